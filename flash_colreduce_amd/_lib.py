@@ -15,6 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libfcr.so")
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
+DTYPE_INT8, DTYPE_E4M3 = 3, 4
 REDUCE_SUM, REDUCE_MAX, REDUCE_MEAN = 0, 1, 2
 OPT_SINGLE_SWEEP, OPT_WAIT_POLLS = 0, 1
 E_WAIT = -8
@@ -85,6 +86,20 @@ def _declare(lib):
     lib.fcr_set_option.argtypes = [c.c_int, c.c_longlong]
     lib.fcr_colreduce_status.restype = c.c_int
     lib.fcr_colreduce_status.argtypes = [c.c_void_p] + [c.c_int] * 6 + [c.c_void_p]
+    i64p, table = c.POINTER(c.c_int64), [c.c_void_p, c.c_int64, c.c_int]
+    lib.fcr_cache_write.restype = c.c_int
+    lib.fcr_cache_write.argtypes = ([c.c_void_p] + table + [c.c_void_p, i64p, c.c_void_p, i64p, c.c_void_p, c.c_void_p, c.c_int,
+                                    c.c_int, c.c_int, i64p, i64p, c.c_void_p])
+    lib.fcr_cache_read.restype = c.c_int
+    lib.fcr_cache_read.argtypes = [c.c_void_p] + table + [c.c_void_p, i64p, c.c_void_p, c.c_void_p, c.c_int, c.c_int, c.c_int, c.c_void_p]
+    lib.fcr_cache_keep.restype = c.c_int
+    lib.fcr_cache_keep.argtypes = ([c.c_void_p] + table + [c.c_void_p, i64p, c.c_void_p, c.c_int, c.c_void_p] + table +
+                                   [c.c_void_p, c.c_int, c.c_void_p])
+    lib.fcr_tree_attention_bytes.restype = c.c_size_t
+    lib.fcr_tree_attention_bytes.argtypes = [c.c_int] * 5 + [c.c_int64]
+    lib.fcr_tree_attention.restype = c.c_int
+    lib.fcr_tree_attention.argtypes = ([c.c_void_p, c.c_void_p] + table + [c.c_void_p, i64p, c.c_void_p, c.c_int64] + [c.c_void_p] * 4 +
+                                       [c.c_size_t, c.c_int, c.c_int, c.c_int, c.c_int, i64p, c.c_float, c.c_void_p])
     lib.fcr_colreduce_ws_status.restype = c.c_int
     lib.fcr_colreduce_ws_status.argtypes = [c.c_void_p, c.c_size_t] + [c.c_int] * 6 + [c.c_void_p]
     return lib

@@ -13,12 +13,17 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = os.path.join(HERE, "csrc", "fcr.hip")
+CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(HERE, "libfcr.so")
 
 OBJ_DIR = os.path.join(HERE, "_build")
-PARTS = (0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13)   # -DFCR_PART=n, see the top of csrc/fcr.hip
+# sources of libfcr.so and their parts (-DFCR_PART=n, see the top of each), compiled side by side
+SOURCES = {
+    "fcr": (0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13),
+    "cache": (0,),
+    "tree_attention": (0, 1, 2, 3, 4),
+}
 
 HIPCC_FLAGS = [
     "-O3",
@@ -40,23 +45,28 @@ def hipcc_path() -> str:
     return exe
 
 
-def build(verbose: bool = True, extra_flags=()) -> str:
-    """Compiles the parts of csrc/fcr.hip side by side (one hipcc each) and links them into libfcr.so."""
+def build(verbose: bool = True, extra_flags=(), only=None) -> str:
+    """Compiles the parts of the sources side by side (one hipcc each) and links them into libfcr.so.  `only`: names of the
+    sources to compile; the objects of the others are those of the last build."""
     hipcc = hipcc_path()
     os.makedirs(OBJ_DIR, exist_ok=True)
-    jobs = []
-    for part in PARTS:
-        obj = os.path.join(OBJ_DIR, f"fcr_part{part}.o")
-        # a part uses a subset of the file's helpers
-        cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, f"-DFCR_PART={part}", "-Wno-unused-function", "-I", INCLUDE,
-               "-c", SRC, "-o", obj]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        jobs.append((cmd, obj, subprocess.Popen(cmd)))
+    jobs, objects = [], []
+    for name, parts in SOURCES.items():
+        for part in parts:
+            obj = os.path.join(OBJ_DIR, f"{name}_part{part}.o")
+            objects.append(obj)
+            if only is not None and name not in only and os.path.exists(obj):
+                continue
+            # a part uses a subset of the file's helpers
+            cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, f"-DFCR_PART={part}", "-Wno-unused-function", "-I", INCLUDE,
+                   "-c", os.path.join(CSRC, name + ".hip"), "-o", obj]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            jobs.append((cmd, obj, subprocess.Popen(cmd)))
     failed = [cmd for cmd, _, proc in jobs if proc.wait() != 0]
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
-    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-fno-gpu-rdc", *[obj for _, obj, _ in jobs], "-o", LIB]
+    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-fno-gpu-rdc", *objects, "-o", LIB]
     if verbose:
         print(" ".join(link), flush=True)
     subprocess.run(link, check=True)

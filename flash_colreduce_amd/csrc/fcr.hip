@@ -110,6 +110,9 @@ void sweeps_f16_both(const Params& p, int ksteps, bool causal, int mode, hipStre
 void sweeps_bf16_both(const Params& p, int ksteps, bool causal, int mode, hipStream_t s);
 void sweeps_f16_long_rows(int which, const Params& p, int ksteps, bool causal, int mode, hipStream_t s);
 void sweeps_bf16_long_rows(int which, const Params& p, int ksteps, bool causal, int mode, hipStream_t s);
+int fail(int code, const char* what);      // for the library's other files: the error text of this thread,
+int launched(const char* what);            //   a launch's status as a return code,
+int chip_cus_of_current_device();          //   and the number of compute units
 extern thread_local bool fused_refused;   // set by a launcher of col_fused_kernel that did not launch
 }  // namespace fcr_detail
 
@@ -5913,6 +5916,9 @@ size_t fcr_lse_bytes_two_kernels(int B, int H, int M, int N) {
 
 }  // namespace
 thread_local bool fcr_detail::fused_refused = false;
+int fcr_detail::fail(int code, const char* what) { return ::fail(code, what); }
+int fcr_detail::launched(const char* what) { return ::launched(what); }
+int fcr_detail::chip_cus_of_current_device() { return chip_cus(); }
 
 extern "C" {
 

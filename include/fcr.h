@@ -58,6 +58,9 @@ extern "C" {
 #define FCR_DTYPE_F16 0
 #define FCR_DTYPE_BF16 1
 #define FCR_DTYPE_F32 2 /* fp32 operands: D a multiple of 4, at most 256 */
+/* element type of a cache (fcr_cache) besides the 16-bit ones: codes of 8 bits, with an fp32 scale per row */
+#define FCR_DTYPE_INT8 3 /* -127 .. 127 */
+#define FCR_DTYPE_E4M3 4 /* 8-bit floats: sign, 4 bits of exponent, 3 of fraction, no infinity, largest value 448 */
 
 /* column reduction over query rows */
 #define FCR_REDUCE_SUM 0 /* also the numerator of 'mean' (flash.py:121-122) */
@@ -280,6 +283,84 @@ int fcr_colreduce_ws_status(const void* ws, size_t ws_bytes, int dtype, int B, i
  * to rounding either way) and the bound on its waits.  For tests and comparisons; returns 0 or FCR_E_SHAPE.
  */
 int fcr_set_option(int option, long long value);
+
+/*
+ * A paged cache of keys and values: what a pruning caller of the column reduction keeps, and what its next tokens attend to.  No
+ * counterpart in the reference.  Nothing of it has a gradient.
+ *
+ * Rows of D elements, in pages of page_size rows of every head: row `j % page_size` of page table[b, j / page_size] holds position j
+ * of sequence b.  k and v are [pages, H, page_size, D] of 16-bit elements or of codes, strides in ELEMENTS in the order (page, head, row):
+ * 16-byte aligned pointers, strides in multiples of 16 bytes, rows that do not overlap and lie less than 2^25 bytes apart; k_scale and
+ * v_scale (codes only) are fp32 [pages, H, page_size] with consecutive scales in a page of a head and 16-byte aligned pages and heads.
+ * page_size is a multiple of 16, D one of 16 in [16, 256].
+ * A row x is held as codes c and a scale s and stands for c s: with a = max |x_d|, FCR_DTYPE_INT8 has s = a / 127 and c = 127 x / a rounded
+ * to a whole number, FCR_DTYPE_E4M3 s = a / 448 and c = 448 x / a rounded to such a float (both to nearest, ties to even; of 16-bit elements
+ * exactly that).  A row of zeros has s = 0.  A row with an infinity or a NaN has s = NaN and codes 0.
+ *
+ * Tables are int32 [B, table_pages], table_stride elements from one sequence to the next.  A page below 0 or not below `pages` is not there:
+ * nothing is written to it, its rows read as zeros, no row attends to its keys.  Lengths (start, counts, lengths, context) are int32
+ * per sequence and head, at at[b * strides[0] + h * strides[1]]; strides[1] = 0 gives every head of a sequence the same one.  Negative
+ * ones count as 0 (start: the tokens in front of position 0 are not written).  Tables and lengths must not change while a call runs.
+ */
+typedef struct fcr_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t k_scale_strides[3];
+  int64_t v_scale_strides[3];
+  int dtype; /* FCR_DTYPE_F16, _BF16, _INT8 or _E4M3 */
+  int pages;
+  int H;
+  int page_size;
+  int D;
+} fcr_cache;
+
+/*
+ * Writes T tokens per sequence: key and value are [B,H,T,D] of `dtype` (FCR_DTYPE_F16, _BF16, _F32; unit d stride, 16-byte aligned
+ * rows), token t goes to position start + t.  With counts (may be NULL) only the first counts tokens of a sequence are written.
+ * Positions behind the table are not written.  Two tokens must not be given the same row.
+ */
+int fcr_cache_write(const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages, const int32_t* start,
+                    const int64_t start_strides[2], const int32_t* counts, const int64_t counts_strides[2], const void* key,
+                    const void* value, int dtype, int B, int T, const int64_t key_strides[4], const int64_t value_strides[4],
+                    void* stream);
+
+/*
+ * Reads positions 0 .. N-1 back: key and value are contiguous [B,H,N,D] of out_dtype, c s in fp32 rounded once.  Rows from `lengths` on
+ * (and behind the table) are zeros.
+ */
+int fcr_cache_read(const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages, const int32_t* lengths,
+                   const int64_t lengths_strides[2], void* key, void* value, int out_dtype, int B, int N, void* stream);
+
+/*
+ * Keeps the rows that a mask names (fcr_topk_mask): keep is contiguous [B,H,N]; of the positions below `lengths` the r-th kept one of a
+ * (sequence, head) goes, codes and scale as they are, to position r of into_table in `into`, which has the same type, heads and D (it may be the
+ * same cache, but no page may be named by both tables).  counts [B,H] receives the number of rows kept, at most what into_table
+ * has room for.  Rows of pages that are not there are not kept.  What lies behind the kept rows is left as it was.
+ */
+int fcr_cache_keep(const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages, const int32_t* lengths,
+                   const int64_t lengths_strides[2], const uint8_t* keep, int N, const fcr_cache* into, const int32_t* into_table,
+                   int64_t into_table_stride, int into_table_pages, int32_t* counts, int B, void* stream);
+
+/*
+ * Attention of T drafted tokens of every sequence over the cache, which holds their keys and values at positions context .. context+T-1.
+ * q is [B, H*G, T, D] (FCR_DTYPE_F16 or _BF16, the cache's type if that holds 16-bit elements), query heads h*G .. h*G+G-1 belong to head h
+ * of the cache.  Token t sees every position below context, and position context + u iff mask[b, t, u] (bytes, [T,T] per sequence, mask_stride
+ * apart, 0: one mask for all) or, with mask NULL, iff u <= t.  tree_lengths [B] (may be NULL): how many of the T tokens a sequence has; the
+ * others are seen by none.  out is contiguous [B, H*G, T, D] of the queries' type: softmax(scale q k^T) v over the keys that a token sees; lse
+ * (may be NULL) fp32 [B, H*G, T], the base-2 log-sum-exp of its scores.  A token that sees nothing, or that the sequence does not have, gets zeros and
+ * -inf.  What hidden keys and values hold has no influence, whatever it is.
+ * ws: fcr_tree_attention_bytes(B, H, G, T, D, table_pages * page_size) bytes, 16-byte aligned (it depends on the number of compute
+ * units: call this with the operands' device current; 0 for sizes that the call refuses), contents irrelevant.
+ */
+size_t fcr_tree_attention_bytes(int B, int H, int G, int T, int D, int64_t positions);
+int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages,
+                       const int32_t* context, const int64_t context_strides[2], const uint8_t* mask, int64_t mask_stride,
+                       const int32_t* tree_lengths, void* out, float* lse, void* ws, size_t ws_bytes, int dtype, int B, int G, int T,
+                       const int64_t q_strides[4], float scale, void* stream);
 
 #ifdef __cplusplus
 }
