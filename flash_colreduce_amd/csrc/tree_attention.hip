@@ -5,23 +5,25 @@
 // sees every key of the context, and of the drafted tokens those that the tree's mask names:
 //   s_j = scale log2(e) <q, c_j> ks_j,   p_j = 2^(s_j - m),   o = sum_j p_j vs_j v_j / sum_j p_j,   lse2 = m + log2 sum_j p_j.
 //
-// The work is bound by reading the cache, so the G query heads of a key head and the drafted tokens are the 16 columns of the matrix
-// instructions (RT column tiles per wave), and every key and value is read once per 16 RT query rows, from global memory into registers
-// without a stop in LDS:
-//   S^T = K Q^T   a lane owns one query (lane & 15) and keys 4 g + i of a 16-key tile (g = lane / 16, register i);
-//   O^T = V^T P^T keeps that query in the lane.  The 8 keys that a lane feeds to one instruction are keys 4 g + i of two tiles, which is
-//                 what the lane holds of P: the probabilities never leave their lane.  V^T is formed from 8 rows of V
-//                 with byte permutes that convert codes at the same time.
-// Softmax statistics are one scalar per lane and in 32 bits.
+// The cache is read once per 16 RT query rows (the G query heads of a key head and the drafted tokens are the columns of the matrix
+// instructions), by one of two kernels.  Both form
+//   S^T = K Q^T   so that a lane owns one query (lane & 15) and keys 4 g + i of a 16-key tile (g = lane / 16, register i), and
+//   O^T = V^T P^T in which that query stays in the lane.  The 8 keys that a lane feeds to one instruction are keys 4 g + i of two tiles,
+//                 which is what it holds of P: probabilities never leave their lane, softmax statistics are one scalar per lane.
+//                 V^T is formed from rows of V with byte permutes that convert codes on the way.
+// tree_attention_kernel (few rows): bound by reading the cache.  Each wave takes 32 keys of a block of 128, from global memory into
+//   registers without a stop in LDS, and all rows; the four waves' results are joined at the end.
+// tall_attention_kernel (many rows): bound by the vector instructions of the softmax and by the matrix units.  Each wave takes 32 rows and
+//   all keys; the operands of a block are converted once, by all waves, and lie in LDS as the matrix instructions take them.
 //
-// Codes are multiplied in fp16, where each of them is exact: bf16 queries are scaled by a power of two per row to fit (elements under
-// 2^-28 of the row's largest lose bits), the keys' scales multiply the scores, the values' scales the probabilities, in 32 bits, before these
-// are rounded to 11 bits.  For that rounding each row has an exponent of its own (State::e), so that weights p_j vs_j fit fp16 whatever
-// the scales are.  16-bit caches are multiplied in their own type.
+// Codes are multiplied in fp16, where each of them is exact: bf16 queries are scaled by one power of two to fit (elements under 2^-38 of
+// the largest are lost, no score changes by more than that part of the largest), the keys' scales multiply the scores, the values' scales the
+// probabilities, in 32 bits, before these are rounded to 11 bits.  16-bit caches are multiplied in their own type.  The reference m of a
+// row is what its weights p_j vs_j ask for, so that they fit fp16 whatever the scales are; sums and statistics are in 32 bits.
 //
-// Distribution: the (batch, head, row tile) items are cut into blocks of 128 keys (a wave takes 32 of each), laid end to end, and every
-// workgroup takes the same number of blocks, found from the lengths on the device.  Parts of an item that was cut are joined by a second
-// kernel, in the order of the keys.
+// Distribution: the (batch, head, row tile) items are cut into blocks of 128 keys, laid end to end, and every workgroup takes the same
+// number of blocks, found from the lengths on the device.  Parts of an item that was cut are joined by tree_join_kernel, in the order of
+// the keys.
 
 #include <math.h>
 
@@ -46,16 +48,17 @@ struct Args {
   char* out;                   // [B, H G, T, D]
   float* lse;                  // [B, H G, T] or null
   int32_t* first;              // [items]: where an item begins, in blocks
-  float* part;                 // [2 workgroups][rows of a tile][D + 2]
+  float* part;                 // [2 workgroups][rows of a tile][D + 4]: reference, sum, 2 unused, weighted values
   int B, H, T, D, rows, row_tiles, bf16;
   Div G;
   float scale2;
   int wgs, least;              // workgroups of the launch; blocks that one takes at least
 };
-void attention_f16(const Args& a, int w, int rt, hipStream_t s);
-void attention_bf16(const Args& a, int w, int rt, hipStream_t s);
-void attention_int8(const Args& a, int w, int rt, hipStream_t s);
-void attention_e4m3(const Args& a, int w, int rt, hipStream_t s);
+// form: see Plan
+void attention_f16(const Args& a, int w, int form, hipStream_t s);
+void attention_bf16(const Args& a, int w, int form, hipStream_t s);
+void attention_int8(const Args& a, int w, int form, hipStream_t s);
+void attention_e4m3(const Args& a, int w, int form, hipStream_t s);
 }  // namespace fcr_tree
 
 namespace {
@@ -64,17 +67,16 @@ using namespace fcr_tree;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kBlock = 32 * kWaves;          // keys of a block
+constexpr int kBlock = 128;                  // keys of a block
 constexpr float kNone = -3.0e38f;            // reference of a row that has seen no key
-constexpr float kLazy = 4.0f;                // scores may pass the reference by this much before it is raised
+constexpr float kMostWeight = 0x1p15f;       // weights above this raise the reference, to where the largest is in (1/2, 1]
+constexpr float kMostSum = 0x1p110f;         // and so do sums above this
 
 __device__ __forceinline__ int blocks_of(int n) { return n <= 0 ? 1 : (n + kBlock - 1) / kBlock; }
 
 // Keys of a sequence: those of the context, then those of the drafted tokens.
 __device__ __forceinline__ void keys_of(const Args& a, int b, int h, int& context, int& n) {
-  const int tree = a.tree_lengths ? min(max(a.tree_lengths[b], 0), a.T) : a.T;
+  const int tree = a.tree_lengths ? min(max(constant_at(a.tree_lengths + b), 0), a.T) : a.T;
   context = max(a.context.of(b, h), 0);
   n = (int)min((int64_t)context + tree, a.c.capacity);
 }
@@ -103,22 +105,10 @@ __device__ __forceinline__ uint32_t halves_of_e4m3(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HI));
 }
 
-// Four codes as four fp16, in their order.
-template <int CD>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (CD == FCR_DTYPE_INT8) {
-    w ^= 0x80808080u;
-    lo = centred(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u));
-    hi = centred(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u));
-  } else {
-    lo = halves_of_e4m3<false>(w);
-    hi = halves_of_e4m3<true>(w);
-  }
-}
-
-// W: D / 64, rounded up.  RT: 16-row tiles of queries per wave.
-template <int CD, int W, int RT>
+// W: D / 64, rounded up.
+template <int CD_, int W>
 struct Form {
+  static constexpr int CD = CD_;
   static constexpr bool codes = CD == FCR_DTYPE_INT8 || CD == FCR_DTYPE_E4M3;
   static constexpr bool bf16 = CD == FCR_DTYPE_BF16;
   static constexpr int KS = 2 * W;                // k-steps of 32 elements
@@ -127,37 +117,37 @@ struct Form {
   static constexpr int VW = codes ? W : 2 * W;    // words that a lane has of a value row
 };
 
-template <class F>
-struct Keys {
-  u32x4 w[2][F::KL];
-  f32x4 scale[2];
-};
-template <class F>
-struct Values {
-  uint32_t w[8][F::VW];
-  f32x4 scale[2];
-};
-
-// Where the two 16-key tiles of a wave's 32 keys lie: page (< 0: not there) and first row in it.
+// Where the 16-key tile from position `pos` on lies: page (< 0: not there, or behind the last key) and first row in it.
 struct Place {
-  int page[2];
-  int row[2];
+  int page, row;
 };
-
 __device__ __forceinline__ Place place_of(const Args& a, int b, int pos, int n) {
-  Place p;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    p.page[t] = -1;
-    p.row[t] = 0;
-    if (pos + 16 * t < n) {
-      uint32_t row;
-      p.page[t] = page_of(a.c, b, (uint32_t)(pos + 16 * t), row);
-      p.row[t] = (int)row;
-    }
+  Place p{-1, 0};
+  if (pos < n) {
+    uint32_t row;
+    p.page = page_of(a.c, b, (uint32_t)pos, row);
+    p.row = (int)row;
   }
   return p;
 }
+
+// The lane's places in rows of keys (lane & 15; 16-byte pieces, of which a row's last one stands for those behind it) and of values (rows
+// 4 g + i, elements from `first` on, where behind the row's end there are elements that another lane has as well).
+template <class F>
+struct Lane {
+  int lane, g, col, first;
+  uint32_t key, piece[F::KL], value;
+  __device__ __forceinline__ Lane(const Args& a, int lane_) {
+    constexpr int e = F::codes ? 1 : 2;
+    lane = lane_, g = lane >> 4, col = lane & 15;
+    first = elements_of(a, col);
+    key = (uint32_t)(col * a.c.side[0].row);
+#pragma unroll
+    for (int i = 0; i < F::KL; ++i) piece[i] = min(64u * i + 16u * g, (uint32_t)(a.D * e) - 16u);
+    value = (uint32_t)(4 * g * a.c.side[1].row) + (uint32_t)(first * e);
+  }
+  __device__ __forceinline__ static int elements_of(const Args& a, int col) { return min(col * F::DT, a.D - F::DT); }
+};
 
 template <int N>
 __device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[N]) {
@@ -180,517 +170,670 @@ __device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[N]) {
   }
 }
 
-// koff: bytes of the lane's key row (lane & 15), kchunk: its 16-byte pieces; a row's last piece stands for those behind it.
+// A 16-key tile as the lane loads it, and its scales of keys 4 g + i.
 template <class F>
-__device__ __forceinline__ void load_keys(const Args& a, int h, const Place& p, uint32_t koff, const uint32_t (&kchunk)[F::KL], int g,
-                                          Keys<F>& k) {
+struct Keys {
+  u32x4 w[F::KL];
+  f32x4 scale;
+  __device__ __forceinline__ void load(const Args& a, int h, const Place& p, const Lane<F>& at) {
+    if (p.page >= 0) {
+      const Side& s = a.c.side[0];
+      const char* base = s.rows + p.page * s.page + h * s.head + p.row * s.row;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    if (p.page[t] >= 0) {
-      const char* base = a.c.side[0].rows + p.page[t] * a.c.side[0].page + h * a.c.side[0].head + p.row[t] * a.c.side[0].row;
-#pragma unroll
-      for (int i = 0; i < F::KL; ++i) k.w[t][i] = *reinterpret_cast<const u32x4*>(base + (koff + kchunk[i]));
-      if constexpr (F::codes)
-        k.scale[t] = *reinterpret_cast<const f32x4*>(a.c.side[0].scale + p.page[t] * a.c.side[0].s_page + h * a.c.side[0].s_head +
-                                                     p.row[t] + 4 * g);
+      for (int i = 0; i < F::KL; ++i) w[i] = *reinterpret_cast<const u32x4*>(base + (at.key + at.piece[i]));
+      if constexpr (F::codes) scale = *reinterpret_cast<const f32x4*>(s.scale + p.page * s.s_page + h * s.s_head + p.row + 4 * at.g);
     } else {
 #pragma unroll
-      for (int i = 0; i < F::KL; ++i) k.w[t][i] = u32x4{0, 0, 0, 0};
-      k.scale[t] = f32x4{0, 0, 0, 0};
+      for (int i = 0; i < F::KL; ++i) w[i] = u32x4{0, 0, 0, 0};
+      scale = f32x4{0, 0, 0, 0};
     }
   }
-}
+  // k-steps 2 i and 2 i + 1 (codes) or i (16-bit) of load i
+  __device__ __forceinline__ u32x4 operand(int ks) const {
+    if constexpr (F::CD == FCR_DTYPE_INT8) {
+      u32x4 f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t x = w[ks / 2][2 * (ks & 1) + j] ^ 0x80808080u;
+        f[2 * j] = centred(__builtin_amdgcn_perm(0x64646464u, x, 0x04010400u));
+        f[2 * j + 1] = centred(__builtin_amdgcn_perm(0x64646464u, x, 0x04030402u));
+      }
+      return f;
+    } else if constexpr (F::CD == FCR_DTYPE_E4M3) {
+      u32x4 f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t x = w[ks / 2][2 * (ks & 1) + j];
+        f[2 * j] = halves_of_e4m3<false>(x);
+        f[2 * j + 1] = halves_of_e4m3<true>(x);
+      }
+      return f;
+    } else {
+      return w[ks];
+    }
+  }
+};
 
-// voff: bytes of row 4 g and of the lane's elements.
 template <class F>
-__device__ __forceinline__ void load_values(const Args& a, int h, const Place& p, uint32_t voff, int g, Values<F>& v) {
+struct Values {
+  uint32_t w[4][F::VW];
+  f32x4 scale;
+  __device__ __forceinline__ void load(const Args& a, int h, const Place& p, const Lane<F>& at) {
+    if (p.page >= 0) {
+      const Side& s = a.c.side[1];
+      const char* base = s.rows + p.page * s.page + h * s.head + p.row * s.row;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    if (p.page[t] >= 0) {
-      const char* base = a.c.side[1].rows + p.page[t] * a.c.side[1].page + h * a.c.side[1].head + p.row[t] * a.c.side[1].row;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) load_words(base + (voff + (uint32_t)(i * a.c.side[1].row)), v.w[4 * t + i]);
-      if constexpr (F::codes)
-        v.scale[t] = *reinterpret_cast<const f32x4*>(a.c.side[1].scale + p.page[t] * a.c.side[1].s_page + h * a.c.side[1].s_head +
-                                                     p.row[t] + 4 * g);
+      for (int i = 0; i < 4; ++i) load_words(base + (at.value + (uint32_t)(i * s.row)), w[i]);
+      if constexpr (F::codes) scale = *reinterpret_cast<const f32x4*>(s.scale + p.page * s.s_page + h * s.s_head + p.row + 4 * at.g);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < F::VW; ++j) v.w[4 * t + i][j] = 0;
-      v.scale[t] = f32x4{0, 0, 0, 0};
+        for (int j = 0; j < F::VW; ++j) w[i][j] = 0;
+      scale = f32x4{0, 0, 0, 0};
     }
   }
-}
-
-// The operand of element d (of the lane's DT) from the 8 rows: V[key][d] for the lane's 8 keys.
-template <int CD, class F>
-__device__ __forceinline__ u32x4 value_operand(const uint32_t (&v)[8][F::VW], int d) {
-  u32x4 f;
-  if constexpr (CD == FCR_DTYPE_INT8) {
-    const uint32_t pick = 0x0c040c00u + 0x00010001u * (d & 3);
+  // Keys that are not there: bits of `there` from bit 0 on.  What their rows hold is not looked at.
+  __device__ __forceinline__ void drop(uint32_t there) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)   // (of codes + 128)
-      f[j] = centred(__builtin_amdgcn_perm(v[2 * j + 1][d / 4], v[2 * j][d / 4], pick) | 0x64006400u);
-  } else if constexpr (CD == FCR_DTYPE_E4M3) {
-    const uint32_t pick = (d & 2) ? 0x07030602u : 0x05010400u;
+    for (int i = 0; i < 4; ++i)
+      if (!((there >> i) & 1u)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = __builtin_amdgcn_perm(v[2 * j + 1][d / 4], v[2 * j][d / 4], pick);
-      f[j] = (d & 1) ? halves_of_e4m3<true>(w) : halves_of_e4m3<false>(w);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      f[j] = __builtin_amdgcn_perm(v[2 * j + 1][d / 2], v[2 * j][d / 2], (d & 1) ? 0x07060302u : 0x05040100u);
+        for (int j = 0; j < F::VW; ++j) w[i][j] = 0;
+        if constexpr (F::codes) scale[i] = 0.0f;
+      }
   }
-  return f;
-}
-
-// Whether a word holds a 16-bit element that is not finite.
-template <bool BF16>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-  return (w & e) == e || ((w >> 16) & e) == e;
-}
+  // Whether a 16-bit element is not finite.
+  __device__ __forceinline__ bool not_finite() const {
+    constexpr uint32_t e = F::bf16 ? 0x7f80u : 0x7c00u;
+    bool is = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < F::VW; ++j) is = is || (w[i][j] & e) == e || ((w[i][j] >> 16) & e) == e;
+    return is;
+  }
+  // Element d (of the lane's DT) of the four rows, as four fp16 or bf16.
+  __device__ __forceinline__ u32x2 operand(int d) const {
+    u32x2 f;
+    if constexpr (F::CD == FCR_DTYPE_INT8) {
+      const uint32_t pick = 0x0c040c00u + 0x00010001u * (d & 3);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        f[j] = centred(__builtin_amdgcn_perm(w[2 * j + 1][d / 4] ^ 0x80808080u, w[2 * j][d / 4] ^ 0x80808080u, pick) | 0x64006400u);
+    } else if constexpr (F::CD == FCR_DTYPE_E4M3) {
+      const uint32_t pick = (d & 2) ? 0x07030602u : 0x05010400u;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t x = __builtin_amdgcn_perm(w[2 * j + 1][d / 4], w[2 * j][d / 4], pick);
+        f[j] = (d & 1) ? halves_of_e4m3<true>(x) : halves_of_e4m3<false>(x);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        f[j] = __builtin_amdgcn_perm(w[2 * j + 1][d / 2], w[2 * j][d / 2], (d & 1) ? 0x07060302u : 0x05040100u);
+    }
+    return f;
+  }
+};
+__device__ __forceinline__ u32x4 joined_operand(u32x2 a, u32x2 b) { return u32x4{a[0], a[1], b[0], b[1]}; }
 
 // What a lane knows of the query of each of its column tiles.
 template <class F, int RT>
 struct State {
-  f32x4 o[RT][F::DT];
-  float m[RT];        // reference exponent, a whole number (raised, not followed: see kLazy); kNone before the first key
-  float l[RT];        // this lane's part of sum 2^(s - m)
-  float e[RT];        // o holds sum 2^(s - m) vs v * 2^e
+  f32x4 o[RT][F::DT];   // sum 2^(s - m) vs v
+  float m[RT];          // reference exponent, a whole number; kNone before the first key
+  float l[RT];          // this lane's part of sum 2^(s - m)
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      m[r] = kNone, l[r] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < F::DT; ++d) o[r][d] = f32x4{0, 0, 0, 0};
+    }
+  }
 };
 
-// The weights of 32 keys from their scores.  `masked`: seen holds the keys that a row sees, bit 4 t + i; else every key is seen.
+// The weights of 32 keys from their products with the queries: 2^(k_scale s - m) v_scale.  `masked`: seen[r] holds the keys that a row
+// sees, bit 4 t + i; else every key is seen.  Bound by the vector unit: per score an fma, an exponential (four slots), the sum, the product
+// with the value's scale, a maximum and half a conversion.  The reference is raised, for the rows that ask for it, where a weight would
+// not fit fp16 or a sum fp32, which a few of the first steps do and hardly any later one: the largest weight may be 2^15 times what the
+// reference was raised for, and nothing needs it to be followed more closely.
 template <class F, int RT>
-__device__ __forceinline__ void weights(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], const f32x4 (&s)[RT][2], const float (&qf)[RT],
-                                        bool masked, const uint32_t (&seen)[RT], State<F, RT>& st, u32x4 (&p)[RT]) {
-  float most_v = 0.0f;
-  if constexpr (F::codes) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most_v = fmaxf(most_v, fabsf(v_scale[e / 4][e % 4]));
-  }
+__device__ __forceinline__ void weights(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], const f32x4 (&s)[RT][2], bool masked,
+                                        const uint32_t (&seen)[RT], State<F, RT>& st, u32x4 (&p)[RT]) {
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    float x[8], by[8];
+    float x[8], sum = 0.0f, most = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      by[e] = F::codes ? qf[r] * k_scale[e / 4][e % 4] : qf[r];
-      x[e] = __builtin_fmaf(s[r][e / 4][e % 4], by[e], -st.m[r]);
-    }
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(s[r][e / 4][e % 4], k_scale[e / 4][e % 4], -st.m[r]);
     if (masked) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = (seen[r] >> e) & 1u ? x[e] : -INFINITY;
     }
-    float most = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) most = fmaxf(most, x[e]);
-    if (__any(most > kLazy)) {
-      // raise the reference of rows whose scores passed it
+    const auto weigh = [&] {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = s[r][e / 4][e % 4] * by[e];
-        if (masked) x[e] = (seen[r] >> e) & 1u ? x[e] : -INFINITY;
-        most = e ? fmaxf(most, x[e]) : x[e];
+        x[e] = __builtin_amdgcn_exp2f(x[e]);
+        sum += x[e];
+        if constexpr (F::codes) x[e] *= v_scale[e / 4][e % 4];
       }
-      most = across(most, true);
-      const float m = most > st.m[r] ? ceilf(most) : st.m[r];
-      float shrink = __builtin_amdgcn_exp2f(st.m[r] - m);
-      st.l[r] *= shrink;
-      if constexpr (F::codes) {
-        // the weights' exponent rises instead of the sums shrinking, as far as fp32 can express 2^e
-        const float e = st.e[r] + (m - st.m[r]);
-        st.e[r] = fminf(e, 120.0f);
-        shrink = __builtin_amdgcn_exp2f(st.e[r] - e);
-      }
-#pragma unroll
-      for (int d = 0; d < F::DT; ++d) st.o[r][d] *= shrink;
-      st.m[r] = m;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] -= m;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = __builtin_amdgcn_exp2f(x[e]);
-      st.l[r] += x[e];
-    }
-    if constexpr (F::codes) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= v_scale[e / 4][e % 4];
-      if (masked) {   // (a hidden value's scale may be a NaN)
+      if (F::codes && masked) {   // (a hidden value's scale may be a NaN)
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = (seen[r] >> e) & 1u ? x[e] : 0.0f;
       }
-      float f = __builtin_amdgcn_exp2f(st.e[r]);
-      if (__any(most_v * f > 0x1p11f)) {
-        // probabilities are 2^kLazy at most: only here can a weight pass fp16
-        float w = 0.0f;
+    };
+    weigh();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w = fmaxf(w, fabsf(x[e]));
-        w = across(w, true);
-        if (w * f > 0x1p15f) {
-          const float to = fminf(st.e[r], (float)(126 - (int)(__builtin_bit_cast(uint32_t, w) >> 23)));   // w 2^to in [1/2, 1)
-          const float by = __builtin_amdgcn_exp2f(to - st.e[r]);
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+    if (__any(most > kMostWeight || !(st.l[r] + sum < kMostSum))) {
+      float of_weights = -INFINITY, of_sum = -INFINITY;
 #pragma unroll
-          for (int d = 0; d < F::DT; ++d) st.o[r][d] *= by;
-          st.e[r] = to;
-          f = __builtin_amdgcn_exp2f(to);
-        }
+      for (int e = 0; e < 8; ++e) {
+        x[e] = s[r][e / 4][e % 4] * k_scale[e / 4][e % 4];
+        if (masked) x[e] = (seen[r] >> e) & 1u ? x[e] : -INFINITY;
+        of_sum = fmaxf(of_sum, x[e]);
+        of_weights = fmaxf(of_weights, F::codes ? x[e] + __builtin_amdgcn_logf(fabsf(v_scale[e / 4][e % 4])) : x[e]);
       }
+      const float top = across(fmaxf(of_weights, of_sum - 100.0f), true);
+      const float m = top > st.m[r] ? ceilf(top) : st.m[r];
+      const float shrink = __builtin_amdgcn_exp2f(st.m[r] - m);
+      st.m[r] = m;
+      st.l[r] *= shrink;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= f;
+      for (int d = 0; d < F::DT; ++d) st.o[r][d] *= shrink;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] -= m;
+      sum = 0.0f;
+      weigh();
     }
+    st.l[r] += sum;
 #pragma unroll
     for (int j = 0; j < 4; ++j) p[r][j] = F::bf16 ? pack2<FCR_DTYPE_BF16>(x[2 * j], x[2 * j + 1]) : pack2<FCR_DTYPE_F16>(x[2 * j], x[2 * j + 1]);
   }
 }
 
-// O^T += V^T P^T where a value that is not finite may stand at a key that some rows do not see: 0 * inf would reach them.  One key
-// at a time, and only rows that see it take the result.
-template <int CD, class F, int RT>
-__device__ __forceinline__ void add_values_one_by_one(const Values<F>& v, const u32x4 (&p)[RT], const uint32_t (&seen)[RT], int lane, State<F, RT>& st) {
+// O^T += V^T P^T of 32 keys, `operand(d)` giving V^T's part.  Where a value that is not finite stands at a key that some rows do not see
+// (one_by_one), 0 * inf would reach them: then one key at a time, and only rows that see it take the result.
+template <class F, int RT, class Operand>
+__device__ __forceinline__ void add_values(const Operand& operand, const u32x4 (&p)[RT], bool one_by_one, const uint32_t (&seen)[RT], const Lane<F>& at,
+                                           State<F, RT>& st) {
+  if (F::codes || !one_by_one) {
+#pragma unroll
+    for (int d = 0; d < F::DT; ++d) {
+      const u32x4 f = operand(d);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(f, p[r], st.o[r][d]);
+    }
+    return;
+  }
   for (int key = 0; key < 32; ++key) {
     const int e = key & 7, g = key >> 3;
-    const bool mine = (lane >> 4) == g;
-    uint32_t row[8][F::VW];
+    u32x4 only;
 #pragma unroll
-    for (int j = 0; j < F::VW; ++j) {
-      uint32_t w = v.w[0][j];
+    for (int j = 0; j < 4; ++j) only[j] = at.g == g && (e >> 1) == j ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+    bool see[RT];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) w = e == i ? v.w[i][j] : w;
-      w = mine ? w : 0;
+    for (int r = 0; r < RT; ++r) see[r] = (__shfl((int)seen[r], 16 * g + at.col) >> e) & 1;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) row[i][j] = i == 0 ? w : 0;   // (the key takes the place of the lane's first)
-    }
+    for (int d = 0; d < F::DT; ++d) {
+      const u32x4 f = operand(d) & only;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      uint32_t w = p[r][0];
+      for (int r = 0; r < RT; ++r) {
+        const f32x4 with = mma<F::bf16>(f, p[r] & only, st.o[r][d]);
 #pragma unroll
-      for (int j = 1; j < 4; ++j) w = (e >> 1) == j ? p[r][j] : w;
-      w = mine ? ((e & 1) ? w >> 16 : w & 0xffffu) : 0;
-      const bool see = (__shfl((int)seen[r], 16 * g + (lane & 15)) >> e) & 1;
-#pragma unroll
-      for (int d = 0; d < F::DT; ++d) {
-        const f32x4 with = mma<F::bf16>(value_operand<CD, F>(row, d), u32x4{w, 0, 0, 0}, st.o[r][d]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.o[r][d][i] = see ? with[i] : st.o[r][d][i];
+        for (int i = 0; i < 4; ++i) st.o[r][d][i] = see[r] ? with[i] : st.o[r][d][i];
       }
     }
   }
 }
 
-template <int CD, int W, int RT>
-__global__ void __launch_bounds__(kThreads) tree_attention_kernel(Args a) {
-  using F = Form<CD, W, RT>;
-  __shared__ float joined[4 * F::DT * 4 * 64];          // [wave][register][tile][lane]
-  __shared__ float stats[kWaves][RT][16][3];            // m, l, e
-  __shared__ int scan[kWaves + 2];
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, col = lane & 15;
-  // workgroups are dealt to 8 dies in turn: consecutive ranges of blocks, which share keys, go to one die
-  const int wg = (blockIdx.x & 7) * (a.wgs >> 3) + (blockIdx.x >> 3);
-
-  // Which blocks are this workgroup's: lengths are known on the device only.  Lengths of sequences: an entry is H heads.
-  const bool by_head = a.context.sh != 0;
-  const int entries = by_head ? a.B * a.H : a.B;
-  const int weight = by_head ? a.row_tiles : a.H * a.row_tiles;
-  const auto entry_blocks = [&](int e) {
-    int context, n;
-    keys_of(a, by_head ? e / a.H : e, by_head ? e % a.H : 0, context, n);
-    return blocks_of(n) * weight;
-  };
-  int total = 0;
-  for (int e = tid; e < entries; e += kThreads) total += entry_blocks(e);
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-  if (lane == 0) scan[wave] = total;
-  __syncthreads();
-  total = scan[0] + scan[1] + scan[2] + scan[3];
-  const int per = max((total + a.wgs - 1) / a.wgs, a.least);
-  int at = wg * per;                                    // (wgs * per is total + wgs at most: checked by the host to fit)
-  const int end = min(at + per, total);
-  if (at >= end) return;
-  int entry = 0, begun = 0;                             // the entry that holds `at`, and its first block
-  for (int base = 0, before = 0;; base += kThreads) {
-    const int e = base + tid;
-    const int mine = e < entries ? entry_blocks(e) : 0;
-    int sum = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(sum, o);
-      if (lane >= o) sum += x;
-    }
-    __syncthreads();
-    if (lane == 63) scan[wave] = sum;
-    if (tid == 0) scan[kWaves] = -1;
-    __syncthreads();
-    int start = before + sum - mine;
-    for (int i = 0; i < wave; ++i) start += scan[i];
-    if (mine > 0 && at >= start && at < start + mine) {
-      scan[kWaves] = e;
-      scan[kWaves + 1] = start;
-    }
-    before += scan[0] + scan[1] + scan[2] + scan[3];
-    __syncthreads();
-    if (scan[kWaves] >= 0) {
-      entry = scan[kWaves], begun = scan[kWaves + 1];
-      break;
-    }
-    if (base + kThreads >= entries) return;             // (only if lengths change under the call)
-  }
-  entry = __builtin_amdgcn_readfirstlane(entry);
-  begun = __builtin_amdgcn_readfirstlane(begun);
-
-  // the lane's places in rows of keys and of values
-  const int e_bytes = F::codes ? 1 : 2;
-  const uint32_t row_bytes = (uint32_t)(a.D * e_bytes);
-  const uint32_t koff = (uint32_t)(col * a.c.side[0].row);
-  uint32_t kchunk[F::KL];
-#pragma unroll
-  for (int i = 0; i < F::KL; ++i) kchunk[i] = min(64u * i + 16u * g, row_bytes - 16u);
-  const int dfirst = min(col * F::DT, a.D - F::DT);     // (behind the row's end: elements that another lane has as well)
-  const uint32_t voff = (uint32_t)(4 * g * a.c.side[1].row) + (uint32_t)(dfirst * e_bytes);
-
-  int b = by_head ? entry / a.H : entry, h = by_head ? entry % a.H : 0;
-  int context, n;
-  keys_of(a, b, h, context, n);
-  int nb = blocks_of(n);
-  int in = at - begun;                                  // blocks from the entry's begin
-  if (!by_head) {
-    h = in / (nb * a.row_tiles);
-    in -= h * nb * a.row_tiles;
-  }
-  int tile = in / nb;
-  int blk = in - tile * nb;
-
-  while (at < end) {
-    context = __builtin_amdgcn_readfirstlane(context);
-    n = __builtin_amdgcn_readfirstlane(n);
-    const int item = (b * a.H + h) * a.row_tiles + tile;
-    const int stop = min(nb, blk + (end - at));         // blocks [blk, stop) of this item
-
-    // queries: column col of tile r is row 16 r + col of the workgroup's, token t, head gq of the key head
-    u32x4 q[RT][F::KS];
-    float qf[RT];
-    int token[RT];
+// The queries of column tiles from row `row0` on: row t G + g is token t and head g of the key head's.  Elements in the order in which
+// the lane has those of a key.
+template <class F, int RT>
+struct Queries {
+  u32x4 w[RT][F::KS];
+  int token[RT];
+  // Returns the largest element's bits where they are to be scaled.
+  __device__ __forceinline__ uint32_t load(const Args& a, int b, int h, int row0, const Lane<F>& at) {
+    uint32_t most = 0;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const int row = (tile * RT + r) * 16 + col;
+      const int row = row0 + 16 * r + at.col;
       const bool live = row < a.rows;
-      const uint32_t t = a.G.of((uint32_t)(live ? row : 0)), gq = (uint32_t)(live ? row : 0) - t * a.G.d;
+      const uint32_t t = a.G.of((uint32_t)(live ? row : 0)), head = (uint32_t)(live ? row : 0) - t * a.G.d;
       token[r] = (int)t;
-      const char* at_q = a.q + b * a.qb + (int64_t)(h * (int)a.G.d + (int)gq) * a.qh + t * a.qt;
-      qf[r] = a.scale2;
-      uint32_t most = 0;
+      const char* from = a.q + b * a.qb + (int64_t)(h * (int)a.G.d + (int)head) * a.qh + t * a.qt;
 #pragma unroll
       for (int s = 0; s < F::KS; ++s) {
-        // the elements that the lane's part of a key stands for in k-step s
-        const int d = F::codes ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
-        q[r][s] = live && d < a.D ? *reinterpret_cast<const u32x4*>(at_q + 2 * d) : u32x4{0, 0, 0, 0};
+        const int d = F::codes ? 64 * (s / 2) + 16 * at.g + 8 * (s & 1) : 32 * s + 8 * at.g;
+        w[r][s] = live && d < a.D ? *reinterpret_cast<const u32x4*>(from + 2 * d) : u32x4{0, 0, 0, 0};
         if constexpr (F::codes) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) most = max(most, max(q[r][s][j] & 0x7fffu, (q[r][s][j] >> 16) & 0x7fffu));
-        }
-      }
-      if constexpr (F::codes) {
-        if (a.bf16) {
-          most = max(most, (uint32_t)__shfl_xor((int)most, 16));
-          most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-          // largest element to [2^14, 2^15); exponents in steps of two halves, each in range
-          const int up = most == 0 || most >= 0x7f80u ? 0 : min(14 - ((int)(most >> 7) - 127), 140);
-          const float by1 = __builtin_bit_cast(float, (uint32_t)(127 + up / 2) << 23), by2 = __builtin_bit_cast(float, (uint32_t)(127 + up - up / 2) << 23);
-          const float undo1 = __builtin_bit_cast(float, (uint32_t)(127 - up / 2) << 23), undo2 = __builtin_bit_cast(float, (uint32_t)(127 - (up - up / 2)) << 23);
-          qf[r] = a.scale2 * undo1 * undo2;
-#pragma unroll
-          for (int s = 0; s < F::KS; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              q[r][s][j] = pack2<FCR_DTYPE_F16>(bf16_of(q[r][s][j], 0) * by1 * by2, bf16_of(q[r][s][j], 1) * by1 * by2);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = w[r][s][j] & 0x7fffu, hi = (w[r][s][j] >> 16) & 0x7fffu;
+            most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));   // (of what is finite)
+          }
         }
       }
     }
+    return most;
+  }
+  // bf16 to fp16, the largest element (its bits: `most`, the same in every lane) to [2^14, 2^15).  Returns what undoes it.
+  __device__ __forceinline__ float scale(uint32_t most) {
+    const int up = most == 0 ? 0 : max(-112, min(14 - ((int)(most >> 7) - 127), 140));
+    // (in two steps, each of which fp32 can express)
+    const float by1 = __builtin_bit_cast(float, (uint32_t)(127 + up / 2) << 23), by2 = __builtin_bit_cast(float, (uint32_t)(127 + up - up / 2) << 23);
+    const float undo1 = __builtin_bit_cast(float, (uint32_t)(127 - up / 2) << 23), undo2 = __builtin_bit_cast(float, (uint32_t)(127 - (up - up / 2)) << 23);
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int s = 0; s < F::KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[r][s][j] = pack2<FCR_DTYPE_F16>(bf16_of(w[r][s][j], 0) * by1 * by2, bf16_of(w[r][s][j], 1) * by1 * by2);
+    return undo1 * undo2;
+  }
+};
+__device__ __forceinline__ uint32_t largest_of_wave(uint32_t x) {
+  for (int o = 1; o < 64; o <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
+  return x;
+}
 
+// Which of the lane's keys from position `pos` on (a 32-key step: bits 4 t + i) the query of token t sees.
+__device__ __forceinline__ uint32_t seen_by(const Args& a, int b, int token, int pos, int context, uint32_t there, int g) {
+  uint32_t seen = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int u = pos + 16 * (e / 4) + 4 * g + e % 4 - context;   // which drafted token
+    bool is = (there >> e) & 1u;
+    if (is && u >= 0) is = a.mask ? a.mask[b * a.mask_b + (int64_t)token * a.T + u] != 0 : u <= token;
+    seen |= is ? 1u << e : 0u;
+  }
+  return seen;
+}
+// Which of the lane's keys are there: in front of n, on a page that is.  Bits 4 t + i.
+__device__ __forceinline__ uint32_t there_of(int pos, int n, bool page0, bool page1, int g) {
+  uint32_t there = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) there |= pos + 16 * (e / 4) + 4 * g + e % 4 < n && (e < 4 ? page0 : page1) ? 1u << e : 0u;
+  return there;
+}
+
+// DT consecutive elements of a row: its result, or its part of one.
+template <class F>
+__device__ __forceinline__ void emit(const Args& a, bool final, float* slot, int b, int h, int row, int row_in_tile, int token, int d0, bool first,
+                                     const float (&x)[F::DT], float m, float l) {
+  if (row >= a.rows) return;
+  if (final) {
+    const bool none = (a.tree_lengths && token >= a.tree_lengths[b]) || l == 0.0f;
+    const float inverse = 1.0f / l;
+    const int64_t to = ((int64_t)b * a.H * a.G.d + (int64_t)h * a.G.d + (row - token * (int)a.G.d)) * a.T + token;
+    uint32_t* const o = reinterpret_cast<uint32_t*>(a.out + (to * a.D + d0) * 2);
+#pragma unroll
+    for (int d = 0; d < F::DT; d += 4) {
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = none ? 0.0f : x[d + j] * inverse;
+      const u32x2 v = a.bf16 ? u32x2{pack2<FCR_DTYPE_BF16>(y[0], y[1]), pack2<FCR_DTYPE_BF16>(y[2], y[3])}
+                             : u32x2{pack2<FCR_DTYPE_F16>(y[0], y[1]), pack2<FCR_DTYPE_F16>(y[2], y[3])};
+      *reinterpret_cast<u32x2*>(o + d / 2) = v;          // (d0 is a multiple of 4)
+    }
+    if (a.lse && first) a.lse[to] = none ? -INFINITY : m + __builtin_amdgcn_logf(l);
+  } else {
+    float* const o = slot + (int64_t)row_in_tile * (a.D + 4);
+#pragma unroll
+    for (int d = 0; d < F::DT; d += 4) *reinterpret_cast<f32x4*>(o + 4 + d0 + d) = f32x4{x[d], x[d + 1], x[d + 2], x[d + 3]};
+    if (first) o[0] = m, o[1] = l;
+  }
+}
+
+// The blocks of a workgroup, as pieces of items.  Lengths are known on the device only: every workgroup adds them up.  Lengths of
+// sequences (not of heads): an entry is all heads of one.
+template <int THREADS>
+struct Deal {
+  int at, end, b, h, tile, blk, nb, context, n;
+  __device__ __forceinline__ bool start(const Args& a, int wg, int* scan) {   // scan: THREADS / 64 + 2 words of LDS
+    constexpr int waves = THREADS / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const bool by_head = a.context.sh != 0;
+    const int entries = by_head ? a.B * a.H : a.B;
+    const int weight = by_head ? a.row_tiles : a.H * a.row_tiles;
+    const auto entry_blocks = [&](int e) {
+      int context, n;
+      keys_of(a, by_head ? e / a.H : e, by_head ? e % a.H : 0, context, n);
+      return blocks_of(n) * weight;
+    };
+    int total = 0;
+    for (int e = tid; e < entries; e += THREADS) total += entry_blocks(e);
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    if (lane == 0) scan[wave] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < waves; ++i) total += scan[i];
+    const int per = max((total + a.wgs - 1) / a.wgs, a.least);
+    at = wg * per;                                      // (wgs * per is total + wgs at most: checked by the host to fit)
+    end = min(at + per, total);
+    if (at >= end) return false;
+    int entry = 0, begun = 0;                           // the entry that holds `at`, and its first block
+    for (int base = 0, before = 0;; base += THREADS) {
+      const int e = base + tid;
+      const int mine = e < entries ? entry_blocks(e) : 0;
+      int sum = mine;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(sum, o);
+        if (lane >= o) sum += x;
+      }
+      __syncthreads();
+      if (lane == 63) scan[wave] = sum;
+      if (tid == 0) scan[waves] = -1;
+      __syncthreads();
+      int start = before + sum - mine;
+      for (int i = 0; i < wave; ++i) start += scan[i];
+      if (mine > 0 && at >= start && at < start + mine) {
+        scan[waves] = e;
+        scan[waves + 1] = start;
+      }
+#pragma unroll
+      for (int i = 0; i < waves; ++i) before += scan[i];
+      __syncthreads();
+      if (scan[waves] >= 0) {
+        entry = scan[waves], begun = scan[waves + 1];
+        break;
+      }
+      if (base + THREADS >= entries) return false;      // (only if lengths change under the call)
+    }
+    entry = __builtin_amdgcn_readfirstlane(entry);
+    int in = at - __builtin_amdgcn_readfirstlane(begun); // blocks from the entry's begin
+    b = by_head ? entry / a.H : entry, h = by_head ? entry % a.H : 0;
+    look(a);
+    if (!by_head) {
+      h = in / (nb * a.row_tiles);
+      in -= h * nb * a.row_tiles;
+    }
+    tile = in / nb;
+    blk = in - tile * nb;
+    return true;
+  }
+  __device__ __forceinline__ void look(const Args& a) {
+    keys_of(a, b, h, context, n);
+    context = __builtin_amdgcn_readfirstlane(context);
+    n = __builtin_amdgcn_readfirstlane(n);
+    nb = blocks_of(n);
+  }
+  __device__ __forceinline__ int stop() const { return min(nb, blk + (end - at)); }   // blocks [blk, stop) of this item
+  __device__ __forceinline__ int item(const Args& a) const { return (b * a.H + h) * a.row_tiles + tile; }
+  // To the next piece; false: there is none.
+  __device__ __forceinline__ bool next(const Args& a) {
+    at += stop() - blk;
+    if (at >= end) return false;
+    blk = 0;
+    if (++tile == a.row_tiles) {
+      tile = 0;
+      if (++h == a.H) h = 0, ++b;
+      look(a);
+    }
+    return true;
+  }
+};
+// workgroups are dealt to 8 dies in turn: consecutive ranges of blocks, whose row tiles share keys, go to one die
+__device__ __forceinline__ int range_of(const Args& a, int block) { return (block & 7) * (a.wgs >> 3) + (block >> 3); }
+
+template <int CD, int W, int RT>
+__global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kernel(Args a) {
+  using F = Form<CD, W>;
+  constexpr int kWaves = 4;
+  __shared__ float joined[kWaves * 4 * F::DT * 64];     // [wave][register][tile][lane]
+  __shared__ float stats[kWaves][RT][16][2];            // m, l
+  __shared__ int scan[kWaves + 2];
+  const int wg = range_of(a, blockIdx.x);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const Lane<F> at(a, threadIdx.x & 63);
+  Deal<256> deal;
+  if (!deal.start(a, wg, scan)) return;
+  do {
+    const int b = deal.b, h = deal.h, n = deal.n, context = deal.context, stop = deal.stop();
+    const int row0 = deal.tile * 16 * RT;
+    Queries<F, RT> q;
+    float by = a.scale2;
+    const uint32_t most = q.load(a, b, h, row0, at);
+    if (F::codes && a.bf16) by *= q.scale(largest_of_wave(most));
     State<F, RT> st;
+    st.clear();
+    Keys<F> k[2];
+    Values<F> v[2];
+    Place here[2], next[2];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      st.m[r] = kNone, st.l[r] = 0.0f, st.e[r] = F::codes ? 120.0f : 0.0f;
-#pragma unroll
-      for (int d = 0; d < F::DT; ++d) st.o[r][d] = f32x4{0, 0, 0, 0};
+    for (int t = 0; t < 2; ++t) {
+      here[t] = place_of(a, b, deal.blk * kBlock + wave * 32 + 16 * t, n);
+      k[t].load(a, h, here[t], at);
+      v[t].load(a, h, here[t], at);
     }
-
-    Keys<F> k;
-    Values<F> v;
-    Place here = place_of(a, b, blk * kBlock + wave * 32, n);
-    load_keys<F>(a, h, here, koff, kchunk, g, k);
-    load_values<F>(a, h, here, voff, g, v);
-    for (int i = blk; i < stop; ++i) {
+    for (int i = deal.blk; i < stop; ++i) {
       const int pos = i * kBlock + wave * 32;
-      const Place next = i + 1 < stop ? place_of(a, b, pos + kBlock, n) : Place{{-1, -1}, {0, 0}};
       if (pos >= n) break;                              // (a wave's later blocks lie behind this one)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) next[t] = place_of(a, b, pos + kBlock + 16 * t, i + 1 < stop ? n : 0);
       f32x4 s[RT][2];
 #pragma unroll
-      for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = f32x4{0, 0, 0, 0};
+      for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int r = 0; r < RT; ++r) s[r][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int c = 0; c < F::KL; ++c) {
-          if constexpr (F::codes) {
-            u32x4 f[2];
+        for (int c = 0; c < F::KS; ++c) {
+          const u32x4 f = k[t].operand(c);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t lo, hi;
-              widen<CD>(k.w[t][c][j], lo, hi);
-              f[j / 2][2 * (j & 1)] = lo, f[j / 2][2 * (j & 1) + 1] = hi;
-            }
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-              s[r][t] = mma<false>(f[0], q[r][2 * c], s[r][t]);
-              s[r][t] = mma<false>(f[1], q[r][2 * c + 1], s[r][t]);
-            }
-          } else {
-#pragma unroll
-            for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(k.w[t][c], q[r][c], s[r][t]);
-          }
+          for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(f, q.w[r][c], s[r][t]);
         }
-      const f32x4 k_scale[2] = {k.scale[0], k.scale[1]};
-      if (i + 1 < stop) load_keys<F>(a, h, next, koff, kchunk, g, k);
-
+      }
+      f32x4 k_scale[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) k_scale[t] = F::codes ? k[t].scale * by : f32x4{by, by, by, by};
+      if (i + 1 < stop) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) k[t].load(a, h, next[t], at);
+      }
       u32x4 p[RT];
       uint32_t seen[RT] = {};
-      const bool masked = pos + 32 > min(context, n) || here.page[0] < 0 || here.page[1] < 0;
+      const bool masked = pos + 32 > min(context, n) || here[0].page < 0 || here[1].page < 0;
       bool one_by_one = false;
       if (masked) {
-        uint32_t there = 0;
+        const uint32_t there = there_of(pos, n, here[0].page >= 0, here[1].page >= 0, at.g);
+        v[0].drop(there);
+        v[1].drop(there >> 4);
+        if constexpr (!F::codes) one_by_one = pos + 32 > context && __any(v[0].not_finite() || v[1].not_finite());
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool is = pos + 16 * (e / 4) + 4 * g + e % 4 < n && here.page[e / 4] >= 0;
-          there |= is ? 1u << e : 0u;
-          if (!is) {
-#pragma unroll
-            for (int j = 0; j < F::VW; ++j) v.w[e][j] = 0;
-            v.scale[e / 4][e % 4] = 0.0f;
-          }
-        }
-        if constexpr (!F::codes) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int j = 0; j < F::VW; ++j) one_by_one = one_by_one || not_finite<F::bf16>(v.w[e][j]);
-          one_by_one = __any(one_by_one) && pos + 32 > context;
-        }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int u = pos + 16 * (e / 4) + 4 * g + e % 4 - context;   // which drafted token
-            bool is = (there >> e) & 1u;
-            if (is && u >= 0) is = a.mask ? a.mask[b * a.mask_b + (int64_t)token[r] * a.T + u] != 0 : u <= token[r];
-            seen[r] |= is ? 1u << e : 0u;
-          }
-        }
+        for (int r = 0; r < RT; ++r) seen[r] = seen_by(a, b, q.token[r], pos, context, there, at.g);
       }
-      weights<F, RT>(k_scale, v.scale, s, qf, masked, seen, st, p);
-      if constexpr (CD == FCR_DTYPE_INT8) {
+      const f32x4 v_scale[2] = {v[0].scale, v[1].scale};
+      weights<F, RT>(k_scale, v_scale, s, masked, seen, st, p);
+      add_values<F, RT>([&](int d) { return joined_operand(v[0].operand(d), v[1].operand(d)); }, p, one_by_one, seen, at, st);
+      if (i + 1 < stop) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int j = 0; j < F::VW; ++j) v.w[e][j] ^= 0x80808080u;   // codes + 128, see value_operand
+        for (int t = 0; t < 2; ++t) v[t].load(a, h, next[t], at);
       }
-      if (one_by_one) {
-        add_values_one_by_one<CD, F, RT>(v, p, seen, lane, st);
-      } else {
-#pragma unroll
-        for (int d = 0; d < F::DT; ++d) {
-          const u32x4 f = value_operand<CD, F>(v.w, d);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(f, p[r], st.o[r][d]);
-        }
-      }
-      if (i + 1 < stop) load_values<F>(a, h, next, voff, g, v);
-      here = next;
+      here[0] = next[0], here[1] = next[1];
     }
 
     // join the four waves
-    const bool final = blk == 0 && stop == nb;
-    float* const slot = a.part + (int64_t)(2 * wg + (blk == 0 ? 1 : 0)) * (16 * RT) * (a.D + 2);
-    if (blk == 0 && tid == 0 && a.first) a.first[item] = at;
+    const bool final = deal.blk == 0 && stop == deal.nb;
+    float* const slot = a.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * (16 * RT) * (a.D + 4);
+    if (deal.blk == 0 && threadIdx.x == 0) a.first[deal.item(a)] = deal.at;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const float l = across(st.l[r], false);
-      if (g == 0) {
-        stats[wave][r][col][0] = st.m[r];
-        stats[wave][r][col][1] = l;
-        stats[wave][r][col][2] = st.e[r];
-      }
+      if (at.g == 0) stats[wave][r][at.col][0] = st.m[r], stats[wave][r][at.col][1] = l;
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      float m = stats[0][r][col][0];
+      float m = stats[0][r][at.col][0], l = 0.0f;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[w][r][col][0]);
-      float l = 0.0f;
+      for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[w][r][at.col][0]);
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) l += stats[w][r][col][1] * __builtin_amdgcn_exp2f(stats[w][r][col][0] - m);
-      const float by = __builtin_amdgcn_exp2f(st.m[r] - m - st.e[r]);
-      // (a wave that has seen nothing has sums of zero; its exponent may not be expressible)
-      const bool none = st.m[r] == kNone;
+      for (int w = 0; w < kWaves; ++w) l += stats[w][r][at.col][1] * __builtin_amdgcn_exp2f(stats[w][r][at.col][0] - m);
+      const float shrink = __builtin_amdgcn_exp2f(st.m[r] - m);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int d = 0; d < F::DT; ++d) joined[((wave * 4 + i) * F::DT + d) * 64 + lane] = none ? 0.0f : st.o[r][d][i] * by;
+        for (int d = 0; d < F::DT; ++d) joined[((wave * 4 + i) * F::DT + d) * 64 + at.lane] = st.o[r][d][i] * shrink;
       __syncthreads();
-      // wave w writes register w of every tile: query col, elements from dfirst of lane 4 g + w on
-      const int row = (tile * RT + r) * 16 + col;
-      const int d0 = min((4 * g + wave) * F::DT, a.D - F::DT);
+      // wave w writes register w of every tile: query col, the elements of lane 4 g + w
       float x[F::DT];
 #pragma unroll
       for (int d = 0; d < F::DT; ++d) {
         x[d] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) x[d] += joined[((w * 4 + wave) * F::DT + d) * 64 + lane];
+        for (int w = 0; w < kWaves; ++w) x[d] += joined[((w * 4 + wave) * F::DT + d) * 64 + at.lane];
       }
-      if (row < a.rows) {
-        if (final) {
-          const bool none = (a.tree_lengths && token[r] >= a.tree_lengths[b]) || l == 0.0f;
-          const float inverse = 1.0f / l;
-          const int64_t to = ((int64_t)b * a.H * a.G.d + (int64_t)h * a.G.d + (row - token[r] * (int)a.G.d)) * a.T + token[r];
-#pragma unroll
-          for (int d = 0; d < F::DT; ++d) x[d] = none ? 0.0f : x[d] * inverse;
-          uint32_t* const o = reinterpret_cast<uint32_t*>(a.out + (to * a.D + d0) * 2);
-#pragma unroll
-          for (int d = 0; d < F::DT / 2; ++d) o[d] = a.bf16 ? pack2<FCR_DTYPE_BF16>(x[2 * d], x[2 * d + 1]) : pack2<FCR_DTYPE_F16>(x[2 * d], x[2 * d + 1]);
-          if (a.lse && wave == 0 && g == 0) a.lse[to] = none ? -INFINITY : m + __builtin_amdgcn_logf(l);
-        } else {
-          float* const o = slot + (16 * r + col) * (a.D + 2);
-#pragma unroll
-          for (int d = 0; d < F::DT; ++d) o[2 + d0 + d] = x[d];
-          if (wave == 0 && g == 0) o[0] = m, o[1] = l;
-        }
-      }
+      emit<F>(a, final, slot, b, h, row0 + 16 * r + at.col, 16 * r + at.col, q.token[r], Lane<F>::elements_of(a, 4 * at.g + wave),
+              wave == 0 && at.g == 0, x, m, l);
       __syncthreads();
     }
+  } while (deal.next(a));
+}
 
-    at += stop - blk;
-    blk = 0;
-    if (++tile == a.row_tiles) {
-      tile = 0;
-      if (++h == a.H) h = 0, ++b;
-      if (at < end) {
-        keys_of(a, b, h, context, n);
-        nb = blocks_of(n);
+// Column tiles per wave: two, where their sums and queries leave room in 256 registers.
+constexpr int tall_tiles(int w) { return w <= 2 ? 2 : 1; }
+
+// A stage holds a block's operands: of every 16-key tile the KS key operands, of every 32 keys the DT value operands,
+// 16 bytes per lane, and the scales.  A wave converts 128 / WAVES keys of it.
+template <int CD, int W, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, WAVES == 4 && W >= 3 ? 1 : 2) tall_attention_kernel(Args a) {
+  using F = Form<CD, W>;
+  constexpr int RT = tall_tiles(W), kTiles = 8 / WAVES;  // 16-key tiles that a wave converts
+  __shared__ __attribute__((aligned(16))) char lds[(8 * F::KS + 4 * F::DT) * 64 * 16 + 2 * kBlock * 4 + (8 + WAVES + 2) * 4];
+  u32x4* const ks = reinterpret_cast<u32x4*>(lds);                       // [8][KS][64]
+  u32x4* const vs = ks + 8 * F::KS * 64;                                 // [4][DT][64]
+  float* const k_scales = reinterpret_cast<float*>(vs + 4 * F::DT * 64); // [128]
+  float* const v_scales = k_scales + kBlock;                             // [128]
+  int* const flags = reinterpret_cast<int*>(v_scales + kBlock);          // [8]: a tile's page is there, and (bit 1) a value is not finite
+  int* const scan = flags + 8;                                           // [WAVES + 2]
+  const int wg = range_of(a, blockIdx.x);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const Lane<F> at(a, threadIdx.x & 63);
+  Deal<64 * WAVES> deal;
+  if (!deal.start(a, wg, scan)) return;
+  do {
+    const int b = deal.b, h = deal.h, n = deal.n, context = deal.context, stop = deal.stop();
+    const int row0 = (deal.tile * WAVES + wave) * 16 * RT;
+    Queries<F, RT> q;
+    float by = a.scale2;
+    uint32_t most = q.load(a, b, h, row0, at);
+    if (F::codes && a.bf16) {
+      // one power of two for all rows of the workgroup, which the keys' scales undo
+      most = largest_of_wave(most);
+      __syncthreads();
+      if (at.lane == 0) scan[wave] = (int)most;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) most = max(most, (uint32_t)scan[w]);
+      by *= q.scale(most);
+    }
+    State<F, RT> st;
+    st.clear();
+    Keys<F> k[kTiles];
+    Values<F> v[kTiles];
+    Place place[kTiles];
+    const auto fetch = [&](int i) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        place[t] = place_of(a, b, i * kBlock + (wave * kTiles + t) * 16, n);
+        k[t].load(a, h, place[t], at);
+        v[t].load(a, h, place[t], at);
+      }
+    };
+    fetch(deal.blk);
+    for (int i = deal.blk; i < stop; ++i) {
+      __syncthreads();                                  // (the block before has been used)
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const int tile = wave * kTiles + t, pos = i * kBlock + tile * 16;
+        int flag = place[t].page >= 0 ? 1 : 0;
+        if (!flag || pos + 16 > min(context, n)) {
+          v[t].drop(there_of(pos, n, flag, flag, at.g));
+          if constexpr (!F::codes) flag |= pos + 16 > context && __any(v[t].not_finite()) ? 2 : 0;
+        }
+#pragma unroll
+        for (int c = 0; c < F::KS; ++c) ks[(tile * F::KS + c) * 64 + at.lane] = k[t].operand(c);
+        if constexpr (F::codes) {
+          if (at.col == 0) {
+            *reinterpret_cast<f32x4*>(k_scales + tile * 16 + 4 * at.g) = k[t].scale * by;
+            *reinterpret_cast<f32x4*>(v_scales + tile * 16 + 4 * at.g) = v[t].scale;
+          }
+        }
+        if (at.lane == 0) flags[tile] = flag;
+      }
+      if constexpr (kTiles == 2) {
+#pragma unroll
+        for (int d = 0; d < F::DT; ++d) vs[(wave * F::DT + d) * 64 + at.lane] = joined_operand(v[0].operand(d), v[1].operand(d));
+      } else {
+#pragma unroll
+        for (int d = 0; d < F::DT; ++d)
+          reinterpret_cast<u32x2*>(vs + ((wave / 2) * F::DT + d) * 64 + at.lane)[wave & 1] = v[0].operand(d);
+      }
+      if (i + 1 < stop) fetch(i + 1);
+      __syncthreads();
+#pragma unroll 1
+      for (int step = 0; step < 4; ++step) {
+        const int pos = i * kBlock + step * 32;
+        if (pos >= n) break;
+        f32x4 s[RT][2], k_scale[2], v_scale[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int r = 0; r < RT; ++r) s[r][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int c = 0; c < F::KS; ++c) {
+            const u32x4 f = ks[((2 * step + t) * F::KS + c) * 64 + at.lane];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(f, q.w[r][c], s[r][t]);
+          }
+          if constexpr (F::codes) {
+            k_scale[t] = *reinterpret_cast<const f32x4*>(k_scales + step * 32 + 16 * t + 4 * at.g);
+            v_scale[t] = *reinterpret_cast<const f32x4*>(v_scales + step * 32 + 16 * t + 4 * at.g);
+          } else {
+            k_scale[t] = f32x4{by, by, by, by};
+            v_scale[t] = f32x4{1, 1, 1, 1};
+          }
+        }
+        u32x4 p[RT];
+        uint32_t seen[RT] = {};
+        const int flag0 = __builtin_amdgcn_readfirstlane(flags[2 * step]), flag1 = __builtin_amdgcn_readfirstlane(flags[2 * step + 1]);
+        const bool masked = pos + 32 > min(context, n) || !(flag0 & flag1 & 1);
+        if (masked) {
+          const uint32_t there = there_of(pos, n, flag0 & 1, flag1 & 1, at.g);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) seen[r] = seen_by(a, b, q.token[r], pos, context, there, at.g);
+        }
+        weights<F, RT>(k_scale, v_scale, s, masked, seen, st, p);
+        add_values<F, RT>([&](int d) { return vs[(step * F::DT + d) * 64 + at.lane]; }, p, ((flag0 | flag1) & 2) != 0, seen, at, st);
       }
     }
-  }
+    const bool final = deal.blk == 0 && stop == deal.nb;
+    float* const slot = a.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * (16 * RT * WAVES) * (a.D + 4);
+    if (deal.blk == 0 && threadIdx.x == 0) a.first[deal.item(a)] = deal.at;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float l = across(st.l[r], false);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x[F::DT];
+#pragma unroll
+        for (int d = 0; d < F::DT; ++d) x[d] = st.o[r][d][i];
+        emit<F>(a, final, slot, b, h, row0 + 16 * r + at.col, (wave * RT + r) * 16 + at.col, q.token[r], Lane<F>::elements_of(a, 4 * at.g + i),
+                at.g == 0 && i == 0, x, st.m[r], l);
+      }
+    }
+  } while (deal.next(a));
 }
 
 #if FCR_HAS(0)
-// Joins the parts of items that were cut: a thread per two elements of a row.
-__global__ void __launch_bounds__(256) tree_join_kernel(Args a, int tile_rows) {
-  const int item = blockIdx.x;
+// Joins the parts of items that were cut, in the order of their keys: a thread per four elements of a row.
+__global__ void __launch_bounds__(256) tree_join_kernel(Args a, int tile_rows, int groups) {
+  const int item = blockIdx.x / groups;
   const int tile = item % a.row_tiles, bh = item / a.row_tiles;
   const int b = bh / a.H, h = bh - b * a.H;
   // how many blocks a workgroup took, as the first kernel found it
@@ -698,9 +841,8 @@ __global__ void __launch_bounds__(256) tree_join_kernel(Args a, int tile_rows) {
   const bool by_head = a.context.sh != 0;
   const int entries = by_head ? a.B * a.H : a.B;
   const int weight = by_head ? a.row_tiles : a.H * a.row_tiles;
-  int total = 0;
+  int total = 0, context, n;
   for (int e = threadIdx.x; e < entries; e += 256) {
-    int context, n;
     keys_of(a, by_head ? e / a.H : e, by_head ? e % a.H : 0, context, n);
     total += blocks_of(n) * weight;
   }
@@ -709,69 +851,77 @@ __global__ void __launch_bounds__(256) tree_join_kernel(Args a, int tile_rows) {
   __syncthreads();
   total = scan[0] + scan[1] + scan[2] + scan[3];
   const int per = max((total + a.wgs - 1) / a.wgs, a.least);
-  int context, n;
   keys_of(a, b, h, context, n);
   const int begin = a.first[item];
   const int from = begin / per, to = (begin + blocks_of(n) - 1) / per;
   if (from == to) return;
-  const int pairs = a.D / 2;
+  const int pieces = a.D / 4;
   const int rows = min(tile_rows, a.rows - tile * tile_rows);
-  const int64_t stride = a.D + 2;
-  for (int i = threadIdx.x; i < rows * pairs; i += 256) {
-    const int r = i / pairs, d = 2 * (i - r * pairs);
-    float m = kNone;
-    for (int w = from; w <= to; ++w) m = fmaxf(m, a.part[((2 * (int64_t)w + (w == from ? 1 : 0)) * tile_rows + r) * stride]);
-    float l = 0.0f, x0 = 0.0f, x1 = 0.0f;
+  const int64_t stride = a.D + 4, part = (int64_t)tile_rows * stride;
+  const float* const parts = a.part + 2 * part * from + part;       // the first part; the next ones are from the others' first slots
+  for (int i = (blockIdx.x % groups) * 256 + threadIdx.x; i < rows * pieces; i += 256 * groups) {
+    const int r = i / pieces, d = 4 * (i - r * pieces);
+    float m = kNone, l = 0.0f;
+    f32x4 x = {0, 0, 0, 0};
+    const float* at_part = parts + r * stride;
     for (int w = from; w <= to; ++w) {
-      const float* o = a.part + ((2 * (int64_t)w + (w == from ? 1 : 0)) * tile_rows + r) * stride;
-      const float by = __builtin_amdgcn_exp2f(o[0] - m);
-      l += o[1] * by;
-      x0 += o[2 + d] * by;
-      x1 += o[3 + d] * by;
+      const float pm = at_part[0], pl = at_part[1];
+      const f32x4 y = *reinterpret_cast<const f32x4*>(at_part + 4 + d);
+      const float top = fmaxf(m, pm);
+      const float mine = __builtin_amdgcn_exp2f(m - top), its = __builtin_amdgcn_exp2f(pm - top);
+      l = l * mine + pl * its;
+      x = x * mine + y * its;
+      m = top;
+      at_part += w == from ? part : 2 * part;
     }
     const int row = tile * tile_rows + r;
-    const int t = (int)a.G.of((uint32_t)row), gq = row - t * (int)a.G.d;
-    const bool drafted = !a.tree_lengths || t < a.tree_lengths[b];
-    const bool none = !drafted || l == 0.0f;
-    const float inverse = none ? 0.0f : 1.0f / l;
-    const int64_t at = (((int64_t)b * a.H + h) * a.G.d + gq) * a.T + t;
-    x0 = none ? 0.0f : x0 * inverse, x1 = none ? 0.0f : x1 * inverse;
-    *reinterpret_cast<uint32_t*>(a.out + (at * a.D + d) * 2) = a.bf16 ? pack2<FCR_DTYPE_BF16>(x0, x1) : pack2<FCR_DTYPE_F16>(x0, x1);
+    const int t = (int)a.G.of((uint32_t)row), head = row - t * (int)a.G.d;
+    const bool none = (a.tree_lengths && t >= a.tree_lengths[b]) || l == 0.0f;
+    const float inverse = 1.0f / l;
+    const int64_t at = (((int64_t)b * a.H + h) * a.G.d + head) * a.T + t;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = none ? 0.0f : x[j] * inverse;
+    *reinterpret_cast<u32x2*>(a.out + (at * a.D + d) * 2) = a.bf16 ? u32x2{pack2<FCR_DTYPE_BF16>(x[0], x[1]), pack2<FCR_DTYPE_BF16>(x[2], x[3])}
+                                                                  : u32x2{pack2<FCR_DTYPE_F16>(x[0], x[1]), pack2<FCR_DTYPE_F16>(x[2], x[3])};
     if (a.lse && d == 0) a.lse[at] = none ? -INFINITY : m + __builtin_amdgcn_logf(l);
   }
 }
 #endif
 
 template <int CD, int W>
-void launch_w(const Args& a, int rt, hipStream_t s) {
+void launch_w(const Args& a, int form, hipStream_t s) {
   const dim3 grid((unsigned)a.wgs);
-  switch (rt) {
-    case 1: hipLaunchKernelGGL((tree_attention_kernel<CD, W, 1>), grid, dim3(kThreads), 0, s, a); break;
-    default: hipLaunchKernelGGL((tree_attention_kernel<CD, W, 2>), grid, dim3(kThreads), 0, s, a); break;
+  switch (form) {
+    case 1: hipLaunchKernelGGL((tree_attention_kernel<CD, W, 1>), grid, dim3(256), 0, s, a); break;
+    case 2:
+      if constexpr (W <= 2) hipLaunchKernelGGL((tree_attention_kernel<CD, W, 2>), grid, dim3(256), 0, s, a);
+      break;
+    case 4: hipLaunchKernelGGL((tall_attention_kernel<CD, W, 4>), grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL((tall_attention_kernel<CD, W, 8>), grid, dim3(512), 0, s, a); break;
   }
 }
 template <int CD>
-void launch(const Args& a, int w, int rt, hipStream_t s) {
+void launch(const Args& a, int w, int form, hipStream_t s) {
   switch (w) {
-    case 1: launch_w<CD, 1>(a, rt, s); break;
-    case 2: launch_w<CD, 2>(a, rt, s); break;
-    case 3: launch_w<CD, 3>(a, rt, s); break;
-    default: launch_w<CD, 4>(a, rt, s); break;
+    case 1: launch_w<CD, 1>(a, form, s); break;
+    case 2: launch_w<CD, 2>(a, form, s); break;
+    case 3: launch_w<CD, 3>(a, form, s); break;
+    default: launch_w<CD, 4>(a, form, s); break;
   }
 }
 }  // namespace
 
 #if FCR_HAS(1)
-void fcr_tree::attention_f16(const Args& a, int w, int rt, hipStream_t s) { launch<FCR_DTYPE_F16>(a, w, rt, s); }
+void fcr_tree::attention_f16(const Args& a, int w, int form, hipStream_t s) { launch<FCR_DTYPE_F16>(a, w, form, s); }
 #endif
 #if FCR_HAS(2)
-void fcr_tree::attention_bf16(const Args& a, int w, int rt, hipStream_t s) { launch<FCR_DTYPE_BF16>(a, w, rt, s); }
+void fcr_tree::attention_bf16(const Args& a, int w, int form, hipStream_t s) { launch<FCR_DTYPE_BF16>(a, w, form, s); }
 #endif
 #if FCR_HAS(3)
-void fcr_tree::attention_int8(const Args& a, int w, int rt, hipStream_t s) { launch<FCR_DTYPE_INT8>(a, w, rt, s); }
+void fcr_tree::attention_int8(const Args& a, int w, int form, hipStream_t s) { launch<FCR_DTYPE_INT8>(a, w, form, s); }
 #endif
 #if FCR_HAS(4)
-void fcr_tree::attention_e4m3(const Args& a, int w, int rt, hipStream_t s) { launch<FCR_DTYPE_E4M3>(a, w, rt, s); }
+void fcr_tree::attention_e4m3(const Args& a, int w, int form, hipStream_t s) { launch<FCR_DTYPE_E4M3>(a, w, form, s); }
 #endif
 
 #if FCR_HAS(0)
@@ -780,24 +930,27 @@ using fcr_detail::fail;
 using fcr_detail::launched;
 
 struct Plan {
-  int rt, row_tiles, wgs, least;
+  int form;                  // 1, 2: tree_attention_kernel of as many column tiles; 4, 8: tall_attention_kernel of as many waves
+  int tile_rows, row_tiles, wgs, least;
   int64_t items, first_bytes, bytes;
 };
 // What depends on sizes alone.  false: too large.
 bool plan_of(int B, int H, int G, int T, int D, int64_t capacity, Plan& p) {
   const int64_t rows = (int64_t)T * G;
-  p.rt = rows <= 16 ? 1 : 2;
-  const int64_t tiles = (rows + 16 * p.rt - 1) / (16 * p.rt);
+  const int w = (D + 63) / 64, tall = 16 * tall_tiles(w);
+  p.form = rows <= 16 ? 1 : rows <= 32 && w <= 2 ? 2 : rows <= 4 * tall ? 4 : 8;
+  p.tile_rows = p.form <= 2 ? 16 * p.form : tall * p.form;
+  const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.items = (int64_t)B * H * tiles;
   const int64_t blocks = p.items * ((capacity + kBlock - 1) / kBlock);
   if (rows > (1 << 24) || p.items > (1 << 24) || blocks > (1 << 30)) return false;
   p.row_tiles = (int)tiles;
-  int64_t wgs = 2 * (int64_t)fcr_detail::chip_cus_of_current_device();
+  int64_t wgs = (p.form == 8 ? 1 : 2) * (int64_t)fcr_detail::chip_cus_of_current_device();
   if (blocks < wgs) wgs = blocks;
   p.wgs = (int)((wgs + 7) / 8 * 8);
   p.least = 1;
   p.first_bytes = (p.items * 4 + 15) / 16 * 16;
-  p.bytes = p.first_bytes + 2ll * p.wgs * 16 * p.rt * (D + 2) * 4;
+  p.bytes = p.first_bytes + 2ll * p.wgs * p.tile_rows * (D + 4) * 4;
   return true;
 }
 }  // namespace
@@ -853,13 +1006,15 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
   const int w = (D + 63) / 64;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (cache->dtype) {
-    case FCR_DTYPE_F16: attention_f16(a, w, plan.rt, s); break;
-    case FCR_DTYPE_BF16: attention_bf16(a, w, plan.rt, s); break;
-    case FCR_DTYPE_INT8: attention_int8(a, w, plan.rt, s); break;
-    default: attention_e4m3(a, w, plan.rt, s); break;
+    case FCR_DTYPE_F16: attention_f16(a, w, plan.form, s); break;
+    case FCR_DTYPE_BF16: attention_bf16(a, w, plan.form, s); break;
+    case FCR_DTYPE_INT8: attention_int8(a, w, plan.form, s); break;
+    default: attention_e4m3(a, w, plan.form, s); break;
   }
   if ((rc = launched("tree_attention_kernel"))) return rc;
-  hipLaunchKernelGGL(tree_join_kernel, dim3((unsigned)plan.items), dim3(256), 0, s, a, 16 * plan.rt);
+  const int pieces = (plan.tile_rows < a.rows ? plan.tile_rows : a.rows) * (D / 4);
+  const int groups = (pieces + 255) / 256;
+  hipLaunchKernelGGL(tree_join_kernel, dim3((unsigned)(plan.items * groups)), dim3(256), 0, s, a, plan.tile_rows, groups);
   return launched("tree_join_kernel");
 }
 
