@@ -67,6 +67,15 @@ using namespace fcr_tree;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+// The kernel's arguments, read again where they are used: kept for the whole kernel they would not fit the scalar registers, and their
+// spills take vector registers and instructions of the inner loops.  (Args is the only parameter of the kernels that call this.)
+__device__ __forceinline__ const Args& arguments() {
+  typedef const __attribute__((address_space(4))) Args* Pointer;
+  Pointer p = (Pointer)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Args*)p;
+}
+
 constexpr int kBlock = 128;                  // keys of a block
 constexpr float kNone = -3.0e38f;            // reference of a row that has seen no key
 constexpr float kMostWeight = 0x1p15f;       // weights above this raise the reference, to where the largest is in (1/2, 1]
@@ -125,48 +134,59 @@ __device__ __forceinline__ Place place_of(const Args& a, int b, int pos, int n) 
   Place p{-1, 0};
   if (pos < n) {
     uint32_t row;
-    p.page = page_of(a.c, b, (uint32_t)pos, row);
+    p.page = __builtin_amdgcn_readfirstlane(page_of(a.c, b, (uint32_t)pos, row));
     p.row = (int)row;
   }
   return p;
 }
 
-// The lane's places in rows of keys (lane & 15; 16-byte pieces, of which a row's last one stands for those behind it) and of values (rows
-// 4 g + i, elements from `first` on, where behind the row's end there are elements that another lane has as well).
+// The lane's places in a 16-key tile: of keys (row lane & 15; 16-byte pieces, of which a row's last one stands for those behind it) and of
+// values (rows 4 g + i, elements from elements_of(col) on, where behind the row's end there are elements that another lane has as well).
 template <class F>
 struct Lane {
-  int lane, g, col, first;
-  uint32_t key, piece[F::KL], value;
-  __device__ __forceinline__ Lane(const Args& a, int lane_) {
-    constexpr int e = F::codes ? 1 : 2;
-    lane = lane_, g = lane >> 4, col = lane & 15;
-    first = elements_of(a, col);
-    key = (uint32_t)(col * a.c.side[0].row);
-#pragma unroll
-    for (int i = 0; i < F::KL; ++i) piece[i] = min(64u * i + 16u * g, (uint32_t)(a.D * e) - 16u);
-    value = (uint32_t)(4 * g * a.c.side[1].row) + (uint32_t)(first * e);
+  static constexpr uint32_t kBytes = F::codes ? 1 : 2;
+  int lane, g, col;
+  __device__ __forceinline__ Lane(int lane_) : lane(lane_), g(lane_ >> 4), col(lane_ & 15) {}
+  __device__ __forceinline__ Lane again() const {        // (what is derived from it is formed again, not kept in registers)
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    return Lane(l);
+  }
+  __device__ __forceinline__ uint32_t key(const Args& a) const { return (uint32_t)(col * (int)a.c.side[0].row); }
+  __device__ __forceinline__ uint32_t piece(const Args& a, int i) const { return min(64u * i + 16u * g, (uint32_t)a.D * kBytes - 16u); }
+  __device__ __forceinline__ uint32_t value(const Args& a) const {
+    return (uint32_t)(4 * g * (int)a.c.side[1].row) + (uint32_t)elements_of(a, col) * kBytes;
   }
   __device__ __forceinline__ static int elements_of(const Args& a, int col) { return min(col * F::DT, a.D - F::DT); }
 };
 
+// A tile's rows, or its scales, as a view that reads as zeros where its page is not there: the loads need no branch.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const Side& s, int h, const Place& p) {
+  return __builtin_amdgcn_make_buffer_rsrc(s.rows + p.page * s.page + h * s.head + p.row * s.row, 0, p.page >= 0 ? (int)(16 * s.row) : 0, 0x00020000);
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t scales_of(const Side& s, int h, const Place& p) {
+  return __builtin_amdgcn_make_buffer_rsrc(s.scale + p.page * s.s_page + h * s.s_head + p.row, 0, p.page >= 0 ? 64 : 0, 0x00020000);
+}
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t v, uint32_t at) { return __builtin_amdgcn_raw_buffer_load_b128(v, (int)at, 0, 0); }
+
 template <int N>
-__device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[N]) {
+__device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t v, uint32_t at, int row, uint32_t (&w)[N]) {
   // (a lane's part of a row is 4 N bytes: aligned to 16 where N is a multiple of 4, to 8 where it is even)
   if constexpr (N % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const u32x4 v = reinterpret_cast<const u32x4*>(at)[i];
-      w[4 * i] = v[0], w[4 * i + 1] = v[1], w[4 * i + 2] = v[2], w[4 * i + 3] = v[3];
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(v, (int)at + 16 * i, row, 0);
+      w[4 * i] = x[0], w[4 * i + 1] = x[1], w[4 * i + 2] = x[2], w[4 * i + 3] = x[3];
     }
   } else if constexpr (N % 2 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-      const u32x2 v = reinterpret_cast<const u32x2*>(at)[i];
-      w[2 * i] = v[0], w[2 * i + 1] = v[1];
+      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(v, (int)at + 8 * i, row, 0);
+      w[2 * i] = x[0], w[2 * i + 1] = x[1];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(at)[i];
+    for (int i = 0; i < N; ++i) w[i] = __builtin_amdgcn_raw_buffer_load_b32(v, (int)at + 4 * i, row, 0);
   }
 }
 
@@ -176,17 +196,10 @@ struct Keys {
   u32x4 w[F::KL];
   f32x4 scale;
   __device__ __forceinline__ void load(const Args& a, int h, const Place& p, const Lane<F>& at) {
-    if (p.page >= 0) {
-      const Side& s = a.c.side[0];
-      const char* base = s.rows + p.page * s.page + h * s.head + p.row * s.row;
+    const __amdgpu_buffer_rsrc_t rows = rows_of(a.c.side[0], h, p);
 #pragma unroll
-      for (int i = 0; i < F::KL; ++i) w[i] = *reinterpret_cast<const u32x4*>(base + (at.key + at.piece[i]));
-      if constexpr (F::codes) scale = *reinterpret_cast<const f32x4*>(s.scale + p.page * s.s_page + h * s.s_head + p.row + 4 * at.g);
-    } else {
-#pragma unroll
-      for (int i = 0; i < F::KL; ++i) w[i] = u32x4{0, 0, 0, 0};
-      scale = f32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < F::KL; ++i) w[i] = load16(rows, at.key(a) + at.piece(a, i));
+    if constexpr (F::codes) scale = __builtin_bit_cast(f32x4, load16(scales_of(a.c.side[0], h, p), 16 * at.g));
   }
   // k-steps 2 i and 2 i + 1 (codes) or i (16-bit) of load i
   __device__ __forceinline__ u32x4 operand(int ks) const {
@@ -219,19 +232,10 @@ struct Values {
   uint32_t w[4][F::VW];
   f32x4 scale;
   __device__ __forceinline__ void load(const Args& a, int h, const Place& p, const Lane<F>& at) {
-    if (p.page >= 0) {
-      const Side& s = a.c.side[1];
-      const char* base = s.rows + p.page * s.page + h * s.head + p.row * s.row;
+    const __amdgpu_buffer_rsrc_t rows = rows_of(a.c.side[1], h, p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) load_words(base + (at.value + (uint32_t)(i * s.row)), w[i]);
-      if constexpr (F::codes) scale = *reinterpret_cast<const f32x4*>(s.scale + p.page * s.s_page + h * s.s_head + p.row + 4 * at.g);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < F::VW; ++j) w[i][j] = 0;
-      scale = f32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < 4; ++i) load_words(rows, at.value(a), i * (int)a.c.side[1].row, w[i]);
+    if constexpr (F::codes) scale = __builtin_bit_cast(f32x4, load16(scales_of(a.c.side[1], h, p), 16 * at.g));
   }
   // Keys that are not there: bits of `there` from bit 0 on.  What their rows hold is not looked at.
   __device__ __forceinline__ void drop(uint32_t there) {
@@ -294,79 +298,89 @@ struct State {
   }
 };
 
-// The weights of 32 keys from their products with the queries: 2^(k_scale s - m) v_scale.  `masked`: seen[r] holds the keys that a row
+// The weights of 32 keys from their products with the queries: 2^(k_scale s - m) v_scale.  MASKED: seen[r] holds the keys that a row
 // sees, bit 4 t + i; else every key is seen.  Bound by the vector unit: per score an fma, an exponential (four slots), the sum, the product
-// with the value's scale, a maximum and half a conversion.  The reference is raised, for the rows that ask for it, where a weight would
-// not fit fp16 or a sum fp32, which a few of the first steps do and hardly any later one: the largest weight may be 2^15 times what the
-// reference was raised for, and nothing needs it to be followed more closely.
-template <class F, int RT>
-__device__ __forceinline__ void weights(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], const f32x4 (&s)[RT][2], bool masked,
-                                        const uint32_t (&seen)[RT], State<F, RT>& st, u32x4 (&p)[RT]) {
+// with the value's scale, half a maximum and half a conversion.  Returns whether some row's reference has to be raised, where a weight would
+// not fit fp16 or a sum fp32.  A few of the first steps ask for it and hardly any later one: the
+// largest weight may be 2^15 times what the reference was raised for, and nothing needs it to be followed more closely.
+template <bool MASKED, class F, int RT>
+__device__ __forceinline__ bool weights(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], const f32x4 (&s)[RT][2], const uint32_t (&seen)[RT],
+                                        const State<F, RT>& st, float (&sum)[RT], u32x4 (&p)[RT]) {
+  bool raise = false;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    float x[8], sum = 0.0f, most = 0.0f;
+    float x[8], most = 0.0f, part[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(s[r][e / 4][e % 4], k_scale[e / 4][e % 4], -st.m[r]);
-    if (masked) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (seen[r] >> e) & 1u ? x[e] : -INFINITY;
+    for (int e = 0; e < 8; ++e) {
+      x[e] = __builtin_fmaf(s[r][e / 4][e % 4], k_scale[e / 4][e % 4], -st.m[r]);
+      if (MASKED) x[e] = (seen[r] >> e) & 1u ? x[e] : -INFINITY;
+      x[e] = __builtin_amdgcn_exp2f(x[e]);
+      part[e & 1] += x[e];
+      if constexpr (F::codes) {
+        x[e] *= v_scale[e / 4][e % 4];
+        if (MASKED) x[e] = (seen[r] >> e) & 1u ? x[e] : 0.0f;      // (a hidden value's scale may be a NaN)
+      }
+      most = fmaxf(most, fabsf(x[e]));
     }
-    const auto weigh = [&] {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = __builtin_amdgcn_exp2f(x[e]);
-        sum += x[e];
-        if constexpr (F::codes) x[e] *= v_scale[e / 4][e % 4];
-      }
-      if (F::codes && masked) {   // (a hidden value's scale may be a NaN)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (seen[r] >> e) & 1u ? x[e] : 0.0f;
-      }
-    };
-    weigh();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
-    if (__any(most > kMostWeight || !(st.l[r] + sum < kMostSum))) {
-      float of_weights = -INFINITY, of_sum = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = s[r][e / 4][e % 4] * k_scale[e / 4][e % 4];
-        if (masked) x[e] = (seen[r] >> e) & 1u ? x[e] : -INFINITY;
-        of_sum = fmaxf(of_sum, x[e]);
-        of_weights = fmaxf(of_weights, F::codes ? x[e] + __builtin_amdgcn_logf(fabsf(v_scale[e / 4][e % 4])) : x[e]);
-      }
-      const float top = across(fmaxf(of_weights, of_sum - 100.0f), true);
-      const float m = top > st.m[r] ? ceilf(top) : st.m[r];
-      const float shrink = __builtin_amdgcn_exp2f(st.m[r] - m);
-      st.m[r] = m;
-      st.l[r] *= shrink;
-#pragma unroll
-      for (int d = 0; d < F::DT; ++d) st.o[r][d] *= shrink;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] -= m;
-      sum = 0.0f;
-      weigh();
-    }
-    st.l[r] += sum;
+    sum[r] = st.l[r] + (part[0] + part[1]);
+    raise = raise || most > kMostWeight || !(sum[r] < kMostSum);
 #pragma unroll
     for (int j = 0; j < 4; ++j) p[r][j] = F::bf16 ? pack2<FCR_DTYPE_BF16>(x[2 * j], x[2 * j + 1]) : pack2<FCR_DTYPE_F16>(x[2 * j], x[2 * j + 1]);
   }
+  return __any(raise);
 }
 
-// O^T += V^T P^T of 32 keys, `operand(d)` giving V^T's part.  Where a value that is not finite stands at a key that some rows do not see
-// (one_by_one), 0 * inf would reach them: then one key at a time, and only rows that see it take the result.
-template <class F, int RT, class Operand>
-__device__ __forceinline__ void add_values(const Operand& operand, const u32x4 (&p)[RT], bool one_by_one, const uint32_t (&seen)[RT], const Lane<F>& at,
-                                           State<F, RT>& st) {
-  if (F::codes || !one_by_one) {
+// Raises references so that the largest weight of these keys is in (1/2, 1].
+template <class F, int RT>
+__device__ __forceinline__ void raise(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], const f32x4 (&s)[RT][2], const uint32_t (&seen)[RT],
+                                      State<F, RT>& st) {
 #pragma unroll
-    for (int d = 0; d < F::DT; ++d) {
-      const u32x4 f = operand(d);
+  for (int r = 0; r < RT; ++r) {
+    float of_weights = -INFINITY, of_sum = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(f, p[r], st.o[r][d]);
+    for (int e = 0; e < 8; ++e) {
+      float x = s[r][e / 4][e % 4] * k_scale[e / 4][e % 4];
+      x = (seen[r] >> e) & 1u ? x : -INFINITY;
+      of_sum = fmaxf(of_sum, x);
+      of_weights = fmaxf(of_weights, F::codes ? x + __builtin_amdgcn_logf(fabsf(v_scale[e / 4][e % 4])) : x);
     }
-    return;
+    const float top = across(fmaxf(of_weights, of_sum - 100.0f), true);
+    const float m = top > st.m[r] ? ceilf(top) : st.m[r];
+    const float shrink = __builtin_amdgcn_exp2f(st.m[r] - m);
+    st.m[r] = m;
+    st.l[r] *= shrink;
+#pragma unroll
+    for (int d = 0; d < F::DT; ++d) st.o[r][d] *= shrink;
   }
+}
+
+template <class F, int RT>
+__device__ __forceinline__ void weigh(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], const f32x4 (&s)[RT][2], bool masked,
+                                      const uint32_t (&seen)[RT], State<F, RT>& st, u32x4 (&p)[RT]) {
+  float sum[RT];
+  const bool up = masked ? weights<true, F, RT>(k_scale, v_scale, s, seen, st, sum, p) : weights<false, F, RT>(k_scale, v_scale, s, seen, st, sum, p);
+  if (__builtin_expect(up, 0)) {
+    raise<F, RT>(k_scale, v_scale, s, seen, st);
+    weights<true, F, RT>(k_scale, v_scale, s, seen, st, sum, p);
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r) st.l[r] = sum[r];
+}
+
+// O^T += V^T P^T of 32 keys, for the lane's elements [D0, D1).
+template <class F, int RT, int D0, int D1>
+__device__ __forceinline__ void add_values(const u32x4 (&v)[F::DT], const u32x4 (&p)[RT], State<F, RT>& st) {
+#pragma unroll
+  for (int d = D0; d < D1; ++d)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(v[d], p[r], st.o[r][d]);
+}
+// The same where a value that is not finite stands at a key that some rows do not see: 0 * inf would reach them.  One key at a time, and
+// only rows that see it take the result.
+template <class F, int RT>
+__device__ __forceinline__ void add_values_one_by_one(const u32x4 (&v)[F::DT], const u32x4 (&p)[RT], const uint32_t (&seen)[RT], const Lane<F>& at,
+                                                      State<F, RT>& st) {
+#pragma unroll 1
   for (int key = 0; key < 32; ++key) {
     const int e = key & 7, g = key >> 3;
     u32x4 only;
@@ -377,10 +391,9 @@ __device__ __forceinline__ void add_values(const Operand& operand, const u32x4 (
     for (int r = 0; r < RT; ++r) see[r] = (__shfl((int)seen[r], 16 * g + at.col) >> e) & 1;
 #pragma unroll
     for (int d = 0; d < F::DT; ++d) {
-      const u32x4 f = operand(d) & only;
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        const f32x4 with = mma<F::bf16>(f, p[r] & only, st.o[r][d]);
+        const f32x4 with = mma<F::bf16>(v[d] & only, p[r] & only, st.o[r][d]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) st.o[r][d][i] = see[r] ? with[i] : st.o[r][d][i];
       }
@@ -393,7 +406,6 @@ __device__ __forceinline__ void add_values(const Operand& operand, const u32x4 (
 template <class F, int RT>
 struct Queries {
   u32x4 w[RT][F::KS];
-  int token[RT];
   // Returns the largest element's bits where they are to be scaled.
   __device__ __forceinline__ uint32_t load(const Args& a, int b, int h, int row0, const Lane<F>& at) {
     uint32_t most = 0;
@@ -402,7 +414,6 @@ struct Queries {
       const int row = row0 + 16 * r + at.col;
       const bool live = row < a.rows;
       const uint32_t t = a.G.of((uint32_t)(live ? row : 0)), head = (uint32_t)(live ? row : 0) - t * a.G.d;
-      token[r] = (int)t;
       const char* from = a.q + b * a.qb + (int64_t)(h * (int)a.G.d + (int)head) * a.qh + t * a.qt;
 #pragma unroll
       for (int s = 0; s < F::KS; ++s) {
@@ -441,16 +452,19 @@ __device__ __forceinline__ uint32_t largest_of_wave(uint32_t x) {
 }
 
 // Which of the lane's keys from position `pos` on (a 32-key step: bits 4 t + i) the query of token t sees.
-__device__ __forceinline__ uint32_t seen_by(const Args& a, int b, int token, int pos, int context, uint32_t there, int g) {
+// (row: the query's; rows that are none are given token 0)
+__device__ __forceinline__ uint32_t seen_by(const Args& a, int b, int row, int pos, int context, uint32_t there, int g) {
+  const int token = row < a.rows ? (int)a.G.of((uint32_t)row) : 0;
+  const uint8_t* const mask = a.mask ? a.mask + b * a.mask_b + (int64_t)token * a.T : nullptr;
   uint32_t seen = 0;
-#pragma unroll
+#pragma unroll 1
   for (int e = 0; e < 8; ++e) {
-    const int u = pos + 16 * (e / 4) + 4 * g + e % 4 - context;   // which drafted token
-    bool is = (there >> e) & 1u;
-    if (is && u >= 0) is = a.mask ? a.mask[b * a.mask_b + (int64_t)token * a.T + u] != 0 : u <= token;
+    const int u = pos + 16 * (e / 4) + 4 * g + e % 4 - context;   // which drafted token; below 0: of the context
+    bool is = u <= token;
+    if (mask) is = u < 0 || mask[min(max(u, 0), a.T - 1)] != 0;
     seen |= is ? 1u << e : 0u;
   }
-  return seen;
+  return seen & there;
 }
 // Which of the lane's keys are there: in front of n, on a page that is.  Bits 4 t + i.
 __device__ __forceinline__ uint32_t there_of(int pos, int n, bool page0, bool page1, int g) {
@@ -462,10 +476,11 @@ __device__ __forceinline__ uint32_t there_of(int pos, int n, bool page0, bool pa
 
 // DT consecutive elements of a row: its result, or its part of one.
 template <class F>
-__device__ __forceinline__ void emit(const Args& a, bool final, float* slot, int b, int h, int row, int row_in_tile, int token, int d0, bool first,
+__device__ __forceinline__ void emit(const Args& a, bool final, float* slot, int b, int h, int row, int row_in_tile, int d0, bool first,
                                      const float (&x)[F::DT], float m, float l) {
   if (row >= a.rows) return;
   if (final) {
+    const int token = (int)a.G.of((uint32_t)row);
     const bool none = (a.tree_lengths && token >= a.tree_lengths[b]) || l == 0.0f;
     const float inverse = 1.0f / l;
     const int64_t to = ((int64_t)b * a.H * a.G.d + (int64_t)h * a.G.d + (row - token * (int)a.G.d)) * a.T + token;
@@ -581,18 +596,19 @@ struct Deal {
 __device__ __forceinline__ int range_of(const Args& a, int block) { return (block & 7) * (a.wgs >> 3) + (block >> 3); }
 
 template <int CD, int W, int RT>
-__global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kernel(Args a) {
+__global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kernel(Args args) {
   using F = Form<CD, W>;
   constexpr int kWaves = 4;
   __shared__ float joined[kWaves * 4 * F::DT * 64];     // [wave][register][tile][lane]
   __shared__ float stats[kWaves][RT][16][2];            // m, l
   __shared__ int scan[kWaves + 2];
-  const int wg = range_of(a, blockIdx.x);
+  const int wg = range_of(args, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const Lane<F> at(a, threadIdx.x & 63);
+  const Lane<F> at(threadIdx.x & 63);
   Deal<256> deal;
-  if (!deal.start(a, wg, scan)) return;
+  if (!deal.start(arguments(), wg, scan)) return;
   do {
+    const Args& a = arguments();
     const int b = deal.b, h = deal.h, n = deal.n, context = deal.context, stop = deal.stop();
     const int row0 = deal.tile * 16 * RT;
     Queries<F, RT> q;
@@ -635,7 +651,9 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
         for (int t = 0; t < 2; ++t) k[t].load(a, h, next[t], at);
       }
       u32x4 p[RT];
-      uint32_t seen[RT] = {};
+      uint32_t seen[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) seen[r] = 0xff;
       const bool masked = pos + 32 > min(context, n) || here[0].page < 0 || here[1].page < 0;
       bool one_by_one = false;
       if (masked) {
@@ -644,11 +662,23 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
         v[1].drop(there >> 4);
         if constexpr (!F::codes) one_by_one = pos + 32 > context && __any(v[0].not_finite() || v[1].not_finite());
 #pragma unroll
-        for (int r = 0; r < RT; ++r) seen[r] = seen_by(a, b, q.token[r], pos, context, there, at.g);
+        for (int r = 0; r < RT; ++r) seen[r] = seen_by(a, b, row0 + 16 * r + at.col, pos, context, there, at.g);
       }
       const f32x4 v_scale[2] = {v[0].scale, v[1].scale};
-      weights<F, RT>(k_scale, v_scale, s, masked, seen, st, p);
-      add_values<F, RT>([&](int d) { return joined_operand(v[0].operand(d), v[1].operand(d)); }, p, one_by_one, seen, at, st);
+      weigh<F, RT>(k_scale, v_scale, s, masked, seen, st, p);
+      if (__builtin_expect(!F::codes && one_by_one, 0)) {
+        u32x4 f[F::DT];
+#pragma unroll
+        for (int d = 0; d < F::DT; ++d) f[d] = joined_operand(v[0].operand(d), v[1].operand(d));
+        add_values_one_by_one<F, RT>(f, p, seen, at, st);
+      } else {
+#pragma unroll
+        for (int d = 0; d < F::DT; ++d) {
+          const u32x4 f = joined_operand(v[0].operand(d), v[1].operand(d));
+#pragma unroll
+          for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(f, p[r], st.o[r][d]);
+        }
+      }
       if (i + 1 < stop) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) v[t].load(a, h, next[t], at);
@@ -657,9 +687,10 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
     }
 
     // join the four waves
+    const Args& a_end = arguments();
     const bool final = deal.blk == 0 && stop == deal.nb;
-    float* const slot = a.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * (16 * RT) * (a.D + 4);
-    if (deal.blk == 0 && threadIdx.x == 0) a.first[deal.item(a)] = deal.at;
+    float* const slot = a_end.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * (16 * RT) * (a_end.D + 4);
+    if (deal.blk == 0 && threadIdx.x == 0) a_end.first[deal.item(a_end)] = deal.at;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -688,44 +719,57 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) x[d] += joined[((w * 4 + wave) * F::DT + d) * 64 + at.lane];
       }
-      emit<F>(a, final, slot, b, h, row0 + 16 * r + at.col, 16 * r + at.col, q.token[r], Lane<F>::elements_of(a, 4 * at.g + wave),
+      emit<F>(a_end, final, slot, b, h, row0 + 16 * r + at.col, 16 * r + at.col, Lane<F>::elements_of(a_end, 4 * at.g + wave),
               wave == 0 && at.g == 0, x, m, l);
       __syncthreads();
     }
-  } while (deal.next(a));
+  } while (deal.next(arguments()));
 }
 
 // Column tiles per wave: two, where their sums and queries leave room in 256 registers.
 constexpr int tall_tiles(int w) { return w <= 2 ? 2 : 1; }
+// Keys of a stage: two stages in LDS, of one workgroup of eight waves, or of two of four.
+constexpr int tall_keys(int w, int waves) { return w == 1 || (w == 2 && waves == 8) ? 128 : 64; }
 
-// A stage holds a block's operands: of every 16-key tile the KS key operands, of every 32 keys the DT value operands,
-// 16 bytes per lane, and the scales.  A wave converts 128 / WAVES keys of it.
+// A stage holds the operands of its keys: of every 16-key tile the KS key operands, of every 32 keys the DT value operands, 16 bytes per
+// lane, and the scales.  The waves share its conversion.  While one stage is used the next one is written.
+// A SIMD has two waves.  While one forms weights (vector unit) the other one multiplies, values with weights and the next keys with the
+// queries (matrix unit, at a higher priority: where both ask for it the one that multiplies goes on, and they part).  The later half of the
+// waves converts later in the stage, for the same reason.
+// One barrier per stage, before the products of its last step, which read the first keys of the next stage: that has been written by then, and
+// the stage before, whose place it takes, was last read before the last such barrier.
 template <int CD, int W, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, WAVES == 4 && W >= 3 ? 1 : 2) tall_attention_kernel(Args a) {
+__global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args) {
   using F = Form<CD, W>;
-  constexpr int RT = tall_tiles(W), kTiles = 8 / WAVES;  // 16-key tiles that a wave converts
-  __shared__ __attribute__((aligned(16))) char lds[(8 * F::KS + 4 * F::DT) * 64 * 16 + 2 * kBlock * 4 + (8 + WAVES + 2) * 4];
-  u32x4* const ks = reinterpret_cast<u32x4*>(lds);                       // [8][KS][64]
-  u32x4* const vs = ks + 8 * F::KS * 64;                                 // [4][DT][64]
-  float* const k_scales = reinterpret_cast<float*>(vs + 4 * F::DT * 64); // [128]
-  float* const v_scales = k_scales + kBlock;                             // [128]
-  int* const flags = reinterpret_cast<int*>(v_scales + kBlock);          // [8]: a tile's page is there, and (bit 1) a value is not finite
-  int* const scan = flags + 8;                                           // [WAVES + 2]
-  const int wg = range_of(a, blockIdx.x);
+  constexpr int RT = tall_tiles(W), kKeys = tall_keys(W, WAVES), kSteps = kKeys / 32, kTiles = kKeys / 16;
+  constexpr int kMine = kTiles > WAVES ? kTiles / WAVES : 1;             // 16-key tiles that a wave converts
+  constexpr bool kApart = kTiles < WAVES;                                // a wave converts a tile's keys or its values
+  constexpr int kValues = kTiles * F::KS * 64;                           // where the values begin, in 16 bytes
+  constexpr int kStage = kValues + kSteps * F::DT * 64;
+  static_assert(kTiles * (kApart ? 2 : 1) == WAVES * kMine, "every wave has its share of a stage");
+  __shared__ u32x4 operands[2 * kStage];
+  __shared__ __attribute__((aligned(16))) float scales[2][2][kKeys];     // of keys, of values
+  __shared__ int flags[2][kTiles];                                       // a tile's page is there, and (bit 1) a value is not finite
+  __shared__ int scan[WAVES + 2];
+  const int wg = range_of(args, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const Lane<F> at(a, threadIdx.x & 63);
+  const Lane<F> at(threadIdx.x & 63);
+  const int my_tile = kApart ? wave % kTiles : wave * kMine;
+  const bool my_keys = !kApart || wave < kTiles, my_values = !kApart || wave >= kTiles;
   Deal<64 * WAVES> deal;
-  if (!deal.start(a, wg, scan)) return;
+  if (!deal.start(arguments(), wg, scan)) return;
   do {
     const int b = deal.b, h = deal.h, n = deal.n, context = deal.context, stop = deal.stop();
     const int row0 = (deal.tile * WAVES + wave) * 16 * RT;
+    const bool idle = row0 >= arguments().rows;                                    // (it converts all the same)
+    const bool late = WAVES == 8 && wave >= 4;
     Queries<F, RT> q;
-    float by = a.scale2;
-    uint32_t most = q.load(a, b, h, row0, at);
-    if (F::codes && a.bf16) {
+    float by = arguments().scale2;
+    uint32_t most = q.load(arguments(), b, h, row0, at);
+    __syncthreads();                                                     // (the piece before has been used)
+    if (F::codes && arguments().bf16) {
       // one power of two for all rows of the workgroup, which the keys' scales undo
       most = largest_of_wave(most);
-      __syncthreads();
       if (at.lane == 0) scan[wave] = (int)most;
       __syncthreads();
 #pragma unroll
@@ -734,84 +778,147 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 4 && W >= 3 ? 1 : 2) tall
     }
     State<F, RT> st;
     st.clear();
-    Keys<F> k[kTiles];
-    Values<F> v[kTiles];
-    Place place[kTiles];
-    const auto fetch = [&](int i) {
+    Keys<F> k[kMine];
+    Values<F> v[kMine];
+    Place place[kMine];
+    const int pos0 = deal.blk * kBlock;
+    const int steps = (stop - deal.blk) * (kBlock / 32), stages = steps / kSteps;
+    const auto fetch = [&](int stage) {
+      const Args& a = arguments();
+      const Lane<F> here = at.again();
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        place[t] = place_of(a, b, i * kBlock + (wave * kTiles + t) * 16, n);
-        k[t].load(a, h, place[t], at);
-        v[t].load(a, h, place[t], at);
+      for (int t = 0; t < kMine; ++t) {
+        place[t] = place_of(a, b, pos0 + stage * kKeys + (my_tile + t) * 16, n);
+        if (my_keys) k[t].load(a, h, place[t], here);
+        if (my_values) v[t].load(a, h, place[t], here);
       }
     };
-    fetch(deal.blk);
-    for (int i = deal.blk; i < stop; ++i) {
-      __syncthreads();                                  // (the block before has been used)
+    const auto convert = [&](int stage) {
+      u32x4* const to = operands + (stage & 1) * kStage + at.lane;
+      float* const sc = scales[stage & 1][0];
+      int flag[kMine];
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        const int tile = wave * kTiles + t, pos = i * kBlock + tile * 16;
-        int flag = place[t].page >= 0 ? 1 : 0;
-        if (!flag || pos + 16 > min(context, n)) {
-          v[t].drop(there_of(pos, n, flag, flag, at.g));
-          if constexpr (!F::codes) flag |= pos + 16 > context && __any(v[t].not_finite()) ? 2 : 0;
+      for (int t = 0; t < kMine; ++t) {
+        const int pos = pos0 + stage * kKeys + (my_tile + t) * 16;
+        flag[t] = place[t].page >= 0 ? 1 : 0;
+        if (my_values && (!flag[t] || pos + 16 > min(context, n))) {
+          v[t].drop(there_of(pos, n, flag[t], flag[t], at.g));
+          if constexpr (!F::codes) flag[t] |= pos + 16 > context && __any(v[t].not_finite()) ? 2 : 0;
         }
+        if (my_keys) {
 #pragma unroll
-        for (int c = 0; c < F::KS; ++c) ks[(tile * F::KS + c) * 64 + at.lane] = k[t].operand(c);
+          for (int c = 0; c < F::KS; ++c) to[((my_tile + t) * F::KS + c) * 64] = k[t].operand(c);
+          if (F::codes && at.col == 0) *reinterpret_cast<f32x4*>(sc + (my_tile + t) * 16 + 4 * at.g) = k[t].scale * by;
+        }
+        if (my_values) {
+          if (F::codes && at.col == 0) *reinterpret_cast<f32x4*>(sc + kKeys + (my_tile + t) * 16 + 4 * at.g) = v[t].scale;
+          if (at.lane == 0) flags[stage & 1][my_tile + t] = flag[t];
+          if constexpr (kMine == 1) {
+#pragma unroll
+            for (int d = 0; d < F::DT; ++d)
+              reinterpret_cast<u32x2*>(to + kValues + ((my_tile / 2) * F::DT + d) * 64)[my_tile & 1] = v[0].operand(d);
+          } else if (t & 1) {
+#pragma unroll
+            for (int d = 0; d < F::DT; ++d)
+              to[kValues + ((my_tile + t) / 2 * F::DT + d) * 64] = joined_operand(v[t - 1].operand(d), v[t].operand(d));
+          }
+        }
+      }
+    };
+    // What a step reads from LDS is read ahead: keys, scales and flags under the products of the step before, values under the weights.
+    // (Left to itself the scheduler reads each operand in front of its use, to save registers, and waits for it.)
+    f32x4 s[RT][2], k_scale[2], v_scale[2];
+    u32x4 kf[2][F::KS];
+    int flag[2];
+    const auto read_keys = [&](int i, int t) {
+      const u32x4* const from = operands + ((i / kSteps) & 1) * kStage + ((i % kSteps) * 2 + t) * F::KS * 64 + at.lane;
+#pragma unroll
+      for (int c = 0; c < F::KS; ++c) kf[t][c] = from[c * 64];
+    };
+    const auto read_scales = [&](int i) {
+      const int buffer = (i / kSteps) & 1, j = i % kSteps;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         if constexpr (F::codes) {
-          if (at.col == 0) {
-            *reinterpret_cast<f32x4*>(k_scales + tile * 16 + 4 * at.g) = k[t].scale * by;
-            *reinterpret_cast<f32x4*>(v_scales + tile * 16 + 4 * at.g) = v[t].scale;
-          }
+          const float* const sc = scales[buffer][0] + j * 32 + 16 * t + 4 * at.g;
+          k_scale[t] = *reinterpret_cast<const f32x4*>(sc);
+          v_scale[t] = *reinterpret_cast<const f32x4*>(sc + kKeys);
+        } else {
+          k_scale[t] = f32x4{by, by, by, by};
+          v_scale[t] = f32x4{1, 1, 1, 1};
         }
-        if (at.lane == 0) flags[tile] = flag;
+        flag[t] = flags[buffer][2 * j + t];
       }
-      if constexpr (kTiles == 2) {
+    };
+    const auto products = [&] {                                          // of the keys read last with the queries
 #pragma unroll
-        for (int d = 0; d < F::DT; ++d) vs[(wave * F::DT + d) * 64 + at.lane] = joined_operand(v[0].operand(d), v[1].operand(d));
-      } else {
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int d = 0; d < F::DT; ++d)
-          reinterpret_cast<u32x2*>(vs + ((wave / 2) * F::DT + d) * 64 + at.lane)[wave & 1] = v[0].operand(d);
-      }
-      if (i + 1 < stop) fetch(i + 1);
-      __syncthreads();
-#pragma unroll 1
-      for (int step = 0; step < 4; ++step) {
-        const int pos = i * kBlock + step * 32;
-        if (pos >= n) break;
-        f32x4 s[RT][2], k_scale[2], v_scale[2];
+        for (int c = 0; c < F::KS; ++c)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+          for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(kf[t][c], q.w[r][c], c ? s[r][t] : f32x4{0, 0, 0, 0});
+    };
+    fetch(0);
+    convert(0);
+    if (stages > 1) fetch(1);
+    __syncthreads();
+    if (!idle) {
+      read_keys(0, 0);
+      read_keys(0, 1);
+      read_scales(0);
+      products();
+    }
+    for (int i = 0; i < steps; ++i) {
+      const int stage = i / kSteps, j = i % kSteps, pos = pos0 + i * 32;
+      const bool work = !idle && pos < n;
+      u32x4 vf[F::DT], p[RT];
+      uint32_t seen[RT];
+      bool one_by_one = false;
+      if (work) {
+        const u32x4* const from = operands + (stage & 1) * kStage + kValues + j * F::DT * 64 + at.lane;
 #pragma unroll
-          for (int r = 0; r < RT; ++r) s[r][t] = f32x4{0, 0, 0, 0};
+        for (int d = 0; d < F::DT; ++d) vf[d] = from[d * 64];
+        const int f0 = __builtin_amdgcn_readfirstlane(flag[0]), f1 = __builtin_amdgcn_readfirstlane(flag[1]);
+        const bool masked = pos + 32 > min(context, n) || !(f0 & f1 & 1);
+        one_by_one = ((f0 | f1) & 2) != 0;
 #pragma unroll
-          for (int c = 0; c < F::KS; ++c) {
-            const u32x4 f = ks[((2 * step + t) * F::KS + c) * 64 + at.lane];
-#pragma unroll
-            for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(f, q.w[r][c], s[r][t]);
-          }
-          if constexpr (F::codes) {
-            k_scale[t] = *reinterpret_cast<const f32x4*>(k_scales + step * 32 + 16 * t + 4 * at.g);
-            v_scale[t] = *reinterpret_cast<const f32x4*>(v_scales + step * 32 + 16 * t + 4 * at.g);
-          } else {
-            k_scale[t] = f32x4{by, by, by, by};
-            v_scale[t] = f32x4{1, 1, 1, 1};
-          }
-        }
-        u32x4 p[RT];
-        uint32_t seen[RT] = {};
-        const int flag0 = __builtin_amdgcn_readfirstlane(flags[2 * step]), flag1 = __builtin_amdgcn_readfirstlane(flags[2 * step + 1]);
-        const bool masked = pos + 32 > min(context, n) || !(flag0 & flag1 & 1);
+        for (int r = 0; r < RT; ++r) seen[r] = 0xff;
         if (masked) {
-          const uint32_t there = there_of(pos, n, flag0 & 1, flag1 & 1, at.g);
+          const uint32_t there = there_of(pos, n, f0 & 1, f1 & 1, at.g);
 #pragma unroll
-          for (int r = 0; r < RT; ++r) seen[r] = seen_by(a, b, q.token[r], pos, context, there, at.g);
+          for (int r = 0; r < RT; ++r) seen[r] = seen_by(arguments(), b, row0 + 16 * r + at.col, pos, context, there, at.g);
         }
-        weights<F, RT>(k_scale, v_scale, s, masked, seen, st, p);
-        add_values<F, RT>([&](int d) { return vs[(step * F::DT + d) * 64 + at.lane]; }, p, ((flag0 | flag1) & 2) != 0, seen, at, st);
+        weigh<F, RT>(k_scale, v_scale, s, masked, seen, st, p);
+      }
+      if (j == (late ? kSteps / 2 : 0) && stage + 1 < stages) {
+        convert(stage + 1);
+        if (stage + 2 < stages) fetch(stage + 2);
+      }
+      if (j == kSteps - 1) __syncthreads();
+      if (work) {
+        __builtin_amdgcn_s_setprio(1);
+        // (behind the last step: what is read is not used)
+        const int next = min(i + 1, steps - 1);
+        if (__builtin_expect(!F::codes && one_by_one, 0)) {
+          add_values_one_by_one<F, RT>(vf, p, seen, at, st);
+          read_keys(next, 0);
+          read_keys(next, 1);
+          read_scales(next);
+        } else {
+          read_keys(next, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          add_values<F, RT, 0, F::DT / 2>(vf, p, st);
+          __builtin_amdgcn_sched_barrier(0);
+          read_keys(next, 1);
+          read_scales(next);
+          __builtin_amdgcn_sched_barrier(0);
+          add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
+        }
+        products();
+        __builtin_amdgcn_s_setprio(0);
       }
     }
+    const Args& a = arguments();
     const bool final = deal.blk == 0 && stop == deal.nb;
     float* const slot = a.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * (16 * RT * WAVES) * (a.D + 4);
     if (deal.blk == 0 && threadIdx.x == 0) a.first[deal.item(a)] = deal.at;
@@ -823,11 +930,11 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 4 && W >= 3 ? 1 : 2) tall
         float x[F::DT];
 #pragma unroll
         for (int d = 0; d < F::DT; ++d) x[d] = st.o[r][d][i];
-        emit<F>(a, final, slot, b, h, row0 + 16 * r + at.col, (wave * RT + r) * 16 + at.col, q.token[r], Lane<F>::elements_of(a, 4 * at.g + i),
+        emit<F>(a, final, slot, b, h, row0 + 16 * r + at.col, (wave * RT + r) * 16 + at.col, Lane<F>::elements_of(a, 4 * at.g + i),
                 at.g == 0 && i == 0, x, st.m[r], l);
       }
     }
-  } while (deal.next(a));
+  } while (deal.next(arguments()));
 }
 
 #if FCR_HAS(0)
@@ -896,7 +1003,9 @@ void launch_w(const Args& a, int form, hipStream_t s) {
     case 2:
       if constexpr (W <= 2) hipLaunchKernelGGL((tree_attention_kernel<CD, W, 2>), grid, dim3(256), 0, s, a);
       break;
-    case 4: hipLaunchKernelGGL((tall_attention_kernel<CD, W, 4>), grid, dim3(256), 0, s, a); break;
+    case 4:
+      if constexpr (W <= 2) hipLaunchKernelGGL((tall_attention_kernel<CD, W, 4>), grid, dim3(256), 0, s, a);
+      break;
     default: hipLaunchKernelGGL((tall_attention_kernel<CD, W, 8>), grid, dim3(512), 0, s, a); break;
   }
 }
@@ -938,7 +1047,7 @@ struct Plan {
 bool plan_of(int B, int H, int G, int T, int D, int64_t capacity, Plan& p) {
   const int64_t rows = (int64_t)T * G;
   const int w = (D + 63) / 64, tall = 16 * tall_tiles(w);
-  p.form = rows <= 16 ? 1 : rows <= 32 && w <= 2 ? 2 : rows <= 4 * tall ? 4 : 8;
+  p.form = rows <= 16 ? 1 : rows <= 32 && w <= 2 ? 2 : rows <= 4 * tall && w <= 2 ? 4 : 8;
   p.tile_rows = p.form <= 2 ? 16 * p.form : tall * p.form;
   const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.items = (int64_t)B * H * tiles;
