@@ -126,19 +126,41 @@ struct Form {
   static constexpr int VW = codes ? W : 2 * W;    // words that a lane has of a value row
 };
 
-// Where the 16-key tile from position `pos` on lies: page (< 0: not there, or behind the last key) and first row in it.
+// Where a sequence's keys of one head lie: what a tile's address is formed from, and nothing else that would be kept in scalar registers.
+struct Source {
+  const char* rows[2];
+  const float* scale[2];
+  int64_t page[2], s_page[2];     // bytes; elements
+  int row[2];                     // bytes
+  const int32_t* table;
+  Div page_size;
+  int pages, n;
+  __device__ __forceinline__ Source(const Args& a, int b, int h, int n_) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const Side& s = a.c.side[i];
+      rows[i] = s.rows + h * s.head;
+      scale[i] = s.scale + h * s.s_head;
+      page[i] = s.page, s_page[i] = s.s_page, row[i] = (int)s.row;
+    }
+    table = a.c.table + b * a.c.table_stride;
+    page_size = a.c.page_size;
+    pages = a.c.pages, n = n_;
+  }
+};
+// Where the 16-key tile from position `pos` on lies: page (not below Source::pages: not there, or behind the last key) and first row in it.
 struct Place {
   int page, row;
-};
-__device__ __forceinline__ Place place_of(const Args& a, int b, int pos, int n) {
-  Place p{-1, 0};
-  if (pos < n) {
-    uint32_t row;
-    p.page = __builtin_amdgcn_readfirstlane(page_of(a.c, b, (uint32_t)pos, row));
-    p.row = (int)row;
+  __device__ __forceinline__ Place() {}
+  __device__ __forceinline__ Place(const Source& s, int pos) : page(-1), row(0) {
+    if (pos < s.n) {
+      const uint32_t i = s.page_size.of((uint32_t)pos);
+      row = pos - (int)(i * s.page_size.d);
+      page = constant_at(s.table + i);
+    }
   }
-  return p;
-}
+  __device__ __forceinline__ bool there(const Source& s) const { return (uint32_t)page < (uint32_t)s.pages; }
+};
 
 // The lane's places in a 16-key tile: of keys (row lane & 15; 16-byte pieces, of which a row's last one stands for those behind it) and of
 // values (rows 4 g + i, elements from elements_of(col) on, where behind the row's end there are elements that another lane has as well).
@@ -152,20 +174,20 @@ struct Lane {
     asm volatile("" : "+v"(l));
     return Lane(l);
   }
-  __device__ __forceinline__ uint32_t key(const Args& a) const { return (uint32_t)(col * (int)a.c.side[0].row); }
-  __device__ __forceinline__ uint32_t piece(const Args& a, int i) const { return min(64u * i + 16u * g, (uint32_t)a.D * kBytes - 16u); }
-  __device__ __forceinline__ uint32_t value(const Args& a) const {
-    return (uint32_t)(4 * g * (int)a.c.side[1].row) + (uint32_t)elements_of(a, col) * kBytes;
+  __device__ __forceinline__ uint32_t key(const Source& s, int i, int D) const {
+    return (uint32_t)(col * s.row[0]) + min(64u * i + 16u * g, (uint32_t)D * kBytes - 16u);
   }
-  __device__ __forceinline__ static int elements_of(const Args& a, int col) { return min(col * F::DT, a.D - F::DT); }
+  __device__ __forceinline__ uint32_t value(const Source& s, int D) const { return (uint32_t)(4 * g * s.row[1]) + (uint32_t)elements_of(D, col) * kBytes; }
+  __device__ __forceinline__ static int elements_of(int D, int col) { return min(col * F::DT, D - F::DT); }
 };
 
 // A tile's rows, or its scales, as a view that reads as zeros where its page is not there: the loads need no branch.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const Side& s, int h, const Place& p) {
-  return __builtin_amdgcn_make_buffer_rsrc(s.rows + p.page * s.page + h * s.head + p.row * s.row, 0, p.page >= 0 ? (int)(16 * s.row) : 0, 0x00020000);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const Source& s, int side, const Place& p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(s.rows[side]) + p.page * s.page[side] + (int64_t)p.row * s.row[side], 0,
+                                           p.there(s) ? 16 * s.row[side] : 0, 0x00020000);
 }
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t scales_of(const Side& s, int h, const Place& p) {
-  return __builtin_amdgcn_make_buffer_rsrc(s.scale + p.page * s.s_page + h * s.s_head + p.row, 0, p.page >= 0 ? 64 : 0, 0x00020000);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t scales_of(const Source& s, int side, const Place& p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(s.scale[side]) + p.page * s.s_page[side] + p.row, 0, p.there(s) ? 64 : 0, 0x00020000);
 }
 __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t v, uint32_t at) { return __builtin_amdgcn_raw_buffer_load_b128(v, (int)at, 0, 0); }
 
@@ -195,11 +217,11 @@ template <class F>
 struct Keys {
   u32x4 w[F::KL];
   f32x4 scale;
-  __device__ __forceinline__ void load(const Args& a, int h, const Place& p, const Lane<F>& at) {
-    const __amdgpu_buffer_rsrc_t rows = rows_of(a.c.side[0], h, p);
+  __device__ __forceinline__ void load(const Source& s, int D, const Place& p, const Lane<F>& at) {
+    const __amdgpu_buffer_rsrc_t rows = rows_of(s, 0, p);
 #pragma unroll
-    for (int i = 0; i < F::KL; ++i) w[i] = load16(rows, at.key(a) + at.piece(a, i));
-    if constexpr (F::codes) scale = __builtin_bit_cast(f32x4, load16(scales_of(a.c.side[0], h, p), 16 * at.g));
+    for (int i = 0; i < F::KL; ++i) w[i] = load16(rows, at.key(s, i, D));
+    if constexpr (F::codes) scale = __builtin_bit_cast(f32x4, load16(scales_of(s, 0, p), 16 * at.g));
   }
   // k-steps 2 i and 2 i + 1 (codes) or i (16-bit) of load i
   __device__ __forceinline__ u32x4 operand(int ks) const {
@@ -231,11 +253,11 @@ template <class F>
 struct Values {
   uint32_t w[4][F::VW];
   f32x4 scale;
-  __device__ __forceinline__ void load(const Args& a, int h, const Place& p, const Lane<F>& at) {
-    const __amdgpu_buffer_rsrc_t rows = rows_of(a.c.side[1], h, p);
+  __device__ __forceinline__ void load(const Source& s, int D, const Place& p, const Lane<F>& at) {
+    const __amdgpu_buffer_rsrc_t rows = rows_of(s, 1, p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_words(rows, at.value(a), i * (int)a.c.side[1].row, w[i]);
-    if constexpr (F::codes) scale = __builtin_bit_cast(f32x4, load16(scales_of(a.c.side[1], h, p), 16 * at.g));
+    for (int i = 0; i < 4; ++i) load_words(rows, at.value(s, D), i * s.row[1], w[i]);
+    if constexpr (F::codes) scale = __builtin_bit_cast(f32x4, load16(scales_of(s, 1, p), 16 * at.g));
   }
   // Keys that are not there: bits of `there` from bit 0 on.  What their rows hold is not looked at.
   __device__ __forceinline__ void drop(uint32_t there) {
@@ -619,18 +641,21 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
     st.clear();
     Keys<F> k[2];
     Values<F> v[2];
-    Place here[2], next[2];
+    // (places are a block further ahead than the loads, which need them)
+    const Source src(a, b, h, n);
+    Place here[2], next[2], then[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      here[t] = place_of(a, b, deal.blk * kBlock + wave * 32 + 16 * t, n);
-      k[t].load(a, h, here[t], at);
-      v[t].load(a, h, here[t], at);
+      here[t] = Place(src, deal.blk * kBlock + wave * 32 + 16 * t);
+      k[t].load(src, a.D, here[t], at);
+      v[t].load(src, a.D, here[t], at);
+      next[t] = Place(src, (deal.blk + 1) * kBlock + wave * 32 + 16 * t);
     }
     for (int i = deal.blk; i < stop; ++i) {
       const int pos = i * kBlock + wave * 32;
       if (pos >= n) break;                              // (a wave's later blocks lie behind this one)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) next[t] = place_of(a, b, pos + kBlock + 16 * t, i + 1 < stop ? n : 0);
+      for (int t = 0; t < 2; ++t) then[t] = Place(src, pos + 2 * kBlock + 16 * t);
       f32x4 s[RT][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -648,16 +673,17 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
       for (int t = 0; t < 2; ++t) k_scale[t] = F::codes ? k[t].scale * by : f32x4{by, by, by, by};
       if (i + 1 < stop) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) k[t].load(a, h, next[t], at);
+        for (int t = 0; t < 2; ++t) k[t].load(src, a.D, next[t], at);
       }
       u32x4 p[RT];
       uint32_t seen[RT];
 #pragma unroll
       for (int r = 0; r < RT; ++r) seen[r] = 0xff;
-      const bool masked = pos + 32 > min(context, n) || here[0].page < 0 || here[1].page < 0;
+      const bool there0 = here[0].there(src), there1 = here[1].there(src);
+      const bool masked = pos + 32 > min(context, n) || !there0 || !there1;
       bool one_by_one = false;
       if (masked) {
-        const uint32_t there = there_of(pos, n, here[0].page >= 0, here[1].page >= 0, at.g);
+        const uint32_t there = there_of(pos, n, there0, there1, at.g);
         v[0].drop(there);
         v[1].drop(there >> 4);
         if constexpr (!F::codes) one_by_one = pos + 32 > context && __any(v[0].not_finite() || v[1].not_finite());
@@ -681,9 +707,10 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
       }
       if (i + 1 < stop) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) v[t].load(a, h, next[t], at);
+        for (int t = 0; t < 2; ++t) v[t].load(src, a.D, next[t], at);
       }
       here[0] = next[0], here[1] = next[1];
+      next[0] = then[0], next[1] = then[1];
     }
 
     // join the four waves
@@ -719,7 +746,7 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) x[d] += joined[((w * 4 + wave) * F::DT + d) * 64 + at.lane];
       }
-      emit<F>(a_end, final, slot, b, h, row0 + 16 * r + at.col, 16 * r + at.col, Lane<F>::elements_of(a_end, 4 * at.g + wave),
+      emit<F>(a_end, final, slot, b, h, row0 + 16 * r + at.col, 16 * r + at.col, Lane<F>::elements_of(a_end.D, 4 * at.g + wave),
               wave == 0 && at.g == 0, x, m, l);
       __syncthreads();
     }
@@ -780,18 +807,24 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
     st.clear();
     Keys<F> k[kMine];
     Values<F> v[kMine];
-    Place place[kMine];
+    const Source src(arguments(), b, h, n);
+    Place place[kMine], ahead[kMine];                                    // of the rows loaded last, and of the next ones
     const int pos0 = deal.blk * kBlock;
     const int steps = (stop - deal.blk) * (kBlock / 32), stages = steps / kSteps;
+    const auto look = [&](int stage) {
+#pragma unroll
+      for (int t = 0; t < kMine; ++t) ahead[t] = Place(src, pos0 + stage * kKeys + (my_tile + t) * 16);
+    };
     const auto fetch = [&](int stage) {
-      const Args& a = arguments();
+      const int D = arguments().D;
       const Lane<F> here = at.again();
 #pragma unroll
       for (int t = 0; t < kMine; ++t) {
-        place[t] = place_of(a, b, pos0 + stage * kKeys + (my_tile + t) * 16, n);
-        if (my_keys) k[t].load(a, h, place[t], here);
-        if (my_values) v[t].load(a, h, place[t], here);
+        place[t] = ahead[t];
+        if (my_keys) k[t].load(src, D, place[t], here);
+        if (my_values) v[t].load(src, D, place[t], here);
       }
+      look(stage + 1);
     };
     const auto convert = [&](int stage) {
       u32x4* const to = operands + (stage & 1) * kStage + at.lane;
@@ -800,7 +833,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
       for (int t = 0; t < kMine; ++t) {
         const int pos = pos0 + stage * kKeys + (my_tile + t) * 16;
-        flag[t] = place[t].page >= 0 ? 1 : 0;
+        flag[t] = place[t].there(src) ? 1 : 0;
         if (my_values && (!flag[t] || pos + 16 > min(context, n))) {
           v[t].drop(there_of(pos, n, flag[t], flag[t], at.g));
           if constexpr (!F::codes) flag[t] |= pos + 16 > context && __any(v[t].not_finite()) ? 2 : 0;
@@ -858,6 +891,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
           for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(kf[t][c], q.w[r][c], c ? s[r][t] : f32x4{0, 0, 0, 0});
     };
+    look(0);
     fetch(0);
     convert(0);
     if (stages > 1) fetch(1);
@@ -930,7 +964,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         float x[F::DT];
 #pragma unroll
         for (int d = 0; d < F::DT; ++d) x[d] = st.o[r][d][i];
-        emit<F>(a, final, slot, b, h, row0 + 16 * r + at.col, (wave * RT + r) * 16 + at.col, Lane<F>::elements_of(a, 4 * at.g + i),
+        emit<F>(a, final, slot, b, h, row0 + 16 * r + at.col, (wave * RT + r) * 16 + at.col, Lane<F>::elements_of(a.D, 4 * at.g + i),
                 at.g == 0 && i == 0, x, st.m[r], l);
       }
     }
