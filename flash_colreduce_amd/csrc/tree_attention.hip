@@ -50,9 +50,10 @@ struct Args {
   int32_t* first;              // [items]: where an item begins, in blocks
   float* part;                 // [2 workgroups][rows of a tile][D + 4]: reference, sum, 2 unused, weighted values
   int B, H, T, D, rows, row_tiles, bf16;
-  Div G;
+  Div G, per_head, heads, all; // by G, by row_tiles, by H, by wgs
   float scale2;
   int wgs, least;              // workgroups of the launch; blocks that one takes at least
+  int positions;               // that a row of the table names
 };
 // form: see Plan
 void attention_f16(const Args& a, int w, int form, hipStream_t s);
@@ -87,7 +88,7 @@ __device__ __forceinline__ int blocks_of(int n) { return n <= 0 ? 1 : (n + kBloc
 __device__ __forceinline__ void keys_of(const Args& a, int b, int h, int& context, int& n) {
   const int tree = a.tree_lengths ? min(max(constant_at(a.tree_lengths + b), 0), a.T) : a.T;
   context = max(a.context.of(b, h), 0);
-  n = (int)min((int64_t)context + tree, a.c.capacity);
+  n = (int)min((uint32_t)context + (uint32_t)tree, (uint32_t)a.positions);   // (each below 2^31)
 }
 
 __device__ __forceinline__ float across(float x, bool largest) {   // over the four lanes that share a query
@@ -428,44 +429,55 @@ __device__ __forceinline__ void add_values_one_by_one(const u32x4 (&v)[F::DT], c
 template <class F, int RT>
 struct Queries {
   u32x4 w[RT][F::KS];
-  // Returns the largest element's bits where they are to be scaled.
+  // Returns the largest finite element's bits (of codes: where they are bf16 they are to be scaled).
   __device__ __forceinline__ uint32_t load(const Args& a, int b, int h, int row0, const Lane<F>& at) {
-    uint32_t most = 0;
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    constexpr int mine = F::codes ? 16 : 8;   // elements that lanes are apart
+    s16x2 most = {0, 0};
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int row = row0 + 16 * r + at.col;
-      const bool live = row < a.rows;
-      const uint32_t t = a.G.of((uint32_t)(live ? row : 0)), head = (uint32_t)(live ? row : 0) - t * a.G.d;
-      const char* from = a.q + b * a.qb + (int64_t)(h * (int)a.G.d + (int)head) * a.qh + t * a.qt;
+      const uint32_t t = a.G.of((uint32_t)row), head = (uint32_t)row - t * a.G.d;
+      const char* from = a.q + b * a.qb + (int64_t)(h * (int)a.G.d + (int)head) * a.qh + t * a.qt + 2 * mine * at.g;
 #pragma unroll
-      for (int s = 0; s < F::KS; ++s) {
-        const int d = F::codes ? 64 * (s / 2) + 16 * at.g + 8 * (s & 1) : 32 * s + 8 * at.g;
-        w[r][s] = live && d < a.D ? *reinterpret_cast<const u32x4*>(from + 2 * d) : u32x4{0, 0, 0, 0};
-        if constexpr (F::codes) {
+      for (int s = 0; s < F::KS; ++s) w[r][s] = u32x4{0, 0, 0, 0};
+      if (row < a.rows) {
+        const int d0 = mine * at.g;
+        if (a.D == 64 * (F::KS / 2)) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = w[r][s][j] & 0x7fffu, hi = (w[r][s][j] >> 16) & 0x7fffu;
-            most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));   // (of what is finite)
-          }
+          for (int s = 0; s < F::KS; ++s) w[r][s] = *reinterpret_cast<const u32x4*>(from + 2 * element(s));
+        } else {
+#pragma unroll
+          for (int s = 0; s < F::KS; ++s)
+            if (d0 + element(s) < a.D) w[r][s] = *reinterpret_cast<const u32x4*>(from + 2 * element(s));
         }
       }
     }
-    return most;
+    // magnitudes with 0x80 added: as signed halves bf16's infinities and NaNs are below all others
+    if (F::codes && a.bf16) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int s = 0; s < F::KS; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, (w[r][s][j] & 0x7fff7fffu) + 0x00800080u));
+    }
+    return (uint32_t)max(max((int)most[0], (int)most[1]) - 0x80, 0);
   }
-  // bf16 to fp16, the largest element (its bits: `most`, the same in every lane) to [2^14, 2^15).  Returns what undoes it.
-  __device__ __forceinline__ float scale(uint32_t most) {
-    const int up = most == 0 ? 0 : max(-112, min(14 - ((int)(most >> 7) - 127), 140));
-    // (in two steps, each of which fp32 can express)
-    const float by1 = __builtin_bit_cast(float, (uint32_t)(127 + up / 2) << 23), by2 = __builtin_bit_cast(float, (uint32_t)(127 + up - up / 2) << 23);
-    const float undo1 = __builtin_bit_cast(float, (uint32_t)(127 - up / 2) << 23), undo2 = __builtin_bit_cast(float, (uint32_t)(127 - (up - up / 2)) << 23);
+  // Where in a row the lanes' first elements of k-step s are.
+  __device__ __forceinline__ static constexpr int element(int s) { return F::codes ? 64 * (s / 2) + 8 * (s & 1) : 32 * s; }
+  // bf16 to fp16, the largest element (its bits: `most`, the same in every lane) to [2^14, 2^15): times 2^ what is returned.
+  __device__ __forceinline__ int scale(uint32_t most) {
+    const int up = most == 0 ? 0 : 14 - ((int)(most >> 7) - 127);
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
       for (int s = 0; s < F::KS; ++s)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          w[r][s][j] = pack2<FCR_DTYPE_F16>(bf16_of(w[r][s][j], 0) * by1 * by2, bf16_of(w[r][s][j], 1) * by1 * by2);
-    return undo1 * undo2;
+          w[r][s][j] = pack2<FCR_DTYPE_F16>(__builtin_amdgcn_ldexpf(bf16_of(w[r][s][j], 0), up), __builtin_amdgcn_ldexpf(bf16_of(w[r][s][j], 1), up));
+    return up;
   }
 };
 __device__ __forceinline__ uint32_t largest_of_wave(uint32_t x) {
@@ -473,18 +485,22 @@ __device__ __forceinline__ uint32_t largest_of_wave(uint32_t x) {
   return x;
 }
 
-// Which of the lane's keys from position `pos` on (a 32-key step: bits 4 t + i) the query of token t sees.
-// (row: the query's; rows that are none are given token 0)
+// Which of the lane's keys from position `pos` on (a 32-key step: bits 4 t + i) the query of a row sees.  (Rows that are none are given
+// token 0.  Bytes in front of the mask's row, for keys of the context, and behind it, for keys that are not there, do not count.)
 __device__ __forceinline__ uint32_t seen_by(const Args& a, int b, int row, int pos, int context, uint32_t there, int g) {
   const int token = row < a.rows ? (int)a.G.of((uint32_t)row) : 0;
-  const uint8_t* const mask = a.mask ? a.mask + b * a.mask_b + (int64_t)token * a.T : nullptr;
+  const int u = pos + 4 * g - context;   // which drafted token the lane's first key is; below 0: of the context
   uint32_t seen = 0;
-#pragma unroll 1
-  for (int e = 0; e < 8; ++e) {
-    const int u = pos + 16 * (e / 4) + 4 * g + e % 4 - context;   // which drafted token; below 0: of the context
-    bool is = u <= token;
-    if (mask) is = u < 0 || mask[min(max(u, 0), a.T - 1)] != 0;
-    seen |= is ? 1u << e : 0u;
+  if (a.mask) {
+    const __amdgpu_buffer_rsrc_t mask = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.mask) + b * a.mask_b, 0, a.T * a.T, 0x00020000);
+    uint32_t is[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) is[e] = __builtin_amdgcn_raw_buffer_load_b8(mask, token * a.T + u + 16 * (e / 4) + e % 4, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) seen |= u + 16 * (e / 4) + e % 4 < 0 || (is[e] & 0xffu) ? 1u << e : 0u;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) seen |= u + 16 * (e / 4) + e % 4 <= token ? 1u << e : 0u;
   }
   return seen & there;
 }
@@ -496,33 +512,33 @@ __device__ __forceinline__ uint32_t there_of(int pos, int n, bool page0, bool pa
   return there;
 }
 
-// DT consecutive elements of a row: its result, or its part of one.
-template <class F>
-__device__ __forceinline__ void emit(const Args& a, bool final, float* slot, int b, int h, int row, int row_in_tile, int d0, bool first,
-                                     const float (&x)[F::DT], float m, float l) {
-  if (row >= a.rows) return;
-  if (final) {
-    const int token = (int)a.G.of((uint32_t)row);
-    const bool none = (a.tree_lengths && token >= a.tree_lengths[b]) || l == 0.0f;
-    const float inverse = 1.0f / l;
-    const int64_t to = ((int64_t)b * a.H * a.G.d + (int64_t)h * a.G.d + (row - token * (int)a.G.d)) * a.T + token;
-    uint32_t* const o = reinterpret_cast<uint32_t*>(a.out + (to * a.D + d0) * 2);
-#pragma unroll
-    for (int d = 0; d < F::DT; d += 4) {
-      float y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = none ? 0.0f : x[d + j] * inverse;
-      const u32x2 v = a.bf16 ? u32x2{pack2<FCR_DTYPE_BF16>(y[0], y[1]), pack2<FCR_DTYPE_BF16>(y[2], y[3])}
-                             : u32x2{pack2<FCR_DTYPE_F16>(y[0], y[1]), pack2<FCR_DTYPE_F16>(y[2], y[3])};
-      *reinterpret_cast<u32x2*>(o + d / 2) = v;          // (d0 is a multiple of 4)
-    }
-    if (a.lse && first) a.lse[to] = none ? -INFINITY : m + __builtin_amdgcn_logf(l);
-  } else {
-    float* const o = slot + (int64_t)row_in_tile * (a.D + 4);
-#pragma unroll
-    for (int d = 0; d < F::DT; d += 4) *reinterpret_cast<f32x4*>(o + 4 + d0 + d) = f32x4{x[d], x[d + 1], x[d + 2], x[d + 3]};
-    if (first) o[0] = m, o[1] = l;
+// A query row's place in the outputs.
+struct Output {
+  int64_t row;
+  bool live, none;     // there is such a row; the sequence has no such token, or it sees nothing
+  __device__ __forceinline__ Output(const Args& a, int b, int h, int r, float l) : live(r < a.rows) {
+    const int token = (int)a.G.of((uint32_t)r);
+    none = (a.tree_lengths && token >= a.tree_lengths[live ? b : 0]) || l == 0.0f;
+    row = ((int64_t)b * a.H * a.G.d + (int64_t)h * a.G.d + (r - token * (int)a.G.d)) * a.T + token;
   }
+};
+// DT consecutive elements of a row, from d0 (a multiple of 4) on: its result, or its part of one (`to` is the row's in the part).
+template <class F>
+__device__ __forceinline__ void emit(const Args& a, const Output& out, int d0, const float (&x)[F::DT], float inverse) {
+  uint32_t* const o = reinterpret_cast<uint32_t*>(a.out + (out.row * a.D + d0) * 2);
+#pragma unroll
+  for (int d = 0; d < F::DT; d += 4) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = out.none ? 0.0f : x[d + j] * inverse;
+    *reinterpret_cast<u32x2*>(o + d / 2) = a.bf16 ? u32x2{pack2<FCR_DTYPE_BF16>(y[0], y[1]), pack2<FCR_DTYPE_BF16>(y[2], y[3])}
+                                                  : u32x2{pack2<FCR_DTYPE_F16>(y[0], y[1]), pack2<FCR_DTYPE_F16>(y[2], y[3])};
+  }
+}
+template <class F>
+__device__ __forceinline__ void emit_part(float* to, int d0, const float (&x)[F::DT]) {
+#pragma unroll
+  for (int d = 0; d < F::DT; d += 4) *reinterpret_cast<f32x4*>(to + 4 + d0 + d) = f32x4{x[d], x[d + 1], x[d + 2], x[d + 3]};
 }
 
 // The blocks of a workgroup, as pieces of items.  Lengths are known on the device only: every workgroup adds them up.  Lengths of
@@ -530,6 +546,8 @@ __device__ __forceinline__ void emit(const Args& a, bool final, float* slot, int
 template <int THREADS>
 struct Deal {
   int at, end, b, h, tile, blk, nb, context, n;
+  // (Short on purpose: this and what else runs once per workgroup costs about 200 cycles per 64 bytes of instructions, which come
+  // from memory at that point.)
   __device__ __forceinline__ bool start(const Args& a, int wg, int* scan) {   // scan: THREADS / 64 + 2 words of LDS
     constexpr int waves = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -537,60 +555,66 @@ struct Deal {
     const int entries = by_head ? a.B * a.H : a.B;
     const int weight = by_head ? a.row_tiles : a.H * a.row_tiles;
     const auto entry_blocks = [&](int e) {
-      int context, n;
-      keys_of(a, by_head ? e / a.H : e, by_head ? e % a.H : 0, context, n);
+      if (e >= entries) return 0;
+      int eb = e, eh = 0, context, n;
+      if (by_head) eb = (int)a.heads.of((uint32_t)e), eh = e - eb * a.H;
+      keys_of(a, eb, eh, context, n);
       return blocks_of(n) * weight;
     };
-    int total = 0;
-    for (int e = tid; e < entries; e += THREADS) total += entry_blocks(e);
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-    if (lane == 0) scan[wave] = total;
-    __syncthreads();
-    total = 0;
+    const auto in_front = [&](int x, int& sum) {        // of this thread; the sum over all
+      int upto = x;
 #pragma unroll
-    for (int i = 0; i < waves; ++i) total += scan[i];
-    const int per = max((total + a.wgs - 1) / a.wgs, a.least);
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(upto, o);
+        upto += lane >= o ? y : 0;
+      }
+      if (lane == 63) scan[wave] = upto;
+      __syncthreads();
+      sum = 0;
+      int before = upto - x;
+#pragma unroll
+      for (int i = 0; i < waves; ++i) {
+        before += i < wave ? scan[i] : 0;
+        sum += scan[i];
+      }
+      return before;
+    };
+    int mine = entry_blocks(tid), round, total;         // a round: as many entries as there are threads
+    int start = in_front(mine, round);
+    total = round;
+    if (__builtin_expect(entries > THREADS, 0)) {
+      int rest = 0;
+      for (int e = tid + THREADS; e < entries; e += THREADS) rest += entry_blocks(e);
+      __syncthreads();
+      in_front(rest, total);
+      total += round;
+    }
+    const int per = max((int)a.all.of((uint32_t)(total + a.wgs - 1)), a.least);
     at = wg * per;                                      // (wgs * per is total + wgs at most: checked by the host to fit)
     end = min(at + per, total);
     if (at >= end) return false;
-    int entry = 0, begun = 0;                           // the entry that holds `at`, and its first block
-    for (int base = 0, before = 0;; base += THREADS) {
-      const int e = base + tid;
-      const int mine = e < entries ? entry_blocks(e) : 0;
-      int sum = mine;
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(sum, o);
-        if (lane >= o) sum += x;
-      }
+    int base = 0;
+    for (int before = round; __builtin_expect(at >= before, 0); before += round) {
+      base += THREADS;
+      if (base >= entries) return false;                // (only if lengths change under the call)
       __syncthreads();
-      if (lane == 63) scan[wave] = sum;
-      if (tid == 0) scan[waves] = -1;
-      __syncthreads();
-      int start = before + sum - mine;
-      for (int i = 0; i < wave; ++i) start += scan[i];
-      if (mine > 0 && at >= start && at < start + mine) {
-        scan[waves] = e;
-        scan[waves + 1] = start;
-      }
-#pragma unroll
-      for (int i = 0; i < waves; ++i) before += scan[i];
-      __syncthreads();
-      if (scan[waves] >= 0) {
-        entry = scan[waves], begun = scan[waves + 1];
-        break;
-      }
-      if (base + THREADS >= entries) return false;      // (only if lengths change under the call)
+      mine = entry_blocks(base + tid);
+      start = before + in_front(mine, round);
     }
-    entry = __builtin_amdgcn_readfirstlane(entry);
-    int in = at - __builtin_amdgcn_readfirstlane(begun); // blocks from the entry's begin
-    b = by_head ? entry / a.H : entry, h = by_head ? entry % a.H : 0;
+    if (at >= start && at < start + mine) {             // the entry that holds `at`, and its first block
+      scan[waves] = base + tid;
+      scan[waves + 1] = start;
+    }
+    __syncthreads();
+    const int entry = __builtin_amdgcn_readfirstlane(scan[waves]);
+    const int in = at - __builtin_amdgcn_readfirstlane(scan[waves + 1]);
+    b = by_head ? (int)a.heads.of((uint32_t)entry) : entry;
+    h = by_head ? entry - b * a.H : 0;
     look(a);
-    if (!by_head) {
-      h = in / (nb * a.row_tiles);
-      in -= h * nb * a.row_tiles;
-    }
-    tile = in / nb;
-    blk = in - tile * nb;
+    int item_of_entry = (int)((uint32_t)in / (uint32_t)nb);
+    blk = in - item_of_entry * nb;
+    if (!by_head) h = (int)a.per_head.of((uint32_t)item_of_entry), item_of_entry -= h * a.row_tiles;
+    tile = item_of_entry;
     return true;
   }
   __device__ __forceinline__ void look(const Args& a) {
@@ -636,7 +660,7 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
     Queries<F, RT> q;
     float by = a.scale2;
     const uint32_t most = q.load(a, b, h, row0, at);
-    if (F::codes && a.bf16) by *= q.scale(largest_of_wave(most));
+    if (F::codes && a.bf16) by = __builtin_amdgcn_ldexpf(by, -q.scale(largest_of_wave(most)));
     State<F, RT> st;
     st.clear();
     Keys<F> k[2];
@@ -746,8 +770,19 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) x[d] += joined[((w * 4 + wave) * F::DT + d) * 64 + at.lane];
       }
-      emit<F>(a_end, final, slot, b, h, row0 + 16 * r + at.col, 16 * r + at.col, Lane<F>::elements_of(a_end.D, 4 * at.g + wave),
-              wave == 0 && at.g == 0, x, m, l);
+      const int row = row0 + 16 * r + at.col, d0 = Lane<F>::elements_of(a_end.D, 4 * at.g + wave);
+      const bool first = wave == 0 && at.g == 0;
+      if (row < a_end.rows) {
+        if (final) {
+          const Output out(a_end, b, h, row, l);
+          emit<F>(a_end, out, d0, x, 1.0f / l);
+          if (a_end.lse && first) a_end.lse[out.row] = out.none ? -INFINITY : m + __builtin_amdgcn_logf(l);
+        } else {
+          float* const to = slot + (int64_t)(16 * r + at.col) * (a_end.D + 4);
+          emit_part<F>(to, d0, x);
+          if (first) to[0] = m, to[1] = l;
+        }
+      }
       __syncthreads();
     }
   } while (deal.next(arguments()));
@@ -790,21 +825,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
     const int row0 = (deal.tile * WAVES + wave) * 16 * RT;
     const bool idle = row0 >= arguments().rows;                                    // (it converts all the same)
     const bool late = WAVES == 8 && wave >= 4;
-    Queries<F, RT> q;
-    float by = arguments().scale2;
-    uint32_t most = q.load(arguments(), b, h, row0, at);
-    __syncthreads();                                                     // (the piece before has been used)
-    if (F::codes && arguments().bf16) {
-      // one power of two for all rows of the workgroup, which the keys' scales undo
-      most = largest_of_wave(most);
-      if (at.lane == 0) scan[wave] = (int)most;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) most = max(most, (uint32_t)scan[w]);
-      by *= q.scale(most);
-    }
-    State<F, RT> st;
-    st.clear();
     Keys<F> k[kMine];
     Values<F> v[kMine];
     const Source src(arguments(), b, h, n);
@@ -826,6 +846,23 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       }
       look(stage + 1);
     };
+    look(0);
+    fetch(0);
+    Queries<F, RT> q;
+    float by = arguments().scale2;
+    uint32_t most = q.load(arguments(), b, h, row0, at);
+    __syncthreads();                                                     // (the piece before has been used)
+    if (F::codes && arguments().bf16) {
+      // one power of two for all rows of the workgroup, which the keys' scales undo
+      most = largest_of_wave(most);
+      if (at.lane == 0) scan[wave] = (int)most;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) most = max(most, (uint32_t)scan[w]);
+      by = __builtin_amdgcn_ldexpf(by, -q.scale(most));
+    }
+    State<F, RT> st;
+    st.clear();
     const auto convert = [&](int stage) {
       u32x4* const to = operands + (stage & 1) * kStage + at.lane;
       float* const sc = scales[stage & 1][0];
@@ -891,8 +928,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
           for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(kf[t][c], q.w[r][c], c ? s[r][t] : f32x4{0, 0, 0, 0});
     };
-    look(0);
-    fetch(0);
     convert(0);
     if (stages > 1) fetch(1);
     __syncthreads();
@@ -959,13 +994,29 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const float l = across(st.l[r], false);
+      const int row = row0 + 16 * r + at.col;
+      if (row >= a.rows) continue;
+      if (final) {
+        const Output out(a, b, h, row, l);
+        const float inverse = 1.0f / l;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x[F::DT];
+        for (int i = 0; i < 4; ++i) {
+          float x[F::DT];
 #pragma unroll
-        for (int d = 0; d < F::DT; ++d) x[d] = st.o[r][d][i];
-        emit<F>(a, final, slot, b, h, row0 + 16 * r + at.col, (wave * RT + r) * 16 + at.col, Lane<F>::elements_of(a.D, 4 * at.g + i),
-                at.g == 0 && i == 0, x, st.m[r], l);
+          for (int d = 0; d < F::DT; ++d) x[d] = st.o[r][d][i];
+          emit<F>(a, out, Lane<F>::elements_of(a.D, 4 * at.g + i), x, inverse);
+        }
+        if (a.lse && at.g == 0) a.lse[out.row] = out.none ? -INFINITY : st.m[r] + __builtin_amdgcn_logf(l);
+      } else {
+        float* const to = slot + (int64_t)((wave * RT + r) * 16 + at.col) * (a.D + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x[F::DT];
+#pragma unroll
+          for (int d = 0; d < F::DT; ++d) x[d] = st.o[r][d][i];
+          emit_part<F>(to, Lane<F>::elements_of(a.D, 4 * at.g + i), x);
+        }
+        if (at.g == 0) to[0] = st.m[r], to[1] = l;
       }
     }
   } while (deal.next(arguments()));
@@ -991,7 +1042,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(Args a, int tile_rows, i
   if ((threadIdx.x & 63) == 0) scan[threadIdx.x >> 6] = total;
   __syncthreads();
   total = scan[0] + scan[1] + scan[2] + scan[3];
-  const int per = max((total + a.wgs - 1) / a.wgs, a.least);
+  const int per = max((int)a.all.of((uint32_t)(total + a.wgs - 1)), a.least);
   keys_of(a, b, h, context, n);
   const int begin = a.first[item];
   const int from = begin / per, to = (begin + blocks_of(n) - 1) / per;
@@ -1119,6 +1170,7 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
   const int H = cache->H, D = cache->D;
   const int64_t capacity = (int64_t)table_pages * cache->page_size;
   Plan plan;
+  if (mask && T > 46340) return fail(FCR_E_SHAPE, "a mask of more than 2^31 bytes");
   if (G < 1 || T < 1 || T > (1 << 24) || G > (1 << 24) || (int64_t)B * H > (1 << 24) || (int64_t)H * G > (1 << 24) || !plan_of(B, H, G, T, D, capacity, plan))
     return fail(FCR_E_SHAPE, "G and T must be >= 1; B, H, G, T and the table are too large for one call otherwise");
   if (!isfinite(scale)) return fail(FCR_E_SCALE, "scale must be finite");
@@ -1143,7 +1195,8 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
   a.first = static_cast<int32_t*>(ws);
   a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + plan.first_bytes);
   a.B = B, a.H = H, a.T = T, a.D = D, a.rows = T * G, a.row_tiles = plan.row_tiles, a.bf16 = dtype == FCR_DTYPE_BF16;
-  a.G.set((uint32_t)G);
+  a.G.set((uint32_t)G), a.per_head.set((uint32_t)plan.row_tiles), a.heads.set((uint32_t)H), a.all.set((uint32_t)plan.wgs);
+  a.positions = (int)capacity;
   a.scale2 = scale * 1.44269504088896340736f;
   a.wgs = plan.wgs, a.least = plan.least;
   const int w = (D + 63) / 64;
