@@ -323,30 +323,31 @@ struct State {
 
 // The weights of 32 keys from their products with the queries: 2^(k_scale s - m) v_scale.  MASKED: seen[r] holds the keys that a row
 // sees, bit 4 t + i; else every key is seen.  Bound by the vector unit: per score an fma, an exponential (four slots), the sum, the product
-// with the value's scale, half a maximum and half a conversion.  Returns whether some row's reference has to be raised, where a weight would
-// not fit fp16 or a sum fp32.  A few of the first steps ask for it and hardly any later one: the
-// largest weight may be 2^15 times what the reference was raised for, and nothing needs it to be followed more closely.
+// with the value's scale and half a conversion.  Returns whether some row's reference has to be raised, because a weight might not fit fp16 (the
+// sum of the lane's probabilities times most_v, the largest scale of the 32 values: nothing asks for a maximum of weights) or a sum fp32.
+// A few of the first steps ask for it and hardly any later one: the largest weight may be 2^12 times what the reference was raised for, and
+// nothing needs it to be followed more closely.
 template <bool MASKED, class F, int RT>
-__device__ __forceinline__ bool weights(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], const f32x4 (&s)[RT][2], const uint32_t (&seen)[RT],
-                                        const State<F, RT>& st, float (&sum)[RT], u32x4 (&p)[RT]) {
+__device__ __forceinline__ bool weights(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], float most_v, const f32x4 (&s)[RT][2],
+                                        const uint32_t (&seen)[RT], const State<F, RT>& st, float (&sum)[RT], u32x4 (&p)[RT]) {
   bool raise = false;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    float x[8], most = 0.0f, part[2] = {0.0f, 0.0f};
+    float x[8], part[2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       x[e] = __builtin_fmaf(s[r][e / 4][e % 4], k_scale[e / 4][e % 4], -st.m[r]);
       if (MASKED) x[e] = (seen[r] >> e) & 1u ? x[e] : -INFINITY;
       x[e] = __builtin_amdgcn_exp2f(x[e]);
-      part[e & 1] += x[e];
+      part[e & 1] = e < 2 ? x[e] : part[e & 1] + x[e];
       if constexpr (F::codes) {
         x[e] *= v_scale[e / 4][e % 4];
         if (MASKED) x[e] = (seen[r] >> e) & 1u ? x[e] : 0.0f;      // (a hidden value's scale may be a NaN)
       }
-      most = fmaxf(most, fabsf(x[e]));
     }
-    sum[r] = st.l[r] + (part[0] + part[1]);
-    raise = raise || most > kMostWeight || !(sum[r] < kMostSum);
+    part[0] += part[1];
+    sum[r] = st.l[r] + part[0];
+    raise = raise || part[0] * most_v > kMostWeight || !(sum[r] < kMostSum);
 #pragma unroll
     for (int j = 0; j < 4; ++j) p[r][j] = F::bf16 ? pack2<FCR_DTYPE_BF16>(x[2 * j], x[2 * j + 1]) : pack2<FCR_DTYPE_F16>(x[2 * j], x[2 * j + 1]);
   }
@@ -378,13 +379,14 @@ __device__ __forceinline__ void raise(const f32x4 (&k_scale)[2], const f32x4 (&v
 }
 
 template <class F, int RT>
-__device__ __forceinline__ void weigh(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], const f32x4 (&s)[RT][2], bool masked,
+__device__ __forceinline__ void weigh(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], float most_v, const f32x4 (&s)[RT][2], bool masked,
                                       const uint32_t (&seen)[RT], State<F, RT>& st, u32x4 (&p)[RT]) {
   float sum[RT];
-  const bool up = masked ? weights<true, F, RT>(k_scale, v_scale, s, seen, st, sum, p) : weights<false, F, RT>(k_scale, v_scale, s, seen, st, sum, p);
+  const bool up = masked ? weights<true, F, RT>(k_scale, v_scale, most_v, s, seen, st, sum, p)
+                         : weights<false, F, RT>(k_scale, v_scale, most_v, s, seen, st, sum, p);
   if (__builtin_expect(up, 0)) {
     raise<F, RT>(k_scale, v_scale, s, seen, st);
-    weights<true, F, RT>(k_scale, v_scale, s, seen, st, sum, p);
+    weights<true, F, RT>(k_scale, v_scale, most_v, s, seen, st, sum, p);
   }
 #pragma unroll
   for (int r = 0; r < RT; ++r) st.l[r] = sum[r];
@@ -715,7 +717,12 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
         for (int r = 0; r < RT; ++r) seen[r] = seen_by(a, b, row0 + 16 * r + at.col, pos, context, there, at.g);
       }
       const f32x4 v_scale[2] = {v[0].scale, v[1].scale};
-      weigh<F, RT>(k_scale, v_scale, s, masked, seen, st, p);
+      float most_v = F::codes ? 0.0f : 1.0f;
+      if constexpr (F::codes) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most_v = fmaxf(most_v, fabsf(v_scale[e / 4][e % 4]));
+      }
+      weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
       if (__builtin_expect(!F::codes && one_by_one, 0)) {
         u32x4 f[F::DT];
 #pragma unroll
@@ -811,6 +818,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   static_assert(kTiles * (kApart ? 2 : 1) == WAVES * kMine, "every wave has its share of a stage");
   __shared__ u32x4 operands[2 * kStage];
   __shared__ __attribute__((aligned(16))) float scales[2][2][kKeys];     // of keys, of values
+  __shared__ float most[2][kTiles];                                      // the largest scale of a tile's values
   __shared__ int flags[2][kTiles];                                       // a tile's page is there, and (bit 1) a value is not finite
   __shared__ int scan[WAVES + 2];
   const int wg = range_of(args, blockIdx.x);
@@ -850,16 +858,16 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
     fetch(0);
     Queries<F, RT> q;
     float by = arguments().scale2;
-    uint32_t most = q.load(arguments(), b, h, row0, at);
+    uint32_t largest = q.load(arguments(), b, h, row0, at);
     __syncthreads();                                                     // (the piece before has been used)
     if (F::codes && arguments().bf16) {
       // one power of two for all rows of the workgroup, which the keys' scales undo
-      most = largest_of_wave(most);
-      if (at.lane == 0) scan[wave] = (int)most;
+      largest = largest_of_wave(largest);
+      if (at.lane == 0) scan[wave] = (int)largest;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) most = max(most, (uint32_t)scan[w]);
-      by = __builtin_amdgcn_ldexpf(by, -q.scale(most));
+      for (int w = 0; w < WAVES; ++w) largest = max(largest, (uint32_t)scan[w]);
+      by = __builtin_amdgcn_ldexpf(by, -q.scale(largest));
     }
     State<F, RT> st;
     st.clear();
@@ -881,7 +889,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
           if (F::codes && at.col == 0) *reinterpret_cast<f32x4*>(sc + (my_tile + t) * 16 + 4 * at.g) = k[t].scale * by;
         }
         if (my_values) {
-          if (F::codes && at.col == 0) *reinterpret_cast<f32x4*>(sc + kKeys + (my_tile + t) * 16 + 4 * at.g) = v[t].scale;
+          if constexpr (F::codes) {
+            if (at.col == 0) *reinterpret_cast<f32x4*>(sc + kKeys + (my_tile + t) * 16 + 4 * at.g) = v[t].scale;
+            const f32x4 x = v[t].scale;
+            const float m = across(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))), true);
+            if (at.lane == 0) most[stage & 1][my_tile + t] = fmaxf(m, 0.0f);   // (a NaN does not count)
+          }
           if (at.lane == 0) flags[stage & 1][my_tile + t] = flag[t];
           if constexpr (kMine == 1) {
 #pragma unroll
@@ -899,6 +912,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
     // (Left to itself the scheduler reads each operand in front of its use, to save registers, and waits for it.)
     f32x4 s[RT][2], k_scale[2], v_scale[2];
     u32x4 kf[2][F::KS];
+    float most_v = 1.0f;
     int flag[2];
     const auto read_keys = [&](int i, int t) {
       const u32x4* const from = operands + ((i / kSteps) & 1) * kStage + ((i % kSteps) * 2 + t) * F::KS * 64 + at.lane;
@@ -919,6 +933,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         }
         flag[t] = flags[buffer][2 * j + t];
       }
+      if constexpr (F::codes) most_v = fmaxf(most[buffer][2 * j], most[buffer][2 * j + 1]);
     };
     const auto products = [&] {                                          // of the keys read last with the queries
 #pragma unroll
@@ -957,7 +972,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
           for (int r = 0; r < RT; ++r) seen[r] = seen_by(arguments(), b, row0 + 16 * r + at.col, pos, context, there, at.g);
         }
-        weigh<F, RT>(k_scale, v_scale, s, masked, seen, st, p);
+        weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
       }
       if (j == (late ? kSteps / 2 : 0) && stage + 1 < stages) {
         convert(stage + 1);
