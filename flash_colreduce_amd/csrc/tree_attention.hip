@@ -270,15 +270,19 @@ struct Values {
         if constexpr (F::codes) scale[i] = 0.0f;
       }
   }
-  // Whether a 16-bit element is not finite.
-  __device__ __forceinline__ bool not_finite() const {
+  // 16-bit elements that are not finite become 0 (see add_not_finite); returns whether there was one.
+  __device__ __forceinline__ bool clean() {
     constexpr uint32_t e = F::bf16 ? 0x7f80u : 0x7c00u;
-    bool is = false;
+    uint32_t found = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < F::VW; ++j) is = is || (w[i][j] & e) == e || ((w[i][j] >> 16) & e) == e;
-    return is;
+      for (int j = 0; j < F::VW; ++j) {
+        const uint32_t bad = ((w[i][j] & e) == e ? 0xffffu : 0u) | (((w[i][j] >> 16) & e) == e ? 0xffff0000u : 0u);
+        found |= bad;
+        w[i][j] &= ~bad;
+      }
+    return found != 0;
   }
   // Element d (of the lane's DT) of the four rows, as four fp16 or bf16.
   __device__ __forceinline__ u32x2 operand(int d) const {
@@ -400,27 +404,32 @@ __device__ __forceinline__ void add_values(const u32x4 (&v)[F::DT], const u32x4 
 #pragma unroll
     for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(v[d], p[r], st.o[r][d]);
 }
-// The same where a value that is not finite stands at a key that some rows do not see: 0 * inf would reach them.  One key at a time, and
-// only rows that see it take the result.
+// Values that are not finite, at keys that only some rows see: in a matrix product 0 * inf would reach the others.  They are 0 there, and
+// come here from the cache: p v for the rows that see the key.  (pos: the first of the 32 keys.  Rare, and as short as can be.)
 template <class F, int RT>
-__device__ __forceinline__ void add_values_one_by_one(const u32x4 (&v)[F::DT], const u32x4 (&p)[RT], const uint32_t (&seen)[RT], const Lane<F>& at,
-                                                      State<F, RT>& st) {
+__device__ __forceinline__ void add_not_finite(const Source& src, int D, int pos, const u32x4 (&p)[RT], const uint32_t (&seen)[RT], const Lane<F>& at,
+                                               State<F, RT>& st) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const Place place(src, pos + 16 * t);
+    if (!place.there(src)) continue;
+    const char* row = src.rows[1] + place.page * src.page[1] + (int64_t)place.row * src.row[1];
 #pragma unroll 1
-  for (int key = 0; key < 32; ++key) {
-    const int e = key & 7, g = key >> 3;
-    u32x4 only;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) only[j] = at.g == g && (e >> 1) == j ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
-    bool see[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) see[r] = (__shfl((int)seen[r], 16 * g + at.col) >> e) & 1;
-#pragma unroll
-    for (int d = 0; d < F::DT; ++d) {
+    for (int k = 0; k < 16; ++k, row += src.row[1]) {
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        const f32x4 with = mma<F::bf16>(v[d] & only, p[r] & only, st.o[r][d]);
+        const int from = 16 * (k >> 2) + at.col;                             // the lane that has this key's weight
+        const bool see = (__shfl((int)seen[r], from) >> (4 * t + (k & 3))) & 1;
+        const uint32_t two = (uint32_t)__shfl((int)(k & 2 ? p[r][2 * t + 1] : p[r][2 * t]), from);
+        const float w = element<F::CD>(k & 1 ? two >> 16 : two, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st.o[r][d][i] = see[r] ? with[i] : st.o[r][d][i];
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < F::DT; ++d) {
+            const uint32_t x = *reinterpret_cast<const uint16_t*>(row + 2 * (Lane<F>::elements_of(D, 4 * at.g + i) + d));
+            constexpr uint32_t e = F::bf16 ? 0x7f80u : 0x7c00u;
+            if (see && (x & e) == e) st.o[r][d][i] += w * element<F::CD>(x, 0);
+          }
       }
     }
   }
@@ -707,12 +716,15 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
       for (int r = 0; r < RT; ++r) seen[r] = 0xff;
       const bool there0 = here[0].there(src), there1 = here[1].there(src);
       const bool masked = pos + 32 > min(context, n) || !there0 || !there1;
-      bool one_by_one = false;
+      bool not_finite = false;
       if (masked) {
         const uint32_t there = there_of(pos, n, there0, there1, at.g);
         v[0].drop(there);
         v[1].drop(there >> 4);
-        if constexpr (!F::codes) one_by_one = pos + 32 > context && __any(v[0].not_finite() || v[1].not_finite());
+        if constexpr (!F::codes) {
+          if (pos + 32 > context) not_finite = v[0].clean() | v[1].clean();
+          not_finite = __any(not_finite);
+        }
 #pragma unroll
         for (int r = 0; r < RT; ++r) seen[r] = seen_by(a, b, row0 + 16 * r + at.col, pos, context, there, at.g);
       }
@@ -723,18 +735,14 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
         for (int e = 0; e < 8; ++e) most_v = fmaxf(most_v, fabsf(v_scale[e / 4][e % 4]));
       }
       weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
-      if (__builtin_expect(!F::codes && one_by_one, 0)) {
-        u32x4 f[F::DT];
 #pragma unroll
-        for (int d = 0; d < F::DT; ++d) f[d] = joined_operand(v[0].operand(d), v[1].operand(d));
-        add_values_one_by_one<F, RT>(f, p, seen, at, st);
-      } else {
+      for (int d = 0; d < F::DT; ++d) {
+        const u32x4 f = joined_operand(v[0].operand(d), v[1].operand(d));
 #pragma unroll
-        for (int d = 0; d < F::DT; ++d) {
-          const u32x4 f = joined_operand(v[0].operand(d), v[1].operand(d));
-#pragma unroll
-          for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(f, p[r], st.o[r][d]);
-        }
+        for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(f, p[r], st.o[r][d]);
+      }
+      if constexpr (!F::codes) {
+        if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(src, arguments().D, pos, p, seen, at, st);
       }
       if (i + 1 < stop) {
 #pragma unroll
@@ -815,11 +823,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   constexpr bool kApart = kTiles < WAVES;                                // a wave converts a tile's keys or its values
   constexpr int kValues = kTiles * F::KS * 64;                           // where the values begin, in 16 bytes
   constexpr int kStage = kValues + kSteps * F::DT * 64;
+  constexpr int kEarly = W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights
   static_assert(kTiles * (kApart ? 2 : 1) == WAVES * kMine, "every wave has its share of a stage");
   __shared__ u32x4 operands[2 * kStage];
   __shared__ __attribute__((aligned(16))) float scales[2][2][kKeys];     // of keys, of values
   __shared__ float most[2][kTiles];                                      // the largest scale of a tile's values
-  __shared__ int flags[2][kTiles];                                       // a tile's page is there, and (bit 1) a value is not finite
+  __shared__ int flags[2][kTiles];                                       // a tile's page is there, and (bit 1) a drafted value was not finite
   __shared__ int scan[WAVES + 2];
   const int wg = range_of(args, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -881,7 +890,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         flag[t] = place[t].there(src) ? 1 : 0;
         if (my_values && (!flag[t] || pos + 16 > min(context, n))) {
           v[t].drop(there_of(pos, n, flag[t], flag[t], at.g));
-          if constexpr (!F::codes) flag[t] |= pos + 16 > context && __any(v[t].not_finite()) ? 2 : 0;
+          if constexpr (!F::codes) flag[t] |= pos + 16 > context && __any(v[t].clean()) ? 2 : 0;
         }
         if (my_keys) {
 #pragma unroll
@@ -957,14 +966,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       const bool work = !idle && pos < n;
       u32x4 vf[F::DT], p[RT];
       uint32_t seen[RT];
-      bool one_by_one = false;
+      bool not_finite = false;
       if (work) {
         const u32x4* const from = operands + (stage & 1) * kStage + kValues + j * F::DT * 64 + at.lane;
 #pragma unroll
-        for (int d = 0; d < F::DT; ++d) vf[d] = from[d * 64];
+        for (int d = 0; d < kEarly; ++d) vf[d] = from[d * 64];
         const int f0 = __builtin_amdgcn_readfirstlane(flag[0]), f1 = __builtin_amdgcn_readfirstlane(flag[1]);
         const bool masked = pos + 32 > min(context, n) || !(f0 & f1 & 1);
-        one_by_one = ((f0 | f1) & 2) != 0;
+        not_finite = !F::codes && ((f0 | f1) & 2) != 0;
 #pragma unroll
         for (int r = 0; r < RT; ++r) seen[r] = 0xff;
         if (masked) {
@@ -978,25 +987,46 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         convert(stage + 1);
         if (stage + 2 < stages) fetch(stage + 2);
       }
-      if (j == kSteps - 1) __syncthreads();
-      if (work) {
-        __builtin_amdgcn_s_setprio(1);
-        // (behind the last step: what is read is not used)
-        const int next = min(i + 1, steps - 1);
-        if (__builtin_expect(!F::codes && one_by_one, 0)) {
-          add_values_one_by_one<F, RT>(vf, p, seen, at, st);
+      const auto read_values = [&](int from_d) {
+        const u32x4* const from = operands + (stage & 1) * kStage + kValues + j * F::DT * 64 + at.lane;
+#pragma unroll
+        for (int d = 0; d < F::DT / 2; ++d) vf[from_d + d] = from[(from_d + d) * 64];
+      };
+      // (behind the last step: what is read is not used)
+      const int next = min(i + 1, steps - 1);
+      if constexpr (W == 4) {
+        // no registers for both halves of the values, or for keys next to them
+        if (work) {
+          add_values<F, RT, 0, F::DT / 2>(vf, p, st);
+          read_values(F::DT / 2);
+          add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
+        }
+        if (j == kSteps - 1) __syncthreads();
+        if (work) {
           read_keys(next, 0);
           read_keys(next, 1);
           read_scales(next);
-        } else {
-          read_keys(next, 0);
+        }
+      } else {
+        if (kEarly < F::DT && work) read_values(F::DT / 2);                // (before the barrier: the stage's place is written behind it)
+        if (j == kSteps - 1) __syncthreads();
+        if (work) {
+          __builtin_amdgcn_s_setprio(1);
+          if (kEarly == F::DT) read_keys(next, 0);
           __builtin_amdgcn_sched_barrier(0);
           add_values<F, RT, 0, F::DT / 2>(vf, p, st);
           __builtin_amdgcn_sched_barrier(0);
-          read_keys(next, 1);
+          read_keys(next, kEarly == F::DT ? 1 : 0);
           read_scales(next);
           __builtin_amdgcn_sched_barrier(0);
           add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
+          __builtin_amdgcn_sched_barrier(0);
+          if (kEarly < F::DT) read_keys(next, 1);
+        }
+      }
+      if (work) {
+        if constexpr (!F::codes) {
+          if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(src, arguments().D, pos, p, seen, at, st);
         }
         products();
         __builtin_amdgcn_s_setprio(0);
