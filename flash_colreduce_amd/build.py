@@ -33,9 +33,10 @@ HIPCC_FLAGS = [
     "-fno-gpu-rdc",
     # keep packed fp32 VALU forms out of the generated code
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    # the scheduler that favours instruction-level parallelism: the masked row sweep gains 3-4 %, the rest is unchanged
-    "-mllvm", "-amdgpu-sched-strategy=max-ilp",
 ]
+# flags of one source.  The scheduler that favours instruction-level parallelism: in fcr the masked row sweep gains 3-4 %, the rest is
+# unchanged; the kernels of tree_attention that use every register would spill up to 10 more.
+SOURCE_FLAGS = {"fcr": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]}
 
 
 def hipcc_path() -> str:
@@ -58,7 +59,7 @@ def build(verbose: bool = True, extra_flags=(), only=None) -> str:
             if only is not None and name not in only and os.path.exists(obj):
                 continue
             # a part uses a subset of the file's helpers
-            cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, f"-DFCR_PART={part}", "-Wno-unused-function", "-I", INCLUDE,
+            cmd = [hipcc, *HIPCC_FLAGS, *SOURCE_FLAGS.get(name, ()), *extra_flags, f"-DFCR_PART={part}", "-Wno-unused-function", "-I", INCLUDE,
                    "-c", os.path.join(CSRC, name + ".hip"), "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)

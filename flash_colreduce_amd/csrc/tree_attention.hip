@@ -27,6 +27,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 #include "paged.h"
 
 #ifndef FCR_PART
@@ -47,7 +49,7 @@ struct Args {
   int64_t mask_b;
   char* out;                   // [B, H G, T, D]
   float* lse;                  // [B, H G, T] or null
-  int32_t* first;              // [items]: where an item begins, in blocks
+  int32_t* first;              // [4]: blocks of a workgroup; [items][2]: the first workgroup that has a part of an item, blocks of others
   float* part;                 // [2 workgroups][rows of a tile][D + 4]: reference, sum, 2 unused, weighted values
   int B, H, T, D, rows, row_tiles, bf16;
   Div G, per_head, heads, all; // by G, by row_tiles, by H, by wgs
@@ -78,6 +80,7 @@ __device__ __forceinline__ const Args& arguments() {
 }
 
 constexpr int kBlock = 128;                  // keys of a block
+constexpr int kFirst = 4;                    // words in front of the items in Args::first
 constexpr float kNone = -3.0e38f;            // reference of a row that has seen no key
 constexpr float kMostWeight = 0x1p15f;       // weights above this raise the reference, to where the largest is in (1/2, 1]
 constexpr float kMostSum = 0x1p110f;         // and so do sums above this
@@ -492,6 +495,7 @@ struct Queries {
   }
 };
 __device__ __forceinline__ uint32_t largest_of_wave(uint32_t x) {
+#pragma unroll
   for (int o = 1; o < 64; o <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
   return x;
 }
@@ -601,6 +605,7 @@ struct Deal {
       total += round;
     }
     const int per = max((int)a.all.of((uint32_t)(total + a.wgs - 1)), a.least);
+    if (wg == 0 && tid == 0) a.first[0] = per;
     at = wg * per;                                      // (wgs * per is total + wgs at most: checked by the host to fit)
     end = min(at + per, total);
     if (at >= end) return false;
@@ -636,6 +641,12 @@ struct Deal {
   }
   __device__ __forceinline__ int stop() const { return min(nb, blk + (end - at)); }   // blocks [blk, stop) of this item
   __device__ __forceinline__ int item(const Args& a) const { return (b * a.H + h) * a.row_tiles + tile; }
+  // For the join, by the workgroup that has an item's first part.
+  __device__ __forceinline__ void tell(const Args& a, int wg) const {
+    int32_t* const to = a.first + kFirst + 2 * (int64_t)item(a);
+    to[0] = wg;
+    to[1] = nb - (end - at);
+  }
   // To the next piece; false: there is none.
   __device__ __forceinline__ bool next(const Args& a) {
     at += stop() - blk;
@@ -652,8 +663,9 @@ struct Deal {
 // workgroups are dealt to 8 dies in turn: consecutive ranges of blocks, whose row tiles share keys, go to one die
 __device__ __forceinline__ int range_of(const Args& a, int block) { return (block & 7) * (a.wgs >> 3) + (block >> 3); }
 
-template <int CD, int W, int RT>
-__global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kernel(Args args) {
+template <int CD, int W>
+__global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) tree_attention_kernel(Args args) {
+  constexpr int RT = 1;                                 // tiles of 16 rows: two read the cache once for both, but were never faster
   using F = Form<CD, W>;
   constexpr int kWaves = 4;
   __shared__ float joined[kWaves * 4 * F::DT * 64];     // [wave][register][tile][lane]
@@ -668,24 +680,25 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
     const Args& a = arguments();
     const int b = deal.b, h = deal.h, n = deal.n, context = deal.context, stop = deal.stop();
     const int row0 = deal.tile * 16 * RT;
-    Queries<F, RT> q;
-    float by = a.scale2;
-    const uint32_t most = q.load(a, b, h, row0, at);
-    if (F::codes && a.bf16) by = __builtin_amdgcn_ldexpf(by, -q.scale(largest_of_wave(most)));
-    State<F, RT> st;
-    st.clear();
     Keys<F> k[2];
     Values<F> v[2];
     // (places are a block further ahead than the loads, which need them)
     const Source src(a, b, h, n);
     Place here[2], next[2], then[2];
 #pragma unroll
+    for (int t = 0; t < 2; ++t) here[t] = Place(src, deal.blk * kBlock + wave * 32 + 16 * t);
+#pragma unroll
     for (int t = 0; t < 2; ++t) {
-      here[t] = Place(src, deal.blk * kBlock + wave * 32 + 16 * t);
       k[t].load(src, a.D, here[t], at);
       v[t].load(src, a.D, here[t], at);
       next[t] = Place(src, (deal.blk + 1) * kBlock + wave * 32 + 16 * t);
     }
+    Queries<F, RT> q;
+    float by = a.scale2;
+    const uint32_t most = q.load(a, b, h, row0, at);
+    if (F::codes && a.bf16) by = __builtin_amdgcn_ldexpf(by, -q.scale(largest_of_wave(most)));
+    State<F, RT> st;
+    st.clear();
     for (int i = deal.blk; i < stop; ++i) {
       const int pos = i * kBlock + wave * 32;
       if (pos >= n) break;                              // (a wave's later blocks lie behind this one)
@@ -756,7 +769,7 @@ __global__ void __launch_bounds__(256, RT * W <= 2 ? 2 : 1) tree_attention_kerne
     const Args& a_end = arguments();
     const bool final = deal.blk == 0 && stop == deal.nb;
     float* const slot = a_end.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * (16 * RT) * (a_end.D + 4);
-    if (deal.blk == 0 && threadIdx.x == 0) a_end.first[deal.item(a_end)] = deal.at;
+    if (deal.blk == 0 && threadIdx.x == 0) deal.tell(a_end, wg);
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -823,7 +836,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   constexpr bool kApart = kTiles < WAVES;                                // a wave converts a tile's keys or its values
   constexpr int kValues = kTiles * F::KS * 64;                           // where the values begin, in 16 bytes
   constexpr int kStage = kValues + kSteps * F::DT * 64;
-  constexpr int kEarly = W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights
+  // Rows of 256 elements leave no registers for both halves of a step's values, or for keys next to them; 16-bit ones none for a tile's
+  // keys next to its values, which a wave has one or the other of, or for the keys of two tiles (64 rows over 4 x 8 heads of 8192 keys:
+  // 135 us with what then spills, 84 us; where nothing spills 8 % are lost).
+  constexpr bool kLean = W == 4, kTight = kLean && !F::codes;
+  constexpr int kEarly = kTight ? 0 : W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights
   static_assert(kTiles * (kApart ? 2 : 1) == WAVES * kMine, "every wave has its share of a stage");
   __shared__ u32x4 operands[2 * kStage];
   __shared__ __attribute__((aligned(16))) float scales[2][2][kKeys];     // of keys, of values
@@ -838,16 +855,16 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   Deal<64 * WAVES> deal;
   if (!deal.start(arguments(), wg, scan)) return;
   do {
-    const int b = deal.b, h = deal.h, n = deal.n, context = deal.context, stop = deal.stop();
+    const int b = deal.b, n = deal.n, context = deal.context;
     const int row0 = (deal.tile * WAVES + wave) * 16 * RT;
     const bool idle = row0 >= arguments().rows;                                    // (it converts all the same)
     const bool late = WAVES == 8 && wave >= 4;
     Keys<F> k[kMine];
-    Values<F> v[kMine];
-    const Source src(arguments(), b, h, n);
+    Values<F> v[kMine];                                                  // (tight: of keys too, in the same registers)
+    const Source src(arguments(), b, deal.h, n);
     Place place[kMine], ahead[kMine];                                    // of the rows loaded last, and of the next ones
     const int pos0 = deal.blk * kBlock;
-    const int steps = (stop - deal.blk) * (kBlock / 32), stages = steps / kSteps;
+    const int steps = (deal.stop() - deal.blk) * (kBlock / 32), stages = steps / kSteps;
     const auto look = [&](int stage) {
 #pragma unroll
       for (int t = 0; t < kMine; ++t) ahead[t] = Place(src, pos0 + stage * kKeys + (my_tile + t) * 16);
@@ -858,7 +875,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
       for (int t = 0; t < kMine; ++t) {
         place[t] = ahead[t];
-        if (my_keys) k[t].load(src, D, place[t], here);
+        if (kTight || my_keys) k[t].load(src, D, place[t], here);
+        if constexpr (kTight) v[t] = __builtin_bit_cast(Values<F>, k[t]);
         if (my_values) v[t].load(src, D, place[t], here);
       }
       look(stage + 1);
@@ -867,7 +885,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
     fetch(0);
     Queries<F, RT> q;
     float by = arguments().scale2;
-    uint32_t largest = q.load(arguments(), b, h, row0, at);
+    uint32_t largest = q.load(arguments(), b, deal.h, row0, at);
     __syncthreads();                                                     // (the piece before has been used)
     if (F::codes && arguments().bf16) {
       // one power of two for all rows of the workgroup, which the keys' scales undo
@@ -893,6 +911,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
           if constexpr (!F::codes) flag[t] |= pos + 16 > context && __any(v[t].clean()) ? 2 : 0;
         }
         if (my_keys) {
+          if constexpr (kTight) k[t] = __builtin_bit_cast(Keys<F>, v[t]);
 #pragma unroll
           for (int c = 0; c < F::KS; ++c) to[((my_tile + t) * F::KS + c) * 64] = k[t].operand(c);
           if (F::codes && at.col == 0) *reinterpret_cast<f32x4*>(sc + (my_tile + t) * 16 + 4 * at.g) = k[t].scale * by;
@@ -944,13 +963,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       }
       if constexpr (F::codes) most_v = fmaxf(most[buffer][2 * j], most[buffer][2 * j + 1]);
     };
-    const auto products = [&] {                                          // of the keys read last with the queries
+    const auto products_of = [&](int t) {                                // of the keys read last with the queries
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int c = 0; c < F::KS; ++c)
 #pragma unroll
-        for (int c = 0; c < F::KS; ++c)
-#pragma unroll
-          for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(kf[t][c], q.w[r][c], c ? s[r][t] : f32x4{0, 0, 0, 0});
+        for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(kf[t][c], q.w[r][c], c ? s[r][t] : f32x4{0, 0, 0, 0});
     };
     convert(0);
     if (stages > 1) fetch(1);
@@ -959,7 +976,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       read_keys(0, 0);
       read_keys(0, 1);
       read_scales(0);
-      products();
+      products_of(0);
+      products_of(1);
     }
     for (int i = 0; i < steps; ++i) {
       const int stage = i / kSteps, j = i % kSteps, pos = pos0 + i * 32;
@@ -994,18 +1012,22 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       };
       // (behind the last step: what is read is not used)
       const int next = min(i + 1, steps - 1);
-      if constexpr (W == 4) {
-        // no registers for both halves of the values, or for keys next to them
+      if constexpr (kLean) {
         if (work) {
+          if (kEarly == 0) read_values(0);
           add_values<F, RT, 0, F::DT / 2>(vf, p, st);
           read_values(F::DT / 2);
           add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
         }
         if (j == kSteps - 1) __syncthreads();
         if (work) {
-          read_keys(next, 0);
-          read_keys(next, 1);
           read_scales(next);
+          read_keys(next, 0);
+          if (kTight) {
+            products_of(0);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          read_keys(next, 1);
         }
       } else {
         if (kEarly < F::DT && work) read_values(F::DT / 2);                // (before the barrier: the stage's place is written behind it)
@@ -1028,21 +1050,22 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         if constexpr (!F::codes) {
           if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(src, arguments().D, pos, p, seen, at, st);
         }
-        products();
+        if (!kTight) products_of(0);
+        products_of(1);
         __builtin_amdgcn_s_setprio(0);
       }
     }
     const Args& a = arguments();
-    const bool final = deal.blk == 0 && stop == deal.nb;
+    const bool final = deal.blk == 0 && deal.stop() == deal.nb;
     float* const slot = a.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * (16 * RT * WAVES) * (a.D + 4);
-    if (deal.blk == 0 && threadIdx.x == 0) a.first[deal.item(a)] = deal.at;
+    if (deal.blk == 0 && threadIdx.x == 0) deal.tell(a, wg);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const float l = across(st.l[r], false);
       const int row = row0 + 16 * r + at.col;
       if (row >= a.rows) continue;
       if (final) {
-        const Output out(a, b, h, row, l);
+        const Output out(a, b, deal.h, row, l);
         const float inverse = 1.0f / l;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1068,59 +1091,64 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 }
 
 #if FCR_HAS(0)
-// Joins the parts of items that were cut, in the order of their keys: a thread per four elements of a row.
-__global__ void __launch_bounds__(256) tree_join_kernel(Args a, int tile_rows, int groups) {
-  const int item = blockIdx.x / groups;
-  const int tile = item % a.row_tiles, bh = item / a.row_tiles;
-  const int b = bh / a.H, h = bh - b * a.H;
-  // how many blocks a workgroup took, as the first kernel found it
-  __shared__ int scan[4];
-  const bool by_head = a.context.sh != 0;
-  const int entries = by_head ? a.B * a.H : a.B;
-  const int weight = by_head ? a.row_tiles : a.H * a.row_tiles;
-  int total = 0, context, n;
-  for (int e = threadIdx.x; e < entries; e += 256) {
-    keys_of(a, by_head ? e / a.H : e, by_head ? e % a.H : 0, context, n);
-    total += blocks_of(n) * weight;
-  }
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-  if ((threadIdx.x & 63) == 0) scan[threadIdx.x >> 6] = total;
-  __syncthreads();
-  total = scan[0] + scan[1] + scan[2] + scan[3];
-  const int per = max((int)a.all.of((uint32_t)(total + a.wgs - 1)), a.least);
-  keys_of(a, b, h, context, n);
-  const int begin = a.first[item];
-  const int from = begin / per, to = (begin + blocks_of(n) - 1) / per;
-  if (from == to) return;
-  const int pieces = a.D / 4;
+// Joins the parts of items that were cut, in the order of their keys.  Units are four elements of a row; a unit has `shares` threads, a
+// power of two that take the parts in turn and meet in LDS: an item of few rows may have a part in every workgroup of the first kernel.
+__global__ void __launch_bounds__(256) tree_join_kernel(Args a, int tile_rows, int shares, Div groups, Div pieces) {
+  __shared__ f32x4 sums[256];
+  __shared__ float stats[256][2];
+  const int item = (int)groups.of(blockIdx.x);
+  const int32_t* const told = a.first + kFirst + 2 * (int64_t)item;
+  const int per = constant_at(a.first), from = constant_at(told), others = constant_at(told + 1);
+  if (others <= 0) return;
+  // workgroups behind the first (no more than there are, should lengths have changed under the call)
+  const int more = min((int)(((uint32_t)others + (uint32_t)per - 1) / (uint32_t)per), a.wgs - 1 - from);
+  const int bh = (int)a.per_head.of((uint32_t)item), tile = item - bh * a.row_tiles;
   const int rows = min(tile_rows, a.rows - tile * tile_rows);
-  const int64_t stride = a.D + 4, part = (int64_t)tile_rows * stride;
-  const float* const parts = a.part + 2 * part * from + part;       // the first part; the next ones are from the others' first slots
-  for (int i = (blockIdx.x % groups) * 256 + threadIdx.x; i < rows * pieces; i += 256 * groups) {
-    const int r = i / pieces, d = 4 * (i - r * pieces);
+  const int units = 256 / shares, mine = (int)threadIdx.x / units;
+  for (uint32_t group = blockIdx.x - (uint32_t)item * groups.d; group * units < (uint32_t)rows * pieces.d; group += groups.d) {
+    const int unit = (int)group * units + ((int)threadIdx.x & (units - 1));
+    const int r = (int)pieces.of((uint32_t)unit), d = 4 * (unit - r * (int)pieces.d);
+    const bool live = r < rows;
+    const int64_t stride = a.D + 4, part = (int64_t)tile_rows * stride;
+    // the first part is in its workgroup's second slot, the others are in their workgroups' first ones
+    const float* const parts = a.part + 2 * part * from + (live ? r : 0) * stride;
     float m = kNone, l = 0.0f;
     f32x4 x = {0, 0, 0, 0};
-    const float* at_part = parts + r * stride;
-    for (int w = from; w <= to; ++w) {
-      const float pm = at_part[0], pl = at_part[1];
-      const f32x4 y = *reinterpret_cast<const f32x4*>(at_part + 4 + d);
+    const auto take = [&](float pm, float pl, f32x4 y) {
       const float top = fmaxf(m, pm);
-      const float mine = __builtin_amdgcn_exp2f(m - top), its = __builtin_amdgcn_exp2f(pm - top);
-      l = l * mine + pl * its;
-      x = x * mine + y * its;
-      m = top;
-      at_part += w == from ? part : 2 * part;
-    }
-    const int row = tile * tile_rows + r;
-    const int t = (int)a.G.of((uint32_t)row), head = row - t * (int)a.G.d;
-    const bool none = (a.tree_lengths && t >= a.tree_lengths[b]) || l == 0.0f;
-    const float inverse = 1.0f / l;
-    const int64_t at = (((int64_t)b * a.H + h) * a.G.d + head) * a.T + t;
+      const float old = __builtin_amdgcn_exp2f(m - top), its = __builtin_amdgcn_exp2f(pm - top);
+      l = l * old + pl * its;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = none ? 0.0f : x[j] * inverse;
-    *reinterpret_cast<u32x2*>(a.out + (at * a.D + d) * 2) = a.bf16 ? u32x2{pack2<FCR_DTYPE_BF16>(x[0], x[1]), pack2<FCR_DTYPE_BF16>(x[2], x[3])}
-                                                                  : u32x2{pack2<FCR_DTYPE_F16>(x[0], x[1]), pack2<FCR_DTYPE_F16>(x[2], x[3])};
-    if (a.lse && d == 0) a.lse[at] = none ? -INFINITY : m + __builtin_amdgcn_logf(l);
+      for (int j = 0; j < 4; ++j) x[j] = x[j] * old + y[j] * its;
+      m = top;
+    };
+    if (live) {
+      for (int w = mine; w <= more; w += shares) {
+        const float* const p = parts + (w == 0 ? part : 2 * part * w);
+        take(p[0], p[1], *reinterpret_cast<const f32x4*>(p + 4 + d));
+      }
+    }
+    if (shares > 1) {
+      __syncthreads();     // (of the units before)
+      sums[threadIdx.x] = x;
+      stats[threadIdx.x][0] = m, stats[threadIdx.x][1] = l;
+      __syncthreads();
+      if (mine == 0 && live) {
+        for (int i = 1; i < shares && i <= more; ++i) {
+          const int other = threadIdx.x + units * i;
+          take(stats[other][0], stats[other][1], sums[other]);
+        }
+      }
+    }
+    if (mine != 0 || !live) continue;
+    const int b = (int)a.heads.of((uint32_t)bh), h = bh - b * a.H;
+    const Output out(a, b, h, tile * tile_rows + r, l);
+    const float inverse = 1.0f / l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = out.none ? 0.0f : x[j] * inverse;
+    *reinterpret_cast<u32x2*>(a.out + (out.row * a.D + d) * 2) = a.bf16 ? u32x2{pack2<FCR_DTYPE_BF16>(x[0], x[1]), pack2<FCR_DTYPE_BF16>(x[2], x[3])}
+                                                                       : u32x2{pack2<FCR_DTYPE_F16>(x[0], x[1]), pack2<FCR_DTYPE_F16>(x[2], x[3])};
+    if (a.lse && d == 0) a.lse[out.row] = out.none ? -INFINITY : m + __builtin_amdgcn_logf(l);
   }
 }
 #endif
@@ -1129,10 +1157,7 @@ template <int CD, int W>
 void launch_w(const Args& a, int form, hipStream_t s) {
   const dim3 grid((unsigned)a.wgs);
   switch (form) {
-    case 1: hipLaunchKernelGGL((tree_attention_kernel<CD, W, 1>), grid, dim3(256), 0, s, a); break;
-    case 2:
-      if constexpr (W <= 2) hipLaunchKernelGGL((tree_attention_kernel<CD, W, 2>), grid, dim3(256), 0, s, a);
-      break;
+    case 1: hipLaunchKernelGGL((tree_attention_kernel<CD, W>), grid, dim3(256), 0, s, a); break;
     case 4:
       if constexpr (W <= 2) hipLaunchKernelGGL((tall_attention_kernel<CD, W, 4>), grid, dim3(256), 0, s, a);
       break;
@@ -1169,26 +1194,29 @@ using fcr_detail::fail;
 using fcr_detail::launched;
 
 struct Plan {
-  int form;                  // 1, 2: tree_attention_kernel of as many column tiles; 4, 8: tall_attention_kernel of as many waves
+  int form;                  // 1: tree_attention_kernel; 4, 8: tall_attention_kernel of as many waves
   int tile_rows, row_tiles, wgs, least;
   int64_t items, first_bytes, bytes;
 };
 // What depends on sizes alone.  false: too large.
-bool plan_of(int B, int H, int G, int T, int D, int64_t capacity, Plan& p) {
+bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Plan& p) {
   const int64_t rows = (int64_t)T * G;
   const int w = (D + 63) / 64, tall = 16 * tall_tiles(w);
-  p.form = rows <= 16 ? 1 : rows <= 32 && w <= 2 ? 2 : rows <= 4 * tall && w <= 2 ? 4 : 8;
-  p.tile_rows = p.form <= 2 ? 16 * p.form : tall * p.form;
+  // Both sides, us, at 4 sequences x 8 heads x 8192 keys, int8 (bf16): 48 rows of 64 elements 31 (30) by form 1, 36 (33) by form 4, 64 rows 39
+  // (44) and 36 (33); of 128 elements 41 (43) and 46 (45), 52 (87) and 47 (47); 48 rows of 256 elements 58 (88) by form 1, 67 (76) by form 8, 64
+  // rows 95 (167) and 71 (84); 128 rows of 128 elements 58 (57) by form 4, 60 (64) by form 8, 192 rows 77 (79) and 72 (74).
+  p.form = rows <= (w <= 2 || codes ? 48 : 16) ? 1 : rows <= 4 * tall && w <= 2 ? 4 : 8;
+  p.tile_rows = p.form == 1 ? 16 : tall * p.form;
   const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.items = (int64_t)B * H * tiles;
   const int64_t blocks = p.items * ((capacity + kBlock - 1) / kBlock);
-  if (rows > (1 << 24) || p.items > (1 << 24) || blocks > (1 << 30)) return false;
+  if (rows > (1 << 24) || p.items > (1 << 22) || blocks > (1 << 30)) return false;
   p.row_tiles = (int)tiles;
   int64_t wgs = (p.form == 8 ? 1 : 2) * (int64_t)fcr_detail::chip_cus_of_current_device();
   if (blocks < wgs) wgs = blocks;
   p.wgs = (int)((wgs + 7) / 8 * 8);
   p.least = 1;
-  p.first_bytes = (p.items * 4 + 15) / 16 * 16;
+  p.first_bytes = (kFirst * 4 + p.items * 8 + 15) / 16 * 16;
   p.bytes = p.first_bytes + 2ll * p.wgs * p.tile_rows * (D + 4) * 4;
   return true;
 }
@@ -1197,9 +1225,9 @@ bool plan_of(int B, int H, int G, int T, int D, int64_t capacity, Plan& p) {
 extern "C" {
 
 size_t fcr_tree_attention_bytes(int B, int H, int G, int T, int D, int64_t positions) {
-  Plan p;
+  Plan p[2];             // for either kind of cache
   if (B < 1 || H < 1 || G < 1 || T < 1 || D < 16 || D > 256 || positions < 1 || positions > (1 << 30) || (int64_t)B * H > (1 << 24)) return 0;
-  return plan_of(B, H, G, T, D, positions, p) ? (size_t)p.bytes : 0;
+  return plan_of(true, B, H, G, T, D, positions, p[0]) && plan_of(false, B, H, G, T, D, positions, p[1]) ? (size_t)std::max(p[0].bytes, p[1].bytes) : 0;
 }
 
 int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages,
@@ -1216,7 +1244,8 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
   const int64_t capacity = (int64_t)table_pages * cache->page_size;
   Plan plan;
   if (mask && T > 46340) return fail(FCR_E_SHAPE, "a mask of more than 2^31 bytes");
-  if (G < 1 || T < 1 || T > (1 << 24) || G > (1 << 24) || (int64_t)B * H > (1 << 24) || (int64_t)H * G > (1 << 24) || !plan_of(B, H, G, T, D, capacity, plan))
+  if (G < 1 || T < 1 || T > (1 << 24) || G > (1 << 24) || (int64_t)B * H > (1 << 24) || (int64_t)H * G > (1 << 24) || 
+      !plan_of(has_codes(cache->dtype), B, H, G, T, D, capacity, plan))
     return fail(FCR_E_SHAPE, "G and T must be >= 1; B, H, G, T and the table are too large for one call otherwise");
   if (!isfinite(scale)) return fail(FCR_E_SCALE, "scale must be finite");
   bool ok = q_strides[3] == 1 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
@@ -1253,9 +1282,12 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
     default: attention_e4m3(a, w, plan.form, s); break;
   }
   if ((rc = launched("tree_attention_kernel"))) return rc;
-  const int pieces = (plan.tile_rows < a.rows ? plan.tile_rows : a.rows) * (D / 4);
-  const int groups = (pieces + 255) / 256;
-  hipLaunchKernelGGL(tree_join_kernel, dim3((unsigned)(plan.items * groups)), dim3(256), 0, s, a, plan.tile_rows, groups);
+  Div groups, pieces;
+  const int rows = std::min(plan.tile_rows, a.rows), shares = plan.wgs >= 16 * plan.items ? 8 : 1, units = 256 / shares;
+  const int64_t most = (1 << 22) / plan.items;
+  pieces.set((uint32_t)D / 4);
+  groups.set((uint32_t)std::max<int64_t>(1, std::min<int64_t>(most, (rows * (D / 4) + units - 1) / units)));
+  hipLaunchKernelGGL(tree_join_kernel, dim3((unsigned)(plan.items * groups.d)), dim3(256), 0, s, a, plan.tile_rows, shares, groups, pieces);
   return launched("tree_join_kernel");
 }
 
