@@ -128,6 +128,8 @@ class _PythonOnly:
     def keep(*args):
         return None
 
+    cache_write = cache_read = cache_keep = tree_attention = keep
+
 
 def host():
     """The module of csrc/host.cpp (the usual call in native code), its errors raised by check().

@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import _lib
+from . import _lib, flash
 from .flash import _DTYPES, _raw_stream
 
 __all__ = ["KVCache", "cache_write", "cache_read", "cache_keep", "tree_attention"]
@@ -62,6 +62,11 @@ class _Cache(ctypes.Structure):   # fcr_cache
                 ("D", ctypes.c_int)]
 
 
+def _host():
+    """csrc/host.cpp: answers the calls that need neither a copy nor a message, and None to all others."""
+    return flash._native or flash._host()
+
+
 _I64x2 = ctypes.c_int64 * 2
 _I64x3 = ctypes.c_int64 * 3
 
@@ -74,7 +79,9 @@ def _check_cache(cache: KVCache, name: str = "cache") -> torch.device:
         raise ValueError(f"The {name}'s keys and values must be (pages, heads, page_size, D) of one float16, bfloat16, int8 or "
                          f"float8_e4m3fn type on one device. Got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}.")
     pages, heads, page_size, d = k.shape
-    if pages < 1 or heads < 1 or page_size < 16 or page_size % 16 or d < 16 or d > 256 or d % 16:
+    if k.stride(3) != 1 or cache.v.stride(3) != 1:
+        raise ValueError(f"The elements of a row of the {name} must be consecutive.")
+    if max(k.shape) >= 2**31 or pages < 1 or heads < 1 or page_size < 16 or page_size % 16 or d < 16 or d > 256 or d % 16:
         raise ValueError(f"The {name} needs pages of a multiple of 16 rows, and D a multiple of 16 up to 256. Got {tuple(k.shape)}.")
     for x in (cache.k_scale, cache.v_scale):
         if k.dtype in _CODES:
@@ -131,6 +138,8 @@ def cache_write(cache: KVCache, key: torch.Tensor, value: torch.Tensor, table: t
     codes.  table is int32 (B, pages per sequence); start and counts are int32 (B,), or (B, H) where the heads of a
     sequence differ in length.  With counts only the first counts[b] tokens are written.  Positions outside the table, or on a page
     that is not there, are skipped.  No row may be the place of two tokens (a page shared between sequences must not be written)."""
+    if _host().cache_write(cache, key, value, table, start, counts):
+        return
     dev = _check_cache(cache)
     h, d = cache.k.shape[1], cache.k.shape[3]
     if key.dim() != 4 or key.shape != value.shape or key.shape[1] != h or key.shape[3] != d or key.device != dev or value.device != dev:
@@ -156,6 +165,9 @@ def cache_read(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, n: in
     """Positions 0 .. n-1 of every sequence and head as (key, value), each a contiguous (B, H, n, D) of out_dtype (fp16, bf16 or fp32; by
     default the cache's type, bf16 for codes), the form that flash_colreduce takes.  A code times its scale is formed in fp32 and rounded
     once.  Rows from lengths[b] (or lengths[b, h]) on are zeros."""
+    kv = _host().cache_read(cache, table, lengths, n, out_dtype)
+    if kv is not None:
+        return kv
     dev = _check_cache(cache)
     _, h, _, d = cache.k.shape
     b = table.shape[0] if table.dim() == 2 else -1
@@ -187,6 +199,9 @@ def cache_keep(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, keep:
     keep is bool (B, H, N), as topk_keep_mask gives it for the scores of flash_colreduce; positions from lengths on, and those on a page
     that is not there, are not kept.  `into` has the cache's type, heads and D, and may be the same cache; into_table must name no page
     that `table` names.  What does not fit into_table is dropped; rows behind the kept ones are left as they were."""
+    counts = _host().cache_keep(cache, table, lengths, keep, into, into_table)
+    if counts is not None:
+        return counts
     dev = _check_cache(cache)
     if _check_cache(into, "cache to keep rows in") != dev:
         raise ValueError("Both caches must be on the same device.")
@@ -234,6 +249,9 @@ def tree_attention(query: torch.Tensor, cache: KVCache, table: torch.Tensor, con
     Returns (B, Hq, T, D) of query's type, and with return_lse2 the base-2 log-sum-exp of every row's scores, fp32 (B, Hq, T), as row_lse2 has it.
     A row that sees nothing (or that the sequence does not have) is zeros, its log-sum-exp -inf.  What hidden rows of the cache hold, NaNs included,
     has no influence."""
+    out = _host().tree_attention(query, cache, table, context, tree_mask, scale, tree_lengths, return_lse2)
+    if out is not None:
+        return out
     dev = _check_cache(cache)
     _, h, page_size, d = cache.k.shape
     if query.dim() != 4 or query.shape[3] != d or query.shape[1] % h or query.shape[1] == 0 or query.device != dev:

@@ -158,6 +158,23 @@ def test_workspace_size_of_tree_attention():
     assert 0 < lib.fcr_tree_attention_bytes(1, 8, 4, 1, 128, 1000) <= lib.fcr_tree_attention_bytes(64, 8, 4, 1, 128, 1000)
 
 
+def test_native_host_path_leaves_the_rest_to_python():
+    """Tensors on the host, other objects, wrong counts of arguments."""
+    host, x = cache_module._host(), torch.zeros(1, 1, 1, 16)
+    cache, ints = KVCache(x, x), torch.zeros(1, 1, dtype=torch.int32)
+    assert host.cache_write(cache, x, x, ints, ints[0], None) is None and host.cache_read(None, ints, ints[0], 1, None) is None
+    assert host.cache_keep(cache, ints, ints[0], x, (), ints) is None and host.cache_read((1, 2, 3, 4), ints, ints[0], 1, None) is None
+    assert host.tree_attention(x, cache, ints, ints[0], None, None, None, False) is None
+    if host is not _lib._PythonOnly:
+        for f in (host.cache_write, host.cache_read, host.cache_keep, host.tree_attention):
+            with pytest.raises(TypeError):
+                f(cache)
+
+
+def test_masks_past_32_bits_are_refused_without_a_device():
+    assert _c_call("attention", _c_cache(), mask=16, T=46341, G=1) == -3
+
+
 def test_python_refuses_without_a_device():
     c = KVCache.zeros(2, 1, 16, 16, I8, device="cpu")
     i = torch.zeros(1, 1, dtype=torch.int32)
@@ -506,6 +523,28 @@ def test_attention_matches_64_bits(shape, kind, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("shape", [  # more rows than one tile of every kernel has, and rows either side of where another kernel takes over
+    (2, 1, 5, 55, 300, 64, 16), (1, 2, 7, 80, 333, 128, 32), (1, 1, 3, 91, 250, 192, 16), (2, 1, 2, 77, 170, 256, 16), (1, 1, 1, 48, 200, 64, 16),
+    (1, 2, 7, 7, 200, 128, 16), (1, 1, 1, 129, 150, 96, 16), (1, 2, 4, 4, 300, 176, 16), (3, 1, 17, 1, 210, 256, 16), (1, 1, 128, 1, 100, 32, 16)])
+def test_attention_of_many_rows(shape, kind, dtype):
+    query, cache, table, context = problem(*shape, kind, dtype)
+    check_attention(query, cache, table, context, random_tree(shape[0], shape[3], 3) if shape[3] % 2 else None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [(BF16, BF16), (I8, F16)])
+@pytest.mark.parametrize("b,h,t,g", [(700, 2, 1, 2), (530, 1, 33, 2)])
+def test_attention_of_more_sequences_than_threads(kind, dtype, b, h, t, g):
+    """Lengths per sequence and per head, among them zeros, for more of them than a workgroup has threads."""
+    query, cache, table, context = problem(b, h, g, t, 20, 32, 16, kind, dtype)
+    check_attention(query, cache, table, context)
+    heads = torch.randint(0, 21, (b, h), generator=torch.Generator().manual_seed(9)).int()
+    heads[1], heads[-1] = 0, 20
+    check_attention(query, cache, table, heads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", KINDS)
 def test_attention_of_a_chain_a_shared_mask_and_any_mask(kind, dtype):
     """The same drafted tokens with no mask, one mask for all sequences, and masks that hide tokens from themselves; heads of own lengths."""
     b, h, g, t, n, d = 3, 2, 2, 9, 150, 64
@@ -766,6 +805,56 @@ def test_prune_then_decode(kind):
     # the rows behind are the ones that the mask named
     pk, pv = fca.cache_read(pruned, pruned_table, counts, kept)
     assert torch.equal(pk, k[keep].view(b, h, kept, d)) and torch.equal(pv, v[keep].view(b, h, kept, d))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F16, BF16, I8, E4M3])
+def test_native_host_path_gives_what_the_general_one_gives(kind, monkeypatch):
+    """The native path answers the usual calls, leaves the others to Python, and both run the same kernels."""
+    b, h, g, t, n, d = 2, 3, 2, 5, 150, 64
+    dtype = kind if kind in (F16, BF16) else BF16
+    query, cache, table, context = problem(b, h, g, t, n, d, 16, kind, dtype)
+    query, cache, table, context = query.cuda(), device(cache), table.cuda(), context.cuda()
+    by_head = context[:, None].repeat(1, h)
+    x = randn(b, h, t, d, seed=9, dtype=dtype).cuda()
+    mask, lengths = random_tree(b, t, 3).cuda(), torch.tensor([t, 2], dtype=torch.int32, device="cuda")
+    keep = torch.rand((b, h, n), generator=torch.Generator().manual_seed(3)).cuda() < 0.3
+    into_table = torch.arange(table.numel(), device="cuda").view(b, -1).int()
+
+    def run():
+        into = KVCache.zeros(cache.k.shape[0], h, 16, d, kind)
+        fca.cache_write(cache, x, x, table, context)
+        got = [fca.tree_attention(query, cache, table, context), *fca.tree_attention(query, cache, table, by_head, mask, 0.3, return_lse2=True),
+               fca.tree_attention(query, cache, table, context, mask[0], tree_lengths=lengths), fca.cache_keep(cache, table, by_head, keep, into, into_table),
+               *fca.cache_read(cache, table, context, n), *fca.cache_read(cache, table, by_head, n + 7, out_dtype=F32), *into]
+        fca.cache_write(cache, x * 2, x, table, by_head, counts=lengths)
+        got += fca.cache_read(cache, table, context + t, n + t)
+        # what the native path leaves to Python
+        strided = x.transpose(2, 3).contiguous().transpose(2, 3)
+        fca.cache_write(cache, strided, x, table, context)
+        got += [fca.tree_attention(query, cache, table, context, mask.transpose(1, 2).contiguous().transpose(1, 2), 1),
+                fca.cache_keep(cache, table, context, keep.transpose(0, 1).contiguous().transpose(0, 1), into, into_table)]
+        return [None if y is None else y.float() if y.dtype == E4M3 else y for y in got]
+
+    native = run()
+    host = cache_module._host()
+    assert host.cache_write(cache, x, x, table, context, None) is True and host.cache_read(cache, table, context, n, None) is not None
+    assert host.tree_attention(query, cache, table, context, None, None, None, False) is not None
+    assert host.cache_keep(cache, table, context, keep, KVCache.zeros(cache.k.shape[0], h, 16, d, kind), into_table) is not None
+    assert host.tree_attention(query, cache, table, context, None, 1, None, False) is None
+    monkeypatch.setattr(cache_module.flash, "_native", _lib._PythonOnly)
+    for a, z in zip(run(), native):
+        assert (a is None and z is None) or torch.equal(a, z)
+
+
+@pytest.mark.gpu
+def test_rows_whose_elements_are_apart_are_refused():
+    cache = KVCache.zeros(4, 2, 16, 32, BF16)
+    apart = KVCache(cache.k.transpose(2, 3).contiguous().transpose(2, 3), cache.v)
+    table, lengths = torch.arange(4, device="cuda").view(2, 2).int(), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for bad in (apart, KVCache(apart[1], apart[0])):
+        with pytest.raises(ValueError, match="consecutive"):
+            fca.cache_read(bad, table, lengths, 3)
 
 
 @pytest.mark.gpu
