@@ -216,42 +216,49 @@ struct KeepArgs {
   Lengths lengths;
   const uint8_t* keep;   // [B, H, N]
   int32_t* counts;       // [B, H]
-  int N, chunk, chunks, row_bytes;
+  int N, chunk;
+  Div chunks, H, pieces; // by chunks of N, by heads, by 16-byte pieces of a row
 };
 
-// How many of the 16 rows from `first` on stay, as a mask: kept, shorter than the length, and on a page that is there.  The rows lie in
-// one page (`first` and the page size are multiples of 16).
-__device__ __forceinline__ uint32_t kept16(const KeepArgs& p, const uint8_t* keep, int b, int first, int n) {
-  if (first >= n) return 0;
-  uint32_t row;
-  if (page_of(p.c, b, (uint32_t)first, row) < 0) return 0;
+// 16 bytes of a mask as 16 bits.
+__device__ __forceinline__ uint32_t bits_of(const uint8_t* at) {
+  u32x4 w;
+  __builtin_memcpy(&w, at, 16);   // (any alignment)
   uint32_t bits = 0;
-  if (first + 16 <= n) {
-    u32x4 w;
-    __builtin_memcpy(&w, keep + first, 16);   // (any alignment)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // any bit of a byte, moved to its lowest; then the four of them side by side
-      uint32_t v = w[i];
-      v |= v >> 4, v |= v >> 2, v |= v >> 1;
-      v &= 0x01010101u;
-      bits |= ((v * 0x01020408u) >> 24) << (4 * i);
-    }
-  } else {
-    for (int i = 0; i < 16 && first + i < n; ++i) bits |= (keep[first + i] != 0 ? 1u : 0u) << i;
+  for (int i = 0; i < 4; ++i) {
+    // any bit of a byte, moved to its lowest; then the four of them side by side
+    uint32_t v = w[i];
+    v |= v >> 4, v |= v >> 2, v |= v >> 1;
+    v &= 0x01010101u;
+    bits |= ((v * 0x01020408u) >> 24) << (4 * i);
   }
   return bits;
 }
+// Which of the 16 rows from `first` on stay: kept, shorter than the length, and on a page that is there.  The rows lie in one page (`first`
+// and the page size are multiples of 16).
+__device__ __forceinline__ uint32_t kept16(const KeepArgs& p, const uint8_t* keep, int b, int first, int n, int& page, uint32_t& row) {
+  page = -1, row = 0;
+  if (first >= n) return 0;
+  page = page_of(p.c, b, (uint32_t)first, row);
+  uint32_t bits = 0;
+  if (first + 16 <= n) {
+    bits = bits_of(keep + first);
+  } else {
+    for (int i = 0; first + i < n; ++i) bits |= (keep[first + i] != 0 ? 1u : 0u) << i;
+  }
+  return page < 0 ? 0 : bits;
+}
 
 // A workgroup takes `chunk` rows of one (batch, head): it counts the kept rows in front of them (the mask is read again by every
-// chunk, at a byte per row next to the 2 D bytes of a kept one), lists its own, and copies them, codes and scales as they are.
-constexpr int kKeepRows = 2048;   // rows listed at once
+// chunk, at a byte per row next to the 2 D bytes of a kept one), lists where its own lie and go, and copies them, codes and scales as they are.
+constexpr int kKeepRows = 512;   // rows listed at once
 
 __global__ void __launch_bounds__(kThreads) cache_keep_kernel(KeepArgs p) {
   __shared__ int counted[kThreads / 64];
-  __shared__ int list[kKeepRows];
-  const int bh = blockIdx.x / p.chunks, part = blockIdx.x - bh * p.chunks;
-  const int b = bh / p.c.H, h = bh - b * p.c.H;
+  __shared__ int4 list[kKeepRows];         // page and row, from and to; a page to go to below 0: none
+  const int bh = (int)p.chunks.of(blockIdx.x), part = blockIdx.x - bh * p.chunks.d;
+  const int b = (int)p.H.of((uint32_t)bh), h = bh - b * p.H.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int n = p.lengths.of(b, h);
   n = min(n, p.N);
@@ -259,18 +266,25 @@ __global__ void __launch_bounds__(kThreads) cache_keep_kernel(KeepArgs p) {
   const uint8_t* keep = p.keep + (int64_t)bh * p.N;
   const int begin = part * p.chunk, end = min(begin + p.chunk, n);
 
-  int before = 0;
-  for (int i = tid * 16; i < begin; i += kThreads * 16) before += __popc(kept16(p, keep, b, i, n));
+  int before = 0, page;
+  uint32_t row;
+  const int whole = min(begin, max(n, 0) & ~15);
+#pragma unroll 4
+  for (int i = tid * 16; i < whole; i += kThreads * 16) {
+    const uint32_t bits = bits_of(keep + i);
+    before += page_of(p.c, b, (uint32_t)i, row) < 0 ? 0 : __popc(bits);
+  }
+  if (tid == 0 && whole < begin) before += __popc(kept16(p, keep, b, whole, n, page, row));
   for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
   if (lane == 0) counted[wave] = before;
   __syncthreads();
   int at = counted[0] + counted[1] + counted[2] + counted[3];
 
-  const int pieces = p.row_bytes / 16;    // 16-byte pieces of a row
   for (int first = begin; first < end; first += kKeepRows) {
     // rows of this round: at most 16 per thread for the first kKeepRows / 16 threads
     __syncthreads();
-    uint32_t bits = tid < kKeepRows / 16 && first + tid * 16 < end ? kept16(p, keep, b, first + tid * 16, n) : 0;
+    const int mine0 = first + tid * 16;
+    uint32_t bits = tid < kKeepRows / 16 && mine0 < end ? kept16(p, keep, b, mine0, n, page, row) : 0;
     int mine = __popc(bits), sum = mine;
     for (int o = 1; o < 64; o <<= 1) {
       const int v = __shfl_up(sum, o);
@@ -284,34 +298,36 @@ __global__ void __launch_bounds__(kThreads) cache_keep_kernel(KeepArgs p) {
     while (bits) {
       const int i = __ffs(bits) - 1;
       bits &= bits - 1;
-      list[place++] = first + tid * 16 + i;
+      list[place++] = int4{page, (int)row + i, -1, 0};
     }
     __syncthreads();
-    // pieces of keys and values, then scales
-    for (int which = 0; which < 2; ++which) {
-      const Side s = p.c.side[which], d = p.into.side[which];
-      for (int i = tid; i < total * pieces; i += kThreads) {
-        const int k = i / pieces, piece = i - k * pieces;
-        if (at + k >= p.into.capacity) break;
-        uint32_t from_row, to_row;
-        const int from = page_of(p.c, b, list[k], from_row), to = page_of(p.into, b, at + k, to_row);
-        if (to < 0) continue;
-        *reinterpret_cast<u32x4*>(d.rows + to * d.page + h * d.head + to_row * d.row + piece * 16) =
-            *reinterpret_cast<const u32x4*>(s.rows + from * s.page + h * s.head + from_row * s.row + piece * 16);
-      }
-      if (s.scale) {
-        for (int k = tid; k < total; k += kThreads) {
-          if (at + k >= p.into.capacity) break;
-          uint32_t from_row, to_row;
-          const int from = page_of(p.c, b, list[k], from_row), to = page_of(p.into, b, at + k, to_row);
-          if (to < 0) continue;
-          d.scale[to * d.s_page + h * d.s_head + to_row] = s.scale[from * s.s_page + h * s.s_head + from_row];
-        }
+    for (int k = tid; k < total; k += kThreads) {
+      uint32_t to_row = 0;
+      list[k].z = at + k < p.into.capacity ? page_of(p.into, b, at + k, to_row) : -1;
+      list[k].w = (int)to_row;
+    }
+    __syncthreads();
+    const Side ks = p.c.side[0], vs = p.c.side[1], kd = p.into.side[0], vd = p.into.side[1];
+    for (int i = tid; i < total * (int)p.pieces.d; i += kThreads) {
+      const int k = (int)p.pieces.of((uint32_t)i), piece = i - k * p.pieces.d;
+      const int4 l = list[k];
+      if (l.z < 0) continue;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(ks.rows + l.x * ks.page + h * ks.head + l.y * ks.row + piece * 16);
+      const u32x4 y = *reinterpret_cast<const u32x4*>(vs.rows + l.x * vs.page + h * vs.head + l.y * vs.row + piece * 16);
+      *reinterpret_cast<u32x4*>(kd.rows + l.z * kd.page + h * kd.head + l.w * kd.row + piece * 16) = x;
+      *reinterpret_cast<u32x4*>(vd.rows + l.z * vd.page + h * vd.head + l.w * vd.row + piece * 16) = y;
+    }
+    if (ks.scale) {
+      for (int k = tid; k < total; k += kThreads) {
+        const int4 l = list[k];
+        if (l.z < 0) continue;
+        kd.scale[l.z * kd.s_page + h * kd.s_head + l.w] = ks.scale[l.x * ks.s_page + h * ks.s_head + l.y];
+        vd.scale[l.z * vd.s_page + h * vd.s_head + l.w] = vs.scale[l.x * vs.s_page + h * vs.s_head + l.y];
       }
     }
     at += total;
   }
-  if (part == p.chunks - 1 && tid == 0) p.counts[bh] = (int)min((int64_t)at, p.into.capacity);
+  if (part == (int)p.chunks.d - 1 && tid == 0) p.counts[bh] = (int)min((int64_t)at, p.into.capacity);
 }
 
 int check_lengths(const int32_t* at, const int64_t strides[2], const char* what) {
@@ -452,13 +468,14 @@ int fcr_cache_keep(const fcr_cache* cache, const int32_t* table, int64_t table_s
   p.keep = keep;
   p.counts = counts;
   p.N = N;
-  p.row_bytes = cache->D * element_bytes(cache->dtype);
-  // short ranges while there are few pairs; a mask is counted again by every range behind, so no more than 64 of them
-  int chunk = 512;
+  p.pieces.set((uint32_t)(cache->D * element_bytes(cache->dtype) / 16));
+  p.H.set((uint32_t)cache->H);
+  // short ranges, but a mask is counted again by every range behind, so no more than 64 of them
+  int chunk = 128;
   while ((N + chunk - 1) / chunk > 64) chunk *= 2;
   p.chunk = chunk;
-  p.chunks = (N + chunk - 1) / chunk;
-  const int64_t blocks = (int64_t)B * cache->H * p.chunks;
+  p.chunks.set((uint32_t)((N + chunk - 1) / chunk));
+  const int64_t blocks = (int64_t)B * cache->H * p.chunks.d;
   if (blocks >= kMaxBlocks) return fail(FCR_E_SHAPE, "B*H and N are too many for one call");
   hipLaunchKernelGGL(cache_keep_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
   return launched("cache_keep_kernel");
