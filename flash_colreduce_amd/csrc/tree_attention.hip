@@ -447,6 +447,13 @@ __device__ __forceinline__ void add_not_finite(const Source& src, int D, int pos
 template <class F, int RT>
 struct Queries {
   u32x4 w[RT][F::KS];
+  // Waits for the loads here: a loop that is entered with them on the way would wait, in every turn, for all that it has on the way itself.
+  __device__ __forceinline__ void arrive() {
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int c = 0; c < F::KS; ++c) asm volatile("" : "+v"(w[r][c]));
+  }
   // Returns the largest finite element's bits (of codes: where they are bf16 they are to be scaled).
   __device__ __forceinline__ uint32_t load(const Args& a, int b, int h, int row0, const Lane<F>& at) {
     typedef short s16x2 __attribute__((ext_vector_type(2)));
@@ -701,6 +708,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
     float by = a.scale2;
     const uint32_t most = q.load(a, b, h, row0, at);
     if (F::codes && a.bf16) by = __builtin_amdgcn_ldexpf(by, -q.scale(largest_of_wave(most)));
+    q.arrive();
     State<F, RT> st;
     st.clear();
     for (int i = deal.blk; i < stop; ++i) {
@@ -900,6 +908,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       for (int w = 0; w < WAVES; ++w) largest = max(largest, (uint32_t)scan[w]);
       by = __builtin_amdgcn_ldexpf(by, -q.scale(largest));
     }
+    q.arrive();
     State<F, RT> st;
     st.clear();
     const auto convert = [&](int stage) {
