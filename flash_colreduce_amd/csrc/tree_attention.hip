@@ -569,7 +569,7 @@ __device__ __forceinline__ void emit_part(float* to, int d0, const float (&x)[F:
 
 // The blocks of a workgroup, as pieces of items.  Lengths are known on the device only: every workgroup adds them up.  Lengths of
 // sequences (not of heads): an entry is all heads of one.
-template <int THREADS>
+template <int THREADS, bool WHOLE_PIECES>
 struct Deal {
   int at, end, b, h, tile, blk, nb, context, n;
   // (Short on purpose: this and what else runs once per workgroup costs about 200 cycles per 64 bytes of instructions, which come
@@ -616,9 +616,23 @@ struct Deal {
       total += round;
     }
     const int per = max((int)a.all.of((uint32_t)(total + a.wgs - 1)), a.least);
-    if (wg == 0 && tid == 0) a.first[0] = per;
-    at = wg * per;                                      // (wgs * per is total + wgs at most: checked by the host to fit)
-    end = min(at + per, total);
+    // A second piece costs a workgroup of many rows as much as 2.6 blocks.  If pieces of one item each, of up to two blocks more, are no more
+    // than the workgroups, every workgroup takes one.
+    int most = 0;
+    if (WHOLE_PIECES && entries <= THREADS) {
+      const int blocks = tid < entries ? mine / weight : 0;
+      for (int p = per; p <= per + 2 && !most; ++p) {
+        const int pieces = (int)((uint32_t)(blocks + p - 1) / (uint32_t)p) * weight;
+        int sum;
+        __syncthreads();
+        const int before = in_front(pieces, sum);
+        if (__builtin_amdgcn_readfirstlane(sum) <= a.wgs) most = p, mine = pieces, start = before, round = total = sum;
+      }
+    }
+    const int unit = most ? 1 : per;
+    if (wg == 0 && tid == 0) a.first[0] = most ? most : per;
+    at = wg * unit;                                     // (wgs * per is total + wgs at most: checked by the host to fit)
+    end = min(at + unit, total);
     if (at >= end) return false;
     int base = 0;
     for (int before = round; __builtin_expect(at >= before, 0); before += round) {
@@ -638,8 +652,14 @@ struct Deal {
     b = by_head ? (int)a.heads.of((uint32_t)entry) : entry;
     h = by_head ? entry - b * a.H : 0;
     look(a);
-    int item_of_entry = (int)((uint32_t)in / (uint32_t)nb);
-    blk = in - item_of_entry * nb;
+    const int pieces = most ? (int)((uint32_t)(nb + most - 1) / (uint32_t)most) : nb;
+    int item_of_entry = (int)((uint32_t)in / (uint32_t)pieces);
+    blk = in - item_of_entry * pieces;
+    if (most) {                                         // (the last of ceil(nb / most) pieces of equal length has a block at least)
+      const int length = (int)((uint32_t)(nb + pieces - 1) / (uint32_t)pieces);
+      blk *= length;
+      at = 0, end = min(length, nb - blk);
+    }
     if (!by_head) h = (int)a.per_head.of((uint32_t)item_of_entry), item_of_entry -= h * a.row_tiles;
     tile = item_of_entry;
     return true;
@@ -685,7 +705,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
   const int wg = range_of(args, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const Lane<F> at(threadIdx.x & 63);
-  Deal<256> deal;
+  Deal<256, false> deal;
   if (!deal.start(arguments(), wg, scan)) return;
   do {
     const Args& a = arguments();
@@ -864,7 +884,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   const Lane<F> at(threadIdx.x & 63);
   const int my_tile = kApart ? wave % kTiles : wave * kMine;
   const bool my_keys = !kApart || wave < kTiles, my_values = !kApart || wave >= kTiles;
-  Deal<64 * WAVES> deal;
+  Deal<64 * WAVES, true> deal;
   if (!deal.start(arguments(), wg, scan)) return;
   do {
     const int b = deal.b, n = deal.n, context = deal.context;

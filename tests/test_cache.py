@@ -79,6 +79,17 @@ def test_attention_blocks_are_dealt_once_and_joined_in_order():
         assert not parts
 
 
+def test_pieces_of_one_item_each_cover_it_once():
+    """The other distribution: pieces of at most `most` blocks, a workgroup for each; and what the join derives from the first one's length."""
+    for blocks in range(1, 400):
+        for most in range(1, 60):
+            pieces = -(-blocks // most)
+            length = -(-blocks // pieces)
+            ends = [(i * length, min(i * length + length, blocks)) for i in range(pieces)]
+            assert all(a < z <= a + most for a, z in ends) and ends[0][0] == 0 and ends[-1][1] == blocks
+            assert -(-(blocks - ends[0][1]) // most) == pieces - 1
+
+
 def _c_cache(**over):
     a = dict(k=16, v=32, k_scale=48, v_scale=64, k_strides=(16384, 2048, 64), v_strides=(16384, 2048, 64), k_scale_strides=(256, 32, 1),
              v_scale_strides=(256, 32, 1), dtype=3, pages=4, H=8, page_size=32, D=64)
