@@ -18,7 +18,7 @@
 // tall_attention_kernel (many rows): bound by the vector instructions of the softmax and by the matrix units.  Each wave takes 32 rows and
 //   all keys; the operands of a block are converted once, by all waves, and lie in LDS as the matrix instructions take them.  64 drafted tokens of 4
 //   query heads over 8 x 8 heads of 32768 int8 keys, D = 128: 265 us, 780 TFLOP/s (1049 with operands formed by every wave from global memory, 341
-//   with one stage in LDS); over 4 x 8 heads of 8192 keys 67 us.
+//   with one stage in LDS); over 4 x 8 heads of 8192 keys 61 us, a quarter of it what runs once per workgroup.
 //
 // Codes are multiplied in fp16, where each of them is exact: bf16 queries are scaled by one power of two to fit (elements under 2^-38 of
 // the largest are lost, no score changes by more than that part of the largest), the keys' scales multiply the scores, the values' scales the
@@ -26,8 +26,8 @@
 // row is what its weights p_j vs_j ask for, so that they fit fp16 whatever the scales are; sums and statistics are in 32 bits.
 //
 // Distribution: the (batch, head, row tile) items are cut into blocks of 128 keys, laid end to end, and every workgroup takes the same
-// number of blocks, found from the lengths on the device.  Parts of an item that was cut are joined by tree_join_kernel, in the order of
-// the keys.
+// number of blocks, found from the lengths on the device; with many rows, where a second piece costs a workgroup most, one piece of one item if that is
+// no more than two blocks longer.  Parts of an item that was cut are joined by tree_join_kernel, in the order of the keys.
 
 #include <math.h>
 
@@ -616,8 +616,9 @@ struct Deal {
       total += round;
     }
     const int per = max((int)a.all.of((uint32_t)(total + a.wgs - 1)), a.least);
-    // A second piece costs a workgroup of many rows as much as 2.6 blocks.  If pieces of one item each, of up to two blocks more, are no more
-    // than the workgroups, every workgroup takes one.
+    // A second piece costs a workgroup of many rows as much as 2.6 blocks (first stage, partial results, code that runs for the first time).  If
+    // pieces of one item each, of up to two blocks more, are no more than the workgroups, every workgroup takes one: 256 rows over 4 x 8 heads of
+    // 8192 keys of 128 elements 77 -> 73 us bf16, 79 -> 74 int8; where no such pieces are found, the search costs 1 us.
     int most = 0;
     if (WHOLE_PIECES && entries <= THREADS) {
       const int blocks = tid < entries ? mine / weight : 0;
