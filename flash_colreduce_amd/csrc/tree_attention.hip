@@ -20,8 +20,8 @@
 //   query heads over 8 x 8 heads of 32768 int8 keys, D = 128: 265 us, 780 TFLOP/s (1049 with operands formed by every wave from global memory, 341
 //   with one stage in LDS); over 4 x 8 heads of 8192 keys 61 us, a quarter of it what runs once per workgroup.
 //
-// Codes are multiplied in fp16, where each of them is exact: bf16 queries are scaled by one power of two to fit (elements under 2^-38 of
-// the largest are lost, no score changes by more than that part of the largest), the keys' scales multiply the scores, the values' scales the
+// Codes are multiplied in fp16, where each of them is exact: bf16 queries are scaled by a power of two to fit, of their own or (many rows) of rows
+// that are up to 2^16 larger (an element keeps its 8 bits down to 2^-15 of its row's largest, and is off by 2^-23 of that at most below), the keys' scales multiply the scores, the values' scales the
 // probabilities, in 32 bits, before these are rounded to 11 bits.  16-bit caches are multiplied in their own type.  The reference m of a
 // row is what its weights p_j vs_j ask for, so that they fit fp16 whatever the scales are; sums and statistics are in 32 bits.
 //
@@ -85,6 +85,7 @@ __device__ __forceinline__ const Args& arguments() {
 
 constexpr int kBlock = 128;                  // keys of a block
 constexpr int kFirst = 4;                    // words in front of the items in Args::first
+constexpr int kNoPower = 200;                // of a row without a finite element but zeros; above all others
 constexpr float kNone = -3.0e38f;            // reference of a row that has seen no key
 constexpr float kMostWeight = 0x1p15f;       // weights above this raise the reference, to where the largest is in (1/2, 1]
 constexpr float kMostSum = 0x1p110f;         // and so do sums above this
@@ -332,6 +333,12 @@ struct State {
   }
 };
 
+// A product that is not joined with the sum it goes into.
+__device__ __forceinline__ float rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 // The weights of 32 keys from their products with the queries: 2^(k_scale s - m) v_scale.  MASKED: seen[r] holds the keys that a row
 // sees, bit 4 t + i; else every key is seen.  Bound by the vector unit: per score an fma, an exponential (four slots), the sum, the product
 // with the value's scale and half a conversion.  Returns whether some row's reference has to be raised, because a weight might not fit fp16 (the
@@ -347,7 +354,10 @@ __device__ __forceinline__ bool weights(const f32x4 (&k_scale)[2], const f32x4 (
     float x[8], part[2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      x[e] = __builtin_fmaf(s[r][e / 4][e % 4], k_scale[e / 4][e % 4], -st.m[r]);
+      // (of scores whose last bit is worth more than a weight's exponent, the rounded one is at the reference that `raise` chose; one rounding
+      // less may put it far above, which raises the reference again and comes here)
+      x[e] = MASKED ? rounded(s[r][e / 4][e % 4] * k_scale[e / 4][e % 4]) - st.m[r]
+                    : __builtin_fmaf(s[r][e / 4][e % 4], k_scale[e / 4][e % 4], -st.m[r]);
       if (MASKED) x[e] = (seen[r] >> e) & 1u ? x[e] : -INFINITY;
       x[e] = __builtin_amdgcn_exp2f(x[e]);
       part[e & 1] = e < 2 ? x[e] : part[e & 1] + x[e];
@@ -374,7 +384,7 @@ __device__ __forceinline__ void raise(const f32x4 (&k_scale)[2], const f32x4 (&v
     float of_weights = -INFINITY, of_sum = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float x = s[r][e / 4][e % 4] * k_scale[e / 4][e % 4];
+      float x = rounded(s[r][e / 4][e % 4] * k_scale[e / 4][e % 4]);
       x = (seen[r] >> e) & 1u ? x : -INFINITY;
       of_sum = fmaxf(of_sum, x);
       of_weights = fmaxf(of_weights, F::codes ? x + __builtin_amdgcn_logf(fabsf(v_scale[e / 4][e % 4])) : x);
@@ -454,11 +464,8 @@ struct Queries {
 #pragma unroll
       for (int c = 0; c < F::KS; ++c) asm volatile("" : "+v"(w[r][c]));
   }
-  // Returns the largest finite element's bits (of codes: where they are bf16 they are to be scaled).
-  __device__ __forceinline__ uint32_t load(const Args& a, int b, int h, int row0, const Lane<F>& at) {
-    typedef short s16x2 __attribute__((ext_vector_type(2)));
+  __device__ __forceinline__ void load(const Args& a, int b, int h, int row0, const Lane<F>& at) {
     constexpr int mine = F::codes ? 16 : 8;   // elements that lanes are apart
-    s16x2 most = {0, 0};
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int row = row0 + 16 * r + at.col;
@@ -478,38 +485,33 @@ struct Queries {
         }
       }
     }
+  }
+  // The power of two that takes the largest finite element of the lane's row r of bf16 to [2^14, 2^15), kNoPower for a row without one.
+  __device__ __forceinline__ int power(int r) const {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    s16x2 most = {0, 0};
     // magnitudes with 0x80 added: as signed halves bf16's infinities and NaNs are below all others
-    if (F::codes && a.bf16) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+    for (int s = 0; s < F::KS; ++s)
 #pragma unroll
-        for (int s = 0; s < F::KS; ++s)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, (w[r][s][j] & 0x7fff7fffu) + 0x00800080u));
-    }
-    return (uint32_t)max(max((int)most[0], (int)most[1]) - 0x80, 0);
+      for (int j = 0; j < 4; ++j)
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, (w[r][s][j] & 0x7fff7fffu) + 0x00800080u));
+    int x = max((int)most[0], (int)most[1]) - 0x80;
+    x = max(x, __shfl_xor(x, 16));
+    x = max(x, __shfl_xor(x, 32));
+    return x <= 0 ? kNoPower : 14 - ((x >> 7) - 127);
   }
   // Where in a row the lanes' first elements of k-step s are.
   __device__ __forceinline__ static constexpr int element(int s) { return F::codes ? 64 * (s / 2) + 8 * (s & 1) : 32 * s; }
-  // bf16 to fp16, the largest element (its bits: `most`, the same in every lane) to [2^14, 2^15): times 2^ what is returned.
-  __device__ __forceinline__ int scale(uint32_t most) {
-    const int up = most == 0 ? 0 : 14 - ((int)(most >> 7) - 127);
+  // Row r from bf16 to fp16, times 2^up.
+  __device__ __forceinline__ void scale(int r, int up) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+    for (int s = 0; s < F::KS; ++s)
 #pragma unroll
-      for (int s = 0; s < F::KS; ++s)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[r][s][j] = pack2<FCR_DTYPE_F16>(__builtin_amdgcn_ldexpf(bf16_of(w[r][s][j], 0), up), __builtin_amdgcn_ldexpf(bf16_of(w[r][s][j], 1), up));
-    return up;
+      for (int j = 0; j < 4; ++j)
+        w[r][s][j] = pack2<FCR_DTYPE_F16>(__builtin_amdgcn_ldexpf(bf16_of(w[r][s][j], 0), up), __builtin_amdgcn_ldexpf(bf16_of(w[r][s][j], 1), up));
   }
 };
-__device__ __forceinline__ uint32_t largest_of_wave(uint32_t x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
-  return x;
-}
 
 // Which of the lane's keys from position `pos` on (a 32-key step: bits 4 t + i) the query of a row sees.  (Rows that are none are given
 // token 0.  Bytes in front of the mask's row, for keys of the context, and behind it, for keys that are not there, do not count.)
@@ -727,8 +729,13 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
     }
     Queries<F, RT> q;
     float by = a.scale2;
-    const uint32_t most = q.load(a, b, h, row0, at);
-    if (F::codes && a.bf16) by = __builtin_amdgcn_ldexpf(by, -q.scale(largest_of_wave(most)));
+    q.load(a, b, h, row0, at);
+    if (F::codes && a.bf16) {
+      int up = q.power(0);
+      up = up == kNoPower ? 0 : up;
+      q.scale(0, up);
+      by = __builtin_amdgcn_ldexpf(by, -up);            // (of the lane's row)
+    }
     q.arrive();
     State<F, RT> st;
     st.clear();
@@ -879,6 +886,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   __shared__ __attribute__((aligned(16))) float scales[2][2][kKeys];     // of keys, of values
   __shared__ float most[2][kTiles];                                      // the largest scale of a tile's values
   __shared__ int flags[2][kTiles];                                       // a tile's page is there, and (bit 1) a drafted value was not finite
+  __shared__ float rest[WAVES][RT][16];                                  // powers of two that rows' scores are still to be multiplied by
   __shared__ int scan[WAVES + 2];
   const int wg = range_of(args, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -918,16 +926,32 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
     fetch(0);
     Queries<F, RT> q;
     float by = arguments().scale2;
-    uint32_t largest = q.load(arguments(), b, deal.h, row0, at);
+    q.load(arguments(), b, deal.h, row0, at);
     __syncthreads();                                                     // (the piece before has been used)
+    bool apart = false;
     if (F::codes && arguments().bf16) {
-      // one power of two for all rows of the workgroup, which the keys' scales undo
-      largest = largest_of_wave(largest);
-      if (at.lane == 0) scan[wave] = (int)largest;
+      // One power of two for all rows of the workgroup, which the keys' scales undo; rows that it would leave under 2^-16 of the largest have
+      // their own, and their scores are multiplied by the rest.
+      int up[RT], least = kNoPower;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) least = min(least, up[r] = q.power(r));
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
+      if (at.lane == 0) scan[wave] = least;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) largest = max(largest, (uint32_t)scan[w]);
-      by = __builtin_amdgcn_ldexpf(by, -q.scale(largest));
+      for (int w = 0; w < WAVES; ++w) least = min(least, scan[w]);
+      least = __builtin_amdgcn_readfirstlane(least);
+      least = least == kNoPower ? 0 : least;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const int mine = up[r] - least > 16 && up[r] != kNoPower ? up[r] : least;
+        q.scale(r, mine);
+        apart = apart || mine != least;
+        if (at.g == 0) rest[wave][r][at.col] = __builtin_amdgcn_ldexpf(1.0f, least - mine);
+      }
+      apart = __any(apart);
+      by = __builtin_amdgcn_ldexpf(by, -least);
     }
     q.arrive();
     State<F, RT> st;
@@ -1032,6 +1056,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
           const uint32_t there = there_of(pos, n, f0 & 1, f1 & 1, at.g);
 #pragma unroll
           for (int r = 0; r < RT; ++r) seen[r] = seen_by(arguments(), b, row0 + 16 * r + at.col, pos, context, there, at.g);
+        }
+        if (F::codes && __builtin_expect(apart, 0)) {
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const float by_row = rest[wave][r][at.col];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[r][t] = s[r][t] * by_row;
+          }
         }
         weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
       }

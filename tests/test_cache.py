@@ -668,6 +668,42 @@ def test_scales_and_scores_far_apart(kind, dtype, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("t,d", [(1, 64), (2, 256), (60, 128), (40, 192)])
+def test_scores_whose_last_bit_is_above_one(kind, dtype, t, d):
+    """Scores of 2^24 to 2^90, where fp32 has no fractions: one key has all the weight, and nothing overflows."""
+    query, cache, table, context = problem(2, 2, 2, t, 400, d, 16, kind, dtype)
+    for scale in (2.0 ** 24, -2.0 ** 40, 2.0 ** 90):
+        check_attention(query, cache, table, context, scale=scale)
+        check_attention(query, cache, table, context, random_tree(2, t, 3), scale=scale, tree_lengths=torch.tensor([t, t - 1]).int())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("t,g", [(1, 4), (3, 5), (40, 4), (90, 3)])
+def test_query_rows_far_apart(kind, t, g):
+    """bf16 rows whose magnitudes differ by 2^80, rows of zeros and rows that are not finite, side by side: each has its own result."""
+    b, h, n, d = 2, 2, 300, 64
+    query, cache, table, context = problem(b, h, g, t, n, d, 16, kind, BF16)
+    power = torch.randint(-80, 1, (b, h * g, t, 1), generator=torch.Generator().manual_seed(4)).double()
+    power[:, 0, 0] = 0
+    far = (query.double() * 2.0 ** power).to(BF16)
+    check_attention(far, cache, table, context)
+    check_attention(far, cache, table, context, scale=2.0 ** 40)
+    far[0, 0, 0] = 0
+    check_attention(far, cache, table, context)
+    bad = far.clone()
+    bad[0, 1, 0, 3] = math.nan
+    bad[1, h * g - 1, t - 1, 5] = math.inf
+    want = list(ref_attention(far, cache, table, context, None, None, None))
+    got, lse = (x.cpu() for x in fca.tree_attention(bad.cuda(), device(cache), table.cuda(), context.cuda(), return_lse2=True))
+    for at in ((0, 1, 0), (1, h * g - 1, t - 1)):
+        assert got[at].isnan().all() and not lse[at].isfinite()
+        got[at], lse[at] = want[0].to(BF16)[at], want[1].float()[at]
+    compare_attention(got, lse, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind,dtype", [(F16, F16), (BF16, BF16), (I8, BF16), (E4M3, F16)])
 def test_layouts(kind, dtype):
     """Keys and values of one allocation, token-major pages, token-major and expanded queries, tables and lengths that are views."""
