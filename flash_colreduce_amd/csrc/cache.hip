@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) cache_keep_kernel(KeepArgs p) {
   int at = counted[0] + counted[1] + counted[2] + counted[3];
 
   for (int first = begin; first < end; first += kKeepRows) {
-    // rows of this round: at most 16 per thread for the first kKeepRows / 16 threads
+    // rows of this turn: at most 16 per thread for the first kKeepRows / 16 threads
     __syncthreads();
     const int mine0 = first + tid * 16;
     uint32_t bits = tid < kKeepRows / 16 && mine0 < end ? kept16(p, keep, b, mine0, n, page, row) : 0;
