@@ -26,8 +26,7 @@
 // row is what its weights p_j vs_j ask for, so that they fit fp16 whatever the scales are; sums and statistics are in 32 bits.
 //
 // Distribution: the (batch, head, row tile) items are cut into blocks of 128 keys, laid end to end, and every workgroup takes the same
-// number of blocks, found from the lengths on the device; with many rows, where a second piece costs a workgroup most, one piece of one item if that is
-// no more than two blocks longer.  Parts of an item that was cut are joined by tree_join_kernel, in the order of the keys.
+// number of blocks, found from the lengths on the device; or, where that takes little longer, one piece of one item.  Parts of an item that was cut are joined by tree_join_kernel, in the order of the keys.
 
 #include <math.h>
 
@@ -571,7 +570,7 @@ __device__ __forceinline__ void emit_part(float* to, int d0, const float (&x)[F:
 
 // The blocks of a workgroup, as pieces of items.  Lengths are known on the device only: every workgroup adds them up.  Lengths of
 // sequences (not of heads): an entry is all heads of one.
-template <int THREADS, bool WHOLE_PIECES>
+template <int THREADS, bool TALL>
 struct Deal {
   int at, end, b, h, tile, blk, nb, context, n;
   // (Short on purpose: this and what else runs once per workgroup costs about 200 cycles per 64 bytes of instructions, which come
@@ -618,18 +617,29 @@ struct Deal {
       total += round;
     }
     const int per = max((int)a.all.of((uint32_t)(total + a.wgs - 1)), a.least);
-    // A second piece costs a workgroup of many rows as much as 2.6 blocks (first stage, partial results, code that runs for the first time).  If
-    // pieces of one item each, of up to two blocks more, are no more than the workgroups, every workgroup takes one: 256 rows over 4 x 8 heads of
-    // 8192 keys of 128 elements 77 -> 73 us bf16, 79 -> 74 int8; where no such pieces are found, the search costs 1 us.
+    // Pieces of one item each, a workgroup for each, where some number of blocks a little above `per` makes them no more than the workgroups.  A
+    // second piece costs a workgroup of many rows as much as 2.6 blocks (first stage, partial results, code that runs for the first time), and row
+    // tiles whose pieces are cut alike read the same keys at the same time.  256 rows over 4 x 8 heads of 8192 keys of 128 elements: 77 -> 73 us bf16,
+    // 79 -> 74 int8; 32 rows: 53 -> 35 bf16, 36 -> 34 int8; 40 rows over 3 x 7 heads of 30000 keys bf16 139 -> 97.  Few rows of one tile gain 3 % from
+    // 200 us on and lose as much, the search, at 20.
     int most = 0;
-    if (WHOLE_PIECES && entries <= THREADS) {
+    if (entries <= THREADS && (TALL || a.row_tiles > 1 || per >= 16)) {
       const int blocks = tid < entries ? mine / weight : 0;
-      for (int p = per; p <= per + 2 && !most; ++p) {
+      const int limit = per + (TALL ? 2 : 0) + min(per / 8, a.row_tiles > 1 ? 6 : TALL ? 0 : 2);
+      int p = limit;                                    // (first whether there is one)
+      for (bool found = false;;) {
         const int pieces = (int)((uint32_t)(blocks + p - 1) / (uint32_t)p) * weight;
         int sum;
         __syncthreads();
         const int before = in_front(pieces, sum);
-        if (__builtin_amdgcn_readfirstlane(sum) <= a.wgs) most = p, mine = pieces, start = before, round = total = sum;
+        const bool fits = __builtin_amdgcn_readfirstlane(sum) <= a.wgs;
+        if (!found && !fits) break;
+        if (fits && (found || p == per)) {
+          most = p, mine = pieces, start = before, round = total = sum;
+          break;
+        }
+        p = found ? p + 1 : per;                        // (`limit` again at most)
+        found = true;
       }
     }
     const int unit = most ? 1 : per;
@@ -1268,9 +1278,9 @@ struct Plan {
 bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Plan& p) {
   const int64_t rows = (int64_t)T * G;
   const int w = (D + 63) / 64, tall = 16 * tall_tiles(w);
-  // Both sides, us, at 4 sequences x 8 heads x 8192 keys, int8 (bf16): 48 rows of 64 elements 31 (30) by form 1, 36 (33) by form 4, 64 rows 39
-  // (44) and 36 (33); of 128 elements 41 (43) and 46 (45), 52 (87) and 47 (47); 48 rows of 256 elements 58 (88) by form 1, 67 (76) by form 8, 64
-  // rows 95 (167) and 71 (84); 128 rows of 128 elements 58 (57) by form 4, 60 (64) by form 8, 192 rows 77 (79) and 72 (74).
+  // Both sides, us, at 4 sequences x 8 heads x 8192 keys, int8 (bf16): 48 rows of 64 elements 33 (31) by form 1, 37 (33) by form 4, 64 rows 38
+  // (35) and 38 (34); of 128 elements 42 (45) and 47 (46), 48 (52) and 49 (47); 48 rows of 256 elements 59 (89) by form 1, 62 (71) by form 8, 64
+  // rows 69 (108) and 66 (76); 128 rows of 128 elements 58 (57) by form 4, 60 (64) by form 8, 192 rows 77 (79) and 72 (74).
   p.form = rows <= (w <= 2 || codes ? 48 : 16) ? 1 : rows <= 4 * tall && w <= 2 ? 4 : 8;
   p.tile_rows = p.form == 1 ? 16 : tall * p.form;
   const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;

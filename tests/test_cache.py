@@ -543,6 +543,19 @@ def test_attention_of_many_rows(shape, kind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [(F16, F16), (I8, BF16)])
+@pytest.mark.parametrize("shape", [(1, 64, 1, 1, 16400, 16, 16), (2, 16, 1, 32, 8200, 32, 16), (2, 16, 1, 300, 2000, 32, 16)])
+def test_attention_of_many_blocks_per_workgroup(shape, kind, dtype):
+    """Enough blocks for pieces of one item each, of equal lengths and, with one short sequence, of lengths that leave none."""
+    query, cache, table, context = problem(*shape, kind, dtype)
+    context[:] = shape[4]
+    check_attention(query, cache, table, context)
+    context = of_heads(context, shape[1]).clone()
+    context[0, ::3] //= 5
+    check_attention(query, cache, table, context)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind,dtype", [(BF16, BF16), (I8, F16)])
 @pytest.mark.parametrize("b,h,t,g", [(700, 2, 1, 2), (530, 1, 33, 2)])
 def test_attention_of_more_sequences_than_threads(kind, dtype, b, h, t, g):
