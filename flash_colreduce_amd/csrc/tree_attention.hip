@@ -291,6 +291,23 @@ struct Values {
       }
     return found != 0;
   }
+  // Codes that are NaNs become 0, and the scale of their row, in every lane that has it, a NaN: a row that is hidden from some of the
+  // queries must not reach these by a product with their weight of 0.
+  __device__ __forceinline__ void clean_codes(const Lane<F>& at) {
+    if constexpr (F::CD == FCR_DTYPE_E4M3) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t found = 0;
+#pragma unroll
+        for (int j = 0; j < F::VW; ++j) {
+          const uint32_t bad = (((w[i][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+          found |= bad;
+          w[i][j] &= ~(bad * 0xffu);
+        }
+        if ((__ballot(found != 0) >> (16 * at.g)) & 0xffff) scale[i] = __builtin_nanf("");
+      }
+    }
+  }
   // Element d (of the lane's DT) of the four rows, as four fp16 or bf16.
   __device__ __forceinline__ u32x2 operand(int d) const {
     u32x2 f;
@@ -784,6 +801,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
         const uint32_t there = there_of(pos, n, there0, there1, at.g);
         v[0].drop(there);
         v[1].drop(there >> 4);
+        if (pos + 32 > context) v[0].clean_codes(at), v[1].clean_codes(at);
         if constexpr (!F::codes) {
           if (pos + 32 > context) not_finite = v[0].clean() | v[1].clean();
           not_finite = __any(not_finite);
@@ -976,6 +994,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         flag[t] = place[t].there(src) ? 1 : 0;
         if (my_values && (!flag[t] || pos + 16 > min(context, n))) {
           v[t].drop(there_of(pos, n, flag[t], flag[t], at.g));
+          if (pos + 16 > context) v[t].clean_codes(at);
           if constexpr (!F::codes) flag[t] |= pos + 16 > context && __any(v[t].clean()) ? 2 : 0;
         }
         if (my_keys) {

@@ -657,6 +657,27 @@ def test_what_hidden_rows_hold_has_no_influence(kind, dtype, t, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("t,d", [(5, 64), (14, 96), (30, 128), (5, 256), (60, 192)])
+def test_codes_that_are_nans_reach_the_rows_that_see_them_only(dtype, t, d):
+    """cache_write makes no such codes; a cache that is filled otherwise may have them."""
+    b, h, g, n = 2, 2, 2, 75
+    query, cache, table, context = problem(b, h, g, t, n, d, 16, E4M3, dtype)
+    mask = random_tree(b, t, 3)
+    want = ref_attention(query, cache, table, context, mask, None, None)
+    j = int(context[0]) + t // 2
+    page = int(table[0, j // 16])
+    cache.v.view(torch.uint8)[page, 1, j % 16, d - 1] = 0xff
+    cache.k.view(torch.uint8)[page, 0, j % 16, 3] = 0x7f
+    got, lse = (x.cpu() for x in fca.tree_attention(query.cuda(), device(cache), table.cuda(), context.cuda(), mask.cuda(), return_lse2=True))
+    sees = mask[0, :, t // 2]
+    assert sees.any() and not sees.all()
+    assert got[0, :g, sees].isnan().all() and got[0, g:, sees, d - 1].isnan().all()
+    got[0, :, sees], lse[0, :, sees] = want[0].to(got.dtype)[0, :, sees], want[1].float()[0, :, sees]
+    compare_attention(got, lse, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [I8, E4M3])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("t", [1, 12])
