@@ -98,6 +98,25 @@ __device__ __forceinline__ void keys_of(const Args& a, int b, int h, int& contex
   n = (int)min((uint32_t)context + (uint32_t)tree, (uint32_t)a.positions);   // (each below 2^31)
 }
 
+// The sum over the wave's lanes up to this one: within rows of 16 lanes, then each row's last sum to the rows behind.  (Lanes exchange
+// within the vector unit; exchanges by way of LDS take ten times as long.)
+__device__ __forceinline__ int sum_up_to(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast:15, to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast:31, to rows 2 and 3
+  return x;
+}
+// The least over 16 lanes that lie together.
+__device__ __forceinline__ int least_of_row(int x) {
+  x = min(x, __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false));   // row_ror:8
+  x = min(x, __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false));
+  x = min(x, __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, false));
+  return min(x, __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false));
+}
+
 __device__ __forceinline__ float across(float x, bool largest) {   // over the four lanes that share a query
   float y = __shfl_xor(x, 16);
   x = largest ? fmaxf(x, y) : x + y;
@@ -606,12 +625,7 @@ struct Deal {
       return blocks_of(n) * weight;
     };
     const auto in_front = [&](int x, int& sum) {        // of this thread; the sum over all
-      int upto = x;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(upto, o);
-        upto += lane >= o ? y : 0;
-      }
+      const int upto = sum_up_to(x);
       if (lane == 63) scan[wave] = upto;
       __syncthreads();
       sum = 0;
@@ -963,8 +977,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       int up[RT], least = kNoPower;
 #pragma unroll
       for (int r = 0; r < RT; ++r) least = min(least, up[r] = q.power(r));
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
+      least = least_of_row(least);
       if (at.lane == 0) scan[wave] = least;
       __syncthreads();
 #pragma unroll
