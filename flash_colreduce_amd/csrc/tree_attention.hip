@@ -117,11 +117,18 @@ __device__ __forceinline__ int least_of_row(int x) {
   return min(x, __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false));
 }
 
-__device__ __forceinline__ float across(float x, bool largest) {   // over the four lanes that share a query
-  float y = __shfl_xor(x, 16);
-  x = largest ? fmaxf(x, y) : x + y;
-  y = __shfl_xor(x, 32);
-  return largest ? fmaxf(x, y) : x + y;
+// Over the four lanes that share a query, those of the four rows of 16: a swap of two copies leaves one row's values in the one and its
+// neighbour's in the other.
+template <class T, class Op>
+__device__ __forceinline__ T across(T x, Op op) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, x);
+  const auto rows = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const uint32_t c = __builtin_bit_cast(uint32_t, op(__builtin_bit_cast(T, (uint32_t)rows[0]), __builtin_bit_cast(T, (uint32_t)rows[1])));
+  const auto halves = __builtin_amdgcn_permlane32_swap(c, c, false, false);
+  return op(__builtin_bit_cast(T, (uint32_t)halves[0]), __builtin_bit_cast(T, (uint32_t)halves[1]));
+}
+__device__ __forceinline__ float across(float x, bool largest) {
+  return across(x, [&](float y, float z) { return largest ? fmaxf(y, z) : y + z; });
 }
 
 template <bool BF16>
@@ -532,8 +539,7 @@ struct Queries {
       for (int j = 0; j < 4; ++j)
         most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, (w[r][s][j] & 0x7fff7fffu) + 0x00800080u));
     int x = max((int)most[0], (int)most[1]) - 0x80;
-    x = max(x, __shfl_xor(x, 16));
-    x = max(x, __shfl_xor(x, 32));
+    x = across(x, [](int y, int z) { return max(y, z); });
     return x <= 0 ? kNoPower : 14 - ((x >> 7) - 127);
   }
   // Where in a row the lanes' first elements of k-step s are.
