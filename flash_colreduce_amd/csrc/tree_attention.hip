@@ -14,19 +14,21 @@
 // tree_attention_kernel (few rows): bound by reading the cache.  Each wave takes 32 keys of a block of 128, from global memory into
 //   registers without a stop in LDS, and 16 rows; the four waves' results are joined at the end.  32 ragged sequences of up to 16384 e4m3 keys, 8 heads
 //   of 4 queries, D = 128: 156 us, 5.3 TB/s; 8 tokens over 4 x 32 heads of up to 9001 fp16 keys of 64 elements: 48 us, 4.6 TB/s; one token
-//   over 1000 keys 11.3 us, most of it the two launches and code that is fetched for the first time.
-// tall_attention_kernel (many rows): bound by the vector instructions of the softmax and by the matrix units.  Each wave takes 32 rows and
-//   all keys; the operands of a block are converted once, by all waves, and lie in LDS as the matrix instructions take them.  64 drafted tokens of 4
+//   over 1000 keys 10.8 us, two launches and a chain of loads: lengths, table, keys.
+// tall_attention_kernel (many rows): bound by the vector instructions of the softmax and by the matrix units.  Each wave takes 32 rows (of
+//   more than 128 elements 16) and all keys; the operands of a block are converted once, by all waves, and lie in LDS as the matrix instructions take them.  64 drafted tokens of 4
 //   query heads over 8 x 8 heads of 32768 int8 keys, D = 128: 265 us, 780 TFLOP/s (1049 with operands formed by every wave from global memory, 341
 //   with one stage in LDS); over 4 x 8 heads of 8192 keys 61 us, a quarter of it what runs once per workgroup.
 //
-// Codes are multiplied in fp16, where each of them is exact: bf16 queries are scaled by a power of two to fit, of their own or (many rows) of rows
-// that are up to 2^16 larger (an element keeps its 8 bits down to 2^-15 of its row's largest, and is off by 2^-23 of that at most below), the keys' scales multiply the scores, the values' scales the
-// probabilities, in 32 bits, before these are rounded to 11 bits.  16-bit caches are multiplied in their own type.  The reference m of a
-// row is what its weights p_j vs_j ask for, so that they fit fp16 whatever the scales are; sums and statistics are in 32 bits.
+// Codes are multiplied in fp16, where each of them is exact: bf16 rows of queries are scaled by a power of two to fit, of their own or (many rows)
+// of rows that are up to 2^16 larger (an element keeps its 8 bits down to 2^-15 of its row's largest, and is off by 2^-23 of that at most
+// below), the keys' scales multiply the scores, the values' scales the probabilities, in 32 bits, before these are rounded to 11 bits, as
+// the matrix instructions take them.  16-bit caches are multiplied in their own type (probabilities against bf16 values have 8 bits).  The reference m
+// of a row is what its weights p_j vs_j ask for, so that they fit fp16 whatever the scales are; sums and statistics are in 32 bits.
 //
 // Distribution: the (batch, head, row tile) items are cut into blocks of 128 keys, laid end to end, and every workgroup takes the same
-// number of blocks, found from the lengths on the device; or, where that takes little longer, one piece of one item.  Parts of an item that was cut are joined by tree_join_kernel, in the order of the keys.
+// number of blocks, found from the lengths on the device; or, where that takes little longer, one piece of one item.  Parts of an item that
+// was cut are joined by tree_join_kernel, in the order of the keys.
 
 #include <math.h>
 
