@@ -930,6 +930,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   // keys next to its values, which a wave has one or the other of, or for the keys of two tiles (64 rows over 4 x 8 heads of 8192 keys:
   // 135 us with what then spills, 84 us; where nothing spills 8 % are lost).
   constexpr bool kLean = W == 4, kTight = kLean && !F::codes;
+  // The first stage is converted in the loop, and not by code in front of it, which made 16-bit kernels of more than 64 elements spill 5 to 39
+  // registers: 128 rows over 4 x 8 heads of 8192 bf16 keys of 128 elements 57 -> 54 us, 1024 rows of 256 elements 451 -> 413, int8 393 -> 383.
+  // With 64 elements, where nothing spills, 1 to 10 % are lost.
+  constexpr bool kInLoop = W >= 2;
   constexpr int kEarly = kTight ? 0 : W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights
   static_assert(kTiles * (kApart ? 2 : 1) == WAVES * kMine, "every wave has its share of a stage");
   __shared__ u32x4 operands[2 * kStage];
@@ -1077,19 +1081,22 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
         for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(kf[t][c], q.w[r][c], c ? s[r][t] : f32x4{0, 0, 0, 0});
     };
-    convert(0);
-    if (stages > 1) fetch(1);
-    __syncthreads();
-    if (!idle) {
-      read_keys(0, 0);
-      read_keys(0, 1);
-      read_scales(0);
-      products_of(0);
-      products_of(1);
+    if constexpr (!kInLoop) {
+      convert(0);
+      if (stages > 1) fetch(1);
+      __syncthreads();
+      if (!idle) {
+        read_keys(0, 0);
+        read_keys(0, 1);
+        read_scales(0);
+        products_of(0);
+        products_of(1);
+      }
     }
-    for (int i = 0; i < steps; ++i) {
-      const int stage = i / kSteps, j = i % kSteps, pos = pos0 + i * 32;
-      const bool work = !idle && pos < n;
+    // (in the loop: the step before the first one does this, with values and weights of 0)
+    for (int i = kInLoop ? -1 : 0; i < steps; ++i) {
+      const int stage = i < 0 ? -1 : i / kSteps, j = i < 0 ? kSteps - 1 : i % kSteps, pos = pos0 + i * 32;
+      const bool run = !idle && pos < n, work = run && (!kInLoop || i >= 0);
       u32x4 vf[F::DT], p[RT];
       uint32_t seen[RT];
       bool not_finite = false;
@@ -1116,8 +1123,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
           }
         }
         weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
+      } else if (kInLoop) {
+#pragma unroll
+        for (int d = 0; d < F::DT; ++d) vf[d] = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < RT; ++r) p[r] = u32x4{0, 0, 0, 0}, seen[r] = 0;
       }
-      if (j == (late ? kSteps / 2 : 0) && stage + 1 < stages) {
+      if (((kInLoop && i < 0) || j == (late ? kSteps / 2 : 0)) && stage + 1 < stages) {
         convert(stage + 1);
         if (stage + 2 < stages) fetch(stage + 2);
       }
@@ -1136,7 +1148,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
           add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
         }
         if (j == kSteps - 1) __syncthreads();
-        if (work) {
+        if (run) {
           read_scales(next);
           read_keys(next, 0);
           if (kTight) {
@@ -1148,7 +1160,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       } else {
         if (kEarly < F::DT && work) read_values(F::DT / 2);                // (before the barrier: the stage's place is written behind it)
         if (j == kSteps - 1) __syncthreads();
-        if (work) {
+        if (run) {
           __builtin_amdgcn_s_setprio(1);
           if (kEarly == F::DT) read_keys(next, 0);
           __builtin_amdgcn_sched_barrier(0);
@@ -1162,7 +1174,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
           if (kEarly < F::DT) read_keys(next, 1);
         }
       }
-      if (work) {
+      if (run) {
         if constexpr (!F::codes) {
           if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(src, arguments().D, pos, p, seen, at, st);
         }
