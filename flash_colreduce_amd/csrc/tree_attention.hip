@@ -926,15 +926,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   constexpr bool kApart = kTiles < WAVES;                                // a wave converts a tile's keys or its values
   constexpr int kValues = kTiles * F::KS * 64;                           // where the values begin, in 16 bytes
   constexpr int kStage = kValues + kSteps * F::DT * 64;
-  // Rows of 256 elements leave no registers for both halves of a step's values, or for keys next to them; 16-bit ones none for a tile's
-  // keys next to its values, which a wave has one or the other of, or for the keys of two tiles (64 rows over 4 x 8 heads of 8192 keys:
-  // 135 us with what then spills, 84 us; where nothing spills 8 % are lost).
-  constexpr bool kLean = W == 4, kTight = kLean && !F::codes;
+  // Rows of 256 elements leave no registers for both halves of a step's values, or for keys next to them.
+  constexpr bool kLean = W == 4;
   // The first stage is converted in the loop, and not by code in front of it, which made 16-bit kernels of more than 64 elements spill 5 to 39
-  // registers: 128 rows over 4 x 8 heads of 8192 bf16 keys of 128 elements 57 -> 54 us, 1024 rows of 256 elements 451 -> 413, int8 393 -> 383.
+  // registers: 128 rows over 4 x 8 heads of 8192 bf16 keys of 128 elements 57 -> 54 us, 1024 rows of 256 elements 451 -> 360, int8 393 -> 383.
   // With 64 elements, where nothing spills, 1 to 10 % are lost.
   constexpr bool kInLoop = W >= 2;
-  constexpr int kEarly = kTight ? 0 : W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights
+  constexpr int kEarly = W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights
   static_assert(kTiles * (kApart ? 2 : 1) == WAVES * kMine, "every wave has its share of a stage");
   __shared__ u32x4 operands[2 * kStage];
   __shared__ __attribute__((aligned(16))) float scales[2][2][kKeys];     // of keys, of values
@@ -955,7 +953,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
     const bool idle = row0 >= arguments().rows;                                    // (it converts all the same)
     const bool late = WAVES == 8 && wave >= 4;
     Keys<F> k[kMine];
-    Values<F> v[kMine];                                                  // (tight: of keys too, in the same registers)
+    Values<F> v[kMine];
     const Source src(arguments(), b, deal.h, n);
     Place place[kMine], ahead[kMine];                                    // of the rows loaded last, and of the next ones
     const int pos0 = deal.blk * kBlock;
@@ -970,8 +968,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
       for (int t = 0; t < kMine; ++t) {
         place[t] = ahead[t];
-        if (kTight || my_keys) k[t].load(src, D, place[t], here);
-        if constexpr (kTight) v[t] = __builtin_bit_cast(Values<F>, k[t]);
+        if (my_keys) k[t].load(src, D, place[t], here);
         if (my_values) v[t].load(src, D, place[t], here);
       }
       look(stage + 1);
@@ -1023,7 +1020,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
           if constexpr (!F::codes) flag[t] |= pos + 16 > context && __any(v[t].clean()) ? 2 : 0;
         }
         if (my_keys) {
-          if constexpr (kTight) k[t] = __builtin_bit_cast(Keys<F>, v[t]);
 #pragma unroll
           for (int c = 0; c < F::KS; ++c) to[((my_tile + t) * F::KS + c) * 64] = k[t].operand(c);
           if (F::codes && at.col == 0) *reinterpret_cast<f32x4*>(sc + (my_tile + t) * 16 + 4 * at.g) = k[t].scale * by;
@@ -1142,7 +1138,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       const int next = min(i + 1, steps - 1);
       if constexpr (kLean) {
         if (work) {
-          if (kEarly == 0) read_values(0);
           add_values<F, RT, 0, F::DT / 2>(vf, p, st);
           read_values(F::DT / 2);
           add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
@@ -1151,10 +1146,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         if (run) {
           read_scales(next);
           read_keys(next, 0);
-          if (kTight) {
-            products_of(0);
-            __builtin_amdgcn_sched_barrier(0);
-          }
           read_keys(next, 1);
         }
       } else {
@@ -1178,7 +1169,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         if constexpr (!F::codes) {
           if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(src, arguments().D, pos, p, seen, at, st);
         }
-        if (!kTight) products_of(0);
+        products_of(0);
         products_of(1);
         __builtin_amdgcn_s_setprio(0);
       }
@@ -1331,8 +1322,8 @@ bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Pl
   const int64_t rows = (int64_t)T * G;
   const int w = (D + 63) / 64, tall = 16 * tall_tiles(w);
   // Both sides, us, at 4 sequences x 8 heads x 8192 keys, int8 (bf16): 48 rows of 64 elements 33 (31) by form 1, 37 (33) by form 4, 64 rows 38
-  // (35) and 38 (34); of 128 elements 42 (45) and 47 (46), 48 (52) and 49 (47); 48 rows of 256 elements 59 (89) by form 1, 62 (71) by form 8, 64
-  // rows 69 (108) and 66 (76); 128 rows of 128 elements 58 (57) by form 4, 60 (64) by form 8, 192 rows 77 (79) and 72 (74).
+  // (35) and 38 (34); of 128 elements 42 (45) and 47 (46), 48 (52) and 49 (47); 48 rows of 256 elements 59 (89) by form 1, 62 (61) by form 8, 64
+  // rows 69 (108) and 65 (67); 128 rows of 128 elements 58 (57) by form 4, 60 (64) by form 8, 192 rows 77 (79) and 72 (74).
   p.form = rows <= (w <= 2 || codes ? 48 : 16) ? 1 : rows <= 4 * tall && w <= 2 ? 4 : 8;
   p.tile_rows = p.form == 1 ? 16 : tall * p.form;
   const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
@@ -1340,7 +1331,9 @@ bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Pl
   const int64_t blocks = p.items * ((capacity + kBlock - 1) / kBlock);
   if (rows > (1 << 24) || p.items > (1 << 22) || blocks > (1 << 30)) return false;
   p.row_tiles = (int)tiles;
-  int64_t wgs = (p.form == 8 ? 1 : 2) * (int64_t)fcr_detail::chip_cus_of_current_device();
+  // As many as the CUs hold at once: one of eight waves, or of four that take more than 256 registers (8 x 8 heads of 1000 bf16 keys of 256
+  // elements 21 us, 28 with twice as many, one behind the other); two of the others.
+  int64_t wgs = (p.form == 8 || (!codes && w > 2) ? 1 : 2) * (int64_t)fcr_detail::chip_cus_of_current_device();
   if (blocks < wgs) wgs = blocks;
   p.wgs = (int)((wgs + 7) / 8 * 8);
   p.least = 1;
