@@ -493,6 +493,28 @@ def test_keep_copies_the_named_rows_in_order(kind, b, h, n, d, page, into_page):
             assert torch.equal(x.cpu().view(torch.uint8), y.view(torch.uint8))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, I8])
+@pytest.mark.parametrize("n", [70001, 140016])
+def test_keep_of_more_rows_than_a_workgroup_lists_at_once(kind, n):
+    test_keep_copies_the_named_rows_in_order(kind, 1, 2, n, 16, 16, 32)
+
+
+@pytest.mark.gpu
+def test_keep_of_lengths_inside_and_in_front_of_a_range():
+    """Lengths of 0, below 0, inside 16 rows, at their end, and behind the mask."""
+    b, h, n, d = 2, 3, 700, 16
+    cache = device(make_cache(2 * 44, h, 16, d, F16, F32, seed=1))
+    table = torch.arange(88).view(2, 44).int().cuda()
+    lengths = torch.tensor([[0, -5, 131], [144, 10 ** 6, 1]]).int().cuda()
+    into = KVCache.zeros(88, h, 16, d, F16)
+    counts = fca.cache_keep(cache, table, lengths, torch.ones((b, h, n), dtype=torch.bool, device="cuda"), into, table)
+    assert counts.tolist() == [[0, 0, 131], [144, 700, 1]]
+    want = fca.cache_read(cache, table, counts, n)
+    assert all(torch.equal(x, y) for x, y in zip(fca.cache_read(into, table, counts, n), want))
+    assert not fca.cache_read(into, table, torch.full_like(lengths, n), n)[0][0, :2].any()
+
+
 # tree_attention ------------------------------------------------------------------------------------------------------------
 
 KINDS = [(F16, F16), (BF16, BF16), (I8, F16), (I8, BF16), (E4M3, F16), (E4M3, BF16)]
@@ -857,6 +879,40 @@ def test_streams_graphs_and_repetition():
     want = [y.clone() for y in step()]
     graph.replay()
     assert all(torch.equal(a, z) for a, z in zip(held, want))
+
+
+@pytest.mark.gpu
+def test_two_graphs_of_one_pool_and_two_streams():
+    """Graphs whose workspaces share memory, replayed in turn, and calls on two streams at once."""
+    few = problem(2, 2, 4, 3, 3000, 64, 16, I8, BF16)
+    many = problem(2, 2, 4, 70, 2000, 128, 16, BF16, BF16, seed=5)
+    calls = []
+    for query, cache, table, context in (few, many):
+        query, cache, table, context = query.cuda(), device(cache), table.cuda(), context.cuda()
+        calls.append(lambda q=query, c=cache, t=table, n=context: fca.tree_attention(q, c, t, n, return_lse2=True))
+    want = [[y.clone() for y in c()] for c in calls]
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for c in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            held.append(c())
+        graphs.append(graph)
+    for i in range(3):
+        for graph, got, w, c in zip(graphs, held, want, calls):
+            graph.replay()
+            assert all(torch.equal(a, z) for a, z in zip(got, w)), i
+            assert all(torch.equal(a, z) for a, z in zip(c(), w)), i
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for k, (stream, c) in enumerate(zip(streams, calls)):
+            with torch.cuda.stream(stream):
+                got[k].append(c())
+    torch.cuda.synchronize()
+    for k, w in enumerate(want):
+        assert all(torch.equal(a, z) for g in got[k] for a, z in zip(g, w))
 
 
 @pytest.mark.gpu
