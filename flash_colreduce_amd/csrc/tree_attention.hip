@@ -59,7 +59,7 @@ struct Args {
   int B, H, T, D, rows, row_tiles, bf16;
   Div G, per_head, heads, all; // by G, by row_tiles, by H, by wgs
   float scale2;
-  int wgs, least;              // workgroups of the launch; blocks that one takes at least
+  int wgs;                     // workgroups of the launch
   int positions;               // that a row of the table names
 };
 // form: see Plan
@@ -655,7 +655,7 @@ struct Deal {
       in_front(rest, total);
       total += round;
     }
-    const int per = max((int)a.all.of((uint32_t)(total + a.wgs - 1)), a.least);
+    const int per = (int)a.all.of((uint32_t)(total + a.wgs - 1));
     // Pieces of one item each, a workgroup for each, where some number of blocks a little above `per` makes them no more than the workgroups.  A
     // second piece costs a workgroup of many rows as much as 2.6 blocks (first stage, partial results, code that runs for the first time), and row
     // tiles whose pieces are cut alike read the same keys at the same time.  256 rows over 4 x 8 heads of 8192 keys of 128 elements: 77 -> 73 us bf16,
@@ -1314,7 +1314,7 @@ using fcr_detail::launched;
 
 struct Plan {
   int form;                  // 1: tree_attention_kernel; 4, 8: tall_attention_kernel of as many waves
-  int tile_rows, row_tiles, wgs, least;
+  int tile_rows, row_tiles, wgs;
   int64_t items, first_bytes, bytes;
 };
 // What depends on sizes alone.  false: too large.
@@ -1336,7 +1336,6 @@ bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Pl
   int64_t wgs = (p.form == 8 || (!codes && w > 2) ? 1 : 2) * (int64_t)fcr_detail::chip_cus_of_current_device();
   if (blocks < wgs) wgs = blocks;
   p.wgs = (int)((wgs + 7) / 8 * 8);
-  p.least = 1;
   p.first_bytes = (kFirst * 4 + p.items * 8 + 15) / 16 * 16;
   p.bytes = p.first_bytes + 2ll * p.wgs * p.tile_rows * (D + 4) * 4;
   return true;
@@ -1393,7 +1392,7 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
   a.G.set((uint32_t)G), a.per_head.set((uint32_t)plan.row_tiles), a.heads.set((uint32_t)H), a.all.set((uint32_t)plan.wgs);
   a.positions = (int)capacity;
   a.scale2 = scale * 1.44269504088896340736f;
-  a.wgs = plan.wgs, a.least = plan.least;
+  a.wgs = plan.wgs;
   const int w = (D + 63) / 64;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (cache->dtype) {
