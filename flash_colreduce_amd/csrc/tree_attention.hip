@@ -659,10 +659,10 @@ struct Deal {
     // Pieces of one item each, a workgroup for each, where some number of blocks a little above `per` makes them no more than the workgroups.  A
     // second piece costs a workgroup of many rows as much as 2.6 blocks (first stage, partial results, code that runs for the first time), and row
     // tiles whose pieces are cut alike read the same keys at the same time.  256 rows over 4 x 8 heads of 8192 keys of 128 elements: 77 -> 73 us bf16,
-    // 79 -> 74 int8; 32 rows: 53 -> 35 bf16, 36 -> 34 int8; 40 rows over 3 x 7 heads of 30000 keys bf16 139 -> 97.  Few rows of one tile gain 3 % from
-    // 200 us on and lose as much, the search, at 20.
+    // 79 -> 74 int8; 32 rows: 53 -> 35 bf16, 36 -> 34 int8; 40 rows over 3 x 7 heads of 30000 keys bf16 139 -> 97.  Few rows of one tile
+    // (8 x 8 heads of 8192 keys, one token: 55 -> 50 bf16, 36 -> 33 int8) lose 0.7 us where there is none, too much for less than 8 blocks.
     int most = 0;
-    if (entries <= THREADS && (TALL || a.row_tiles > 1 || per >= 16)) {
+    if (entries <= THREADS && (TALL || a.row_tiles > 1 || per >= 8)) {
       const int blocks = tid < entries ? mine / weight : 0;
       const int limit = per + (TALL ? 2 : 0) + min(per / 8, a.row_tiles > 1 ? 6 : TALL ? 0 : 2);
       int p = limit;                                    // (first whether there is one)
