@@ -198,11 +198,13 @@ struct Place {
   __device__ __forceinline__ bool there(const Source& s) const { return (uint32_t)page < (uint32_t)s.pages; }
 };
 
-// The lane's places in a 16-key tile: of keys (row lane & 15; 16-byte pieces, of which a row's last one stands for those behind it) and of
-// values (rows 4 g + i, elements from elements_of(col) on, where behind the row's end there are elements that another lane has as well).
+// The lane's places in a 16-key tile: of keys (row lane & 15; 16-byte pieces; those behind a row's end, where
+// queries are zeros, are its last one, or with ZEROS are read as zeros, at a place that no view has) and of values (rows 4 g + i, elements from
+// elements_of(col) on, where behind the row's end there are elements that another lane has as well).
 template <class F>
 struct Lane {
   static constexpr uint32_t kBytes = F::codes ? 1 : 2;
+  static constexpr uint32_t kOutside = 0x7ffff000u;      // (views have at most 2^29 bytes)
   int lane, g, col;
   __device__ __forceinline__ Lane(int lane_) : lane(lane_), g(lane_ >> 4), col(lane_ & 15) {}
   __device__ __forceinline__ Lane again() const {        // (what is derived from it is formed again, not kept in registers)
@@ -210,8 +212,12 @@ struct Lane {
     asm volatile("" : "+v"(l));
     return Lane(l);
   }
+  // Whether the lane's piece i lies behind the row's end (D > 64 (W - 1): the last two may).
+  __device__ __forceinline__ bool behind(int i, int D) const { return i >= F::KL - 2 && 64 * i + 16 * g >= (int)kBytes * D; }
+  template <bool ZEROS>
   __device__ __forceinline__ uint32_t key(const Source& s, int i, int D) const {
-    return (uint32_t)(col * s.row[0]) + min(64u * i + 16u * g, (uint32_t)D * kBytes - 16u);
+    const uint32_t at = (uint32_t)(col * s.row[0]) + min(64u * i + 16u * g, (uint32_t)D * kBytes - 16u);
+    return ZEROS && behind(i, D) ? kOutside : at;
   }
   __device__ __forceinline__ uint32_t value(const Source& s, int D) const { return (uint32_t)(4 * g * s.row[1]) + (uint32_t)elements_of(D, col) * kBytes; }
   __device__ __forceinline__ static int elements_of(int D, int col) { return min(col * F::DT, D - F::DT); }
@@ -253,10 +259,12 @@ template <class F>
 struct Keys {
   u32x4 w[F::KL];
   f32x4 scale;
+  // ZEROS: of rows of 16-bit elements, whose infinities must not meet the queries' zeros.  (Codes are finite, or the row's scores are NaNs anyway.)
+  template <bool ZEROS>
   __device__ __forceinline__ void load(const Source& s, int D, const Place& p, const Lane<F>& at) {
     const __amdgpu_buffer_rsrc_t rows = rows_of(s, 0, p);
 #pragma unroll
-    for (int i = 0; i < F::KL; ++i) w[i] = load16(rows, at.key(s, i, D));
+    for (int i = 0; i < F::KL; ++i) w[i] = load16(rows, at.template key<ZEROS && !F::codes>(s, i, D));
     if constexpr (F::codes) scale = __builtin_bit_cast(f32x4, load16(scales_of(s, 0, p), 16 * at.g));
   }
   // k-steps 2 i and 2 i + 1 (codes) or i (16-bit) of load i
@@ -772,7 +780,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
     for (int t = 0; t < 2; ++t) here[t] = Place(src, deal.blk * kBlock + wave * 32 + 16 * t);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      k[t].load(src, a.D, here[t], at);
+      k[t].template load<true>(src, a.D, here[t], at);
       v[t].load(src, a.D, here[t], at);
       next[t] = Place(src, (deal.blk + 1) * kBlock + wave * 32 + 16 * t);
     }
@@ -810,7 +818,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
       for (int t = 0; t < 2; ++t) k_scale[t] = F::codes ? k[t].scale * by : f32x4{by, by, by, by};
       if (i + 1 < stop) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) k[t].load(src, a.D, next[t], at);
+        for (int t = 0; t < 2; ++t) k[t].template load<true>(src, a.D, next[t], at);
       }
       u32x4 p[RT];
       uint32_t seen[RT];
@@ -968,7 +976,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
       for (int t = 0; t < kMine; ++t) {
         place[t] = ahead[t];
-        if (my_keys) k[t].load(src, D, place[t], here);
+        if (my_keys) k[t].template load<false>(src, D, place[t], here);
         if (my_values) v[t].load(src, D, place[t], here);
       }
       look(stage + 1);
@@ -1022,6 +1030,19 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         if (my_keys) {
 #pragma unroll
           for (int c = 0; c < F::KS; ++c) to[((my_tile + t) * F::KS + c) * 64] = k[t].operand(c);
+          if constexpr (!F::codes) {
+            // What lies behind the rows becomes zeros here: addresses of their own cost rows of 256 elements 10 more spilled registers (256 rows over 4 x 8
+            // heads of 8192 fp16 keys 118 -> 158 us).
+            const int D = arguments().D;
+            if (__builtin_expect(D % 64 != 0, 0)) {
+              const Lane<F> here = at.again();
+              uint32_t zero = 0;
+              asm volatile("" : "+v"(zero));       // (formed here, not kept)
+#pragma unroll
+              for (int c = F::KS - 2; c < F::KS; ++c)
+                if (here.behind(c, D)) to[((my_tile + t) * F::KS + c) * 64] = u32x4{zero, zero, zero, zero};
+            }
+          }
           if (F::codes && at.col == 0) *reinterpret_cast<f32x4*>(sc + (my_tile + t) * 16 + 4 * at.g) = k[t].scale * by;
         }
         if (my_values) {

@@ -1039,3 +1039,23 @@ def test_python_refusals_on_the_device():
     assert not out.any() and lse.isneginf().all()
     assert fca.tree_attention(q[:, :, :0], cache, table, lengths).shape == (b, 2 * h, 0, d)
     assert fca.tree_attention(q[:0], cache, table[:0], lengths[:0]).shape == (0, 2 * h, 3, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("t,d", [(1, 16), (3, 48), (2, 80), (33, 96), (60, 112), (1, 176), (40, 240), (2, 64), (70, 128)])
+def test_keys_of_infinite_elements_that_are_seen(kind, t, d):
+    """A score of minus infinity is no weight, wherever in its row the element lies that makes it one; a row that sees no other score is zeros."""
+    query, cache, table, context = problem(2, 2, 2, t, 150, d, 16, kind, kind)
+    elements = (0, d // 2, d - 8, d - 1)
+    query[..., elements] = query[..., elements].abs() + 0.25
+    for i in range(2):
+        n = int(context[i])
+        for j, e in zip((3, 17, 40, n - 1, n, n + t - 1), (*elements, d - 1, d - 5)):
+            cache.k[int(table[i, j // 16]), :, j % 16, e] = -math.inf
+    query[..., d - 5] = query[..., d - 5].abs() + 0.25
+    check_attention(query, cache, table, context)
+    check_attention(query, cache, table, context, random_tree(2, t, 3))
+    for page in table[:, 0].tolist():
+        cache.k[page, :, :, d - 1] = -math.inf
+    check_attention(query, cache, table, torch.tensor([5, 8]).int(), tree_lengths=torch.tensor([min(t, 9), min(t, 4)]).int())
