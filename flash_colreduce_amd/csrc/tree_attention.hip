@@ -150,12 +150,16 @@ __device__ __forceinline__ uint32_t halves_of_e4m3(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HI));
 }
 
+// 1 in the bytes that are e4m3's NaNs, 0x7f and 0xff, else 0.
+__device__ __forceinline__ uint32_t nans_of_e4m3(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; }
+
 // W: D / 64, rounded up.
 template <int CD_, int W>
 struct Form {
   static constexpr int CD = CD_;
   static constexpr bool codes = CD == FCR_DTYPE_INT8 || CD == FCR_DTYPE_E4M3;
   static constexpr bool bf16 = CD == FCR_DTYPE_BF16;
+  static constexpr bool finite = CD == FCR_DTYPE_INT8;   // no element of a row is an infinity or a NaN
   static constexpr int KS = 2 * W;                // k-steps of 32 elements
   static constexpr int DT = 4 * W;                // 16-element tiles of the output; a lane's elements are consecutive
   static constexpr int KL = codes ? W : 2 * W;    // 16-byte loads of a key
@@ -313,36 +317,24 @@ struct Values {
         if constexpr (F::codes) scale[i] = 0.0f;
       }
   }
-  // 16-bit elements that are not finite become 0 (see add_not_finite); returns whether there was one.
+  // Elements that are not finite become 0 (see add_not_finite); returns whether there was one.  (Codes: e4m3's NaNs.)
   __device__ __forceinline__ bool clean() {
-    constexpr uint32_t e = F::bf16 ? 0x7f80u : 0x7c00u;
     uint32_t found = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < F::VW; ++j) {
-        const uint32_t bad = ((w[i][j] & e) == e ? 0xffffu : 0u) | (((w[i][j] >> 16) & e) == e ? 0xffff0000u : 0u);
+        uint32_t bad;
+        if constexpr (F::codes) {
+          bad = nans_of_e4m3(w[i][j]) * 0xffu;
+        } else {
+          constexpr uint32_t e = F::bf16 ? 0x7f80u : 0x7c00u;
+          bad = ((w[i][j] & e) == e ? 0xffffu : 0u) | (((w[i][j] >> 16) & e) == e ? 0xffff0000u : 0u);
+        }
         found |= bad;
         w[i][j] &= ~bad;
       }
     return found != 0;
-  }
-  // Codes that are NaNs become 0, and the scale of their row, in every lane that has it, a NaN: a row that is hidden from some of the
-  // queries must not reach these by a product with their weight of 0.
-  __device__ __forceinline__ void clean_codes(const Lane<F>& at) {
-    if constexpr (F::CD == FCR_DTYPE_E4M3) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t found = 0;
-#pragma unroll
-        for (int j = 0; j < F::VW; ++j) {
-          const uint32_t bad = (((w[i][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-          found |= bad;
-          w[i][j] &= ~(bad * 0xffu);
-        }
-        if ((__ballot(found != 0) >> (16 * at.g)) & 0xffff) scale[i] = __builtin_nanf("");
-      }
-    }
   }
   // Element d (of the lane's DT) of the four rows, as four fp16 or bf16.
   __device__ __forceinline__ u32x2 operand(int d) const {
@@ -474,7 +466,7 @@ __device__ __forceinline__ void add_values(const u32x4 (&v)[F::DT], const u32x4 
     for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(v[d], p[r], st.o[r][d]);
 }
 // Values that are not finite, at keys that only some rows see: in a matrix product 0 * inf would reach the others.  They are 0 there, and
-// come here from the cache: p v for the rows that see the key.  (pos: the first of the 32 keys.  Rare, and as short as can be.)
+// come here from the cache: p v for the rows that see the key, which for e4m3 is always a NaN.  (pos: the first of the 32 keys.  Rare, and as short as can be.)
 template <class F, int RT>
 __device__ __forceinline__ void add_not_finite(const Source& src, int D, int pos, const u32x4 (&p)[RT], const uint32_t (&seen)[RT], const Lane<F>& at,
                                                State<F, RT>& st) {
@@ -489,6 +481,21 @@ __device__ __forceinline__ void add_not_finite(const Source& src, int D, int pos
       for (int r = 0; r < RT; ++r) {
         const int from = 16 * (k >> 2) + at.col;                             // the lane that has this key's weight
         const bool see = (__shfl((int)seen[r], from) >> (4 * t + (k & 3))) & 1;
+        if constexpr (F::codes) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t* const from_row = reinterpret_cast<const uint32_t*>(row + Lane<F>::elements_of(D, 4 * at.again().g + i));
+#pragma unroll
+            for (int j = 0; j < F::VW; ++j) {
+              uint32_t x = from_row[j];
+              x = see ? nans_of_e4m3(x) : 0;
+#pragma unroll
+              for (int d = 0; d < 4; ++d)      // (a NaN or 0 is added)
+                st.o[r][4 * j + d][i] += __builtin_bit_cast(float, (uint32_t)((int32_t)(x << (31 - 8 * d)) >> 31) & 0x7fc00000u);
+            }
+          }
+          continue;
+        }
         const uint32_t two = (uint32_t)__shfl((int)(k & 2 ? p[r][2 * t + 1] : p[r][2 * t]), from);
         const float w = element<F::CD>(k & 1 ? two >> 16 : two, 0);
 #pragma unroll
@@ -831,8 +838,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
         const uint32_t there = there_of(pos, n, there0, there1, at.g);
         v[0].drop(there);
         v[1].drop(there >> 4);
-        if (pos + 32 > context) v[0].clean_codes(at), v[1].clean_codes(at);
-        if constexpr (!F::codes) {
+        if constexpr (!F::finite) {
           if (pos + 32 > context) not_finite = v[0].clean() | v[1].clean();
           not_finite = __any(not_finite);
         }
@@ -852,7 +858,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
 #pragma unroll
         for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(f, p[r], st.o[r][d]);
       }
-      if constexpr (!F::codes) {
+      if constexpr (!F::finite) {
         if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(src, arguments().D, pos, p, seen, at, st);
       }
       if (i + 1 < stop) {
@@ -945,7 +951,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   __shared__ u32x4 operands[2 * kStage];
   __shared__ __attribute__((aligned(16))) float scales[2][2][kKeys];     // of keys, of values
   __shared__ float most[2][kTiles];                                      // the largest scale of a tile's values
-  __shared__ int flags[2][kTiles];                                       // a tile's page is there, and (bit 1) a drafted value was not finite
+  __shared__ int flags[2][kTiles];                                       // a tile's page is there, and (bit 1) one of its values was not finite
   __shared__ float rest[WAVES][RT][16];                                  // powers of two that rows' scores are still to be multiplied by
   __shared__ int scan[WAVES + 2];
   const int wg = range_of(args, blockIdx.x);
@@ -1024,8 +1030,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         flag[t] = place[t].there(src) ? 1 : 0;
         if (my_values && (!flag[t] || pos + 16 > min(context, n))) {
           v[t].drop(there_of(pos, n, flag[t], flag[t], at.g));
-          if (pos + 16 > context) v[t].clean_codes(at);
-          if constexpr (!F::codes) flag[t] |= pos + 16 > context && __any(v[t].clean()) ? 2 : 0;
+          if constexpr (!F::finite) flag[t] |= pos + 16 > context && __any(v[t].clean()) ? 2 : 0;
         }
         if (my_keys) {
 #pragma unroll
@@ -1123,7 +1128,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         for (int d = 0; d < kEarly; ++d) vf[d] = from[d * 64];
         const int f0 = __builtin_amdgcn_readfirstlane(flag[0]), f1 = __builtin_amdgcn_readfirstlane(flag[1]);
         const bool masked = pos + 32 > min(context, n) || !(f0 & f1 & 1);
-        not_finite = !F::codes && ((f0 | f1) & 2) != 0;
+        not_finite = !F::finite && ((f0 | f1) & 2) != 0;
 #pragma unroll
         for (int r = 0; r < RT; ++r) seen[r] = 0xff;
         if (masked) {
@@ -1187,7 +1192,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
         }
       }
       if (run) {
-        if constexpr (!F::codes) {
+        if constexpr (!F::finite) {
           if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(src, arguments().D, pos, p, seen, at, st);
         }
         products_of(0);

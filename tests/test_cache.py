@@ -1059,3 +1059,17 @@ def test_keys_of_infinite_elements_that_are_seen(kind, t, d):
     for page in table[:, 0].tolist():
         cache.k[page, :, :, d - 1] = -math.inf
     check_attention(query, cache, table, torch.tensor([5, 8]).int(), tree_lengths=torch.tensor([min(t, 9), min(t, 4)]).int())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("t,d", [(1, 64), (5, 64), (20, 80), (14, 96), (30, 128), (60, 128), (60, 192), (5, 256), (40, 256)])
+def test_value_codes_that_are_nans_reach_their_own_element_only(dtype, t, d):
+    """Far in front of the drafted tokens, next to them, and among them: the rows that see the code have a NaN where it is, and nowhere else."""
+    query, cache, table, context = problem(2, 2, 2, t, 75, d, 16, E4M3, dtype)
+    codes = cache.v.view(torch.uint8)
+    for i, head, j, e, code in ((0, 0, 74, d - 1, 0x7f), (0, 1, 75 + t // 2, 1, 0xff), (1, 0, 3, d // 2, 0xff), (1, 1, int(context[1]), 0, 0x7f),
+                                (1, 1, int(context[1]) - 1, d - 2, 0xff)):
+        codes[int(table[i, j // 16]), head, j % 16, e] = code
+    check_attention(query, cache, table, context, random_tree(2, t, 3))
+    check_attention(query, cache, table, context, tree_lengths=torch.tensor([t, t // 2]).int())
