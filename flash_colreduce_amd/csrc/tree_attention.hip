@@ -24,7 +24,8 @@
 // of rows that are up to 2^16 larger (an element keeps its 8 bits down to 2^-15 of its row's largest, and is off by 2^-23 of that at most
 // below), the keys' scales multiply the scores, the values' scales the probabilities, in 32 bits, before these are rounded to 11 bits, as
 // the matrix instructions take them.  16-bit caches are multiplied in their own type (probabilities against bf16 values have 8 bits).  The reference m
-// of a row is what its weights p_j vs_j ask for, so that they fit fp16 whatever the scales are; sums and statistics are in 32 bits.
+// of a row is what its weights p_j vs_j ask for, so that they fit fp16 whatever the scales are, the largest near its upper end (see weights); sums and
+// statistics are in 32 bits.
 //
 // Distribution: the (batch, head, row tile) items are cut into blocks of 128 keys, laid end to end, and every workgroup takes the same
 // number of blocks, found from the lengths on the device; or, where that takes little longer, one piece of one item.  Parts of an item that
@@ -88,7 +89,8 @@ constexpr int kBlock = 128;                  // keys of a block
 constexpr int kFirst = 4;                    // words in front of the items in Args::first
 constexpr int kNoPower = 200;                // of a row without a finite element but zeros; above all others
 constexpr float kNone = -3.0e38f;            // reference of a row that has seen no key
-constexpr float kMostWeight = 0x1p15f;       // weights above this raise the reference, to where the largest is in (1/2, 1]
+constexpr float kMostWeight = 65504.0f;      // weights above this (fp16's largest number) raise the reference
+constexpr float kRaised = 9.0f;              // fp16: to where the largest is in (2^8, 2^9]
 constexpr float kMostSum = 0x1p110f;         // and so do sums above this
 
 __device__ __forceinline__ int blocks_of(int n) { return n <= 0 ? 1 : (n + kBlock - 1) / kBlock; }
@@ -387,8 +389,13 @@ __device__ __forceinline__ float rounded(float x) {
 // sees, bit 4 t + i; else every key is seen.  Bound by the vector unit: per score an fma, an exponential (four slots), the sum, the product
 // with the value's scale and half a conversion.  Returns whether some row's reference has to be raised, because a weight might not fit fp16 (the
 // sum of the lane's probabilities times most_v, the largest scale of the 32 values: nothing asks for a maximum of weights) or a sum fp32.
-// A few of the first steps ask for it and hardly any later one: the largest weight may be 2^12 times what the reference was raised for, and
-// nothing needs it to be followed more closely.
+// A few of the first steps ask for it and hardly any later one: a weight may be 2^7 times the one that the reference was raised for, 2^4 where
+// all eight of a lane are as large.
+// In fp16 a row's largest weight is above 2^8 (of scores below 2^24 and scales above 2^-90): others keep their 11 bits down to 2^-22 of it, and what is lost of those below is 2^-33 of it each.
+// (Many keys of little weight share what a few large ones leave: 65536 of them a thousandth, from weights of 2^-26.  Raised to 1 the
+// reference had them lose nine tenths of that.  256 rows over 4 x 8 heads of 8192 keys of 128 elements: 67 us fp16, 72 int8 either way for scores
+// that spread by 1.4 in base 2; 68 -> 74 and 74 -> 84 where they spread by 5.8 and references rise more often.)  bf16 has weights of any size, and
+// the reference is raised to the largest.
 template <bool MASKED, class F, int RT>
 __device__ __forceinline__ bool weights(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], float most_v, const f32x4 (&s)[RT][2],
                                         const uint32_t (&seen)[RT], const State<F, RT>& st, float (&sum)[RT], u32x4 (&p)[RT]) {
@@ -419,7 +426,7 @@ __device__ __forceinline__ bool weights(const f32x4 (&k_scale)[2], const f32x4 (
   return __any(raise);
 }
 
-// Raises references so that the largest weight of these keys is in (1/2, 1].
+// Raises references so that the largest weight of these keys is in (2^8, 2^9] (fp16) or (1/2, 1] (bf16).
 template <class F, int RT>
 __device__ __forceinline__ void raise(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], const f32x4 (&s)[RT][2], const uint32_t (&seen)[RT],
                                       State<F, RT>& st) {
@@ -433,6 +440,8 @@ __device__ __forceinline__ void raise(const f32x4 (&k_scale)[2], const f32x4 (&v
       of_sum = fmaxf(of_sum, x);
       of_weights = fmaxf(of_weights, F::codes ? x + __builtin_amdgcn_logf(fabsf(v_scale[e / 4][e % 4])) : x);
     }
+    // (a reference above 2^24 is not followed by 9: its last bit may be worth 16 and more)
+    if constexpr (!F::bf16) of_weights -= fabsf(of_weights) < 0x1p24f ? kRaised : 0.0f;
     const float top = across(fmaxf(of_weights, of_sum - 100.0f), true);
     const float m = top > st.m[r] ? ceilf(top) : st.m[r];
     const float shrink = __builtin_amdgcn_exp2f(st.m[r] - m);

@@ -1073,3 +1073,42 @@ def test_value_codes_that_are_nans_reach_their_own_element_only(dtype, t, d):
         codes[int(table[i, j // 16]), head, j % 16, e] = code
     check_attention(query, cache, table, context, random_tree(2, t, 3))
     check_attention(query, cache, table, context, tree_lengths=torch.tensor([t, t // 2]).int())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("t,d", [(1, 64), (60, 64)])
+@pytest.mark.parametrize("share", [2.0 ** -7, 2.0 ** -10])
+def test_many_small_weights_next_to_large_ones(kind, dtype, t, d, share):
+    """Four keys have nearly all the weight and one element of value; what the others, 65536 of them, share between them is all of the other elements.
+
+    A row's largest weight is above 2^8 where it is rounded to fp16, so that half of fp16's smallest step, 2^-25, is 2^-33 of it.  Sequences share
+    their pages; as many as there are workgroups, so that hardly a sequence is cut and the others are added to the same sums as the four."""
+    b, n = 2 * torch.cuda.get_device_properties(0).multi_processor_count, 65540
+    pages = -(-(n + t) // 16)
+    x = randn(pages * 16, seed=1) * 0.5
+    top = math.log(65536 * math.exp(0.125) / (4 * share))
+    key, value = torch.zeros(pages * 16, d), torch.rand((pages * 16, d), generator=torch.Generator().manual_seed(2)) / 2 + 0.5
+    key[:, 1], value[:, 0], value[:, 1] = x, 0.0, 1.0
+    for j in (0, 32, 64, 96):
+        key[j, 0], key[j, 1] = top, 0.0
+        value[j], value[j, 0] = 0.0, 1.0
+    rows = [r.view(pages, 1, 16, d) for r in (key, value)]
+    if kind in TOP:
+        codes = [ref_codes(r, kind) for r in rows]
+        cache = KVCache(*(c.to(F32).to(kind) for c, _ in codes), *(s.float() for _, s in codes))
+    else:
+        cache = KVCache(*(r.to(kind) for r in rows))
+    query = torch.zeros(1, 1, t, d, dtype=dtype)
+    query[..., :2] = 1
+    table, context = torch.arange(pages).view(1, -1).int(), torch.full((1,), n, dtype=torch.int32)
+    want, want_lse, _, tol_lse = ref_attention(query, cache, table, context, None, 1.0, None)
+    got, lse = fca.tree_attention(query.cuda().expand(b, 1, t, d), device(cache), table.cuda().expand(b, -1), context.cuda().expand(b), None, 1.0,
+                                  return_lse2=True)
+    ds = (d + 8) * 2.0 ** -24 * top + 2.0 ** -21                # (of a score, as in ref_attention)
+    tol = want * ((HALF_STEP[BF16] if kind == BF16 else HALF_STEP[F16]) + 2 * ds + 1.01 * HALF_STEP[dtype]) + 2.0 ** -25
+    if kind != BF16:
+        tol = tol + (n + t) * 2.0 ** -33 / 4
+    assert (tol[..., 1:] < (2.0 ** -6 if BF16 in (kind, dtype) else 2.0 ** -7) * want[..., 1:]).all()
+    assert ((got.cpu().double() - want).abs() <= tol).all(), ((got.cpu().double() - want).abs() / tol).max()
+    assert ((lse.cpu().double() - want_lse).abs() <= tol_lse).all()
