@@ -35,7 +35,8 @@ class KVCache(NamedTuple):
     which need k_scale and v_scale, fp32 (pages, heads, page_size): a row stands for its codes times its scale.
 
     D is a multiple of 16 up to 256, page_size a multiple of 16 (one page per sequence is a cache that is not paged).  The tensors may
-    be views (keys and values in one allocation, pages of token-major rows) as far as include/fcr.h describes.  A page number of a table
+    be views (keys and values in one allocation, pages of token-major rows) as far as include/fcr.h describes; a cache that is written may not be an
+    expanded one, nor one whose keys and values share memory.  A page number of a table
     that is negative or not below `pages` is not there: nothing is written to it, its rows read as zeros, nothing attends to its keys."""
     k: torch.Tensor
     v: torch.Tensor

@@ -406,6 +406,7 @@ int fcr_cache_write(const fcr_cache* cache, const int32_t* table, int64_t table_
   p.used = cache->D / 16;
   const int64_t blocks = (((int64_t)p.rows << p.lanes_log2) + kThreads - 1) / kThreads;
   if (blocks >= kMaxBlocks / 2) return fail(FCR_E_SHAPE, "too many rows for one call");
+  if ((rc = check_written(*cache, "cache"))) return rc;
   const dim3 grid((unsigned)blocks, 2);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == FCR_DTYPE_F16) launch_write<FCR_DTYPE_F16>(cache->dtype, p, grid, s);
@@ -480,6 +481,7 @@ int fcr_cache_keep(const fcr_cache* cache, const int32_t* table, int64_t table_s
   p.chunks.set((uint32_t)((N + chunk - 1) / chunk));
   const int64_t blocks = (int64_t)B * cache->H * p.chunks.d;
   if (blocks >= kMaxBlocks) return fail(FCR_E_SHAPE, "B*H and N are too many for one call");
+  if ((rc = check_written(*into, "into"))) return rc;
   hipLaunchKernelGGL(cache_keep_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
   return launched("cache_keep_kernel");
 }

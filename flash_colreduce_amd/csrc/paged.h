@@ -5,6 +5,7 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include "apart.h"
 #include "div.h"
 #include "fcr.h"
 
@@ -100,6 +101,23 @@ inline int check_cache(const fcr_cache* c, const char* name) {
     }
   }
   return 0;
+}
+
+// A cache that is written: no two of its rows share memory.
+inline int check_written(const fcr_cache& c, const char* name) {
+  char text[128];
+  Dimension rows[2][3], scales[2][2];
+  for (int i = 0; i < 2; ++i) {
+    const int64_t *s = i ? c.v_strides : c.k_strides, *f = i ? c.v_scale_strides : c.k_scale_strides;
+    rows[i][0] = Dimension{c.pages, s[0]}, rows[i][1] = Dimension{c.H, s[1]}, rows[i][2] = Dimension{c.page_size, s[2]};
+    scales[i][0] = Dimension{c.pages, f[0]}, scales[i][1] = Dimension{c.H, f[1]};
+  }
+  const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  if (rows_apart(c.D, rows[0], at(c.k), rows[1], at(c.v), 3, element_bytes(c.dtype)) &&
+      (!has_codes(c.dtype) || rows_apart(c.page_size, scales[0], at(c.k_scale), scales[1], at(c.v_scale), 2, 4)))
+    return 0;
+  snprintf(text, sizeof(text), "%s: rows that share memory (of an expanded view, of keys and values) cannot be written", name);
+  return fcr_detail::fail(FCR_E_STRIDE, text);
 }
 
 inline int check_table(const int32_t* table, int64_t stride, int pages, int page_size, int B) {

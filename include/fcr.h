@@ -292,7 +292,8 @@ int fcr_set_option(int option, long long value);
  * of sequence b.  k and v are [pages, H, page_size, D] of 16-bit elements or of codes, strides in ELEMENTS in the order (page, head, row):
  * 16-byte aligned pointers, strides in multiples of 16 bytes, rows that do not overlap and lie less than 2^25 bytes apart; k_scale and
  * v_scale (codes only) are fp32 [pages, H, page_size] with consecutive scales in a page of a head and 16-byte aligned pages and heads.
- * page_size is a multiple of 16, D one of 16 in [16, 256].
+ * page_size is a multiple of 16, D one of 16 in [16, 256].  Pages and heads may be expanded (strides of 0) where a cache is read only; one that is
+ * written (fcr_cache_write, `into` of fcr_cache_keep) has rows and scales that share no memory, else FCR_E_STRIDE.
  * A row x is held as codes c and a scale s and stands for c s: with a = max |x_d|, FCR_DTYPE_INT8 has s = a / 127 and c = 127 x / a rounded
  * to a whole number, FCR_DTYPE_E4M3 s = a / 448 and c = 448 x / a rounded to such a float (both to nearest, ties to even; of 16-bit elements
  * exactly that).  A row of zeros has s = 0.  A row with an infinity or a NaN has s = NaN and codes 0.

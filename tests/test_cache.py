@@ -1112,3 +1112,90 @@ def test_many_small_weights_next_to_large_ones(kind, dtype, t, d, share):
     assert (tol[..., 1:] < (2.0 ** -6 if BF16 in (kind, dtype) else 2.0 ** -7) * want[..., 1:]).all()
     assert ((got.cpu().double() - want).abs() <= tol).all(), ((got.cpu().double() - want).abs() / tol).max()
     assert ((lse.cpu().double() - want_lse).abs() <= tol_lse).all()
+
+
+OVERLAPS = [dict(k_strides=(16384, 0, 64)), dict(v_strides=(0, 2048, 64)), dict(k_strides=(16384, 1024, 64)), dict(v_strides=(8192, 2048, 64)),
+            dict(k_strides=(64, 256, 1024)), dict(k_scale_strides=(256, 0, 1)), dict(v_scale_strides=(0, 32, 1)), dict(v_scale_strides=(128, 32, 1)),
+            dict(k=1 << 20), dict(k=(1 << 20) + 32), dict(v_scale=1 << 28),
+            dict(k_strides=(32768, 64, 1024), v_strides=(32768, 64, 1024), k=(1 << 20) + 64 * 7)]
+
+
+@pytest.mark.parametrize("fn", ["write", "keep"])
+@pytest.mark.parametrize("over", OVERLAPS, ids=str)
+def test_caches_whose_rows_share_memory_are_not_written(fn, over):
+    """Pages, heads or rows that lie in one another, keys among values."""
+    cache = _c_cache(**{**dict(v=1 << 20, k=1 << 24, k_scale=1 << 28, v_scale=1 << 21), **over})
+    assert (_c_call("write", cache) if fn == "write" else _c_call("keep", _c_cache(), into=cache)) == -4
+    assert b"share memory" in _lib.load().fcr_last_error()
+
+
+def test_rows_that_lie_apart(tmp_path):
+    """csrc/apart.h against the elements themselves: every slice and transpose of a small tensor is apart, whatever overlaps is not."""
+    (tmp_path / "a.cpp").write_text(
+        '#include "apart.h"\n'
+        'extern "C" int one(int64_t row, const int64_t* d, int n) { return fcr_paged::rows_apart(row, (const fcr_paged::Dimension*)d, n); }\n'
+        'extern "C" int two(int64_t row, const int64_t* x, int64_t xa, const int64_t* y, int64_t ya, int n, int bytes) {\n'
+        '  return fcr_paged::rows_apart(row, (const fcr_paged::Dimension*)x, xa, (const fcr_paged::Dimension*)y, ya, n, bytes); }\n')
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "flash_colreduce_amd", "csrc"),
+                    str(tmp_path / "a.cpp"), "-o", str(tmp_path / "a.so")], check=True)
+    lib = ctypes.CDLL(str(tmp_path / "a.so"))
+    i64 = ctypes.c_int64
+
+    def dims(sizes, strides):
+        return (i64 * 6)(*(x for pair in zip(sizes, strides) for x in pair))
+
+    def elements(at, row, sizes, strides):
+        return [at + a * strides[0] + b * strides[1] + c * strides[2] + e
+                for a in range(sizes[0]) for b in range(sizes[1]) for c in range(sizes[2]) for e in range(row)]
+
+    rng = random.Random(5)
+    for _ in range(3000):
+        sizes, row = [rng.randint(1, 4) for _ in range(3)], rng.randint(1, 3)
+        if rng.random() < 0.5:
+            strides = [rng.randint(0, 30) for _ in range(3)]
+        else:              # a tensor with room between its rows, its dimensions in any order
+            span, strides = row + rng.randint(0, 1), [0] * 3
+            for i in rng.sample(range(3), 3):
+                strides[i] = span
+                span *= sizes[i] + rng.randint(0, 1)
+            assert lib.one(i64(row), dims(sizes, strides), 3) == 1
+        x, z = elements(0, row, sizes, strides), rng.randint(0, 60)
+        if lib.one(i64(row), dims(sizes, strides), 3):
+            assert len(set(x)) == len(x)
+        y = elements(z, row, sizes, strides)
+        if lib.two(i64(row), dims(sizes, strides), i64(1000), dims(sizes, strides), i64(1000 + 2 * z), 3, 2):
+            assert len(set(x + y)) == len(x + y)
+        span = max(x) + 1      # far enough apart, either way round
+        if len(set(x)) == len(x) and lib.one(i64(row), dims(sizes, strides), 3):
+            assert lib.two(i64(row), dims(sizes, strides), i64(1000), dims(sizes, strides), i64(1000 + 2 * span), 3, 2) == 1
+            assert lib.two(i64(row), dims(sizes, strides), i64(1000 + 2 * span), dims(sizes, strides), i64(1000), 3, 2) == 1
+    big = dims((2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1), (2 ** 40 - 1, 16, 2 ** 36))      # spans past 64 bits
+    assert lib.one(i64(16), big, 3) == 0
+    # keys and values in one allocation: side by side, by pages, by rows
+    for sizes, strides, z in (((5, 3, 4), (24, 8, 2), 120), ((5, 3, 4), (48, 8, 2), 24), ((5, 3, 4), (48, 4, 12), 2), ((1, 3, 4), (0, 8, 2), 24)):
+        assert lib.two(i64(2), dims(sizes, strides), i64(2 * z), dims(sizes, strides), i64(0), 3, 2) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, I8])
+def test_expanded_caches_are_read_and_not_written(kind):
+    """Heads that share one's rows: read, attended to and kept elsewhere as their copies are; refused where they would be written."""
+    query, cache, table, context = problem(2, 1, 4, 5, 200, 64, 16, kind, BF16)
+    cache, table, context, query = device(cache), table.cuda(), context.cuda(), query.cuda()
+    wide = KVCache(*(None if x is None else x.expand(-1, 2, *x.shape[2:]) for x in cache))
+    copy = KVCache(*(None if x is None else x.contiguous() for x in wide))
+    for a, z in zip(fca.cache_read(wide, table, context, 200), fca.cache_read(copy, table, context, 200)):
+        assert torch.equal(a, z)
+    assert torch.equal(fca.tree_attention(query, wide, table, context), fca.tree_attention(query, copy, table, context))
+    keep = torch.rand((2, 2, 200), generator=torch.Generator().manual_seed(3)).cuda() < 0.4
+    pages = torch.arange(table.numel(), device="cuda").view(2, -1).int()
+    into = [KVCache.zeros(pages.numel(), 2, 16, 64, kind) for _ in range(2)]
+    counts = [fca.cache_keep(c, table, context, keep, i, pages) for c, i in zip((wide, copy), into)]
+    assert torch.equal(*counts) and all(a is None or torch.equal(a, z) for a, z in zip(*into))
+    x = randn(2, 2, 3, 64, seed=9, dtype=BF16).cuda()
+    for bad in (wide, cache._replace(v=cache.k)):
+        heads = bad.k.shape[1]
+        with pytest.raises(_lib.FcrError, match="share memory"):
+            fca.cache_write(bad, x[:, :heads], x[:, :heads], table, context)
+        with pytest.raises(_lib.FcrError, match="share memory"):
+            fca.cache_keep(KVCache.zeros(cache.k.shape[0], heads, 16, 64, kind), table, context, keep[:, :heads], bad, pages)
