@@ -138,7 +138,8 @@ def cache_write(cache: KVCache, key: torch.Tensor, value: torch.Tensor, table: t
     a = max |x_d| (ties to even); 16-bit caches hold x rounded.  A row with an infinity or a NaN reads back as NaN from a cache of
     codes.  table is int32 (B, pages per sequence); start and counts are int32 (B,), or (B, H) where the heads of a
     sequence differ in length.  With counts only the first counts[b] tokens are written.  Positions outside the table, or on a page
-    that is not there, are skipped.  No row may be the place of two tokens (a page shared between sequences must not be written)."""
+    that is not there, are skipped.  No row may be the place of two tokens (a page shared between sequences must not be written).
+    At most 2^31 - 256 rows times D / 16 (rounded up to a power of two) in one call."""
     if _host().cache_write(cache, key, value, table, start, counts):
         return
     dev = _check_cache(cache)
@@ -165,7 +166,7 @@ def cache_write(cache: KVCache, key: torch.Tensor, value: torch.Tensor, table: t
 def cache_read(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor, n: int, *, out_dtype: Optional[torch.dtype] = None):
     """Positions 0 .. n-1 of every sequence and head as (key, value), each a contiguous (B, H, n, D) of out_dtype (fp16, bf16 or fp32; by
     default the cache's type, bf16 for codes), the form that flash_colreduce takes.  A code times its scale is formed in fp32 and rounded
-    once.  Rows from lengths[b] (or lengths[b, h]) on are zeros."""
+    once.  Rows from lengths[b] (or lengths[b, h]) on are zeros.  At most 2^31 - 256 rows times D / 16 (rounded up to a power of two) in one call."""
     kv = _host().cache_read(cache, table, lengths, n, out_dtype)
     if kv is not None:
         return kv

@@ -345,6 +345,10 @@ int lanes_log2_of(int D) {
   return l;
 }
 
+// Lanes of a launch over heads * n rows of keys; another as many take the values, and a launch has fewer than 2^32.
+constexpr int64_t kMostLanes = (kMaxBlocks / 2 - 1) * kThreads;
+bool too_many_rows(int64_t heads, int64_t n, int D) { return heads * n > (kMostLanes >> lanes_log2_of(D)); }   // (each at most 2^30)
+
 template <int IN>
 void launch_write(int code, const WriteArgs& p, dim3 grid, hipStream_t s) {
   switch (code) {
@@ -380,8 +384,8 @@ int fcr_cache_write(const fcr_cache* cache, const int32_t* table, int64_t table_
   if (!key || !value || !key_strides || !value_strides) return fail(FCR_E_NULL, "null pointer argument");
   if (!tensor_dtype(dtype)) return fail(FCR_E_DTYPE, "dtype must be FCR_DTYPE_F16, FCR_DTYPE_BF16 or FCR_DTYPE_F32");
   const int H = cache->H;
-  if (T < 1 || T > (1 << 30) || (int64_t)B * H > (1 << 30) || (int64_t)B * H * T >= (1ll << 31))
-    return fail(FCR_E_SHAPE, "T must be >= 1 and B*H*T below 2^31");
+  if (T < 1 || T > (1 << 30) || (int64_t)B * H > (1 << 30) || too_many_rows((int64_t)B * H, T, cache->D))
+    return fail(FCR_E_SHAPE, "T must be >= 1 and B*H*T*L at most 2^31 - 256, L being D / 16 rounded up to a power of two");
   WriteArgs p;
   const int e = element_bytes(dtype);
   for (int i = 0; i < 2; ++i) {
@@ -405,7 +409,6 @@ int fcr_cache_write(const fcr_cache* cache, const int32_t* table, int64_t table_
   p.lanes_log2 = lanes_log2_of(cache->D);
   p.used = cache->D / 16;
   const int64_t blocks = (((int64_t)p.rows << p.lanes_log2) + kThreads - 1) / kThreads;
-  if (blocks >= kMaxBlocks / 2) return fail(FCR_E_SHAPE, "too many rows for one call");
   if ((rc = check_written(*cache, "cache"))) return rc;
   const dim3 grid((unsigned)blocks, 2);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -426,8 +429,8 @@ int fcr_cache_read(const fcr_cache* cache, const int32_t* table, int64_t table_s
   if (((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15) != 0)
     return fail(FCR_E_STRIDE, "key, value: 16-byte aligned pointers");
   const int H = cache->H;
-  if (N < 1 || N > (1 << 30) || (int64_t)B * H > (1 << 30) || (int64_t)B * H * N >= (1ll << 31))
-    return fail(FCR_E_SHAPE, "N must be >= 1 and B*H*N below 2^31");
+  if (N < 1 || N > (1 << 30) || (int64_t)B * H > (1 << 30) || too_many_rows((int64_t)B * H, N, cache->D))
+    return fail(FCR_E_SHAPE, "N must be >= 1 and B*H*N*L at most 2^31 - 256, L being D / 16 rounded up to a power of two");
   ReadArgs p;
   p.c = pages_of(*cache, table, table_stride, table_pages);
   p.lengths = lengths_of(lengths, lengths_strides);
@@ -440,7 +443,6 @@ int fcr_cache_read(const fcr_cache* cache, const int32_t* table, int64_t table_s
   p.used = cache->D / 16;
   p.D = cache->D;
   const int64_t blocks = (((int64_t)p.rows << p.lanes_log2) + kThreads - 1) / kThreads;
-  if (blocks >= kMaxBlocks / 2) return fail(FCR_E_SHAPE, "too many rows for one call");
   const dim3 grid((unsigned)blocks, 2);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (cache->dtype) {

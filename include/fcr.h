@@ -323,6 +323,7 @@ typedef struct fcr_cache {
  * Writes T tokens per sequence: key and value are [B,H,T,D] of `dtype` (FCR_DTYPE_F16, _BF16, _F32; unit d stride, 16-byte aligned
  * rows), token t goes to position start + t.  With counts (may be NULL) only the first counts tokens of a sequence are written.
  * Positions behind the table are not written.  Two tokens must not be given the same row.
+ * Limit (FCR_E_SHAPE): B * H * T * L at most 2^31 - 256, where L is D / 16 rounded up to a power of two (the lanes that take a row).
  */
 int fcr_cache_write(const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages, const int32_t* start,
                     const int64_t start_strides[2], const int32_t* counts, const int64_t counts_strides[2], const void* key,
@@ -331,7 +332,7 @@ int fcr_cache_write(const fcr_cache* cache, const int32_t* table, int64_t table_
 
 /*
  * Reads positions 0 .. N-1 back: key and value are contiguous [B,H,N,D] of out_dtype, c s in fp32 rounded once.  Rows from `lengths` on
- * (and behind the table) are zeros.
+ * (and behind the table) are zeros.  Limit (FCR_E_SHAPE): B * H * N * L at most 2^31 - 256, L as above.
  */
 int fcr_cache_read(const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages, const int32_t* lengths,
                    const int64_t lengths_strides[2], void* key, void* value, int out_dtype, int B, int N, void* stream);

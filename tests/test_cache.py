@@ -1199,3 +1199,18 @@ def test_expanded_caches_are_read_and_not_written(kind):
             fca.cache_write(bad, x[:, :heads], x[:, :heads], table, context)
         with pytest.raises(_lib.FcrError, match="share memory"):
             fca.cache_keep(KVCache.zeros(cache.k.shape[0], heads, 16, 64, kind), table, context, keep[:, :heads], bad, pages)
+
+
+@pytest.mark.parametrize("d,lanes", [(64, 4), (80, 8), (256, 16)])
+def test_rows_of_one_call_without_a_device(d, lanes):
+    """B * H * T * L up to 2^31 - 256: a call of as many rows gets as far as the next refusal."""
+    strides = (16 * 8 * d, 16 * d, d)
+    cache = _c_cache(H=8, D=d, page_size=16, k_strides=strides, v_strides=strides, k=1 << 20, v=1 << 20)
+    most, xs = (2 ** 31 - 256) // (64 * lanes), (64 * d, 8 * d, d, 1)
+    assert _c_call("write", cache, B=8, T=most, xs=xs) == -4 and b"share memory" in _lib.load().fcr_last_error()
+    assert _c_call("write", cache, B=8, T=most + 1, xs=xs) == -3 and b"2^31 - 256" in _lib.load().fcr_last_error()
+    assert _c_call("read", cache, B=8, N=most + 1) == -3 and b"2^31 - 256" in _lib.load().fcr_last_error()
+    for n in (1 << 30, (1 << 30) - 1):       # (products past 64 bits)
+        assert _c_call("write", cache, B=1 << 27, T=n, xs=xs) == -3 and _c_call("read", cache, B=1 << 27, N=n) == -3
+    header = open(os.path.join(ROOT, "include", "fcr.h")).read()
+    assert "B * H * T * L at most 2^31 - 256" in header and "B * H * N * L at most 2^31 - 256" in header
