@@ -35,6 +35,7 @@
 
 #include <algorithm>
 
+#include "deal.h"
 #include "paged.h"
 
 #ifndef FCR_PART
@@ -85,15 +86,12 @@ __device__ __forceinline__ const Args& arguments() {
   return *(const Args*)p;
 }
 
-constexpr int kBlock = 128;                  // keys of a block
 constexpr int kFirst = 4;                    // words in front of the items in Args::first
 constexpr int kNoPower = 200;                // of a row without a finite element but zeros; above all others
 constexpr float kNone = -3.0e38f;            // reference of a row that has seen no key
 constexpr float kMostWeight = 65504.0f;      // weights above this (fp16's largest number) raise the reference
 constexpr float kRaised = 9.0f;              // fp16: to where the largest is in (2^8, 2^9]
 constexpr float kMostSum = 0x1p110f;         // and so do sums above this
-
-__device__ __forceinline__ int blocks_of(int n) { return n <= 0 ? 1 : (n + kBlock - 1) / kBlock; }
 
 // Keys of a sequence: those of the context, then those of the drafted tokens.
 __device__ __forceinline__ void keys_of(const Args& a, int b, int h, int& context, int& n) {
@@ -680,30 +678,17 @@ struct Deal {
       total += round;
     }
     const int per = (int)a.all.of((uint32_t)(total + a.wgs - 1));
-    // Pieces of one item each, a workgroup for each, where some number of blocks a little above `per` makes them no more than the workgroups.  A
-    // second piece costs a workgroup of many rows as much as 2.6 blocks (first stage, partial results, code that runs for the first time), and row
-    // tiles whose pieces are cut alike read the same keys at the same time.  256 rows over 4 x 8 heads of 8192 keys of 128 elements: 77 -> 73 us bf16,
-    // 79 -> 74 int8; 32 rows: 53 -> 35 bf16, 36 -> 34 int8; 40 rows over 3 x 7 heads of 30000 keys bf16 139 -> 97.  Few rows of one tile
-    // (8 x 8 heads of 8192 keys, one token: 55 -> 50 bf16, 36 -> 33 int8) lose 0.7 us where there is none, too much for less than 8 blocks.
     int most = 0;
-    if (entries <= THREADS && (TALL || a.row_tiles > 1 || per >= 8)) {
+    if (pieces_are_tried(entries, THREADS, per, a.row_tiles, TALL)) {
       const int blocks = tid < entries ? mine / weight : 0;
-      const int limit = per + (TALL ? 2 : 0) + min(per / 8, a.row_tiles > 1 ? 6 : TALL ? 0 : 2);
-      int p = limit;                                    // (first whether there is one)
-      for (bool found = false;;) {
-        const int pieces = (int)((uint32_t)(blocks + p - 1) / (uint32_t)p) * weight;
-        int sum;
+      int pieces, before, sum;
+      most = most_of(per, most_allowed(per, a.row_tiles, TALL), [&](int p) {
+        pieces = pieces_of(blocks, p) * weight;
         __syncthreads();
-        const int before = in_front(pieces, sum);
-        const bool fits = __builtin_amdgcn_readfirstlane(sum) <= a.wgs;
-        if (!found && !fits) break;
-        if (fits && (found || p == per)) {
-          most = p, mine = pieces, start = before, round = total = sum;
-          break;
-        }
-        p = found ? p + 1 : per;                        // (`limit` again at most)
-        found = true;
-      }
+        before = in_front(pieces, sum);
+        return __builtin_amdgcn_readfirstlane(sum) <= a.wgs;
+      });
+      if (most) mine = pieces, start = before, round = total = sum;
     }
     const int unit = most ? 1 : per;
     if (wg == 0 && tid == 0) a.first[0] = most ? most : per;
@@ -728,11 +713,11 @@ struct Deal {
     b = by_head ? (int)a.heads.of((uint32_t)entry) : entry;
     h = by_head ? entry - b * a.H : 0;
     look(a);
-    const int pieces = most ? (int)((uint32_t)(nb + most - 1) / (uint32_t)most) : nb;
+    const int pieces = most ? pieces_of(nb, most) : nb;
     int item_of_entry = (int)((uint32_t)in / (uint32_t)pieces);
     blk = in - item_of_entry * pieces;
-    if (most) {                                         // (the last of ceil(nb / most) pieces of equal length has a block at least)
-      const int length = (int)((uint32_t)(nb + pieces - 1) / (uint32_t)pieces);
+    if (most) {
+      const int length = piece_length(nb, pieces);
       blk *= length;
       at = 0, end = min(length, nb - blk);
     }
@@ -929,8 +914,6 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
   } while (deal.next(arguments()));
 }
 
-// Column tiles per wave: two, where their sums and queries leave room in 256 registers.
-constexpr int tall_tiles(int w) { return w <= 2 ? 2 : 1; }
 // Keys of a stage: two stages in LDS, of one workgroup of eight waves, or of two of four.
 constexpr int tall_keys(int w, int waves) { return w == 1 || (w == 2 && waves == 8) ? 128 : 64; }
 
@@ -1255,7 +1238,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(Args a, int tile_rows, i
   const int per = constant_at(a.first), from = constant_at(told), others = constant_at(told + 1);
   if (others <= 0) return;
   // workgroups behind the first (no more than there are, should lengths have changed under the call)
-  const int more = min((int)(((uint32_t)others + (uint32_t)per - 1) / (uint32_t)per), a.wgs - 1 - from);
+  const int more = min(followers(others, per), a.wgs - 1 - from);
   const int bh = (int)a.per_head.of((uint32_t)item), tile = item - bh * a.row_tiles;
   const int rows = min(tile_rows, a.rows - tile * tile_rows);
   const int units = 256 / shares, mine = (int)threadIdx.x / units;
@@ -1348,19 +1331,16 @@ using fcr_detail::fail;
 using fcr_detail::launched;
 
 struct Plan {
-  int form;                  // 1: tree_attention_kernel; 4, 8: tall_attention_kernel of as many waves
+  int form;                  // see form_of
   int tile_rows, row_tiles, wgs;
   int64_t items, first_bytes, bytes;
 };
 // What depends on sizes alone.  false: too large.
 bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Plan& p) {
   const int64_t rows = (int64_t)T * G;
-  const int w = (D + 63) / 64, tall = 16 * tall_tiles(w);
-  // Both sides, us, at 4 sequences x 8 heads x 8192 keys, int8 (bf16): 48 rows of 64 elements 33 (31) by form 1, 37 (33) by form 4, 64 rows 38
-  // (35) and 38 (34); of 128 elements 42 (45) and 47 (46), 48 (52) and 49 (47); 48 rows of 256 elements 59 (89) by form 1, 62 (61) by form 8, 64
-  // rows 69 (108) and 65 (67); 128 rows of 128 elements 58 (57) by form 4, 60 (64) by form 8, 192 rows 77 (79) and 72 (74).
-  p.form = rows <= (w <= 2 || codes ? 48 : 16) ? 1 : rows <= 4 * tall && w <= 2 ? 4 : 8;
-  p.tile_rows = p.form == 1 ? 16 : tall * p.form;
+  const int w = (D + 63) / 64;
+  p.form = form_of(rows, w, codes);
+  p.tile_rows = rows_of_tile(p.form, w);
   const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.items = (int64_t)B * H * tiles;
   const int64_t blocks = p.items * ((capacity + kBlock - 1) / kBlock);

@@ -1214,3 +1214,77 @@ def test_rows_of_one_call_without_a_device(d, lanes):
         assert _c_call("write", cache, B=1 << 27, T=n, xs=xs) == -3 and _c_call("read", cache, B=1 << 27, N=n) == -3
     header = open(os.path.join(ROOT, "include", "fcr.h")).read()
     assert "B * H * T * L at most 2^31 - 256" in header and "B * H * N * L at most 2^31 - 256" in header
+
+
+@pytest.fixture(scope="module")
+def deal(tmp_path_factory):
+    """csrc/deal.h, as the kernels include it."""
+    at = tmp_path_factory.mktemp("deal")
+    (at / "d.cpp").write_text(
+        '#include "deal.h"\nusing namespace fcr_tree;\nextern "C" {\n'
+        'int blocks(int n) { return blocks_of(n); }\n'
+        'int tried(int entries, int threads, int per, int tiles, int tall) { return pieces_are_tried(entries, threads, per, tiles, tall); }\n'
+        'int allowed(int per, int tiles, int tall) { return most_allowed(per, tiles, tall); }\n'
+        'int most(int per, int limit, int wgs, const int* nb, const int* weight, int n, int* last) {\n'
+        '  return most_of(per, limit, [&](int p) { int64_t sum = 0; for (int i = 0; i < n; ++i) sum += (int64_t)pieces_of(nb[i], p) * weight[i];\n'
+        '    *last = p; return sum <= wgs; }); }\n'
+        'int pieces(int nb, int most) { return pieces_of(nb, most); }\nint length(int nb, int pieces) { return piece_length(nb, pieces); }\n'
+        'int behind(int others, int unit) { return followers(others, unit); }\n'
+        'int form(int64_t rows, int w, int codes) { return form_of(rows, w, codes); }\nint tile(int form, int w) { return rows_of_tile(form, w); }\n}\n')
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "flash_colreduce_amd", "csrc"), str(at / "d.cpp"), "-o",
+                    str(at / "d.so")], check=True)
+    lib = ctypes.CDLL(str(at / "d.so"))
+    lib.form.argtypes = [ctypes.c_int64, ctypes.c_int, ctypes.c_int]
+    return lib
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_blocks_are_dealt_once_and_the_join_finds_them(deal, seed):
+    """By the header that the kernels use: every block of every item is one workgroup's, and from what the workgroup with an item's first part tells the join
+    finds the others, one behind the other, in the order of the item's keys.  Pieces of one item each are the longest that are needed, and not longer."""
+    rng = random.Random(seed)
+    for _ in range(12):
+        tall, row_tiles, threads = rng.random() < 0.5, rng.choice([1, 1, 2, 3, 7]), rng.choice([16, 256])
+        entries = [deal.blocks(rng.choice([-5, 0, 1, 127, 128, 129, rng.randint(0, 9000), 8192, 8192])) for _ in range(rng.randint(1, 40))]
+        assert all(e >= 1 for e in entries) and deal.blocks(128) == 1 and deal.blocks(129) == 2
+        heads = rng.choice([1, 1, 2, 8])
+        weight = heads * row_tiles
+        wgs = 8 * rng.randint(1, 64)
+        total = sum(entries) * weight
+        per = -(-total // wgs)
+        most = 0
+        if deal.tried(len(entries), threads, per, row_tiles, tall):
+            limit, last, n = deal.allowed(per, row_tiles, tall), ctypes.c_int(), len(entries)
+            most = deal.most(per, limit, wgs, (ctypes.c_int * n)(*entries), (ctypes.c_int * n)(*[weight] * n), n, ctypes.byref(last))
+            fits = [p for p in range(per, limit + 1) if sum(-(-e // p) for e in entries) * weight <= wgs]
+            assert most == (fits[0] if fits else 0) and (not most or last.value == most)
+        items = [e for e in entries for _ in range(weight)]
+        units = [deal.pieces(e, most) if most else e for e in items]
+        unit = 1 if most else per
+        parts, told = {}, {}
+        for w in range(wgs):
+            at, end = w * unit, min(w * unit + unit, sum(units))
+            while at < end:
+                begun, item = 0, 0
+                while at >= begun + units[item]:
+                    begun += units[item]
+                    item += 1
+                nb, blk = items[item], at - begun
+                if most:
+                    length = deal.length(nb, units[item])
+                    blk *= length
+                    stop = min(nb, blk + length)
+                    at = end
+                else:
+                    stop = min(nb, blk + end - at)
+                    at += stop - blk
+                assert 0 <= blk < stop <= nb
+                if blk == 0:
+                    told[item] = (w, nb - (stop - blk))
+                parts.setdefault(item, []).append((w, blk, stop))
+        for item, nb in enumerate(items):
+            got = parts[item]
+            w, others = told[item]
+            assert got[0][1] == 0 and got[-1][2] == nb and all(x[2] == y[1] for x, y in zip(got, got[1:]))
+            assert [g[0] for g in got] == list(range(w, w + 1 + deal.behind(others, most or per)))
+    assert deal.behind(0, 5) == 0 and deal.behind(-3, 5) == 0
