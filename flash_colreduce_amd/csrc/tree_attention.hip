@@ -64,11 +64,11 @@ struct Args {
   int wgs;                     // workgroups of the launch
   int positions;               // that a row of the table names
 };
-// form: see Plan
-void attention_f16(const Args& a, int w, int form, hipStream_t s);
-void attention_bf16(const Args& a, int w, int form, hipStream_t s);
-void attention_int8(const Args& a, int w, int form, hipStream_t s);
-void attention_e4m3(const Args& a, int w, int form, hipStream_t s);
+// form: see form_of.  false: there is no such kernel
+bool attention_f16(const Args& a, int w, int form, hipStream_t s);
+bool attention_bf16(const Args& a, int w, int form, hipStream_t s);
+bool attention_int8(const Args& a, int w, int form, hipStream_t s);
+bool attention_e4m3(const Args& a, int w, int form, hipStream_t s);
 }  // namespace fcr_tree
 
 namespace {
@@ -1291,38 +1291,40 @@ __global__ void __launch_bounds__(256) tree_join_kernel(Args a, int tile_rows, i
 #endif
 
 template <int CD, int W>
-void launch_w(const Args& a, int form, hipStream_t s) {
+bool launch_w(const Args& a, int form, hipStream_t s) {
   const dim3 grid((unsigned)a.wgs);
-  switch (form) {
-    case 1: hipLaunchKernelGGL((tree_attention_kernel<CD, W>), grid, dim3(256), 0, s, a); break;
-    case 4:
-      if constexpr (W <= 2) hipLaunchKernelGGL((tall_attention_kernel<CD, W, 4>), grid, dim3(256), 0, s, a);
-      break;
-    default: hipLaunchKernelGGL((tall_attention_kernel<CD, W, 8>), grid, dim3(512), 0, s, a); break;
+  if (form == 1) {
+    hipLaunchKernelGGL((tree_attention_kernel<CD, W>), grid, dim3(256), 0, s, a);
+  } else if (form == 8) {
+    hipLaunchKernelGGL((tall_attention_kernel<CD, W, 8>), grid, dim3(512), 0, s, a);
+  } else {
+    if constexpr (W > 2) return false;
+    else hipLaunchKernelGGL((tall_attention_kernel<CD, W, 4>), grid, dim3(256), 0, s, a);
   }
+  return true;
 }
 template <int CD>
-void launch(const Args& a, int w, int form, hipStream_t s) {
+bool launch(const Args& a, int w, int form, hipStream_t s) {
   switch (w) {
-    case 1: launch_w<CD, 1>(a, form, s); break;
-    case 2: launch_w<CD, 2>(a, form, s); break;
-    case 3: launch_w<CD, 3>(a, form, s); break;
-    default: launch_w<CD, 4>(a, form, s); break;
+    case 1: return launch_w<CD, 1>(a, form, s);
+    case 2: return launch_w<CD, 2>(a, form, s);
+    case 3: return launch_w<CD, 3>(a, form, s);
+    default: return launch_w<CD, 4>(a, form, s);
   }
 }
 }  // namespace
 
 #if FCR_HAS(1)
-void fcr_tree::attention_f16(const Args& a, int w, int form, hipStream_t s) { launch<FCR_DTYPE_F16>(a, w, form, s); }
+bool fcr_tree::attention_f16(const Args& a, int w, int form, hipStream_t s) { return launch<FCR_DTYPE_F16>(a, w, form, s); }
 #endif
 #if FCR_HAS(2)
-void fcr_tree::attention_bf16(const Args& a, int w, int form, hipStream_t s) { launch<FCR_DTYPE_BF16>(a, w, form, s); }
+bool fcr_tree::attention_bf16(const Args& a, int w, int form, hipStream_t s) { return launch<FCR_DTYPE_BF16>(a, w, form, s); }
 #endif
 #if FCR_HAS(3)
-void fcr_tree::attention_int8(const Args& a, int w, int form, hipStream_t s) { launch<FCR_DTYPE_INT8>(a, w, form, s); }
+bool fcr_tree::attention_int8(const Args& a, int w, int form, hipStream_t s) { return launch<FCR_DTYPE_INT8>(a, w, form, s); }
 #endif
 #if FCR_HAS(4)
-void fcr_tree::attention_e4m3(const Args& a, int w, int form, hipStream_t s) { launch<FCR_DTYPE_E4M3>(a, w, form, s); }
+bool fcr_tree::attention_e4m3(const Args& a, int w, int form, hipStream_t s) { return launch<FCR_DTYPE_E4M3>(a, w, form, s); }
 #endif
 
 #if FCR_HAS(0)
@@ -1410,12 +1412,14 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
   a.wgs = plan.wgs;
   const int w = (D + 63) / 64;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  bool there;
   switch (cache->dtype) {
-    case FCR_DTYPE_F16: attention_f16(a, w, plan.form, s); break;
-    case FCR_DTYPE_BF16: attention_bf16(a, w, plan.form, s); break;
-    case FCR_DTYPE_INT8: attention_int8(a, w, plan.form, s); break;
-    default: attention_e4m3(a, w, plan.form, s); break;
+    case FCR_DTYPE_F16: there = attention_f16(a, w, plan.form, s); break;
+    case FCR_DTYPE_BF16: there = attention_bf16(a, w, plan.form, s); break;
+    case FCR_DTYPE_INT8: there = attention_int8(a, w, plan.form, s); break;
+    default: there = attention_e4m3(a, w, plan.form, s); break;
   }
+  if (!there) return fail(FCR_E_SHAPE, "no kernel for these sizes");
   if ((rc = launched("tree_attention_kernel"))) return rc;
   Div groups, pieces;
   const int rows = std::min(plan.tile_rows, a.rows), shares = plan.wgs >= 16 * plan.items ? 8 : 1, units = 256 / shares;

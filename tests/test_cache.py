@@ -1238,6 +1238,16 @@ def deal(tmp_path_factory):
     return lib
 
 
+def test_forms_have_kernels_and_tiles_that_hold_rows(deal):
+    """Four waves only for rows of at most 128 elements; a tile of form 4 holds all rows, so that none is left to a second one."""
+    for w in range(1, 5):
+        for codes in (0, 1):
+            forms = [deal.form(rows, w, codes) for rows in range(1, 400)]
+            assert sorted(set(forms)) == ([1, 4, 8] if w <= 2 else [1, 8]) and forms == sorted(forms)
+            assert all(f != 4 or rows <= deal.tile(4, w) for rows, f in enumerate(forms, 1))
+            assert deal.form(1 << 24, w, codes) == 8 and deal.tile(1, w) == 16 and deal.tile(8, w) in (128, 256)
+
+
 @pytest.mark.parametrize("seed", range(40))
 def test_blocks_are_dealt_once_and_the_join_finds_them(deal, seed):
     """By the header that the kernels use: every block of every item is one workgroup's, and from what the workgroup with an item's first part tells the join
