@@ -46,18 +46,14 @@ def hipcc_path() -> str:
     return exe
 
 
-def build(verbose: bool = True, extra_flags=(), only=None) -> str:
-    """Compiles the parts of the sources side by side (one hipcc each) and links them into libfcr.so.  `only`: names of the
-    sources to compile; the objects of the others are those of the last build."""
+def build(verbose: bool = True, extra_flags=()) -> str:
+    """Compiles the parts of all sources side by side (one hipcc each) and links them into libfcr.so."""
     hipcc = hipcc_path()
     os.makedirs(OBJ_DIR, exist_ok=True)
-    jobs, objects = [], []
+    jobs = []
     for name, parts in SOURCES.items():
         for part in parts:
             obj = os.path.join(OBJ_DIR, f"{name}_part{part}.o")
-            objects.append(obj)
-            if only is not None and name not in only and os.path.exists(obj):
-                continue
             # a part uses a subset of the file's helpers
             cmd = [hipcc, *HIPCC_FLAGS, *SOURCE_FLAGS.get(name, ()), *extra_flags, f"-DFCR_PART={part}", "-Wno-unused-function", "-I", INCLUDE,
                    "-c", os.path.join(CSRC, name + ".hip"), "-o", obj]
@@ -67,7 +63,7 @@ def build(verbose: bool = True, extra_flags=(), only=None) -> str:
     failed = [cmd for cmd, _, proc in jobs if proc.wait() != 0]
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
-    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-fno-gpu-rdc", *objects, "-o", LIB]
+    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-fno-gpu-rdc", *[obj for _, obj, _ in jobs], "-o", LIB]
     if verbose:
         print(" ".join(link), flush=True)
     subprocess.run(link, check=True)

@@ -299,3 +299,32 @@ def test_which_calls_have_room_for_the_word_of_both_sweeps():
     for shape in ((4, 128, 700, 128), (32, 512, 32768, 128), (68, 1090, 8104, 128), (300, 2000, 2000, 256), (216, 1562, 1562, 256), (1, 6891, 8176, 32),
                   (1, 7061, 7061, 32), (246, 314, 8281, 96), (80, 570, 570, 48), (85, 601, 601, 32), (60, 800, 800, 96), (72, 670, 670, 80)):
         assert more(*shape) == 0, shape
+
+
+def test_a_build_compiles_every_part_of_every_source(tmp_path, monkeypatch):
+    """Objects that are there already are not linked as they are: headers or flags may have changed since."""
+    import inspect
+
+    from flash_colreduce_amd import build as build_module
+
+    ran = []
+
+    class Ended:
+        def __init__(self, cmd):
+            ran.append(cmd)
+
+        def wait(self):
+            return 0
+
+    parts = [f"{name}_part{part}.o" for name, numbers in build_module.SOURCES.items() for part in numbers]
+    for name in parts:
+        (tmp_path / name).write_bytes(b"")
+    monkeypatch.setattr(build_module, "OBJ_DIR", str(tmp_path))
+    monkeypatch.setattr(build_module, "hipcc_path", lambda: "hipcc")
+    monkeypatch.setattr(build_module.subprocess, "Popen", Ended)
+    monkeypatch.setattr(build_module.subprocess, "run", lambda cmd, check: ran.append(cmd))
+    build_module.build(verbose=False)
+    *compiled, link = ran
+    assert sorted(os.path.basename(cmd[cmd.index("-o") + 1]) for cmd in compiled) == sorted(parts)
+    assert [os.path.basename(x) for x in link if x.endswith(".o")] == parts
+    assert set(inspect.signature(build_module.build).parameters) == {"verbose", "extra_flags"}
