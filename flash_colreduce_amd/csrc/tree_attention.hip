@@ -757,11 +757,10 @@ __device__ __forceinline__ int range_of(const Args& a, int block) { return (bloc
 
 template <int CD, int W>
 __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) tree_attention_kernel(Args args) {
-  constexpr int RT = 1;                                 // tiles of 16 rows: two read the cache once for both, but were never faster
   using F = Form<CD, W>;
   constexpr int kWaves = 4;
   __shared__ float joined[kWaves * 4 * F::DT * 64];     // [wave][register][tile][lane]
-  __shared__ float stats[kWaves][RT][16][2];            // m, l
+  __shared__ float stats[kWaves][16][2];                // m, l
   __shared__ int scan[kWaves + 2];
   const int wg = range_of(args, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -771,7 +770,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
   do {
     const Args& a = arguments();
     const int b = deal.b, h = deal.h, n = deal.n, context = deal.context, stop = deal.stop();
-    const int row0 = deal.tile * 16 * RT;
+    const int row = deal.tile * 16 + at.col;
     Keys<F> k[2];
     Values<F> v[2];
     // (places are a block further ahead than the loads, which need them)
@@ -785,9 +784,9 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
       v[t].load(src, a.D, here[t], at);
       next[t] = Place(src, (deal.blk + 1) * kBlock + wave * 32 + 16 * t);
     }
-    Queries<F, RT> q;
+    Queries<F, 1> q;
     float by = a.scale2;
-    q.load(a, b, h, row0, at);
+    q.load(a, b, h, deal.tile * 16, at);
     if (F::codes && a.bf16) {
       int up = q.power(0);
       up = up == kNoPower ? 0 : up;
@@ -795,24 +794,19 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
       by = __builtin_amdgcn_ldexpf(by, -up);            // (of the lane's row)
     }
     q.arrive();
-    State<F, RT> st;
+    State<F, 1> st;
     st.clear();
     for (int i = deal.blk; i < stop; ++i) {
       const int pos = i * kBlock + wave * 32;
       if (pos >= n) break;                              // (a wave's later blocks lie behind this one)
 #pragma unroll
       for (int t = 0; t < 2; ++t) then[t] = Place(src, pos + 2 * kBlock + 16 * t);
-      f32x4 s[RT][2];
+      f32x4 s[1][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
+        s[0][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int r = 0; r < RT; ++r) s[r][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < F::KS; ++c) {
-          const u32x4 f = k[t].operand(c);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(f, q.w[r][c], s[r][t]);
-        }
+        for (int c = 0; c < F::KS; ++c) s[0][t] = mma<F::bf16>(k[t].operand(c), q.w[0][c], s[0][t]);
       }
       f32x4 k_scale[2];
 #pragma unroll
@@ -821,10 +815,8 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
 #pragma unroll
         for (int t = 0; t < 2; ++t) k[t].template load<true>(src, a.D, next[t], at);
       }
-      u32x4 p[RT];
-      uint32_t seen[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) seen[r] = 0xff;
+      u32x4 p[1];
+      uint32_t seen[1] = {0xff};
       const bool there0 = here[0].there(src), there1 = here[1].there(src);
       const bool masked = pos + 32 > min(context, n) || !there0 || !there1;
       bool not_finite = false;
@@ -836,8 +828,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
           if (pos + 32 > context) not_finite = v[0].clean() | v[1].clean();
           not_finite = __any(not_finite);
         }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) seen[r] = seen_by(a, b, row0 + 16 * r + at.col, pos, context, there, at.g);
+        seen[0] = seen_by(a, b, row, pos, context, there, at.g);
       }
       const f32x4 v_scale[2] = {v[0].scale, v[1].scale};
       float most_v = F::codes ? 0.0f : 1.0f;
@@ -845,15 +836,11 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
 #pragma unroll
         for (int e = 0; e < 8; ++e) most_v = fmaxf(most_v, fabsf(v_scale[e / 4][e % 4]));
       }
-      weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
+      weigh<F, 1>(k_scale, v_scale, most_v, s, masked, seen, st, p);
 #pragma unroll
-      for (int d = 0; d < F::DT; ++d) {
-        const u32x4 f = joined_operand(v[0].operand(d), v[1].operand(d));
-#pragma unroll
-        for (int r = 0; r < RT; ++r) st.o[r][d] = mma<F::bf16>(f, p[r], st.o[r][d]);
-      }
+      for (int d = 0; d < F::DT; ++d) st.o[0][d] = mma<F::bf16>(joined_operand(v[0].operand(d), v[1].operand(d)), p[0], st.o[0][d]);
       if constexpr (!F::finite) {
-        if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(src, arguments().D, pos, p, seen, at, st);
+        if (__builtin_expect(not_finite, 0)) add_not_finite<F, 1>(src, arguments().D, pos, p, seen, at, st);
       }
       if (i + 1 < stop) {
 #pragma unroll
@@ -866,51 +853,45 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) t
     // join the four waves
     const Args& a_end = arguments();
     const bool final = deal.blk == 0 && stop == deal.nb;
-    float* const slot = a_end.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * (16 * RT) * (a_end.D + 4);
+    float* const slot = a_end.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * 16 * (a_end.D + 4);
     if (deal.blk == 0 && threadIdx.x == 0) deal.tell(a_end, wg);
     __syncthreads();
+    const float sum = across(st.l[0], false);
+    if (at.g == 0) stats[wave][at.col][0] = st.m[0], stats[wave][at.col][1] = sum;
+    __syncthreads();
+    float m = stats[0][at.col][0], l = 0.0f;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const float l = across(st.l[r], false);
-      if (at.g == 0) stats[wave][r][at.col][0] = st.m[r], stats[wave][r][at.col][1] = l;
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[w][at.col][0]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) l += stats[w][at.col][1] * __builtin_amdgcn_exp2f(stats[w][at.col][0] - m);
+    const float shrink = __builtin_amdgcn_exp2f(st.m[0] - m);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < F::DT; ++d) joined[((wave * 4 + i) * F::DT + d) * 64 + at.lane] = st.o[0][d][i] * shrink;
+    __syncthreads();
+    // wave w writes register w of every tile: query col, the elements of lane 4 g + w
+    float x[F::DT];
+#pragma unroll
+    for (int d = 0; d < F::DT; ++d) {
+      x[d] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) x[d] += joined[((w * 4 + wave) * F::DT + d) * 64 + at.lane];
+    }
+    const int d0 = Lane<F>::elements_of(a_end.D, 4 * at.g + wave);
+    const bool first = wave == 0 && at.g == 0;
+    if (row < a_end.rows) {
+      if (final) {
+        const Output out(a_end, b, h, row, l);
+        emit<F>(a_end, out, d0, x, 1.0f / l);
+        if (a_end.lse && first) a_end.lse[out.row] = out.none ? -INFINITY : m + __builtin_amdgcn_logf(l);
+      } else {
+        float* const to = slot + (int64_t)at.col * (a_end.D + 4);
+        emit_part<F>(to, d0, x);
+        if (first) to[0] = m, to[1] = l;
+      }
     }
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      float m = stats[0][r][at.col][0], l = 0.0f;
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[w][r][at.col][0]);
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) l += stats[w][r][at.col][1] * __builtin_amdgcn_exp2f(stats[w][r][at.col][0] - m);
-      const float shrink = __builtin_amdgcn_exp2f(st.m[r] - m);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int d = 0; d < F::DT; ++d) joined[((wave * 4 + i) * F::DT + d) * 64 + at.lane] = st.o[r][d][i] * shrink;
-      __syncthreads();
-      // wave w writes register w of every tile: query col, the elements of lane 4 g + w
-      float x[F::DT];
-#pragma unroll
-      for (int d = 0; d < F::DT; ++d) {
-        x[d] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) x[d] += joined[((w * 4 + wave) * F::DT + d) * 64 + at.lane];
-      }
-      const int row = row0 + 16 * r + at.col, d0 = Lane<F>::elements_of(a_end.D, 4 * at.g + wave);
-      const bool first = wave == 0 && at.g == 0;
-      if (row < a_end.rows) {
-        if (final) {
-          const Output out(a_end, b, h, row, l);
-          emit<F>(a_end, out, d0, x, 1.0f / l);
-          if (a_end.lse && first) a_end.lse[out.row] = out.none ? -INFINITY : m + __builtin_amdgcn_logf(l);
-        } else {
-          float* const to = slot + (int64_t)(16 * r + at.col) * (a_end.D + 4);
-          emit_part<F>(to, d0, x);
-          if (first) to[0] = m, to[1] = l;
-        }
-      }
-      __syncthreads();
-    }
   } while (deal.next(arguments()));
 }
 
