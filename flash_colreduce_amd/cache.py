@@ -249,8 +249,9 @@ def tree_attention(query: torch.Tensor, cache: KVCache, table: torch.Tensor, con
     1/sqrt(D).  tree_lengths, int32 (B,): sequences that have fewer than T drafted tokens.
 
     Returns (B, Hq, T, D) of query's type, and with return_lse2 the base-2 log-sum-exp of every row's scores, fp32 (B, Hq, T), as row_lse2 has it.
-    A row that sees nothing (or that the sequence does not have) is zeros, its log-sum-exp -inf.  What hidden rows of the cache hold, NaNs included,
-    has no influence."""
+    A row that sees nothing (or that the sequence does not have, or whose every score is -inf) is zeros, its log-sum-exp -inf.  What hidden rows of the
+    cache hold, NaNs included, has no influence.  Probabilities are rounded to fp16 (bf16 against a bf16 cache) as they multiply the values, sums are fp32.
+    The last bits of a sequence's result depend on how the work was cut, and so on the lengths of the others in the batch."""
     out = _host().tree_attention(query, cache, table, context, tree_mask, scale, tree_lengths, return_lse2)
     if out is not None:
         return out

@@ -7,9 +7,10 @@
 // that is not finite has s = NaN and codes 0, so codes are finite always and such a row reads as NaN.
 // The quotient of 16-bit elements is formed so that the code is the one that exact arithmetic gives (see quotient).
 //
-// All three kernels are bound by memory: 16 elements per lane, 16 bytes and more per load and store.  Measured, D = 128 (a large copy
-// reaches 4.95 TB/s): 32 x 8192 rows fp16 to e4m3 49 us (4.1 TB/s), 8 x 32 heads of up to 9001 e4m3 rows to bf16 332 us (4.9 TB/s), half of
-// 4 x 8 x 32768 bf16 rows kept 96 us (4.2 TB/s; rows of 256 bytes with gaps between them), one token of 64 sequences 5 us, one launch.
+// All three kernels are bound by memory: 16 elements per lane, 16 bytes and more per load and store.  Measured per call, D = 128 (a large copy
+// reaches 4.95 TB/s): 32 x 8192 rows fp16 to e4m3 49 us (4.1 TB/s), fp32 to int8 80 (4.2); 8 x 32 heads of 9001 bf16 rows into a bf16 cache 472 us
+// (5.0 TB/s) and back 441 (5.4), up to 9001 e4m3 rows to bf16 333 (4.9); half of up to 4 x 8 x 32768 bf16 rows kept 67 to 101 us by the drawn lengths
+// (4.5 TB/s; rows of 256 bytes with gaps between them); one token of 64 sequences 4.6 us, one launch.
 
 #include "paged.h"
 
@@ -475,7 +476,7 @@ int fcr_cache_keep(const fcr_cache* cache, const int32_t* table, int64_t table_s
   p.N = N;
   p.pieces.set((uint32_t)(cache->D * element_bytes(cache->dtype) / 16));
   p.H.set((uint32_t)cache->H);
-  // short ranges, but a mask is counted again by every range behind, so no more than 128 of them (4 x 8 x 32768 rows of bf16: 79 us; with 64
+  // short ranges, but a mask is counted again by every range behind, so no more than 128 of them (4 x 8 x 32768 rows of bf16, the kernel alone: 79 us; with 64
   // all workgroups count at one time and copy at another, 85; with 256 80)
   int chunk = 128;
   while ((N + chunk - 1) / chunk > 128) chunk *= 2;

@@ -6,19 +6,20 @@
 //   s_j = scale log2(e) <q, c_j> ks_j,   p_j = 2^(s_j - m),   o = sum_j p_j vs_j v_j / sum_j p_j,   lse2 = m + log2 sum_j p_j.
 //
 // The G query heads of a key head and the drafted tokens are the columns of the matrix instructions, 16 to a tile, in one of two kernels
-// (plan_of has the rule, with both sides measured).  Both form
+// (form_of has the rule, with both sides measured).  Both form
 //   S^T = K Q^T   so that a lane owns one query (lane & 15) and keys 4 g + i of a 16-key tile (g = lane / 16, register i), and
 //   O^T = V^T P^T in which that query stays in the lane.  The 8 keys that a lane feeds to one instruction are keys 4 g + i of two tiles,
 //                 which is what it holds of P: probabilities never leave their lane, softmax statistics are one scalar per lane.
 //                 V^T is formed from rows of V with byte permutes that convert codes on the way.
 // tree_attention_kernel (few rows): bound by reading the cache.  Each wave takes 32 keys of a block of 128, from global memory into
 //   registers without a stop in LDS, and 16 rows; the four waves' results are joined at the end.  32 ragged sequences of up to 16384 e4m3 keys, 8 heads
-//   of 4 queries, D = 128: 156 us, 5.3 TB/s; 8 tokens over 4 x 32 heads of up to 9001 fp16 keys of 64 elements: 48 us, 4.6 TB/s; one token
-//   over 1000 keys 10.8 us, two launches and a chain of loads: lengths, table, keys.
-// tall_attention_kernel (many rows): bound by the vector instructions of the softmax and by the matrix units.  Each wave takes 32 rows (of
+//   of 4 queries, D = 128: 154 to 164 us by the drawn lengths, 5.3 TB/s; 8 tokens over 4 x 32 heads of 9001 fp16 keys of 64 elements: 51 us,
+//   5.8 TB/s; one token over 1000 keys 10.7 us, two launches and a chain of loads: lengths, table, keys.
+// tall_attention_kernel (many rows): bound by how far the vector instructions of the softmax (half of a SIMD's time) run beside the products (a third)
+//   and not behind them.  Each wave takes 32 rows (of
 //   more than 128 elements 16) and all keys; the operands of a block are converted once, by all waves, and lie in LDS as the matrix instructions take them.  64 drafted tokens of 4
-//   query heads over 8 x 8 heads of 32768 int8 keys, D = 128: 265 us, 780 TFLOP/s (1049 with operands formed by every wave from global memory, 341
-//   with one stage in LDS); over 4 x 8 heads of 8192 keys 61 us, a quarter of it what runs once per workgroup.
+//   query heads over 8 x 8 heads of 32768 int8 keys, D = 128: 273 us, 760 TFLOP/s (1049 with operands formed by every wave from global memory, 341
+//   with one stage in LDS); over 4 x 8 heads of 8192 keys 63 us, a quarter of it what runs once per workgroup.
 //
 // Codes are multiplied in fp16, where each of them is exact: bf16 rows of queries are scaled by a power of two to fit, of their own or (many rows)
 // of rows that are up to 2^16 larger (an element keeps its 8 bits down to 2^-15 of its row's largest, and is off by 2^-23 of that at most
@@ -916,7 +917,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   // Rows of 256 elements leave no registers for both halves of a step's values, or for keys next to them.
   constexpr bool kLean = W == 4;
   // The first stage is converted in the loop, and not by code in front of it, which made 16-bit kernels of more than 64 elements spill 5 to 39
-  // registers: 128 rows over 4 x 8 heads of 8192 bf16 keys of 128 elements 57 -> 54 us, 1024 rows of 256 elements 451 -> 360, int8 393 -> 383.
+  // registers: 128 rows over 4 x 8 heads of 8192 bf16 keys of 128 elements 57 -> 54 us, 1024 rows of 256 elements 451 -> 413, int8 393 -> 383.
+  // (fp16 and bf16 rows of 256 elements still spill 15, bf16 of 128 and e4m3 of 256 two.)
   // With 64 elements, where nothing spills, 1 to 10 % are lost.
   constexpr bool kInLoop = W >= 2;
   constexpr int kEarly = W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights

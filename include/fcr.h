@@ -354,7 +354,10 @@ int fcr_cache_keep(const fcr_cache* cache, const int32_t* table, int64_t table_s
  * apart, 0: one mask for all) or, with mask NULL, iff u <= t.  tree_lengths [B] (may be NULL): how many of the T tokens a sequence has; the
  * others are seen by none.  out is contiguous [B, H*G, T, D] of the queries' type: softmax(scale q k^T) v over the keys that a token sees; lse
  * (may be NULL) fp32 [B, H*G, T], the base-2 log-sum-exp of its scores.  A token that sees nothing, or that the sequence does not have, gets zeros and
- * -inf.  What hidden keys and values hold has no influence, whatever it is.
+ * -inf; so does one whose every score is -inf.  What hidden keys and values hold has no influence, whatever it is.
+ * Sums and statistics are fp32; probabilities are rounded to fp16 (bf16 against a bf16 cache) before they multiply the values.  In fp16 a weight keeps
+ * 11 bits down to 2^-22 of its row's largest (a probability times its value's scale), and below 2^-33 of it is 0 (times an infinite value: NaN).  Results do not
+ * depend on timing, but in their last bits on where the work was cut, which follows from the lengths of all sequences of the call.
  * ws: fcr_tree_attention_bytes(B, H, G, T, D, table_pages * page_size) bytes, 16-byte aligned (it depends on the number of compute
  * units: call this with the operands' device current; 0 for sizes that the call refuses), contents irrelevant.
  * Limits (FCR_E_SHAPE): with a mask T <= 46340; T * G <= 2^24; 2^22 tiles of at least 16 rows of a (sequence, head); 2^30 blocks of 128 positions
