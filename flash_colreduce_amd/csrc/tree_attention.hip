@@ -390,7 +390,7 @@ __device__ __forceinline__ float rounded(float x) {
 // sum of the lane's probabilities times most_v, the largest scale of the 32 values: nothing asks for a maximum of weights) or a sum fp32.
 // A few of the first steps ask for it and hardly any later one: a weight may be 2^7 times the one that the reference was raised for, 2^4 where
 // all eight of a lane are as large.
-// In fp16 a row's largest weight is above 2^8 (of scores below 2^24 and scales above 2^-90): others keep their 11 bits down to 2^-22 of it, and what is lost of those below is 2^-33 of it each.
+// In fp16 a row's largest weight is above 2^8 (of scores below 2^24 and scales from 2^-90 to 2^90): others keep their 11 bits down to 2^-22 of it, and what is lost of those below is 2^-33 of it each.
 // (Many keys of little weight share what a few large ones leave: 65536 of them a thousandth, from weights of 2^-26.  Raised to 1 the
 // reference had them lose nine tenths of that.  256 rows over 4 x 8 heads of 8192 keys of 128 elements: 67 us fp16, 72 int8 either way for scores
 // that spread by 1.4 in base 2; 68 -> 74 and 74 -> 84 where they spread by 5.8 and references rise more often.)  bf16 has weights of any size, and
@@ -437,7 +437,12 @@ __device__ __forceinline__ void raise(const f32x4 (&k_scale)[2], const f32x4 (&v
       float x = rounded(s[r][e / 4][e % 4] * k_scale[e / 4][e % 4]);
       x = (seen[r] >> e) & 1u ? x : -INFINITY;
       of_sum = fmaxf(of_sum, x);
-      of_weights = fmaxf(of_weights, F::codes ? x + __builtin_amdgcn_logf(fabsf(v_scale[e / 4][e % 4])) : x);
+      if constexpr (F::codes) {
+        // (an infinite scale does not count: a reference of infinity would leave the row no weights at all)
+        const float of_scale = __builtin_amdgcn_logf(fabsf(v_scale[e / 4][e % 4]));
+        x += of_scale < 200.0f ? of_scale : 0.0f;
+      }
+      of_weights = fmaxf(of_weights, x);
     }
     // (a reference above 2^24 is not followed by 9: its last bit may be worth 16 and more)
     if constexpr (!F::bf16) of_weights -= fabsf(of_weights) < 0x1p24f ? kRaised : 0.0f;

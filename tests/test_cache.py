@@ -1298,3 +1298,23 @@ def test_blocks_are_dealt_once_and_the_join_finds_them(deal, seed):
             assert got[0][1] == 0 and got[-1][2] == nb and all(x[2] == y[1] for x, y in zip(got, got[1:]))
             assert [g[0] for g in got] == list(range(w, w + 1 + deal.behind(others, most or per)))
     assert deal.behind(0, 5) == 0 and deal.behind(-3, 5) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [(I8, F16), (I8, BF16), (E4M3, F16), (E4M3, BF16)])
+@pytest.mark.parametrize("t,d", [(1, 64), (5, 128), (40, 64), (60, 192), (30, 256)])
+def test_scales_that_are_infinite(kind, dtype, t, d):
+    """A value row of an infinite scale is infinite where its codes are not 0, and a NaN where they are, for the rows that see it; log-sum-exps are of the
+    scores alone.  cache_write makes no such scales; a cache that is filled otherwise may have them."""
+    query, cache, table, context = problem(2, 2, 2, t, 300, d, 16, kind, dtype)
+    cache.v.view(torch.uint8)[:, :, :, 3] = 0
+    for i, head, j in ((0, 0, 3), (0, 1, 299), (1, 0, int(context[1])), (1, 1, int(context[1]) + t // 2)):
+        cache.v_scale[int(table[i, j // 16]), head, j % 16] = math.inf
+    check_attention(query, cache, table, context)
+    check_attention(query, cache, table, context, random_tree(2, t, 3))
+    # scores of minus infinity: no weight
+    for i, head, j in ((0, 0, 9), (1, 1, 40)):
+        at = (int(table[i, j // 16]), head, j % 16)
+        cache.k[at] = torch.full((d,), 1.0).to(kind)
+        cache.k_scale[at] = -math.inf
+    check_attention(query.abs() + 0.25, cache, table, context)
