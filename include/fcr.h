@@ -356,7 +356,7 @@ int fcr_cache_keep(const fcr_cache* cache, const int32_t* table, int64_t table_s
  * (may be NULL) fp32 [B, H*G, T], the base-2 log-sum-exp of its scores.  A token that sees nothing, or that the sequence does not have, gets zeros and
  * -inf; so does one whose every score is -inf.  What hidden keys and values hold has no influence, whatever it is.
  * Sums and statistics are fp32; probabilities are rounded to fp16 (bf16 against a bf16 cache) before they multiply the values.  In fp16 a weight keeps
- * 11 bits down to 2^-22 of its row's largest (a probability times its value's scale), and below 2^-33 of it is 0 (times an infinite value: NaN).  Results do not
+ * 11 bits down to 2^-22 of its row's largest (a probability times its value's scale; scales from 2^-90 to 2^90), and below 2^-33 of it is 0 (times an infinite value: NaN).  Results do not
  * depend on timing, but in their last bits on where the work was cut, which follows from the lengths of all sequences of the call.
  * ws: fcr_tree_attention_bytes(B, H, G, T, D, table_pages * page_size) bytes, 16-byte aligned (it depends on the number of compute
  * units: call this with the operands' device current; 0 for sizes that the call refuses), contents irrelevant.
