@@ -100,6 +100,15 @@ def _declare(lib):
     lib.fcr_tree_attention.restype = c.c_int
     lib.fcr_tree_attention.argtypes = ([c.c_void_p, c.c_void_p] + table + [c.c_void_p, i64p, c.c_void_p, c.c_int64] + [c.c_void_p] * 4 +
                                        [c.c_size_t, c.c_int, c.c_int, c.c_int, c.c_int, i64p, c.c_float, c.c_void_p])
+    vp, ci = c.c_void_p, c.c_int
+    lib.fcr_verify_drafts_bytes.restype = c.c_size_t
+    lib.fcr_verify_drafts_bytes.argtypes = [ci] * 3
+    lib.fcr_verify_drafts.restype = ci
+    lib.fcr_verify_drafts.argtypes = [vp, i64p, vp, i64p, vp, ci, vp, c.c_int64] + [vp] * 7 + [c.c_size_t] + [ci] * 4 + [vp]
+    lib.fcr_cache_accept.restype = ci
+    lib.fcr_cache_accept.argtypes = [vp] + table + [vp, i64p, vp, vp, vp, ci, ci, vp]
+    lib.fcr_cache_reserve.restype = ci
+    lib.fcr_cache_reserve.argtypes = table + [vp, vp, ci, vp, vp, i64p, ci, ci, vp, ci, vp]
     lib.fcr_colreduce_ws_status.restype = c.c_int
     lib.fcr_colreduce_ws_status.argtypes = [c.c_void_p, c.c_size_t] + [c.c_int] * 6 + [c.c_void_p]
     return lib
@@ -128,7 +137,7 @@ class _PythonOnly:
     def keep(*args):
         return None
 
-    cache_write = cache_read = cache_keep = tree_attention = keep
+    cache_write = cache_read = cache_keep = tree_attention = verify_drafts = cache_accept = cache_reserve = keep
 
 
 def host():

@@ -22,6 +22,7 @@ OBJ_DIR = os.path.join(HERE, "_build")
 SOURCES = {
     "fcr": (0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13),
     "cache": (0,),
+    "drafts": (0,),
     "tree_attention": (0, 1, 2, 3, 4),
 }
 

@@ -434,6 +434,147 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The same for what follows a step of drafted tokens (drafts.py).
+bool same_sizes(const at::Tensor& t, std::initializer_list<int64_t> sizes) { return t.sizes() == at::IntArrayRef(sizes.begin(), sizes.size()); }
+
+// A contiguous tensor of that type and these sizes on the device.
+const at::Tensor* flat(PyObject* o, at::ScalarType type, c10::Device device, std::initializer_list<int64_t> sizes) {
+  const at::Tensor* const t = plain(o);
+  return t && t->scalar_type() == type && t->device() == device && same_sizes(*t, sizes) && t->is_contiguous() ? t : nullptr;
+}
+// Rows of probabilities that are read in place.
+bool rows_in_place(const at::Tensor& t, int64_t (&strides)[2]) {
+  strides[0] = t.stride(0), strides[1] = t.stride(1);
+  return strides[0] >= 0 && strides[1] >= 0 && t.stride(2) == 1;
+}
+
+// verify_drafts(target, tokens, uniform, sample, draft, parents, counts): (accepted, path, token), or None.
+PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "verify_drafts takes seven arguments");
+    return nullptr;
+  }
+  const at::Tensor *const target = plain(args[0]), *const tokens = plain(args[1]);
+  if (!target || !tokens || target->dim() != 3 || c10::hip::current_device() != target->device().index()) Py_RETURN_NONE;
+  const auto device = target->device();
+  const int code = dtype_code(target->scalar_type());
+  const int64_t B = target->size(0), T = target->size(1) - 1, V = target->size(2);
+  if (code < 0 || B < 1 || T < 1 || V < 1 || T > INT32_MAX || V > INT32_MAX || B > INT32_MAX) Py_RETURN_NONE;
+  const bool wide = tokens->scalar_type() == at::kLong;
+  if (!flat(args[1], wide ? at::kLong : at::kInt, device, {B, T})) Py_RETURN_NONE;
+  const at::Tensor *const uniform = flat(args[2], at::kFloat, device, {B, T}), *const sample = flat(args[3], at::kFloat, device, {B});
+  int64_t ts[2], ds[2] = {0, 0};
+  if (!uniform || !sample || !rows_in_place(*target, ts)) Py_RETURN_NONE;
+  const at::Tensor *draft = nullptr, *parents = nullptr, *counts = nullptr;
+  if (args[4] != Py_None) {
+    draft = plain(args[4]);
+    if (!draft || draft->dim() != 3 || draft->scalar_type() != target->scalar_type() || draft->device() != device || !same_sizes(*draft, {B, T, V}) ||
+        !rows_in_place(*draft, ds))
+      Py_RETURN_NONE;
+  }
+  if (args[5] != Py_None && !(parents = flat(args[5], at::kInt, device, {B, T})) && !(parents = flat(args[5], at::kInt, device, {T}))) Py_RETURN_NONE;
+  if (args[6] != Py_None && !(counts = flat(args[6], at::kInt, device, {B}))) Py_RETURN_NONE;
+  const size_t bytes = draft && parents ? 0 : fcr_verify_drafts_bytes((int)B, (int)T, (int)V);
+  if (!bytes) Py_RETURN_NONE;
+  const auto ints = target->options().dtype(at::kInt);
+  at::Tensor accepted = at::empty({B}, ints), path = at::empty({B, T}, ints), token = at::empty({B}, tokens->options());
+  const at::Tensor ws = at::empty({(int64_t)bytes}, target->options().dtype(at::kByte));
+  const auto words = [](const at::Tensor* t) { return t ? static_cast<const int32_t*>(t->const_data_ptr()) : nullptr; };
+  const void *const td = target->const_data_ptr(), *const dd = draft ? draft->const_data_ptr() : nullptr, *const xd = tokens->const_data_ptr();
+  const int32_t *const pd = words(parents), *const cd = words(counts);
+  const float *const ud = static_cast<const float*>(uniform->const_data_ptr()), *const sd = static_cast<const float*>(sample->const_data_ptr());
+  int32_t *const ad = static_cast<int32_t*>(accepted.mutable_data_ptr()), *const hd = static_cast<int32_t*>(path.mutable_data_ptr());
+  void *const nd = token.mutable_data_ptr(), *const wd = ws.mutable_data_ptr(), *const stream = stream_of(*target);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fcr_verify_drafts(td, ts, dd, ds, xd, wide ? 8 : 4, pd, parents && parents->dim() == 2 ? T : 0, cd, ud, sd, ad, hd, nd, wd, bytes, code, (int)B, (int)T,
+                         (int)V, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return failed(rc);
+  PyObject* const a = THPVariable_Wrap(std::move(accepted));
+  PyObject* const h = THPVariable_Wrap(std::move(path));
+  PyObject* const x = THPVariable_Wrap(std::move(token));
+  if (a && h && x) return Py_BuildValue("(NNN)", a, h, x);
+  Py_XDECREF(a);
+  Py_XDECREF(h);
+  Py_XDECREF(x);
+  return nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_accept(cache, table, context, path, accepted): the new context, or None.
+PyObject* cache_accept(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "cache_accept takes five arguments");
+    return nullptr;
+  }
+  Cache cache;
+  Table table;
+  PerHead context;
+  if (!cache_of(args[0], cache) || !table_of(args[1], cache, table) || !lengths_of(args[2], cache, table.B, context)) Py_RETURN_NONE;
+  const at::Tensor *const path = int_tensor(args[3], cache), *const accepted = int_tensor(args[4], cache);
+  if (!path || !accepted || path->dim() != 2 || path->size(0) != table.B || path->size(1) < 1 || path->size(1) > INT32_MAX || !path->is_contiguous() ||
+      !same_sizes(*accepted, {table.B}) || !accepted->is_contiguous())
+    Py_RETURN_NONE;
+  const at::Tensor& lengths = THPVariable_Unpack(args[2]);
+  if (lengths.dim() == 2 && context.strides[1] == 0) Py_RETURN_NONE;
+  at::Tensor out = at::empty(lengths.sizes(), lengths.options());
+  const int32_t *const pd = static_cast<const int32_t*>(path->const_data_ptr()), *const ad = static_cast<const int32_t*>(accepted->const_data_ptr());
+  int32_t* const od = static_cast<int32_t*>(out.mutable_data_ptr());
+  const int T = (int)path->size(1);
+  void* const stream = stream_of(*cache.k);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fcr_cache_accept(&cache.c, table.at, table.stride, table.pages, context.at, context.strides, pd, ad, od, table.B, T, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return failed(rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_reserve(pool, table, lengths, page_size): granted, or None.
+PyObject* cache_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "cache_reserve takes four arguments");
+    return nullptr;
+  }
+  const at::Tensor *const table = plain(args[1]), *const lengths = plain(args[2]);
+  if (!table || !lengths || !PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != 3 || !PyLong_CheckExact(args[3])) Py_RETURN_NONE;
+  const auto device = table->device();
+  if (c10::hip::current_device() != device.index() || table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) < 1 || table->size(1) < 1 ||
+      table->size(0) > INT32_MAX || table->size(1) > INT32_MAX || (table->size(1) > 1 && table->stride(1) != 1) ||
+      (table->size(0) > 1 && table->stride(0) < table->size(1)))
+    Py_RETURN_NONE;
+  const int64_t B = table->size(0);
+  const at::Tensor* const free_pages = plain(PyTuple_GET_ITEM(args[0], 0));
+  const at::Tensor *const available = flat(PyTuple_GET_ITEM(args[0], 1), at::kInt, device, {1}), *const held = flat(PyTuple_GET_ITEM(args[0], 2), at::kInt, device, {B});
+  if (!free_pages || !available || !held || free_pages->scalar_type() != at::kInt || free_pages->device() != device || free_pages->dim() != 1 ||
+      free_pages->size(0) < 1 || free_pages->size(0) > INT32_MAX || !free_pages->is_contiguous() || lengths->scalar_type() != at::kInt || lengths->device() != device ||
+      lengths->dim() < 1 || lengths->dim() > 2 || lengths->size(0) != B || lengths->size(-1) < 1 || lengths->size(-1) > INT32_MAX)
+    Py_RETURN_NONE;
+  int overflow = 0;
+  const long long page_size = PyLong_AsLongLongAndOverflow(args[3], &overflow);
+  if (overflow || page_size < 1 || page_size > (1 << 30) || page_size * table->size(1) > (1 << 30)) Py_RETURN_NONE;
+  at::Tensor granted = at::empty({B}, table->options().dtype(at::kBool));
+  const int64_t strides[2] = {lengths->stride(0), lengths->dim() == 2 ? lengths->stride(1) : 0};
+  const auto words = [](const at::Tensor* t) { return static_cast<int32_t*>(t->mutable_data_ptr()); };
+  int32_t *const td = words(table), *const hd = words(held), *const fd = words(free_pages), *const vd = words(available);
+  const int32_t* const ld = static_cast<const int32_t*>(lengths->const_data_ptr());
+  uint8_t* const gd = static_cast<uint8_t*>(granted.mutable_data_ptr());
+  const int H = lengths->dim() == 2 ? (int)lengths->size(1) : 1;
+  void* const stream = stream_of(*table);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fcr_cache_reserve(td, table->stride(0), (int)table->size(1), hd, fd, (int)free_pages->size(0), vd, ld, strides, H, (int)page_size, gd, (int)B, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return failed(rc);
+  return THPVariable_Wrap(std::move(granted));
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* on_error(PyObject*, PyObject* f) {
   Py_INCREF(f);
   Py_XSETREF(g_check, f);
@@ -447,6 +588,9 @@ PyMethodDef g_methods[] = {
     {"cache_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_read)), METH_FASTCALL, "cache_read(cache, table, lengths, n, out_dtype)"},
     {"cache_keep", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_keep)), METH_FASTCALL, "cache_keep(cache, table, lengths, keep, into, into_table)"},
     {"tree_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tree_attention)), METH_FASTCALL, "tree_attention(query, cache, table, context, tree_mask, scale, tree_lengths, with_lse)"},
+    {"verify_drafts", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(verify_drafts)), METH_FASTCALL, "verify_drafts(target, tokens, uniform, sample, draft, parents, counts)"},
+    {"cache_accept", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_accept)), METH_FASTCALL, "cache_accept(cache, table, context, path, accepted)"},
+    {"cache_reserve", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_reserve)), METH_FASTCALL, "cache_reserve(pool, table, lengths, page_size)"},
     {"on_error", on_error, METH_O, "on_error(f): f(rc) raises for a return code of the library"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", "the usual call in native code", -1, g_methods};

@@ -369,6 +369,49 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
                        const int32_t* tree_lengths, void* out, float* lse, void* ws, size_t ws_bytes, int dtype, int B, int G, int T,
                        const int64_t q_strides[4], float scale, void* stream);
 
+/*
+ * Which of T drafted tokens of every sequence stand, and what comes behind them.  target is [B, T+1, V] probabilities (FCR_DTYPE_F16, _BF16, _F32;
+ * consecutive in V; strides in ELEMENTS of sequences and rows; rows need no alignment): row 0 behind the context, row i+1 behind token i.  tokens [B, T] are of
+ * token_bytes 4 or 8, uniform [B, T] and sample [B] random numbers in [0, 1); these are contiguous.  Token i continues token parents[b, i] < i
+ * (parents_stride from one sequence to the next, 0: one tree for all), the context where that is -1; parents NULL: a chain, token i continues i-1.  counts [B] (may be
+ * NULL): how many of the T tokens a sequence has.  A token is accepted if the one that it continues is, and, p being its probability in its row
+ *   with draft (probabilities [B, T, V] that the tokens of a chain were drawn from, row i for token i; not with parents):  u q < p, u = uniform[b, i], q = draft's;
+ *   without: u = uniform[b, its row] lies in [c, c + p), c the sum of p of its siblings in front of it; a token that one of them has already has p = 0.
+ * A token outside [0, V) or with a parent outside [-1, i) is never accepted.  At the row where the accepted ones end the next token is the first v with
+ * sum of r up to v > sample * sum of r, r = max(p - q, 0) where draft has that row, else p, without the row's own drafted tokens in a call without draft; where
+ * that leaves nothing, p.  A probability below 0 or a NaN counts as 0.  Without any weight, or with an infinite one, the token is -1.
+ * The tokens that this gives are distributed as if the target had drawn each of them.  Sums are in 64 bits.
+ * accepted [B]; path [B, T]: the accepted tokens in their order, then -1; token [B] of token_bytes.  ws: fcr_verify_drafts_bytes bytes, 16-byte aligned, contents
+ * irrelevant (depends on the number of compute units, as above).  T may be 0 (a token is drawn; tokens, uniform and path may be NULL).
+ * Limits (FCR_E_SHAPE): B <= 2^20, T <= 1024, V <= 2^28.
+ */
+size_t fcr_verify_drafts_bytes(int B, int T, int V);
+int fcr_verify_drafts(const void* target, const int64_t target_strides[2], const void* draft, const int64_t draft_strides[2], const void* tokens,
+                      int token_bytes, const int32_t* parents, int64_t parents_stride, const int32_t* counts, const float* uniform,
+                      const float* sample, int32_t* accepted, int32_t* path, void* token, void* ws, size_t ws_bytes, int dtype, int B,
+                      int T, int V, void* stream);
+
+/*
+ * Moves the rows of accepted tokens in place: of sequence b the row at position context + path[b, i] goes, codes and scale as they are, to position
+ * context + i, for every i < accepted[b], in every head.  path is contiguous [B, T], increasing as far as accepted says (as fcr_verify_drafts gives it); rows that
+ * stay where they are, or would come from or go to a page that is not there, are left alone.  out receives context + accepted, [B], or [B, H] where
+ * context_strides[1] is not 0; it must not be context itself.
+ */
+int fcr_cache_accept(const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages, const int32_t* context,
+                     const int64_t context_strides[2], const int32_t* path, const int32_t* accepted, int32_t* out, int B, int T, void* stream);
+
+/*
+ * Gives sequences the pages that their lengths need, and takes back the others.  free_pages [pages] is a stack of page numbers, *available how many lie on it; the first
+ * held[b] entries of row b of the table are the sequence's pages.  With need = lengths / page_size, rounded up (of the longest head where lengths_strides[1] is not 0;
+ * lengths below 0 count as 0): first every sequence that holds more gives back its entries from need on, which become -1, in the order of sequences and
+ * entries, the last one on top; then sequences that hold fewer take theirs from the top, in the order of sequences, up to the first for which too few are
+ * left: that one and those behind it that want more stay as they are.  So does a sequence that needs more than table_pages.
+ * granted [B]: 1 where a sequence now holds what it needs.  table, held, free_pages and *available are changed in place; rows of the table must not overlap.
+ * Limits (FCR_E_SHAPE): B <= 2^20, pages <= 2^28, B * table_pages <= 2^30.
+ */
+int fcr_cache_reserve(int32_t* table, int64_t table_stride, int table_pages, int32_t* held, int32_t* free_pages, int pages, int32_t* available,
+                      const int32_t* lengths, const int64_t lengths_strides[2], int H, int page_size, uint8_t* granted, int B, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
