@@ -101,6 +101,10 @@ def _declare(lib):
     lib.fcr_tree_attention.argtypes = ([c.c_void_p, c.c_void_p] + table + [c.c_void_p, i64p, c.c_void_p, c.c_int64] + [c.c_void_p] * 4 +
                                        [c.c_size_t, c.c_int, c.c_int, c.c_int, c.c_int, i64p, c.c_float, c.c_void_p])
     vp, ci = c.c_void_p, c.c_int
+    lib.fcr_chunk_attention_bytes.restype = c.c_size_t
+    lib.fcr_chunk_attention_bytes.argtypes = [ci] * 5 + [c.c_int64]
+    lib.fcr_chunk_attention.restype = ci
+    lib.fcr_chunk_attention.argtypes = ([vp, vp] + table + [vp, i64p] + [vp] * 6 + [c.c_size_t, ci, ci, ci, ci, i64p, c.c_float, c.c_float, ci, vp])
     lib.fcr_verify_drafts_bytes.restype = c.c_size_t
     lib.fcr_verify_drafts_bytes.argtypes = [ci] * 3
     lib.fcr_verify_drafts.restype = ci
@@ -137,7 +141,7 @@ class _PythonOnly:
     def keep(*args):
         return None
 
-    cache_write = cache_read = cache_keep = tree_attention = verify_drafts = cache_accept = cache_reserve = keep
+    cache_write = cache_read = cache_keep = tree_attention = chunk_attention = verify_drafts = cache_accept = cache_reserve = keep
 
 
 def host():

@@ -24,6 +24,7 @@ SOURCES = {
     "cache": (0,),
     "drafts": (0,),
     "tree_attention": (0, 1, 2, 3, 4),
+    "chunk_attention": (0, 1, 2, 3, 4),
 }
 
 HIPCC_FLAGS = [

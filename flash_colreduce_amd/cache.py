@@ -7,9 +7,10 @@ tokens attend to.
     keep = topk_keep_mask(flash_colreduce(q, k, "sum", True), kept)
     counts = cache_keep(cache, table, lengths, keep, pruned, pruned_table)
     out = tree_attention(query, pruned, pruned_table, counts)        # after cache_write of the drafted tokens at `counts`
+    out = chunk_attention(query, cache, table, start, cap=50.0)      # after cache_write of a prompt's tokens at `start`
 
-The reference has none of this: its callers leave the cache to a serving program.  The kernels are csrc/cache.hip and
-csrc/tree_attention.hip behind the C ABI (include/fcr.h); nothing here has a gradient.  Every call is asynchronous on the current stream of
+The reference has none of this: its callers leave the cache to a serving program.  The kernels are csrc/cache.hip,
+csrc/tree_attention.hip and csrc/chunk_attention.hip behind the C ABI (include/fcr.h); nothing here has a gradient.  Every call is asynchronous on the current stream of
 the cache's device and allocates with torch only.
 """
 from __future__ import annotations
@@ -24,7 +25,7 @@ import torch
 from . import _lib, flash
 from .flash import _DTYPES, _raw_stream
 
-__all__ = ["KVCache", "cache_write", "cache_read", "cache_keep", "tree_attention"]
+__all__ = ["KVCache", "cache_write", "cache_read", "cache_keep", "tree_attention", "chunk_attention"]
 
 _CODES = {torch.int8: _lib.DTYPE_INT8, torch.float8_e4m3fn: _lib.DTYPE_E4M3}
 _CACHED = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, **_CODES}
@@ -291,4 +292,72 @@ def tree_attention(query: torch.Tensor, cache: KVCache, table: torch.Tensor, con
             _strides2(context), None if mask is None else mask.data_ptr(), t * t if mask is not None and mask.dim() == 3 else 0,
             None if tree_lengths is None else tree_lengths.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
             ws.data_ptr(), nbytes, _DTYPES[query.dtype], b, hq // h, t, _lib.strides4(query.stride()), float(scale), _raw_stream(dev)))
+    return (out, lse) if return_lse2 else out
+
+
+@functools.lru_cache(maxsize=4096)
+def _chunk_bytes(dev_index: int, b: int, h: int, g: int, t: int, d: int, positions: int) -> int:
+    with torch.cuda.device(dev_index):
+        return _lib.load().fcr_chunk_attention_bytes(b, h, g, t, d, positions)
+
+
+def chunk_attention(query: torch.Tensor, cache: KVCache, table: torch.Tensor, context: torch.Tensor, scale: Optional[float] = None, *,
+                    counts: Optional[torch.Tensor] = None, cap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
+                    window: Optional[int] = None, prefix: Optional[torch.Tensor] = None, return_lse2: bool = False):
+    """Attention of T new tokens per sequence, a prompt, a part of one or a single token, over a cache that holds their keys and values at positions
+    context .. context+T-1.
+
+    query is (B, Hq, T, D), fp16 or bf16 (the cache's type if that is one of them), Hq a multiple of the cache's heads: heads h*G .. h*G+G-1 attend to
+    head h.  Token t has position i = context[b] + t (or context[b, h] + t) and sees positions j <= i, with window (at least 1) only those above i - window; with
+    prefix, int32 (B,), besides those every j < prefix[b], also behind it (tokens of an image, or the first ones that a window is to keep).  counts,
+    int32 (B,): sequences that have fewer than T new tokens.
+
+    A score is scale * q.k, scale 1/sqrt(D) by default; with cap it becomes cap * tanh(score / cap), and with slopes, fp32 (Hq,), slopes[head] * |i - j| is
+    taken off it.  Positions are those in the cache: after cache_keep they are not those in the text, and distances and windows go by what is left.
+
+    Returns (B, Hq, T, D) of query's type, and with return_lse2 the base-2 log-sum-exp of every row's scores, fp32 (B, Hq, T).  A row that sees nothing (or that the
+    sequence does not have, or whose every score is -inf) is zeros, its log-sum-exp -inf.  What hidden rows of the cache hold, NaNs included, has no
+    influence.  Probabilities are rounded to fp16 (bf16 against a bf16 cache) as they multiply the values, sums are fp32.  The last bits of a
+    sequence's result depend on how the work was cut, and so on the lengths of the others in the batch."""
+    out = _host().chunk_attention(query, cache, table, context, scale, counts, cap, slopes, window, prefix, return_lse2)
+    if out is not None:
+        return out
+    dev = _check_cache(cache)
+    _, h, page_size, d = cache.k.shape
+    if query.dim() != 4 or query.shape[3] != d or query.shape[1] % h or query.shape[1] == 0 or query.device != dev:
+        raise ValueError(f"query must be (B, a multiple of {h}, T, {d}) on the cache's device. Got {tuple(query.shape)}.")
+    if query.dtype not in (torch.float16, torch.bfloat16) or (cache.k.dtype not in _CODES and cache.k.dtype != query.dtype):
+        raise ValueError(f"query must be float16 or bfloat16, and of the type of a cache of either. Got {query.dtype} and {cache.k.dtype}.")
+    b, hq, t, _ = query.shape
+    _check_table(table, dev, b)
+    _check_lengths(context, dev, b, h, "context")
+    for x, name in ((counts, "counts"), (prefix, "prefix")):
+        if x is not None and (x.dtype != torch.int32 or x.shape != (b,) or x.device != dev):
+            raise ValueError(f"{name} must be int32 ({b},) on the cache's device. Got {tuple(x.shape)} {x.dtype}.")
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (hq,) or slopes.device != dev):
+        raise ValueError(f"slopes must be float32 ({hq},) on the cache's device. Got {tuple(slopes.shape)} {slopes.dtype}.")
+    if cap is not None and not 0 < cap < math.inf:
+        raise ValueError(f"cap must be positive and finite. Got {cap}.")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1. Got {window}.")
+    if scale is None:
+        scale = 1 / math.sqrt(d)
+    out = torch.empty((b, hq, t, d), device=dev, dtype=query.dtype)
+    lse = torch.empty((b, hq, t), device=dev, dtype=torch.float32) if return_lse2 else None
+    if b * t * table.shape[1] == 0:
+        out.zero_()
+        if lse is not None:
+            lse.fill_(-math.inf)
+        return (out, lse) if return_lse2 else out
+    query = _rows(query)
+    counts, prefix, slopes = (None if x is None else x.contiguous() for x in (counts, prefix, slopes))
+    nbytes = _chunk_bytes(dev.index if dev.index is not None else torch.cuda.current_device(), b, h, hq // h, t, d,
+                          table.shape[1] * page_size)
+    ws = torch.empty(max(nbytes, 16), device=dev, dtype=torch.uint8)
+    pointers = [None if x is None else x.data_ptr() for x in (counts, prefix, slopes)]
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().fcr_chunk_attention(
+            query.data_ptr(), ctypes.byref(_described(cache)), table.data_ptr(), table.stride(0), table.shape[1], context.data_ptr(),
+            _strides2(context), *pointers, out.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes, _DTYPES[query.dtype], b,
+            hq // h, t, _lib.strides4(query.stride()), float(scale), float(cap or 0), min(window or 0, 2**31 - 1), _raw_stream(dev)))
     return (out, lse) if return_lse2 else out

@@ -48,7 +48,7 @@ FCR_HOST_DEVICE inline int piece_length(int blocks, int pieces) { return quotien
 // Workgroups behind the one with an item's first part that have parts of it: `others` blocks are theirs.  unit: `per`, or the pieces' `most`.
 FCR_HOST_DEVICE inline int followers(int others, int unit) { return others <= 0 ? 0 : quotient_up(others, unit); }
 
-// Which kernel takes `rows` rows of a (sequence, head) of at most 64 w elements: 1, tree_attention_kernel; 4 and 8, tall_attention_kernel of as many
+// Which kernel takes `rows` rows of a (sequence, head) of at most 64 w elements: 1, few_attention_kernel; 4 and 8, tall_attention_kernel of as many
 // waves (4: of at most 128 elements, see tall_tiles).
 // Both sides, us, at 4 sequences x 8 heads x 8192 keys, int8 (bf16): 48 rows of 64 elements 33 (31) by form 1, 37 (33) by form 4, 64 rows 38
 // (35) and 38 (34); of 128 elements 42 (45) and 47 (46), 48 (52) and 49 (47); 48 rows of 256 elements 59 (89) by form 1, 62 (61) by form 8, 64
@@ -61,5 +61,36 @@ FCR_HOST_DEVICE inline int form_of(int64_t rows, int w, bool codes) {
 FCR_HOST_DEVICE constexpr int tall_tiles(int w) { return w <= 2 ? 2 : 1; }
 // Rows of an item.
 FCR_HOST_DEVICE inline int rows_of_tile(int form, int w) { return form == 1 ? 16 : 16 * tall_tiles(w) * form; }
+
+FCR_HOST_DEVICE inline int most_of_two(int a, int b) { return a > b ? a : b; }
+
+// What tokens first .. last of a sequence (those that it has) see in chunk_attention: keys of [lo, n) and [0, prefix), and no others; keys of [all_lo, all_hi) and
+// [0, prefix), every token.  Blocks that begin at gap_at or behind it (a number of keys) lie `gap` keys further back than their number says: between the
+// prefix and lo no key is seen.  (context up to 2^30, T up to 2^24.)
+struct Sight {
+  int context, n, lo, all_lo, all_hi, prefix, gap_at, gap;
+  FCR_HOST_DEVICE Sight() {}
+  FCR_HOST_DEVICE Sight(int context_, int count, int prefix_, int window, int T, int positions, int first, int last) {
+    context = least_of(most_of_two(context_, 0), 1 << 30);
+    count = least_of(most_of_two(count, 0), T);
+    last = least_of(last, count - 1);
+    const bool none = first >= count;
+    const int there = least_of(context + count, positions);
+    prefix = none ? 0 : least_of(most_of_two(prefix_, 0), there);
+    n = none ? 0 : least_of(there, most_of_two(context + last + 1, prefix));
+    lo = least_of(most_of_two(context + first + 1 - window, 0), n);
+    all_lo = most_of_two(context + last + 1 - window, 0);
+    all_hi = least_of(context + first + 1, n);
+    gap_at = (prefix + kBlock - 1) & -kBlock;
+    gap = most_of_two((lo & -kBlock) - gap_at, 0);
+  }
+  FCR_HOST_DEVICE int blocks() const { return most_of_two((n - gap + kBlock - 1) / kBlock, 1); }
+  // of the key that lies `at` keys behind the first one of the blocks, where all of them are laid end to end
+  FCR_HOST_DEVICE int position(int at) const { return at + (at >= gap_at ? gap : 0); }
+  // whether every token sees `len` keys from pos on, and whether one might see one of them
+  FCR_HOST_DEVICE bool whole(int pos, int len) const { return (pos >= all_lo && pos + len <= all_hi) || pos + len <= prefix; }
+  FCR_HOST_DEVICE bool any(int pos, int len) const { return pos < n && (pos + len > lo || pos < prefix); }
+  FCR_HOST_DEVICE bool settled(int pos, int len) const { return whole(pos, len); }
+};
 
 }  // namespace fcr_tree

@@ -372,6 +372,26 @@ PyObject* cache_keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Queries of attention over a cache, the first of the arguments (query, cache, table, context).
+struct Queries {
+  const at::Tensor* t;
+  int64_t strides[4], T;
+  int code, G;
+};
+bool queries_of(PyObject* const* args, Cache& cache, Table& table, PerHead& context, Queries& out) {
+  const at::Tensor* const qp = plain(args[0]);
+  if (!qp || !cache_of(args[1], cache) || !table_of(args[2], cache, table) || !lengths_of(args[3], cache, table.B, context)) return false;
+  const at::Tensor& q = *qp;
+  const int H = cache.c.H;
+  out.t = qp, out.code = dtype_code(q.scalar_type());
+  if ((out.code != FCR_DTYPE_F16 && out.code != FCR_DTYPE_BF16) || (!cache.c.k_scale && out.code != cache.c.dtype) || q.dim() != 4 || q.size(0) != table.B ||
+      q.size(1) < 1 || q.size(1) % H != 0 || q.size(1) > INT32_MAX || q.size(2) < 1 || q.size(2) > INT32_MAX || q.size(3) != cache.c.D ||
+      q.device() != cache.k->device() || !rows_of(q, out.strides))
+    return false;
+  out.T = q.size(2), out.G = (int)q.size(1) / H;
+  return true;
+}
+
 // tree_attention(query, cache, table, context, tree_mask, scale, tree_lengths, with_lse): the result, (result, log-sum-exp), or None.
 PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -382,21 +402,14 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Cache cache;
   Table table;
   PerHead context;
-  const at::Tensor* const qp = plain(args[0]);
-  if (!qp || !cache_of(args[1], cache) || !table_of(args[2], cache, table) || !lengths_of(args[3], cache, table.B, context)) Py_RETURN_NONE;
-  const at::Tensor& q = *qp;
-  const int code = dtype_code(q.scalar_type()), H = cache.c.H;
-  int64_t qs[4];
-  if ((code != FCR_DTYPE_F16 && code != FCR_DTYPE_BF16) || (!cache.c.k_scale && code != cache.c.dtype) || q.dim() != 4 || q.size(0) != table.B ||
-      q.size(1) < 1 || q.size(1) % H != 0 || q.size(1) > INT32_MAX || q.size(2) < 1 || q.size(2) > INT32_MAX || q.size(3) != cache.c.D ||
-      q.device() != cache.k->device() || !rows_of(q, qs))
-    Py_RETURN_NONE;
-  const int64_t T = q.size(2);
+  Queries q;
+  if (!queries_of(args, cache, table, context, q)) Py_RETURN_NONE;
+  const int64_t T = q.T;
   const uint8_t* mask = nullptr;
   int64_t mask_stride = 0;
   if (args[4] != Py_None) {
     const at::Tensor* const m = plain(args[4]);
-    if (!m || m->scalar_type() != at::kBool || m->device() != q.device() || !m->is_contiguous() || m->dim() < 2 || m->dim() > 3 ||
+    if (!m || m->scalar_type() != at::kBool || m->device() != q.t->device() || !m->is_contiguous() || m->dim() < 2 || m->dim() > 3 ||
         m->size(-1) != T || m->size(-2) != T || (m->dim() == 3 && m->size(0) != table.B))
       Py_RETURN_NONE;
     mask = static_cast<const uint8_t*>(m->const_data_ptr());
@@ -414,19 +427,18 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   const int with_lse = PyObject_IsTrue(args[7]);
   if (with_lse < 0) return nullptr;
-  const int G = (int)q.size(1) / H;
-  const size_t bytes = fcr_tree_attention_bytes(table.B, H, G, (int)T, cache.c.D, (int64_t)table.pages * cache.c.page_size);
+  const size_t bytes = fcr_tree_attention_bytes(table.B, cache.c.H, q.G, (int)T, cache.c.D, (int64_t)table.pages * cache.c.page_size);
   if (!bytes) Py_RETURN_NONE;
-  at::Tensor out = at::empty(q.sizes(), q.options()), lse;
-  if (with_lse) lse = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
-  const at::Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-  const void* const qd = q.const_data_ptr();
-  void *const od = out.mutable_data_ptr(), *const wd = ws.mutable_data_ptr(), *const stream = stream_of(q);
+  at::Tensor out = at::empty(q.t->sizes(), q.t->options()), lse;
+  if (with_lse) lse = at::empty(q.t->sizes().slice(0, 3), q.t->options().dtype(at::kFloat));
+  const at::Tensor ws = at::empty({(int64_t)bytes}, q.t->options().dtype(at::kByte));
+  const void* const qd = q.t->const_data_ptr();
+  void *const od = out.mutable_data_ptr(), *const wd = ws.mutable_data_ptr(), *const stream = stream_of(*q.t);
   float* const ld = with_lse ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = fcr_tree_attention(qd, &cache.c, table.at, table.stride, table.pages, context.at, context.strides, mask, mask_stride, tree_lengths, od, ld, wd, bytes,
-                          code, table.B, G, (int)T, qs, (float)scale, stream);
+                          q.code, table.B, q.G, (int)T, q.strides, (float)scale, stream);
   Py_END_ALLOW_THREADS
   if (rc) return failed(rc);
   if (!with_lse) return THPVariable_Wrap(std::move(out));
@@ -446,6 +458,63 @@ const at::Tensor* flat(PyObject* o, at::ScalarType type, c10::Device device, std
 bool rows_in_place(const at::Tensor& t, int64_t (&strides)[2]) {
   strides[0] = t.stride(0), strides[1] = t.stride(1);
   return strides[0] >= 0 && strides[1] >= 0 && t.stride(2) == 1;
+}
+
+// chunk_attention(query, cache, table, context, scale, counts, cap, slopes, window, prefix, with_lse): the result, (result, log-sum-exp), or None.
+PyObject* chunk_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11) {
+    PyErr_SetString(PyExc_TypeError, "chunk_attention takes eleven arguments");
+    return nullptr;
+  }
+  Cache cache;
+  Table table;
+  PerHead context;
+  Queries q;
+  if (!queries_of(args, cache, table, context, q)) Py_RETURN_NONE;
+  const int64_t T = q.T;
+  double scale, cap = 0.0;
+  if (args[4] == Py_None) scale = 1.0 / std::sqrt((double)cache.c.D);
+  else if (PyFloat_CheckExact(args[4])) scale = PyFloat_AS_DOUBLE(args[4]);
+  else Py_RETURN_NONE;
+  if (args[6] != Py_None) {
+    if (!PyFloat_CheckExact(args[6])) Py_RETURN_NONE;
+    cap = PyFloat_AS_DOUBLE(args[6]);
+    if (!(cap > 0.0) || !std::isfinite(cap)) Py_RETURN_NONE;
+  }
+  long long window = 0;
+  if (args[8] != Py_None) {
+    int overflow = 0;
+    if (!PyLong_CheckExact(args[8])) Py_RETURN_NONE;
+    window = PyLong_AsLongLongAndOverflow(args[8], &overflow);
+    if (overflow || window < 1 || window > INT32_MAX) Py_RETURN_NONE;
+  }
+  const at::Tensor *counts = nullptr, *slopes = nullptr, *prefix = nullptr;
+  if (args[5] != Py_None && !(counts = flat(args[5], at::kInt, q.t->device(), {table.B}))) Py_RETURN_NONE;
+  if (args[7] != Py_None && !(slopes = flat(args[7], at::kFloat, q.t->device(), {q.t->size(1)}))) Py_RETURN_NONE;
+  if (args[9] != Py_None && !(prefix = flat(args[9], at::kInt, q.t->device(), {table.B}))) Py_RETURN_NONE;
+  const int32_t *const nd = counts ? static_cast<const int32_t*>(counts->const_data_ptr()) : nullptr,
+                *const fd = prefix ? static_cast<const int32_t*>(prefix->const_data_ptr()) : nullptr;
+  const float* const sd = slopes ? static_cast<const float*>(slopes->const_data_ptr()) : nullptr;
+  const int with_lse = PyObject_IsTrue(args[10]);
+  if (with_lse < 0) return nullptr;
+  const size_t bytes = fcr_chunk_attention_bytes(table.B, cache.c.H, q.G, (int)T, cache.c.D, (int64_t)table.pages * cache.c.page_size);
+  if (!bytes) Py_RETURN_NONE;
+  at::Tensor out = at::empty(q.t->sizes(), q.t->options()), lse;
+  if (with_lse) lse = at::empty(q.t->sizes().slice(0, 3), q.t->options().dtype(at::kFloat));
+  const at::Tensor ws = at::empty({(int64_t)bytes}, q.t->options().dtype(at::kByte));
+  const void* const qd = q.t->const_data_ptr();
+  void *const od = out.mutable_data_ptr(), *const wd = ws.mutable_data_ptr(), *const stream = stream_of(*q.t);
+  float* const ld = with_lse ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fcr_chunk_attention(qd, &cache.c, table.at, table.stride, table.pages, context.at, context.strides, nd, fd, sd, od, ld, wd, bytes, q.code, table.B, q.G,
+                           (int)T, q.strides, (float)scale, (float)cap, (int)window, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return failed(rc);
+  if (!with_lse) return THPVariable_Wrap(std::move(out));
+  return two(std::move(out), std::move(lse));
+  END_HANDLE_TH_ERRORS
 }
 
 // verify_drafts(target, tokens, uniform, sample, draft, parents, counts): (accepted, path, token), or None.
@@ -588,6 +657,7 @@ PyMethodDef g_methods[] = {
     {"cache_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_read)), METH_FASTCALL, "cache_read(cache, table, lengths, n, out_dtype)"},
     {"cache_keep", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_keep)), METH_FASTCALL, "cache_keep(cache, table, lengths, keep, into, into_table)"},
     {"tree_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tree_attention)), METH_FASTCALL, "tree_attention(query, cache, table, context, tree_mask, scale, tree_lengths, with_lse)"},
+    {"chunk_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(chunk_attention)), METH_FASTCALL, "chunk_attention(query, cache, table, context, scale, counts, cap, slopes, window, prefix, with_lse)"},
     {"verify_drafts", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(verify_drafts)), METH_FASTCALL, "verify_drafts(target, tokens, uniform, sample, draft, parents, counts)"},
     {"cache_accept", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_accept)), METH_FASTCALL, "cache_accept(cache, table, context, path, accepted)"},
     {"cache_reserve", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_reserve)), METH_FASTCALL, "cache_reserve(pool, table, lengths, page_size)"},

@@ -370,6 +370,20 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
                        const int64_t q_strides[4], float scale, void* stream);
 
 /*
+ * Attention of T new tokens of every sequence (a prompt, a part of one, a single token) over the cache, which holds their keys and values at positions
+ * context .. context+T-1.  Everything as in fcr_tree_attention, but for what a token sees and what becomes of its scores: token t, at position i = context + t,
+ * sees position j < context + counts (counts [B], may be NULL: T of each) where j <= i and j > i - window (0: no window), or where j < prefix[b] (may be NULL).  Its scores
+ * are scale q k, with cap > 0 then cap tanh(. / cap), with slopes ([H*G], fp32, may be NULL) then less slopes[head] |i - j|; lse is that of the scores so
+ * formed.  Tokens from counts on get zeros and -inf.  With a cap a score of +-infinity is +-cap.  Positions that no token of a tile sees are not read.
+ * ws: fcr_chunk_attention_bytes(B, H, G, T, D, table_pages * page_size) bytes, as above; the same limits.  cap must be finite and >= 0, scale / cap not overflow.
+ */
+size_t fcr_chunk_attention_bytes(int B, int H, int G, int T, int D, int64_t positions);
+int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages,
+                        const int32_t* context, const int64_t context_strides[2], const int32_t* counts, const int32_t* prefix, const float* slopes,
+                        void* out, float* lse, void* ws, size_t ws_bytes, int dtype, int B, int G, int T, const int64_t q_strides[4], float scale,
+                        float cap, int window, void* stream);
+
+/*
  * Which of T drafted tokens of every sequence stand, and what comes behind them.  target is [B, T+1, V] probabilities (FCR_DTYPE_F16, _BF16, _F32;
  * consecutive in V; strides in ELEMENTS of sequences and rows; rows need no alignment): row 0 behind the context, row i+1 behind token i.  tokens [B, T] are of
  * token_bytes 4 or 8, uniform [B, T] and sample [B] random numbers in [0, 1); these are contiguous.  Token i continues token parents[b, i] < i
