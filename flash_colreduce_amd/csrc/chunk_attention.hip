@@ -63,39 +63,40 @@ struct ChunkDeal {
       __syncthreads();
     };
     find(by_head ? at : (int)a.heads.of((uint32_t)at));
+    // (everything found goes through locals to one place: stores on several ways would be joined into one to an address that is chosen, and the deal
+    // would stay in memory, where nothing is known to be uniform)
     int pair = __builtin_amdgcn_readfirstlane(found[0]), in_front = __builtin_amdgcn_readfirstlane(found[1]);
-    const int entry = (int)a.per_head.of((uint32_t)pair);
-    b = by_head ? (int)a.heads.of((uint32_t)entry) : entry;
-    h = by_head ? entry - b * a.H : 0;
-    tile = 0;
+    const int entry = (int)a.per_head.of((uint32_t)pair), q0 = entry * a.row_tiles;
+    int place = at - times * in_front, head = 0;
     if (a.row_tiles == 1) {
-      look(a);
-      const int place = at - times * in_front;
-      if (!by_head) h = (int)((uint32_t)place / (uint32_t)nb);
-      blk = place - (by_head ? 0 : h * nb);
-      return true;
+      const int blocks = __builtin_amdgcn_readfirstlane(blocks_of_pair(pair));
+      if (!by_head) head = (int)((uint32_t)place / (uint32_t)blocks), place -= head * blocks;
+    } else {
+      // blocks in front of the entry's pairs and behind them
+      const int q1 = q0 + a.row_tiles;
+      const auto mark = [&](int q, int to) {
+        if (p0 <= q && q < p1) {
+          int s = before;
+          for (int p = p0; p < q; ++p) s += blocks_of_pair(p);
+          found[to] = s;
+        } else if (q == pairs && tid == 0) {
+          found[to] = sum;
+        }
+      };
+      mark(q0, 2);
+      mark(q1, 3);
+      __syncthreads();
+      const int from = __builtin_amdgcn_readfirstlane(found[2]), blocks = __builtin_amdgcn_readfirstlane(found[3]) - from;
+      place = at - times * from;
+      if (!by_head) head = (int)((uint32_t)place / (uint32_t)blocks), place -= head * blocks;
+      find(from + place);
+      pair = __builtin_amdgcn_readfirstlane(found[0]), in_front = __builtin_amdgcn_readfirstlane(found[1]);
+      place = from + place - in_front;
     }
-    // blocks in front of the entry's pairs and behind them
-    const int q0 = entry * a.row_tiles, q1 = q0 + a.row_tiles;
-    const auto mark = [&](int q, int to) {
-      if (p0 <= q && q < p1) {
-        int s = before;
-        for (int p = p0; p < q; ++p) s += blocks_of_pair(p);
-        found[to] = s;
-      } else if (q == pairs && tid == 0) {
-        found[to] = sum;
-      }
-    };
-    mark(q0, 2);
-    mark(q1, 3);
-    __syncthreads();
-    const int from = __builtin_amdgcn_readfirstlane(found[2]), blocks = __builtin_amdgcn_readfirstlane(found[3]) - from;
-    int place = at - times * from;
-    if (!by_head) h = (int)((uint32_t)place / (uint32_t)blocks), place -= h * blocks;
-    find(from + place);
-    pair = __builtin_amdgcn_readfirstlane(found[0]), in_front = __builtin_amdgcn_readfirstlane(found[1]);
+    b = by_head ? (int)a.heads.of((uint32_t)entry) : entry;
+    h = __builtin_amdgcn_readfirstlane(by_head ? entry - b * a.H : head);
     tile = pair - q0;
-    blk = from + place - in_front;
+    blk = __builtin_amdgcn_readfirstlane(place);
     look(a);
     return true;
   }
@@ -139,6 +140,7 @@ struct Chunk {
     return view_of(a, b, h, min(row0, a.rows - 1), row0 + rows);
   }
   static __device__ __forceinline__ uint32_t seen_by(const Args& a, const Sight& v, int, int row, int pos, uint32_t there, int g) {
+    asm volatile("" : "+v"(row), "+v"(g));       // (formed here, not kept)
     const int token = row < a.rows ? (int)a.G.of((uint32_t)row) : 0;
     const int back = v.context + token - pos - 4 * g, first = v.prefix - pos - 4 * g;     // of the lane's first key: how far behind the token, in front of the prefix's end
     uint32_t seen = 0;
