@@ -852,7 +852,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) f
     st.clear();
     for (int i = deal.blk; i < stop; ++i) {
       const int pos = view.position(i * kBlock) + wave * 32;
-      if (pos >= n) break;                              // (a wave's later blocks lie behind this one)
+      if (P::rising && pos >= n) break;                 // (a wave's later blocks lie behind this one)
 #pragma unroll
       for (int t = 0; t < 2; ++t) then[t] = Place(src, view.position((i + 2) * kBlock) + wave * 32 + 16 * t);
       f32x4 s[1][2];

@@ -185,7 +185,9 @@ bool fcr_tree::chunk_e4m3(const Args& a, int w, int form, hipStream_t s) { retur
 extern "C" {
 
 size_t fcr_chunk_attention_bytes(int B, int H, int G, int T, int D, int64_t positions) {
-  return fcr_tree_attention_bytes(B, H, G, T, D, positions);
+  Plan p[2];             // for either kind of cache
+  if (B < 1 || H < 1 || G < 1 || T < 1 || D < 16 || D > 256 || positions < 1 || positions > (1 << 30) || (int64_t)B * H > (1 << 24)) return 0;
+  return plan_of(true, B, H, G, T, D, positions, p[0]) && plan_of(false, B, H, G, T, D, positions, p[1]) ? (size_t)std::max(p[0].bytes, p[1].bytes) : 0;
 }
 
 int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages,

@@ -63,7 +63,10 @@ __device__ __forceinline__ void numbers(const char* row, int v, int V, float (&x
       x[i] = DT == FCR_DTYPE_F32 ? __builtin_bit_cast(float, (uint32_t)w[i / 4][i % 4]) : element<DT == FCR_DTYPE_F32 ? FCR_DTYPE_F16 : DT>(w[i / 8][i / 2 % 4], i & 1);
   } else {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) x[i] = v + i < V ? number<DT>(row, v + i) : 0.0f;
+    for (int i = 0; i < kEach; ++i) {
+      x[i] = number<DT>(row, min(v + i, V - 1));
+      x[i] = v + i < V ? x[i] : 0.0f;
+    }
   }
 }
 
@@ -146,12 +149,13 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
   __shared__ double p_of[kMostDrafted];
   __shared__ int token_of[kMostDrafted], parent_of[kMostDrafted];     // -1: none of V; kMostDrafted: not there
   __shared__ int up[2][kMostDrafted];                                 // bit 31: not taken; else the predecessor + 1
-  __shared__ int found, hidden;
+  __shared__ uint64_t path[kMostDrafted / 64];
+  __shared__ int hidden;
   __shared__ double part[2][kWaves];
   const int b = (int)a.pieces.of(blockIdx.x), piece = (int)(blockIdx.x - b * a.pieces.d);
   const int tid = threadIdx.x, count = count_of(a, b);
   const char* const target = a.target + b * a.target_b;
-  if (tid == 0) found = 0, hidden = 0;
+  if (tid == 0) hidden = 0;
   for (int i = tid; i < count; i += kThreads) {
     const int64_t x = token_at(a, (int64_t)b * a.T + i);
     const int parent = a.parents ? a.parents[b * a.parents_b + i] : i - 1;
@@ -163,18 +167,18 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
   __syncthreads();
   if (a.parents && !a.draft) {
     // a token that a sibling in front has already has nothing left
-    bool again[kMostDrafted / kThreads];
-#pragma unroll
-    for (int k = 0; k < kMostDrafted / kThreads; ++k) {
-      again[k] = false;
-      const int i = tid + k * kThreads;
-      if (i >= count) continue;
-      for (int j = 0; j < i; ++j) again[k] = again[k] || (parent_of[j] == parent_of[i] && token_of[j] == token_of[i]);
+    uint32_t again = 0;
+#pragma unroll 1
+    for (int i = tid, k = 0; i < count; i += kThreads, ++k) {
+      const int parent = parent_of[i], token = token_of[i];
+      bool found = false;
+#pragma unroll 4
+      for (int j = 0; j < i; ++j) found |= (parent_of[j] == parent) & (token_of[j] == token);
+      again |= (found ? 1u : 0u) << k;
     }
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kMostDrafted / kThreads; ++k)
-      if (again[k]) p_of[tid + k * kThreads] = 0.0;
+    for (int i = tid; again; i += kThreads, again >>= 1)
+      if (again & 1) p_of[i] = 0.0;
     __syncthreads();
   }
   for (int i = tid; i < count; i += kThreads) {
@@ -186,9 +190,10 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
         taken = u * weight(number<DT>(a.draft + b * a.draft_b + i * a.draft_r, token_of[i])) < p_of[i];
       } else {
         double low = 0.0;
-        if (a.parents)
-          for (int j = 0; j < i; ++j)
-            if (parent_of[j] == parent) low += p_of[j];
+        if (a.parents) {
+#pragma unroll 4
+          for (int j = 0; j < i; ++j) low += parent_of[j] == parent ? p_of[j] : 0.0;
+        }
         taken = low <= u && u < low + p_of[i];
       }
     }
@@ -203,29 +208,28 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
     }
     __syncthreads();
   }
-  for (int i = tid; i < count; i += kThreads)
-    if (up[now][i] >= 0) atomicMax(&found, i + 1);
+  // the path, in the order of its tokens, 64 of them to a word
+  for (int i = tid; i < ((count + 63) & ~63); i += kThreads) {
+    const uint64_t on = __ballot(i < count && up[now][i] >= 0);
+    if ((tid & 63) == 0) path[i >> 6] = on;
+  }
   __syncthreads();
-  const int row = found;
+  int row = 0, taken = 0;
+  for (int g = 0; g < (count + 63) / 64; ++g) {
+    const uint64_t on = path[g];
+    if (on) row = 64 * g + 64 - __clzll(on);
+    taken += __popcll(on);
+  }
   if (piece == 0) {
-    // the path, in the order of its tokens: the k-th one has k in front of it
-    int taken = 0;
-    for (int i = tid; i < a.T; i += kThreads) {
+    for (int i = tid; i < count; i += kThreads) {
       int before = 0;
-      const bool on = i < count && up[now][i] >= 0;
-      if (on)
-        for (int j = 0; j < i; ++j) before += up[now][j] >= 0;
-      if (on) a.path[(int64_t)b * a.T + before] = i;
-      if (on && i + 1 == row) taken = before + 1;
+      for (int g = 0; g < i >> 6; ++g) before += __popcll(path[g]);
+      const uint64_t on = path[i >> 6];
+      before += __popcll(on & ((1ull << (i & 63)) - 1));
+      if (on >> (i & 63) & 1) a.path[(int64_t)b * a.T + before] = i;
     }
-    if (taken) hidden = taken;                   // (one thread: the last token on the path)
-    __syncthreads();
-    taken = hidden;
     for (int i = taken + tid; i < a.T; i += kThreads) a.path[(int64_t)b * a.T + i] = -1;
     if (tid == 0) a.accepted[b] = taken, a.row[b] = row;
-    __syncthreads();
-    if (tid == 0) hidden = 0;
-    __syncthreads();
   }
   const int v0 = piece * a.piece, v1 = min(v0 + a.piece, a.V);
   int* const list = parent_of;                   // (read last before several barriers)
@@ -251,6 +255,23 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
   }
 }
 
+// The first thread of the workgroup with `is`, or the last one: its `at`; `none` where there is no such thread.  words: kWaves of LDS; a barrier is in front of the
+// result, and one must be behind it before the words are used again.
+__device__ __forceinline__ int one_of(bool is, int at, bool first, int none, int* words) {
+  const uint64_t lanes = __ballot(is);
+  const int lane = first ? __ffsll((unsigned long long)lanes) - 1 : 63 - __clzll(lanes);
+  const int found = __shfl(at, lanes ? lane : 0);
+  if ((threadIdx.x & 63) == 0) words[threadIdx.x >> 6] = lanes ? found : none;
+  __syncthreads();
+  int x = none;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const int w = words[first ? kWaves - 1 - i : i];
+    x = w == none ? x : w;
+  }
+  return x;
+}
+
 // The piece that holds the sample's place, then the element.  A thread takes consecutive pieces, or elements.  Sums that meet a border from two sides in another order
 // may disagree by a rounding: the last weight above zero stands where none is found.
 template <int DT>
@@ -258,50 +279,49 @@ __global__ void __launch_bounds__(kThreads) next_token_kernel(VerifyArgs a) {
   __shared__ int list[kMostDrafted];
   __shared__ double part[3][kWaves];
   __shared__ double before_piece;
-  __shared__ int hidden, chosen, last;
+  __shared__ int hidden, words[4][kWaves];
   const int b = blockIdx.x, tid = threadIdx.x, count = count_of(a, b), row = a.row[b];
   const int pieces = (int)a.pieces.d, each = (pieces + kThreads - 1) / kThreads;
   const double* const sums = a.sums + 2 * (int64_t)b * pieces;
   const int first = min(tid * each, pieces), end = min(first + each, pieces);
-  if (tid == 0) hidden = 0, chosen = INT32_MAX, last = -1;
+  if (tid == 0) hidden = 0;
   double mine[2] = {0.0, 0.0}, all[2], before[2];
   for (int i = first; i < end; ++i) mine[0] += sums[2 * i], mine[1] += sums[2 * i + 1];
 #pragma unroll
   for (int k = 0; k < 2; ++k) before[k] = sum_in_front(mine[k], part[k], all[k]);
   const int of = all[0] > 0.0 ? 0 : 1;            // nothing is left: the row as it is
   const double place = (double)a.sample[b] * all[of];
-  __syncthreads();
-  double upto = before[of];
+  int chosen = -1, last = -1;
+  double upto = of ? before[1] : before[0], before_mine = 0.0;
   for (int i = first; i < end; ++i) {
     const double s = sums[2 * i + of];
+    if (s > 0.0 && chosen < 0) {
+      last = i, before_mine = upto;
+      if (upto + s > place) chosen = i;
+    }
     upto += s;
-    if (s > 0.0) {
-      atomicMax(&last, i);
-      if (upto > place) atomicMin(&chosen, i);
-    }
   }
-  __syncthreads();
-  const int piece = chosen == INT32_MAX ? last : chosen;
-  if (piece < 0 || !(all[of] < INFINITY)) {       // no weight at all
+  int piece = one_of(chosen >= 0, chosen, true, -1, words[0]);
+  const int last_piece = one_of(last >= 0, last, false, -1, words[1]);
+  piece = piece < 0 ? last_piece : piece;
+  const auto give = [&](int x) {
     if (tid == 0) {
-      if (a.wide) static_cast<int64_t*>(a.token)[b] = -1;
-      else static_cast<int32_t*>(a.token)[b] = -1;
+      if (a.wide) static_cast<int64_t*>(a.token)[b] = x;
+      else static_cast<int32_t*>(a.token)[b] = x;
     }
+  };
+  if (piece < 0 || !(all[of] < INFINITY)) {       // no weight at all
+    give(-1);
     return;
   }
-  if (piece >= first && piece < end) {
-    double s = before[of];
-    for (int i = first; i < piece; ++i) s += sums[2 * i + of];
-    before_piece = s;
-  }
-  __syncthreads();
-  if (tid == 0) chosen = INT32_MAX, last = -1;
+  if (last == piece) before_piece = before_mine;   // (one thread's)
   const int v0 = piece * a.piece, v1 = min(v0 + a.piece, a.V);
   hide(a, b, count, row, v0, v1, list, &hidden);
   __syncthreads();
   const Rest rest = rest_of(a, b, count, row, list, hidden);
   // (a piece is a multiple of kPiece; in turns of kPiece, so that neighbours read what lies together)
   double from = before_piece;
+  int token = -1;
   for (int t0 = v0; t0 < v1; t0 += kPiece) {
     const int v = t0 + tid * kEach;
     double r[kEach], p[kEach], sum = 0.0, turn;
@@ -310,27 +330,29 @@ __global__ void __launch_bounds__(kThreads) next_token_kernel(VerifyArgs a) {
     if (v < v1) rest.weights<DT>(v, a.V, r, p);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      if (of) r[i] = p[i];
+      r[i] = of ? p[i] : r[i];
       sum += r[i];
     }
     double at = from + sum_in_front(sum, part[2], turn);
+    chosen = last = -1;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       at += r[i];
       if (r[i] > 0.0) {
-        atomicMax(&last, v + i);
-        if (at > place) atomicMin(&chosen, v + i);
+        last = v + i;
+        if (chosen < 0 && at > place) chosen = v + i;
       }
     }
+    const int there = one_of(chosen >= 0, chosen, true, -1, words[2]), behind = one_of(last >= 0, last, false, -1, words[3]);
     from += turn;
+    if (there >= 0) {
+      token = there;
+      break;
+    }
+    token = behind >= 0 ? behind : token;
     __syncthreads();
-    if (chosen != INT32_MAX) break;
   }
-  if (tid == 0) {
-    const int x = chosen == INT32_MAX ? last : chosen;
-    if (a.wide) static_cast<int64_t*>(a.token)[b] = x;
-    else static_cast<int32_t*>(a.token)[b] = x;
-  }
+  give(token);
 }
 
 // Accepted rows ------------------------------------------------------------------------------------------------------
@@ -395,9 +417,8 @@ struct ReserveArgs {
   Div page_size;
 };
 
-constexpr int kSequences = 1024;     // threads, and sequences of a turn
-
-__device__ __forceinline__ int sum_upto(int x, int* part) {   // over the workgroup; part: 16 words of LDS
+template <int THREADS>
+__device__ __forceinline__ int sum_upto(int x, int* part) {   // over the workgroup; part: a word of LDS for each wave
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -411,16 +432,13 @@ __device__ __forceinline__ int sum_upto(int x, int* part) {   // over the workgr
 }
 
 // One workgroup.  First the pages of sequences that need fewer go on the stack, then those that need more take theirs.  Sequences are added up
-// a thread each, then every thread moves entries, of any sequence: the k-th of a turn belongs to the last sequence that begins at or before k.
-__global__ void __launch_bounds__(kSequences) cache_reserve_kernel(ReserveArgs a) {
-  __shared__ int start[kSequences], entry[kSequences], part[kSequences / 64], total, refused;
+// a thread each, in turns of as many as there are threads; then every thread moves entries, of any sequence: the k-th of a turn belongs to the last sequence that
+// begins at or before k.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) cache_reserve_kernel(ReserveArgs a) {
+  __shared__ int start[THREADS], entry[THREADS], part[THREADS / 64], total, refused;
   const int tid = threadIdx.x;
   int there = min(max(*a.available, 0), a.pages);
-  const auto needed = [&](int b) {
-    int n = 0;
-    for (int h = 0; h < a.H; ++h) n = max(n, a.lengths.at[b * a.lengths.sb + h * a.lengths.sh]);
-    return (int)a.page_size.of((uint32_t)n) + ((int)(a.page_size.of((uint32_t)n) * a.page_size.d) < n ? 1 : 0);
-  };
   const auto sequence_of = [&](int k, int n) {   // the last one of n with start <= k
     int low = 0, high = n;
     while (high - low > 1) {
@@ -432,37 +450,41 @@ __global__ void __launch_bounds__(kSequences) cache_reserve_kernel(ReserveArgs a
   };
   constexpr int kMoves = 4;                      // of a thread at once, so that its loads overlap
   if (tid == 0) refused = 0;
+  int need = 0, held = 0;
+#pragma unroll 1
   for (int grow = 0; grow < 2; ++grow) {
-    for (int b0 = 0; b0 < a.B; b0 += kSequences) {
-      const int b = b0 + tid, n = min(kSequences, a.B - b0);
-      int need = 0, held = 0, moves = 0;
-      if (b < a.B) {
-        need = needed(b);
+#pragma unroll 1
+    for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+      const int b = b0 + tid, n = min(THREADS, a.B - b0);
+      int moves = 0;
+      if (b < a.B && (!grow || a.B > THREADS)) {
+        int length = 0;
+        for (int h = 0; h < a.H; ++h) length = max(length, a.lengths.at[b * a.lengths.sb + h * a.lengths.sh]);
+        need = (int)a.page_size.of((uint32_t)length);
+        need += need * (int)a.page_size.d < length ? 1 : 0;
         held = min(max(a.held[b], 0), a.table_pages);
-        if (need <= a.table_pages) moves = grow ? max(need - held, 0) : max(held - need, 0);
       }
-      __syncthreads();
-      const int upto = sum_upto(moves, part);
-      bool fits = true;
-      if (grow) fits = !refused && upto <= there;                     // (upto never falls: from the first that does not fit on)
-      else fits = upto <= a.pages - there;
+      if (b < a.B && need <= a.table_pages) moves = max(grow ? need - held : held - need, 0);
+      if (tid == 0) total = 0;
+      const int upto = sum_upto<THREADS>(moves, part);
+      // (of those that grow upto never falls: from the first one that does not fit on)
+      const bool fits = grow ? !refused && upto <= there : upto <= a.pages - there;
       start[tid] = upto - moves;
       entry[tid] = grow ? held : need;
-      if (tid == 0) total = 0;
-      __syncthreads();
-      if (fits) atomicMax(&total, upto);
+      if (fits && moves) atomicMax(&total, upto);
       if (b < a.B) {
-        if (moves && fits) a.held[b] = need;
+        if (moves && fits) a.held[b] = held = need;
         if (grow) a.granted[b] = need <= a.table_pages && (moves == 0 || fits);
       }
       __syncthreads();
       if (grow && !fits && moves) refused = 1;
       const int all = total;
-      for (int k0 = 0; k0 < all; k0 += kMoves * kSequences) {
+#pragma unroll 1
+      for (int k0 = 0; k0 < all; k0 += kMoves * THREADS) {
         int32_t *place[kMoves], x[kMoves];
 #pragma unroll
         for (int j = 0; j < kMoves; ++j) {
-          const int k = k0 + j * kSequences + tid;
+          const int k = k0 + j * THREADS + tid;
           place[j] = nullptr;
           if (k >= all) continue;
           const int s = sequence_of(k, n);
@@ -475,7 +497,7 @@ __global__ void __launch_bounds__(kSequences) cache_reserve_kernel(ReserveArgs a
           if (grow) {
             *place[j] = x[j];
           } else {
-            a.free[there + k0 + j * kSequences + tid] = x[j];
+            a.free[there + k0 + j * THREADS + tid] = x[j];
             *place[j] = -1;
           }
         }
@@ -595,7 +617,9 @@ int fcr_cache_reserve(int32_t* table, int64_t table_stride, int table_pages, int
   a.granted = granted;
   a.B = B, a.H = lengths_strides[1] ? H : 1, a.table_pages = table_pages, a.pages = pages;
   a.page_size.set((uint32_t)page_size);
-  hipLaunchKernelGGL(cache_reserve_kernel, dim3(1), dim3(kSequences), 0, static_cast<hipStream_t>(stream), a);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (B <= 64) hipLaunchKernelGGL((cache_reserve_kernel<256>), dim3(1), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((cache_reserve_kernel<1024>), dim3(1), dim3(1024), 0, s, a);
   return launched("cache_reserve_kernel");
 }
 

@@ -99,6 +99,7 @@ def sight(tmp_path_factory):
         'extern "C" void sight(int context, int count, int prefix, int window, int T, int positions, int first, int last, int* out) {\n'
         '  const Sight s(context, count, prefix, window, T, positions, first, last);\n'
         '  out[0] = s.blocks(); out[1] = s.n;\n'
+        '  if (s.position(128 * out[0]) < s.n || s.position(-32) < s.n) out[0] = -1;\n'
         '  for (int i = 0; i < 4 * out[0]; ++i) { const int p = s.position(32 * i);\n'
         '    out[2 + 3 * i] = p; out[3 + 3 * i] = s.whole(p, 32); out[4 + 3 * i] = s.any(p, 32); } }\n')
     subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "flash_colreduce_amd", "csrc"), str(tmp / "s.cpp"), "-o",
@@ -126,7 +127,12 @@ def test_blocks_of_a_tile_hold_every_key_that_it_sees(sight):
         some = set().union(*seen.values())
         steps = [(out[2 + 3 * i], out[3 + 3 * i], out[4 + 3 * i]) for i in range(4 * out[0])]
         at = [p for p, _, _ in steps]
-        assert all(a < z for a, z in zip(at, at[1:])) and all(p % 32 == 0 for p in at)
+        if not some:
+            assert out[0] == 1
+            continue
+        # blocks from the last one on, the steps of a block in their order
+        assert all(p % 128 == 32 * (i % 4) and p // 128 == at[i - i % 4] // 128 for i, p in enumerate(at))
+        assert all(a > z >= 0 for a, z in zip(at[::4], at[4::4])) and at[-4] >= 0
         assert some <= {j for p in at for j in range(p, p + 32)}
         for p, whole, any_ in steps:
             step = set(range(p, p + 32))
