@@ -439,8 +439,7 @@ __global__ void __launch_bounds__(THREADS) cache_reserve_kernel(ReserveArgs a) {
   __shared__ int start[THREADS], entry[THREADS], part[THREADS / 64], total, refused;
   const int tid = threadIdx.x;
   int there = min(max(*a.available, 0), a.pages);
-  const auto sequence_of = [&](int k, int n) {   // the last one of n with start <= k
-    int low = 0, high = n;
+  const auto sequence_of = [&](int k, int low, int high) {   // the last one of [low, high) with start <= k
     while (high - low > 1) {
       const int mid = (low + high) >> 1;
       if (start[mid] <= k) low = mid;
@@ -448,7 +447,7 @@ __global__ void __launch_bounds__(THREADS) cache_reserve_kernel(ReserveArgs a) {
     }
     return low;
   };
-  constexpr int kMoves = 4;                      // of a thread at once, so that its loads overlap
+  constexpr int kMoves = 16;                     // of a thread at once, at most, so that its loads overlap
   if (tid == 0) refused = 0;
   int need = 0, held = 0;
 #pragma unroll 1
@@ -478,16 +477,20 @@ __global__ void __launch_bounds__(THREADS) cache_reserve_kernel(ReserveArgs a) {
       }
       __syncthreads();
       if (grow && !fits && moves) refused = 1;
-      const int all = total;
+      const int all = total, moved = min((all + THREADS - 1) / THREADS, kMoves);
 #pragma unroll 1
-      for (int k0 = 0; k0 < all; k0 += kMoves * THREADS) {
+      for (int k0 = (tid & ~63) * moved; k0 < all; k0 += moved * THREADS) {
+        // of many moves the wave's first and last one bound the search of the others: a long sequence needs none
+        const int lane = tid & 63;
+        int from = 0, to = n;
+        if (moved > 1) from = sequence_of(k0, 0, n), to = sequence_of(min(k0 + 64 * moved, all) - 1, from, n) + 1;
         int32_t *place[kMoves], x[kMoves];
 #pragma unroll
         for (int j = 0; j < kMoves; ++j) {
-          const int k = k0 + j * THREADS + tid;
+          const int k = k0 + j * 64 + lane;
           place[j] = nullptr;
-          if (k >= all) continue;
-          const int s = sequence_of(k, n);
+          if (j >= moved || k >= all) continue;
+          const int s = sequence_of(k, from, to);
           place[j] = a.table + (b0 + s) * a.table_stride + entry[s] + (k - start[s]);
           x[j] = grow ? a.free[there - 1 - k] : *place[j];
         }
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(THREADS) cache_reserve_kernel(ReserveArgs a) {
           if (grow) {
             *place[j] = x[j];
           } else {
-            a.free[there + k0 + j * THREADS + tid] = x[j];
+            a.free[there + k0 + j * 64 + lane] = x[j];
             *place[j] = -1;
           }
         }
