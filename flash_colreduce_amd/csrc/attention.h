@@ -624,12 +624,11 @@ __device__ __forceinline__ uint32_t tree_seen_by(const Args& a, int b, int row, 
   return seen & there;
 }
 // What the rows of an item of tree_attention see: `position` of the keys that lie `at` keys behind the first one of their blocks; whether every row
-// sees `len` keys from pos on, whether a row might see one of them, and whether no row's mask is asked about them.
+// sees `len` keys from pos on, and whether no row's mask is asked about them.
 struct TreeView {
   int context, n;
   __device__ __forceinline__ int position(int at) const { return at; }
   __device__ __forceinline__ bool whole(int pos, int len) const { return pos + len <= min(context, n); }
-  __device__ __forceinline__ bool any(int pos, int) const { return pos < n; }
   __device__ __forceinline__ bool settled(int pos, int len) const { return pos + len <= context; }
 };
 // Which of the lane's keys are there: in front of n, on a page that is.  Bits 4 t + i.
@@ -671,7 +670,7 @@ __device__ __forceinline__ void emit_part(float* to, int d0, const float (&x)[F:
 
 // The blocks of a workgroup, as pieces of items.  Lengths are known on the device only: every workgroup adds them up.  Lengths of
 // sequences (not of heads): an entry is all heads of one.
-template <int THREADS, bool TALL, int ROWS>
+template <int THREADS, bool TALL>
 struct TreeDeal {
   int at, end, b, h, tile, blk, nb, context, n;
   // (Short on purpose: this and what else runs once per workgroup costs about 200 cycles per 64 bytes of instructions, which come
@@ -791,15 +790,13 @@ struct TreeDeal {
 // workgroups are dealt to 8 dies in turn: consecutive ranges of blocks, whose row tiles share keys, go to one die
 __device__ __forceinline__ int range_of(const Args& a, int block) { return (block & 7) * (a.wgs >> 3) + (block >> 3); }
 
-// How tree_attention cuts its work, and what a wave's rows see.
+// How tree_attention cuts its work, and what its rows see.
 struct Tree {
   static constexpr bool bent = false;              // scores are products times a scale
-  static constexpr bool rising = true;             // a row that sees nothing of a step sees nothing behind it
+  static constexpr bool rising = true;             // the last keys come last
   static constexpr int kScan = 2;                  // words of LDS behind those of the waves
-  template <int THREADS, bool TALL, int ROWS>
-  using Deal = TreeDeal<THREADS, TALL, ROWS>;
-  static __device__ __forceinline__ bool idle(const Args& a, int, int row0) { return row0 >= a.rows; }
-  static __device__ __forceinline__ TreeView of_rows(const Args&, const TreeView& v, int, int, int, int) { return v; }
+  template <int THREADS>
+  using Deal = TreeDeal<THREADS, false>;
   static __device__ __forceinline__ uint32_t seen_by(const Args& a, const TreeView& v, int b, int row, int pos, uint32_t there, int g) {
     return tree_seen_by(a, b, row, pos, v.context, there, g);
   }
@@ -815,7 +812,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) f
   const int wg = range_of(args, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const Lane<F> at(threadIdx.x & 63);
-  typename P::template Deal<256, false, 16> deal;
+  typename P::template Deal<256> deal;
   if (!deal.start(arguments(), wg, scan)) return;
   do {
     const Args& a = arguments();
@@ -960,7 +957,7 @@ constexpr int tall_keys(int w, int waves) { return w == 1 || (w == 2 && waves ==
 // waves converts later in the stage, for the same reason.
 // One barrier per stage, before the products of its last step, which read the first keys of the next stage: that has been written by then, and
 // the stage before, whose place it takes, was last read before the last such barrier.
-template <class P, int CD, int W, int WAVES>
+template <int CD, int W, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args) {
   using F = Form<CD, W>;
   constexpr int RT = tall_tiles(W), kKeys = tall_keys(W, WAVES), kSteps = kKeys / 32, kTiles = kKeys / 16;
@@ -982,31 +979,28 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
   __shared__ float most[2][kTiles];                                      // the largest scale of a tile's values
   __shared__ int flags[2][kTiles];                                       // a tile's page is there, and (bit 1) one of its values was not finite
   __shared__ float rest[WAVES][RT][16];                                  // powers of two that rows' scores are still to be multiplied by
-  __shared__ int scan[WAVES + P::kScan];
+  __shared__ int scan[WAVES + 2];
   const int wg = range_of(args, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const Lane<F> at(threadIdx.x & 63);
   const int my_tile = kApart ? wave % kTiles : wave * kMine;
   const bool my_keys = !kApart || wave < kTiles, my_values = !kApart || wave >= kTiles;
-  typename P::template Deal<64 * WAVES, true, 16 * RT * WAVES> deal;
+  TreeDeal<64 * WAVES, true> deal;
   if (!deal.start(arguments(), wg, scan)) return;
   do {
-    const int b = deal.b;
-    const auto view = deal.view();
-    const int n = view.n;
+    const int b = deal.b, n = deal.n, context = deal.context;
     const int row0 = (deal.tile * WAVES + wave) * 16 * RT;
-    const bool idle = P::idle(arguments(), b, row0);                               // (it converts all the same)
-    const auto mine = P::of_rows(arguments(), view, b, deal.h, row0, 16 * RT);     // what the wave's rows see
+    const bool idle = row0 >= arguments().rows;                                    // (it converts all the same)
     const bool late = WAVES == 8 && wave >= 4;
     Keys<F> k[kMine];
     Values<F> v[kMine];
     const Source src(arguments(), b, deal.h, n);
     Place place[kMine], ahead[kMine];                                    // of the rows loaded last, and of the next ones
-    const int at0 = deal.blk * kBlock;
+    const int pos0 = deal.blk * kBlock;
     const int steps = (deal.stop() - deal.blk) * (kBlock / 32), stages = steps / kSteps;
     const auto look = [&](int stage) {
 #pragma unroll
-      for (int t = 0; t < kMine; ++t) ahead[t] = Place(src, view.position(at0 + stage * kKeys) + (my_tile + t) * 16);
+      for (int t = 0; t < kMine; ++t) ahead[t] = Place(src, pos0 + stage * kKeys + (my_tile + t) * 16);
     };
     const auto fetch = [&](int stage) {
       const int D = arguments().D;
@@ -1050,8 +1044,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       by = __builtin_amdgcn_ldexpf(by, -least);
     }
     q.arrive();
-    Bend<RT> bend;
-    if constexpr (P::bent) bend.load(arguments(), deal.h, row0, view.context, at.col);
     State<F, RT> st;
     st.clear();
     const auto convert = [&](int stage) {
@@ -1060,11 +1052,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
       int flag[kMine];
 #pragma unroll
       for (int t = 0; t < kMine; ++t) {
-        const int pos = view.position(at0 + stage * kKeys) + (my_tile + t) * 16;
+        const int pos = pos0 + stage * kKeys + (my_tile + t) * 16;
         flag[t] = place[t].there(src) ? 1 : 0;
-        if (my_values && (!flag[t] || !view.whole(pos, 16))) {
+        if (my_values && (!flag[t] || pos + 16 > min(context, n))) {
           v[t].drop(there_of(pos, n, flag[t], flag[t], at.g));
-          if constexpr (!F::finite) flag[t] |= !view.settled(pos, 16) && __any(v[t].clean()) ? 2 : 0;
+          if constexpr (!F::finite) flag[t] |= pos + 16 > context && __any(v[t].clean()) ? 2 : 0;
         }
         if (my_keys) {
 #pragma unroll
@@ -1151,10 +1143,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
     }
     // (in the loop: the step before the first one does this, with values and weights of 0)
     for (int i = kInLoop ? -1 : 0; i < steps; ++i) {
-      const int stage = i < 0 ? -1 : i / kSteps, j = i < 0 ? kSteps - 1 : i % kSteps, pos = view.position(at0 + i * 32);
-      const bool some = !idle && mine.any(pos, 32), work = some && (!kInLoop || i >= 0);
-      // (rows that see nothing of this step may need the products of the next one)
-      const bool run = P::rising ? some : work || (!idle && i + 1 < steps && mine.any(view.position(at0 + i * 32 + 32), 32));
+      const int stage = i < 0 ? -1 : i / kSteps, j = i < 0 ? kSteps - 1 : i % kSteps, pos = pos0 + i * 32;
+      const bool run = !idle && pos < n, work = run && (!kInLoop || i >= 0);
       u32x4 vf[F::DT], p[RT];
       uint32_t seen[RT];
       bool not_finite = false;
@@ -1163,14 +1153,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
 #pragma unroll
         for (int d = 0; d < kEarly; ++d) vf[d] = from[d * 64];
         const int f0 = __builtin_amdgcn_readfirstlane(flag[0]), f1 = __builtin_amdgcn_readfirstlane(flag[1]);
-        const bool masked = !mine.whole(pos, 32) || !(f0 & f1 & 1);
+        const bool masked = pos + 32 > min(context, n) || !(f0 & f1 & 1);
         not_finite = !F::finite && ((f0 | f1) & 2) != 0;
 #pragma unroll
         for (int r = 0; r < RT; ++r) seen[r] = 0xff;
         if (masked) {
           const uint32_t there = there_of(pos, n, f0 & 1, f1 & 1, at.g);
 #pragma unroll
-          for (int r = 0; r < RT; ++r) seen[r] = P::seen_by(arguments(), mine, b, row0 + 16 * r + at.col, pos, there, at.g);
+          for (int r = 0; r < RT; ++r) seen[r] = tree_seen_by(arguments(), b, row0 + 16 * r + at.col, pos, context, there, at.g);
         }
         if (F::codes && __builtin_expect(apart, 0)) {
 #pragma unroll
@@ -1180,9 +1170,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) tall_attention_kernel(Args args
             for (int t = 0; t < 2; ++t) s[r][t] = s[r][t] * by_row;
           }
         }
-        if constexpr (P::bent) bend.of(k_scale, pos, at.g, s);
         weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
-      } else if (kInLoop || !P::rising) {
+      } else if (kInLoop) {
 #pragma unroll
         for (int d = 0; d < F::DT; ++d) vf[d] = u32x4{0, 0, 0, 0};
 #pragma unroll
@@ -1334,30 +1323,6 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Args a, int tile_ro
   }
 }
 #endif
-
-template <class P, int CD, int W>
-bool launch_w(const Args& a, int form, hipStream_t s) {
-  const dim3 grid((unsigned)a.wgs);
-  if (form == 1) {
-    hipLaunchKernelGGL((few_attention_kernel<P, CD, W>), grid, dim3(256), 0, s, a);
-  } else if (form == 8) {
-    hipLaunchKernelGGL((tall_attention_kernel<P, CD, W, 8>), grid, dim3(512), 0, s, a);
-  } else {
-    if constexpr (W > 2) return false;
-    else hipLaunchKernelGGL((tall_attention_kernel<P, CD, W, 4>), grid, dim3(256), 0, s, a);
-  }
-  return true;
-}
-// form: see form_of.  false: there is no such kernel
-template <class P, int CD>
-bool launch(const Args& a, int w, int form, hipStream_t s) {
-  switch (w) {
-    case 1: return launch_w<P, CD, 1>(a, form, s);
-    case 2: return launch_w<P, CD, 2>(a, form, s);
-    case 3: return launch_w<P, CD, 3>(a, form, s);
-    default: return launch_w<P, CD, 4>(a, form, s);
-  }
-}
 
 #if FCR_HAS(0)
 using fcr_detail::fail;

@@ -20,7 +20,7 @@ __device__ __forceinline__ Sight view_of(const Args& a, int b, int h, int r0, in
 // Blocks of all items laid end to end, `per` of them for every workgroup, found from the lengths on the device.  A thread adds up the blocks of some consecutive
 // (entry, tile) pairs, an entry being a sequence, or one of its heads where these differ in length; all heads of a sequence have the same number S of blocks.  A place
 // among the blocks is then found in two steps: its entry, by the place over the number of heads, and the tile, by what is left of the place over S.
-template <int THREADS, bool TALL, int ROWS>
+template <int THREADS, int ROWS>
 struct ChunkDeal {
   int at, end, b, h, tile, blk, nb;
   Sight seen;
@@ -131,14 +131,8 @@ template <bool BENT>
 struct Chunk {
   static constexpr bool bent = BENT, rising = false;
   static constexpr int kScan = 4;
-  template <int THREADS, bool TALL, int ROWS>
-  using Deal = ChunkDeal<THREADS, TALL, ROWS>;
-  static __device__ __forceinline__ bool idle(const Args& a, int b, int row0) {
-    return row0 >= a.rows || (a.tree_lengths && (int)a.G.of((uint32_t)row0) >= constant_at(a.tree_lengths + b));
-  }
-  static __device__ __forceinline__ Sight of_rows(const Args& a, const Sight&, int b, int h, int row0, int rows) {
-    return view_of(a, b, h, min(row0, a.rows - 1), row0 + rows);
-  }
+  template <int THREADS>
+  using Deal = ChunkDeal<THREADS, 16>;
   static __device__ __forceinline__ uint32_t seen_by(const Args& a, const Sight& v, int, int row, int pos, uint32_t there, int g) {
     asm volatile("" : "+v"(row), "+v"(g));       // (formed here, not kept)
     const int token = row < a.rows ? (int)a.G.of((uint32_t)row) : 0;
@@ -152,6 +146,349 @@ struct Chunk {
     return seen & there;
   }
 };
+// Many rows: the scheme of tall_attention_kernel (attention.h), two stages of keys in LDS, converted by all waves; a wave has 16 RT rows, of which it leaves out the
+// steps that none sees.  What a step costs beside its products and weights is kept small, since it is the vector and scalar instructions of two waves that a SIMD
+// spends its time on: a step is a slot of a ring in LDS at one address, what the wave sees of it follows from one number that falls by 32 (Steps), and what is used once per
+// stage is formed there from the arguments.
+template <bool BENT, int CD, int W, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args args) {
+  using F = Form<CD, W>;
+  constexpr int RT = tall_tiles(W), kKeys = tall_keys(W, WAVES), kSteps = kKeys / 32, kTiles = kKeys / 16, kStepsLog2 = kSteps == 4 ? 2 : 1;
+  constexpr int kMine = kTiles > WAVES ? kTiles / WAVES : 1;             // 16-key tiles that a wave converts
+  constexpr bool kApart = kTiles < WAVES;                                // a wave converts a tile's keys or its values
+  constexpr int kValues = 2 * F::KS * 64, kStep = kValues + F::DT * 64;  // where a step's values begin, and the next step, in 16 bytes
+  constexpr int kRing = 2 * kSteps;                                      // steps in LDS
+  // Rows of 256 elements leave no registers for both halves of a step's values, or for keys next to them.
+  constexpr bool kLean = W == 4;
+  // The first stage is converted in the loop, and not by code in front of it, which made 16-bit kernels of more than 64 elements spill 5 to 39
+  // registers: 128 rows over 4 x 8 heads of 8192 bf16 keys of 128 elements 57 -> 54 us, 1024 rows of 256 elements 451 -> 413, int8 393 -> 383.
+  // (fp16 and bf16 rows of 256 elements still spill 15, bf16 of 128 and e4m3 of 256 two.)
+  // With 64 elements, where nothing spills, 1 to 10 % are lost.
+  constexpr bool kInLoop = W >= 2;
+  constexpr int kEarly = W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights
+  static_assert(kTiles * (kApart ? 2 : 1) == WAVES * kMine, "every wave has its share of a stage");
+  __shared__ u32x4 operands[kRing * kStep];
+  __shared__ __attribute__((aligned(16))) float scales[kRing][2][32];    // of keys, of values
+  __shared__ float most[kRing][2];                                       // the largest scale of a tile's values
+  __shared__ int2 flags[kRing];                                          // a tile's page is there, and (bit 1) one of its values was not finite
+  __shared__ float rest[WAVES][RT][16];                                  // powers of two that rows' scores are still to be multiplied by
+  __shared__ int scan[WAVES + 4];
+  const int wg = range_of(args, blockIdx.x);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const Lane<F> at(threadIdx.x & 63);
+  const int my_tile = kApart ? wave % kTiles : wave * kMine;
+  const bool my_keys = !kApart || wave < kTiles, my_values = !kApart || wave >= kTiles;
+  ChunkDeal<64 * WAVES, 16 * RT * WAVES> deal;
+  if (!deal.start(arguments(), wg, scan)) return;
+  do {
+    const int b = deal.b, h = deal.h, D = arguments().D;
+    const Sight view = deal.view();
+    const int n = view.n;
+    const int row0 = (deal.tile * WAVES + wave) * 16 * RT;
+    const bool late = WAVES == 8 && wave >= 4;
+    // (a wave without rows converts all the same)
+    const Steps sees(view_of(arguments(), b, h, min(row0, arguments().rows - 1), row0 + 16 * RT), view, row0 < arguments().rows);
+    Keys<F> k[kMine];
+    Values<F> v[kMine];
+    // (formed from the arguments where it is used: it would take 25 scalar registers of all loops)
+    const auto source = [&]() { return Source(arguments(), b, h, n); };
+    Place place[kMine], ahead[kMine];                                    // of the rows loaded last, and of the next ones
+    const int steps = (deal.stop() - deal.blk) * (kBlock / 32), stages = steps / kSteps;
+    const int x0 = (deal.nb - deal.blk) * kBlock - 32;                   // of the first step: the last keys are taken first
+    const auto x_of = [&](int stage, int t) { return x0 - 32 * (stage * kSteps + (my_tile + t) / 2) + 16 * ((my_tile + t) & 1); };
+    const auto look = [&](const Source& src, int stage) {
+#pragma unroll
+      for (int t = 0; t < kMine; ++t) ahead[t] = Place(src, view.key(x_of(stage, t)));
+    };
+    const auto fetch = [&](int stage) {
+      const Source src = source();
+      const Lane<F> here = at.again();
+#pragma unroll
+      for (int t = 0; t < kMine; ++t) {
+        place[t] = ahead[t];
+        if (my_keys) k[t].template load<false>(src, D, place[t], here);
+        if (my_values) v[t].load(src, D, place[t], here);
+      }
+      look(src, stage + 1);
+    };
+    look(source(), 0);
+    fetch(0);
+    Queries<F, RT> q;
+    float by = arguments().scale2;
+    q.load(arguments(), b, h, row0, at);
+    __syncthreads();                                                     // (the piece before has been used)
+    bool apart = false;
+    if (F::codes && arguments().bf16) {
+      // One power of two for all rows of the workgroup, which the keys' scales undo; rows that it would leave under 2^-16 of the largest have
+      // their own, and their scores are multiplied by the rest.
+      int up[RT], least = kNoPower;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) least = min(least, up[r] = q.power(r));
+      least = least_of_row(least);
+      if (at.lane == 0) scan[wave] = least;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) least = min(least, scan[w]);
+      least = __builtin_amdgcn_readfirstlane(least);
+      least = least == kNoPower ? 0 : least;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const int mine = up[r] - least > 16 && up[r] != kNoPower ? up[r] : least;
+        q.scale(r, mine);
+        apart = apart || mine != least;
+        if (at.g == 0) rest[wave][r][at.col] = __builtin_amdgcn_ldexpf(1.0f, least - mine);
+      }
+      apart = __any(apart);
+      by = __builtin_amdgcn_ldexpf(by, -least);
+    }
+    q.arrive();
+    Bend<RT> bend;
+    if constexpr (BENT) bend.load(arguments(), h, row0, view.context, at.col);
+    State<F, RT> st;
+    st.clear();
+    const auto convert = [&](int stage) {
+      const int pages = arguments().c.pages;
+#pragma unroll
+      for (int t = 0; t < kMine; ++t) {
+        const int x = x_of(stage, t), slot = (stage * kSteps + (my_tile + t) / 2) & (kRing - 1), half = (my_tile + t) & 1;
+        u32x4* const to = operands + slot * kStep + at.lane;
+        float* const sc = scales[slot][0] + 16 * half;
+        const int pos = view.key(x);
+        int flag = (uint32_t)place[t].page < (uint32_t)pages ? 1 : 0;
+        if (my_values && (!flag || !view.whole(pos, 16))) {
+          v[t].drop(there_of(pos, n, flag, flag, at.g));
+          if constexpr (!F::finite) flag |= __any(v[t].clean()) ? 2 : 0;
+        }
+        if (my_keys) {
+#pragma unroll
+          for (int c = 0; c < F::KS; ++c) to[(half * F::KS + c) * 64] = k[t].operand(c);
+          if constexpr (!F::codes) {
+            // What lies behind the rows becomes zeros here (see tall_attention_kernel).
+            if (__builtin_expect(D % 64 != 0, 0)) {
+              const Lane<F> here = at.again();
+              uint32_t zero = 0;
+              asm volatile("" : "+v"(zero));       // (formed here, not kept)
+#pragma unroll
+              for (int c = F::KS - 2; c < F::KS; ++c)
+                if (here.behind(c, D)) to[(half * F::KS + c) * 64] = u32x4{zero, zero, zero, zero};
+            }
+          }
+          if (F::codes && at.col == 0) *reinterpret_cast<f32x4*>(sc + 4 * at.g) = k[t].scale * by;
+        }
+        if (my_values) {
+          if constexpr (F::codes) {
+            if (at.col == 0) *reinterpret_cast<f32x4*>(sc + 32 + 4 * at.g) = v[t].scale;
+            const f32x4 x = v[t].scale;
+            const float m = across(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))), true);
+            if (at.lane == 0) most[slot][half] = fmaxf(m, 0.0f);   // (a NaN does not count)
+          }
+          if (at.lane == 0) reinterpret_cast<int*>(flags + slot)[half] = flag;
+          if constexpr (kMine == 1) {
+#pragma unroll
+            for (int d = 0; d < F::DT; ++d) reinterpret_cast<u32x2*>(to + kValues + d * 64)[half] = v[0].operand(d);
+          } else if (t & 1) {
+#pragma unroll
+            for (int d = 0; d < F::DT; ++d) to[kValues + d * 64] = joined_operand(v[t - 1].operand(d), v[t].operand(d));
+          }
+        }
+      }
+    };
+    // What a step reads from LDS is read ahead: keys, scales and flags under the products of the step before, values under the weights.
+    // (Left to itself the scheduler reads each operand in front of its use, to save registers, and waits for it.)
+    f32x4 s[RT][2], k_scale[2], v_scale[2];
+    u32x4 kf[2][F::KS];
+    float most_v = 1.0f;
+    int2 flag;
+    const auto slot_of = [&](int i) { return operands + (i & (kRing - 1)) * kStep + at.lane; };
+    const auto read_keys = [&](int i, int t) {
+      const u32x4* const from = slot_of(i) + t * F::KS * 64;
+#pragma unroll
+      for (int c = 0; c < F::KS; ++c) kf[t][c] = from[c * 64];
+    };
+    const auto read_scales = [&](int i) {
+      const int slot = i & (kRing - 1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (F::codes) {
+          const float* const sc = scales[slot][0] + 16 * t + 4 * at.g;
+          k_scale[t] = *reinterpret_cast<const f32x4*>(sc);
+          v_scale[t] = *reinterpret_cast<const f32x4*>(sc + 32);
+        } else {
+          k_scale[t] = f32x4{by, by, by, by};
+          v_scale[t] = f32x4{1, 1, 1, 1};
+        }
+      }
+      flag = flags[slot];
+      if constexpr (F::codes) most_v = fmaxf(most[slot][0], most[slot][1]);
+    };
+    const auto products_of = [&](int t) {                                // of the keys read last with the queries
+#pragma unroll
+      for (int c = 0; c < F::KS; ++c)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(kf[t][c], q.w[r][c], c ? s[r][t] : f32x4{0, 0, 0, 0});
+    };
+    if constexpr (!kInLoop) {
+      convert(0);
+      if (stages > 1) fetch(1);
+      __syncthreads();
+      if (sees.high | sees.prefix) {
+        read_keys(0, 0);
+        read_keys(0, 1);
+        read_scales(0);
+        products_of(0);
+        products_of(1);
+      }
+    }
+    // (in the loop: the step before the first one does this, with values and weights of 0)
+    int x = kInLoop ? x0 + 32 : x0;
+    bool next = sees.some(x);
+    for (int i = kInLoop ? -1 : 0; i < steps; ++i, x -= 32) {
+      const int stage = i >> kStepsLog2, j = i & (kSteps - 1);
+      const bool work = next && (!kInLoop || i >= 0);
+      next = i + 1 < steps && sees.some(x - 32);
+      const bool run = work || next;                     // (rows that see nothing of this step may need the products of the next one)
+      u32x4 vf[F::DT], p[RT];
+      uint32_t seen[RT];
+      bool not_finite = false;
+      if (work) {
+        const u32x4* const from = slot_of(i) + kValues;
+#pragma unroll
+        for (int d = 0; d < kEarly; ++d) vf[d] = from[d * 64];
+        const int f0 = __builtin_amdgcn_readfirstlane(flag.x), f1 = __builtin_amdgcn_readfirstlane(flag.y);
+        const bool masked = !sees.whole(x) || ((f0 ^ 1) | (f1 ^ 1)) != 0;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) seen[r] = 0xff;
+        if (masked) {
+          not_finite = !F::finite && ((f0 | f1) & 2) != 0;
+          const Lane<F> here = at.again();
+          const int pos = view.key(x);
+          const uint32_t there = there_of(pos, n, f0 & 1, f1 & 1, here.g);
+          const Sight rows = view_of(arguments(), b, h, row0, row0 + 16 * RT);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) seen[r] = Chunk<BENT>::seen_by(arguments(), rows, b, row0 + 16 * r + here.col, pos, there, here.g);
+        }
+        if (F::codes && __builtin_expect(apart, 0)) {
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const float by_row = rest[wave][r][at.col];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[r][t] = s[r][t] * by_row;
+          }
+        }
+        if constexpr (BENT) bend.of(k_scale, view.key(x), at.g, s);
+        weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
+      } else {
+#pragma unroll
+        for (int d = 0; d < F::DT; ++d) vf[d] = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < RT; ++r) p[r] = u32x4{0, 0, 0, 0}, seen[r] = 0;
+      }
+      if (((kInLoop && i < 0) || j == (late ? kSteps / 2 : 0)) && stage + 1 < stages) {
+        convert(stage + 1);
+        if (stage + 2 < stages) fetch(stage + 2);
+      }
+      const auto read_values = [&](int from_d) {
+        const u32x4* const from = slot_of(i) + kValues;
+#pragma unroll
+        for (int d = 0; d < F::DT / 2; ++d) vf[from_d + d] = from[(from_d + d) * 64];
+      };
+      if constexpr (kLean) {
+        if (work) {
+          add_values<F, RT, 0, F::DT / 2>(vf, p, st);
+          read_values(F::DT / 2);
+          add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
+        }
+        if (j == kSteps - 1) __syncthreads();
+        if (run) {
+          read_scales(i + 1);
+          read_keys(i + 1, 0);
+          read_keys(i + 1, 1);
+        }
+      } else {
+        if (kEarly < F::DT && work) read_values(F::DT / 2);                // (before the barrier: the stage's place is written behind it)
+        if (j == kSteps - 1) __syncthreads();
+        if (run) {
+          __builtin_amdgcn_s_setprio(1);
+          if (kEarly == F::DT) read_keys(i + 1, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          add_values<F, RT, 0, F::DT / 2>(vf, p, st);
+          __builtin_amdgcn_sched_barrier(0);
+          read_keys(i + 1, kEarly == F::DT ? 1 : 0);
+          read_scales(i + 1);
+          __builtin_amdgcn_sched_barrier(0);
+          add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
+          __builtin_amdgcn_sched_barrier(0);
+          if (kEarly < F::DT) read_keys(i + 1, 1);
+        }
+      }
+      if (run) {
+        if constexpr (!F::finite) {
+          if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(source(), D, view.key(x), p, seen, at, st);
+        }
+        products_of(0);
+        products_of(1);
+        __builtin_amdgcn_s_setprio(0);
+      }
+    }
+    const Args& a = arguments();
+    const bool final = deal.blk == 0 && deal.stop() == deal.nb;
+    float* const slot = a.part + (int64_t)(2 * wg + (deal.blk == 0 ? 1 : 0)) * (16 * RT * WAVES) * (a.D + 4);
+    if (deal.blk == 0 && threadIdx.x == 0) deal.tell(a, wg);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float l = across(st.l[r], false);
+      const int row = row0 + 16 * r + at.col;
+      if (row >= a.rows) continue;
+      if (final) {
+        const Output out(a, b, h, row, l);
+        const float inverse = 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x[F::DT];
+#pragma unroll
+          for (int d = 0; d < F::DT; ++d) x[d] = st.o[r][d][i];
+          emit<F>(a, out, Lane<F>::elements_of(a.D, 4 * at.g + i), x, inverse);
+        }
+        if (a.lse && at.g == 0) a.lse[out.row] = out.none ? -INFINITY : st.m[r] + __builtin_amdgcn_logf(l);
+      } else {
+        float* const to = slot + (int64_t)((wave * RT + r) * 16 + at.col) * (a.D + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x[F::DT];
+#pragma unroll
+          for (int d = 0; d < F::DT; ++d) x[d] = st.o[r][d][i];
+          emit_part<F>(to, Lane<F>::elements_of(a.D, 4 * at.g + i), x);
+        }
+        if (at.g == 0) to[0] = st.m[r], to[1] = l;
+      }
+    }
+  } while (deal.next(arguments()));
+}
+
+// form: see form_of.  false: there is no such kernel
+template <bool BENT, int CD, int W>
+bool launch_chunk(const Args& a, int form, hipStream_t s) {
+  const dim3 grid((unsigned)a.wgs);
+  if (form == 1) {
+    hipLaunchKernelGGL((few_attention_kernel<Chunk<BENT>, CD, W>), grid, dim3(256), 0, s, a);
+  } else if (form == 8) {
+    hipLaunchKernelGGL((chunk_attention_kernel<BENT, CD, W, 8>), grid, dim3(512), 0, s, a);
+  } else {
+    if constexpr (W > 2) return false;
+    else hipLaunchKernelGGL((chunk_attention_kernel<BENT, CD, W, 4>), grid, dim3(256), 0, s, a);
+  }
+  return true;
+}
+template <int CD>
+bool launch_chunk(const Args& a, int w, int form, hipStream_t s) {
+  const bool bent = a.cap2 != 0.0f || a.slopes;
+  switch (w) {
+    case 1: return bent ? launch_chunk<true, CD, 1>(a, form, s) : launch_chunk<false, CD, 1>(a, form, s);
+    case 2: return bent ? launch_chunk<true, CD, 2>(a, form, s) : launch_chunk<false, CD, 2>(a, form, s);
+    case 3: return bent ? launch_chunk<true, CD, 3>(a, form, s) : launch_chunk<false, CD, 3>(a, form, s);
+    default: return bent ? launch_chunk<true, CD, 4>(a, form, s) : launch_chunk<false, CD, 4>(a, form, s);
+  }
+}
 }  // namespace
 
 namespace fcr_tree {
@@ -160,13 +497,6 @@ bool chunk_bf16(const Args& a, int w, int form, hipStream_t s);
 bool chunk_int8(const Args& a, int w, int form, hipStream_t s);
 bool chunk_e4m3(const Args& a, int w, int form, hipStream_t s);
 }  // namespace fcr_tree
-
-namespace {
-template <int CD>
-bool launch_chunk(const Args& a, int w, int form, hipStream_t s) {
-  return a.cap2 != 0.0f || a.slopes ? launch<Chunk<true>, CD>(a, w, form, s) : launch<Chunk<false>, CD>(a, w, form, s);
-}
-}  // namespace
 
 #if FCR_HAS(1)
 bool fcr_tree::chunk_f16(const Args& a, int w, int form, hipStream_t s) { return launch_chunk<FCR_DTYPE_F16>(a, w, form, s); }

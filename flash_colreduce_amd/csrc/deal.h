@@ -88,16 +88,31 @@ struct Sight {
     gap = most_of_two((lo & -kBlock) - gap_at, 0);
   }
   FCR_HOST_DEVICE int blocks() const { return most_of_two((n - gap + kBlock - 1) / kBlock, 1); }
-  // of the key that lies `at` keys behind the first one of the blocks, where all of them are laid end to end, the last one in front; behind them, and
-  // in front of them, no key
+  // The key at x of the blocks laid end to end; kNoKey in front of them.
+  FCR_HOST_DEVICE int key(int x) const { return x < 0 ? kNoKey : x + (x >= gap_at ? gap : 0); }
+  // The key that lies `at` keys behind the first one of the blocks where the last block is in front.
   FCR_HOST_DEVICE int position(int at) const {
     const int from = ((n - gap + kBlock - 1) & -kBlock) - kBlock - (at & -kBlock);
-    return from < 0 || at < 0 ? kNoKey : (at & (kBlock - 1)) + from + (from >= gap_at ? gap : 0);
+    return from < 0 || at < 0 ? kNoKey : key((at & (kBlock - 1)) + from);
   }
-  // whether every token sees `len` keys from pos on, and whether one might see one of them
+  // whether every token sees `len` keys from pos on
   FCR_HOST_DEVICE bool whole(int pos, int len) const { return (pos >= all_lo && pos + len <= all_hi) || pos + len <= prefix; }
-  FCR_HOST_DEVICE bool any(int pos, int len) const { return pos < n && (pos + len > lo || pos < prefix); }
   FCR_HOST_DEVICE bool settled(int pos, int len) const { return whole(pos, len); }
+};
+
+// What some rows of an item see of the item's steps of 32 keys, a step named by its first key's x.
+struct Steps {
+  int fast, fasts, high, low, prefix;
+  FCR_HOST_DEVICE Steps(const Sight& rows, const Sight& item, bool live) {
+    fast = rows.all_lo - item.gap;
+    fasts = most_of_two(rows.all_hi - 31 - rows.all_lo, 0);
+    high = !live ? 0 : rows.n > item.gap_at ? rows.n - item.gap : rows.n;
+    low = rows.lo - item.gap - 32;
+    prefix = live ? rows.prefix : 0;
+  }
+  // some row might see one of the keys; every row sees all of them
+  FCR_HOST_DEVICE bool some(int x) const { return x < prefix || (x < high && x > low); }
+  FCR_HOST_DEVICE bool whole(int x) const { return (uint32_t)(x - fast) < (uint32_t)fasts || x <= prefix - 32; }
 };
 
 }  // namespace fcr_tree

@@ -34,6 +34,32 @@
 
 #include "attention.h"
 
+namespace {
+template <int CD, int W>
+bool launch_w(const Args& a, int form, hipStream_t s) {
+  const dim3 grid((unsigned)a.wgs);
+  if (form == 1) {
+    hipLaunchKernelGGL((few_attention_kernel<Tree, CD, W>), grid, dim3(256), 0, s, a);
+  } else if (form == 8) {
+    hipLaunchKernelGGL((tall_attention_kernel<CD, W, 8>), grid, dim3(512), 0, s, a);
+  } else {
+    if constexpr (W > 2) return false;
+    else hipLaunchKernelGGL((tall_attention_kernel<CD, W, 4>), grid, dim3(256), 0, s, a);
+  }
+  return true;
+}
+// form: see form_of.  false: there is no such kernel
+template <int CD>
+bool launch(const Args& a, int w, int form, hipStream_t s) {
+  switch (w) {
+    case 1: return launch_w<CD, 1>(a, form, s);
+    case 2: return launch_w<CD, 2>(a, form, s);
+    case 3: return launch_w<CD, 3>(a, form, s);
+    default: return launch_w<CD, 4>(a, form, s);
+  }
+}
+}  // namespace
+
 namespace fcr_tree {
 bool tree_f16(const Args& a, int w, int form, hipStream_t s);
 bool tree_bf16(const Args& a, int w, int form, hipStream_t s);
@@ -42,16 +68,16 @@ bool tree_e4m3(const Args& a, int w, int form, hipStream_t s);
 }  // namespace fcr_tree
 
 #if FCR_HAS(1)
-bool fcr_tree::tree_f16(const Args& a, int w, int form, hipStream_t s) { return launch<Tree, FCR_DTYPE_F16>(a, w, form, s); }
+bool fcr_tree::tree_f16(const Args& a, int w, int form, hipStream_t s) { return launch<FCR_DTYPE_F16>(a, w, form, s); }
 #endif
 #if FCR_HAS(2)
-bool fcr_tree::tree_bf16(const Args& a, int w, int form, hipStream_t s) { return launch<Tree, FCR_DTYPE_BF16>(a, w, form, s); }
+bool fcr_tree::tree_bf16(const Args& a, int w, int form, hipStream_t s) { return launch<FCR_DTYPE_BF16>(a, w, form, s); }
 #endif
 #if FCR_HAS(3)
-bool fcr_tree::tree_int8(const Args& a, int w, int form, hipStream_t s) { return launch<Tree, FCR_DTYPE_INT8>(a, w, form, s); }
+bool fcr_tree::tree_int8(const Args& a, int w, int form, hipStream_t s) { return launch<FCR_DTYPE_INT8>(a, w, form, s); }
 #endif
 #if FCR_HAS(4)
-bool fcr_tree::tree_e4m3(const Args& a, int w, int form, hipStream_t s) { return launch<Tree, FCR_DTYPE_E4M3>(a, w, form, s); }
+bool fcr_tree::tree_e4m3(const Args& a, int w, int form, hipStream_t s) { return launch<FCR_DTYPE_E4M3>(a, w, form, s); }
 #endif
 
 #if FCR_HAS(0)

@@ -96,21 +96,23 @@ def sight(tmp_path_factory):
     tmp = tmp_path_factory.mktemp("sight")
     (tmp / "s.cpp").write_text(
         '#include "deal.h"\nusing namespace fcr_tree;\n'
-        'extern "C" void sight(int context, int count, int prefix, int window, int T, int positions, int first, int last, int* out) {\n'
-        '  const Sight s(context, count, prefix, window, T, positions, first, last);\n'
+        'extern "C" void sight(int context, int count, int prefix, int window, int T, int positions, int first, int last, int some, int to, int* out) {\n'
+        '  const Sight s(context, count, prefix, window, T, positions, first, last), rows(context, count, prefix, window, T, positions, some, to);\n'
+        '  const Steps wave(rows, s, 1);\n'
         '  out[0] = s.blocks(); out[1] = s.n;\n'
-        '  if (s.position(128 * out[0]) < s.n || s.position(-32) < s.n) out[0] = -1;\n'
-        '  for (int i = 0; i < 4 * out[0]; ++i) { const int p = s.position(32 * i);\n'
-        '    out[2 + 3 * i] = p; out[3 + 3 * i] = s.whole(p, 32); out[4 + 3 * i] = s.any(p, 32); } }\n')
+        '  if (s.position(128 * out[0]) < s.n || s.position(-32) < s.n || s.key(-32) < s.n) out[0] = -1;\n'
+        '  for (int i = 0; i < 4 * out[0]; ++i) { const int p = s.position(32 * i), x = 128 * out[0] - 32 - 32 * i, k = s.key(x); int* const o = out + 2 + 5 * i;\n'
+        '    o[0] = p; o[1] = s.whole(p, 32); o[2] = k; o[3] = wave.whole(x); o[4] = wave.some(x); } }\n')
     subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "flash_colreduce_amd", "csrc"), str(tmp / "s.cpp"), "-o",
                     str(tmp / "s.so")], check=True)
     return ctypes.CDLL(str(tmp / "s.so"))
 
 
 def test_blocks_of_a_tile_hold_every_key_that_it_sees(sight):
-    """Every key that a token of the tile sees lies in its blocks, once and in order; steps said to be seen by all are, and those said to be seen by none."""
+    """Every key that a token of the tile sees lies in its blocks, once and in order; steps said to be seen by all of some rows are, those said to be seen by none are
+    seen by none."""
     rng = random.Random(2)
-    for _ in range(3000):
+    for _ in range(4000):
         T = rng.choice([1, 2, 7, 40, 300])
         context, count = rng.choice([0, 1, rng.randint(0, 1000), -5]), rng.randint(-1, T + 1)
         positions = 16 * rng.randint(1, 90)
@@ -118,28 +120,34 @@ def test_blocks_of_a_tile_hold_every_key_that_it_sees(sight):
         prefix = rng.choice([0, 0, -3, rng.randint(0, 500), 1500])
         first = rng.randint(0, T - 1)
         last = rng.randint(first, T - 1)
-        out = (ctypes.c_int * (2 + 3 * 4 * 80))()
-        sight.sight(context, count, prefix, window, T, positions, first, last, out)
+        some = rng.randint(first, last)
+        to = rng.randint(some, last)
+        out = (ctypes.c_int * (2 + 5 * 4 * 80))()
+        sight.sight(context, count, prefix, window, T, positions, first, last, some, to, out)
         start, have = max(context, 0), min(max(count, 0), T)
         tokens = range(first, min(last, have - 1) + 1)
         keys = range(min(start + have, positions))
         seen = {t: {j for j in keys if j <= start + t and j > start + t - window or j < prefix} for t in tokens}
-        some = set().union(*seen.values())
-        steps = [(out[2 + 3 * i], out[3 + 3 * i], out[4 + 3 * i]) for i in range(4 * out[0])]
-        at = [p for p, _, _ in steps]
-        if not some:
+        seen_by_any = set().union(*seen.values())
+        steps = [out[2 + 5 * i: 7 + 5 * i] for i in range(4 * out[0])]
+        at = [p for p, *_ in steps]
+        assert out[0] >= 1
+        if not seen_by_any:
             assert out[0] == 1
             continue
-        # blocks from the last one on, the steps of a block in their order
+        # blocks from the last one on, the steps of a block in their order; and all steps from the last one on
         assert all(p % 128 == 32 * (i % 4) and p // 128 == at[i - i % 4] // 128 for i, p in enumerate(at))
         assert all(a > z >= 0 for a, z in zip(at[::4], at[4::4])) and at[-4] >= 0
-        assert some <= {j for p in at for j in range(p, p + 32)}
-        for p, whole, any_ in steps:
-            step = set(range(p, p + 32))
-            assert not whole or all(step <= s for s in seen.values()) or not tokens
-            assert any_ or not (step & some)
+        assert [k for _, _, k, _, _ in steps] == sorted(at, reverse=True)
+        assert seen_by_any <= {j for p in at for j in range(p, p + 32)}
+        rows = [seen[t] for t in range(some, to + 1) if t in seen]
+        for p, whole, k, wave_whole, wave_some in steps:
+            assert not whole or all(set(range(p, p + 32)) <= s for s in seen.values())
+            step = set(range(k, k + 32))
+            assert not rows or not wave_whole or all(step <= s for s in rows)
+            assert wave_some or not any(step & s for s in rows)
         # and no block without a reason
-        assert out[0] <= max(1, len({j // 128 for j in some}) + 1)
+        assert out[0] <= max(1, len({j // 128 for j in seen_by_any}) + 1)
 
 
 def _chunk_c(**over):
