@@ -365,32 +365,38 @@ __device__ __forceinline__ float rounded(float x) {
 // reference had them lose nine tenths of that.  256 rows over 4 x 8 heads of 8192 keys of 128 elements: 67 us fp16, 72 int8 either way for scores
 // that spread by 1.4 in base 2; 68 -> 74 and 74 -> 84 where they spread by 5.8 and references rise more often.)  bf16 has weights of any size, and
 // the reference is raised to the largest.
+template <bool MASKED, class F>
+__device__ __forceinline__ bool weights_of_row(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], float most_v, const f32x4 (&s)[2], uint32_t seen, float m, float l,
+                                               float& sum, u32x4& p) {
+  float x[8], part[2];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    // (of scores whose last bit is worth more than a weight's exponent, the rounded one is at the reference that `raise` chose; one rounding
+    // less may put it far above, which raises the reference again and comes here)
+    x[e] = MASKED ? rounded(s[e / 4][e % 4] * k_scale[e / 4][e % 4]) - m : __builtin_fmaf(s[e / 4][e % 4], k_scale[e / 4][e % 4], -m);
+    if (MASKED) x[e] = (seen >> e) & 1u ? x[e] : -INFINITY;
+    x[e] = __builtin_amdgcn_exp2f(x[e]);
+    part[e & 1] = e < 2 ? x[e] : part[e & 1] + x[e];
+    if constexpr (F::codes) {
+      x[e] *= v_scale[e / 4][e % 4];
+      if (MASKED) x[e] = (seen >> e) & 1u ? x[e] : 0.0f;      // (a hidden value's scale may be a NaN)
+    }
+  }
+  part[0] += part[1];
+  sum = l + part[0];
+  const bool raise = part[0] * most_v > kMostWeight || !(sum < kMostSum);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) p[j] = F::bf16 ? pack2<FCR_DTYPE_BF16>(x[2 * j], x[2 * j + 1]) : pack2<FCR_DTYPE_F16>(x[2 * j], x[2 * j + 1]);
+  return raise;
+}
 template <bool MASKED, class F, int RT>
 __device__ __forceinline__ bool weights(const f32x4 (&k_scale)[2], const f32x4 (&v_scale)[2], float most_v, const f32x4 (&s)[RT][2],
                                         const uint32_t (&seen)[RT], const State<F, RT>& st, float (&sum)[RT], u32x4 (&p)[RT]) {
   bool raise = false;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    float x[8], part[2];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // (of scores whose last bit is worth more than a weight's exponent, the rounded one is at the reference that `raise` chose; one rounding
-      // less may put it far above, which raises the reference again and comes here)
-      x[e] = MASKED ? rounded(s[r][e / 4][e % 4] * k_scale[e / 4][e % 4]) - st.m[r]
-                    : __builtin_fmaf(s[r][e / 4][e % 4], k_scale[e / 4][e % 4], -st.m[r]);
-      if (MASKED) x[e] = (seen[r] >> e) & 1u ? x[e] : -INFINITY;
-      x[e] = __builtin_amdgcn_exp2f(x[e]);
-      part[e & 1] = e < 2 ? x[e] : part[e & 1] + x[e];
-      if constexpr (F::codes) {
-        x[e] *= v_scale[e / 4][e % 4];
-        if (MASKED) x[e] = (seen[r] >> e) & 1u ? x[e] : 0.0f;      // (a hidden value's scale may be a NaN)
-      }
-    }
-    part[0] += part[1];
-    sum[r] = st.l[r] + part[0];
-    raise = raise || part[0] * most_v > kMostWeight || !(sum[r] < kMostSum);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p[r][j] = F::bf16 ? pack2<FCR_DTYPE_BF16>(x[2 * j], x[2 * j + 1]) : pack2<FCR_DTYPE_F16>(x[2 * j], x[2 * j + 1]);
+    const bool up = weights_of_row<MASKED, F>(k_scale, v_scale, most_v, s[r], seen[r], st.m[r], st.l[r], sum[r], p[r]);
+    raise = raise || up;
   }
   return __any(raise);
 }

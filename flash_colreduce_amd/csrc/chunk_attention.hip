@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
   // registers: 128 rows over 4 x 8 heads of 8192 bf16 keys of 128 elements 57 -> 54 us, 1024 rows of 256 elements 451 -> 413, int8 393 -> 383.
   // (fp16 and bf16 rows of 256 elements still spill 15, bf16 of 128 and e4m3 of 256 two.)
   // With 64 elements, where nothing spills, 1 to 10 % are lost.
-  constexpr bool kInLoop = W >= 2;
+  constexpr bool kPiped = W <= 2;
   constexpr int kEarly = W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights
   static_assert(kTiles * (kApart ? 2 : 1) == WAVES * kMine, "every wave has its share of a stage");
   __shared__ u32x4 operands[kRing * kStep];
@@ -327,107 +327,218 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
 #pragma unroll
         for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(kf[t][c], q.w[r][c], c ? s[r][t] : f32x4{0, 0, 0, 0});
     };
-    if constexpr (!kInLoop) {
-      convert(0);
-      if (stages > 1) fetch(1);
-      __syncthreads();
-      if (sees.high | sees.prefix) {
-        read_keys(0, 0);
-        read_keys(0, 1);
-        read_scales(0);
-        products_of(0);
-        products_of(1);
-      }
-    }
-    // (in the loop: the step before the first one does this, with values and weights of 0)
-    int x = kInLoop ? x0 + 32 : x0;
-    bool next = sees.some(x);
-    for (int i = kInLoop ? -1 : 0; i < steps; ++i, x -= 32) {
-      const int stage = i >> kStepsLog2, j = i & (kSteps - 1);
-      const bool work = next && (!kInLoop || i >= 0);
-      next = i + 1 < steps && sees.some(x - 32);
-      const bool run = work || next;                     // (rows that see nothing of this step may need the products of the next one)
-      u32x4 vf[F::DT], p[RT];
+    // What rows see of the step at x, forms weights of its products s, and adds what is not finite of its values.
+    const auto weigh_step = [&](int i, int x, u32x4 (&p)[RT]) {
+      read_scales(i);
+      const int f0 = __builtin_amdgcn_readfirstlane(flag.x), f1 = __builtin_amdgcn_readfirstlane(flag.y);
+      const bool masked = !sees.whole(x) || ((f0 ^ 1) | (f1 ^ 1)) != 0;
       uint32_t seen[RT];
-      bool not_finite = false;
-      if (work) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) seen[r] = 0xff;
+      if (__builtin_expect(masked, 0)) {
+        const Lane<F> here = at.again();
+        const int pos = view.key(x);
+        const uint32_t there = there_of(pos, n, f0 & 1, f1 & 1, here.g);
+        const Sight rows = view_of(arguments(), b, h, row0, row0 + 16 * RT);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) seen[r] = Chunk<BENT>::seen_by(arguments(), rows, b, row0 + 16 * r + here.col, pos, there, here.g);
+      }
+      if (F::codes && __builtin_expect(apart, 0)) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float by_row = rest[wave][r][at.col];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) s[r][t] = s[r][t] * by_row;
+        }
+      }
+      if constexpr (BENT) bend.of(k_scale, view.key(x), at.g, s);
+      weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
+      if constexpr (!F::finite) {
+        if (__builtin_expect(((f0 | f1) & 2) != 0, 0)) add_not_finite<F, RT>(source(), D, view.key(x), p, seen, at, st);
+      }
+    };
+    if constexpr (kPiped) {
+      // Arrays are declared where they are read from LDS, without a condition: one that might hold an earlier turn's values would take its registers everywhere.
+      const bool none = (sees.high | sees.prefix) == 0;
+      u32x4 p[RT];
+      const auto read_values = [&](int i, u32x4 (&vf)[F::DT]) {
         const u32x4* const from = slot_of(i) + kValues;
 #pragma unroll
-        for (int d = 0; d < kEarly; ++d) vf[d] = from[d * 64];
-        const int f0 = __builtin_amdgcn_readfirstlane(flag.x), f1 = __builtin_amdgcn_readfirstlane(flag.y);
-        const bool masked = !sees.whole(x) || ((f0 ^ 1) | (f1 ^ 1)) != 0;
+        for (int d = 0; d < F::DT; ++d) vf[d] = from[d * 64];
+      };
+      const auto keys = [&](int i, int t, u32x4 (&kf)[F::KS]) {
+        const u32x4* const from = slot_of(i) + t * F::KS * 64;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) seen[r] = 0xff;
-        if (masked) {
-          not_finite = !F::finite && ((f0 | f1) & 2) != 0;
-          const Lane<F> here = at.again();
-          const int pos = view.key(x);
-          const uint32_t there = there_of(pos, n, f0 & 1, f1 & 1, here.g);
-          const Sight rows = view_of(arguments(), b, h, row0, row0 + 16 * RT);
+        for (int c = 0; c < F::KS; ++c) kf[c] = from[c * 64];
+      };
+      const auto products = [&](const u32x4 (&kf)[2][F::KS]) {
 #pragma unroll
-          for (int r = 0; r < RT; ++r) seen[r] = Chunk<BENT>::seen_by(arguments(), rows, b, row0 + 16 * r + here.col, pos, there, here.g);
-        }
-        if (F::codes && __builtin_expect(apart, 0)) {
+        for (int c = 0; c < F::KS; ++c)
 #pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const float by_row = rest[wave][r][at.col];
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) s[r][t] = s[r][t] * by_row;
-          }
-        }
-        if constexpr (BENT) bend.of(k_scale, view.key(x), at.g, s);
-        weigh<F, RT>(k_scale, v_scale, most_v, s, masked, seen, st, p);
-      } else {
-#pragma unroll
-        for (int d = 0; d < F::DT; ++d) vf[d] = u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int r = 0; r < RT; ++r) p[r] = u32x4{0, 0, 0, 0}, seen[r] = 0;
-      }
-      if (((kInLoop && i < 0) || j == (late ? kSteps / 2 : 0)) && stage + 1 < stages) {
+            for (int r = 0; r < RT; ++r) s[r][t] = mma<F::bf16>(kf[t][c], q.w[r][c], c ? s[r][t] : f32x4{0, 0, 0, 0});
+      };
+      const auto next_stage = [&](int stage) {
+        if (stage + 1 >= stages) return;
         convert(stage + 1);
         if (stage + 2 < stages) fetch(stage + 2);
-      }
-      const auto read_values = [&](int from_d) {
-        const u32x4* const from = slot_of(i) + kValues;
-#pragma unroll
-        for (int d = 0; d < F::DT / 2; ++d) vf[from_d + d] = from[(from_d + d) * 64];
       };
-      if constexpr (kLean) {
-        if (work) {
-          add_values<F, RT, 0, F::DT / 2>(vf, p, st);
-          read_values(F::DT / 2);
-          add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) p[r] = u32x4{0, 0, 0, 0};
+      bool live = false, fast = false;                   // p are weights; all rows see all of the stage
+      for (int stage = -1; stage < stages; ++stage) {
+        const int i0 = stage * kSteps;
+        int x = x0 - 32 * i0;
+        if (stage >= 0) {
+          if (!late) next_stage(stage);
+          if (__builtin_expect(fast, 1)) {
+            u32x4 kf[2][F::KS], vf[F::DT];
+            keys(i0 + 1, 0, kf[0]);
+            keys(i0 + 1, 1, kf[1]);
+            read_scales(i0 + 1);
+            read_values(i0, vf);
+#pragma unroll
+            for (int j = 0; j < kSteps - 1; ++j) {
+              float sum[RT];
+              u32x4 following[RT];
+              products(kf);
+              __builtin_amdgcn_sched_barrier(0);
+              if constexpr (BENT) bend.of(k_scale, view.key(x - 32 * (j + 1)), at.g, s);
+              // A part of the products of values for each row tile: they run under the vector instructions of its weights.  Keys come as values go.
+              bool up = false;
+#pragma unroll
+              for (int r = 0; r < RT; ++r) {
+                const bool up_r = weights_of_row<false, F>(k_scale, v_scale, most_v, s[r], 0xff, st.m[r], st.l[r], sum[r], following[r]);
+                up = up || up_r;
+#pragma unroll
+                for (int d = r * F::DT / RT; d < (r + 1) * F::DT / RT; ++d)
+#pragma unroll
+                  for (int i = 0; i < RT; ++i) st.o[i][d] = mma<F::bf16>(vf[d], p[i], st.o[i][d]);
+#pragma unroll
+                for (int k = 0; k < F::DT; ++k) {
+                  __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                  __builtin_amdgcn_sched_group_barrier(0x2, 5, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (j + 2 < kSteps) keys(i0 + j + 2, r, kf[r]);
+                __builtin_amdgcn_sched_barrier(0);
+              }
+              if (__builtin_expect(__any(up), 0)) {
+                uint32_t seen[RT];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) seen[r] = 0xff;
+                raise<F, RT>(k_scale, v_scale, s, seen, st);
+                weights<true, F, RT>(k_scale, v_scale, most_v, s, seen, st, sum, following);
+              }
+#pragma unroll
+              for (int r = 0; r < RT; ++r) st.l[r] = sum[r], p[r] = following[r];
+              if (j + 2 < kSteps) {
+                read_scales(i0 + j + 2);
+                read_values(i0 + j + 1, vf);
+              }
+            }
+          } else if (!none) {
+#pragma unroll 1
+            for (int j = 0; j < kSteps - 1; ++j) {
+              if (live) {
+                u32x4 vf[F::DT];
+                read_values(i0 + j, vf);
+                add_values<F, RT, 0, F::DT>(vf, p, st);
+              }
+              live = sees.some(x - 32 * (j + 1));
+              if (live) {
+                u32x4 kf[2][F::KS];
+                keys(i0 + j + 1, 0, kf[0]);
+                keys(i0 + j + 1, 1, kf[1]);
+                products(kf);
+                weigh_step(i0 + j + 1, x - 32 * (j + 1), p);
+              }
+            }
+          }
         }
-        if (j == kSteps - 1) __syncthreads();
-        if (run) {
-          read_scales(i + 1);
-          read_keys(i + 1, 0);
-          read_keys(i + 1, 1);
-        }
-      } else {
-        if (kEarly < F::DT && work) read_values(F::DT / 2);                // (before the barrier: the stage's place is written behind it)
-        if (j == kSteps - 1) __syncthreads();
-        if (run) {
-          __builtin_amdgcn_s_setprio(1);
-          if (kEarly == F::DT) read_keys(i + 1, 0);
-          __builtin_amdgcn_sched_barrier(0);
-          add_values<F, RT, 0, F::DT / 2>(vf, p, st);
-          __builtin_amdgcn_sched_barrier(0);
-          read_keys(i + 1, kEarly == F::DT ? 1 : 0);
-          read_scales(i + 1);
-          __builtin_amdgcn_sched_barrier(0);
-          add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
-          __builtin_amdgcn_sched_barrier(0);
-          if (kEarly < F::DT) read_keys(i + 1, 1);
-        }
+        if (late || stage < 0) next_stage(stage);
+        u32x4 vf[F::DT], kf[2][F::KS];
+        read_values(i0 + kSteps - 1, vf);                   // (behind the barrier their place is written)
+        __syncthreads();
+        if (none) continue;
+        keys(i0 + kSteps, 0, kf[0]);
+        keys(i0 + kSteps, 1, kf[1]);
+        if (live) add_values<F, RT, 0, F::DT>(vf, p, st);
+        if (stage + 1 == stages) break;
+        x -= 32 * kSteps;
+        live = sees.some(x), fast = false;
+        if (!live) continue;
+        products(kf);
+        const u32x4* const f = reinterpret_cast<const u32x4*>(flags + ((i0 + kSteps) & (kRing - 1)));
+        u32x4 odd = f[0] ^ 1;
+#pragma unroll
+        for (int k = 1; k < kSteps / 2; ++k) odd |= f[k] ^ 1;
+        weigh_step(i0 + kSteps, x, p);
+        fast = sees.whole(x, x - 32 * (kSteps - 1)) && !apart && __builtin_amdgcn_readfirstlane((int)(odd[0] | odd[1] | odd[2] | odd[3])) == 0;
       }
-      if (run) {
-        if constexpr (!F::finite) {
-          if (__builtin_expect(not_finite, 0)) add_not_finite<F, RT>(source(), D, view.key(x), p, seen, at, st);
+    } else {
+      // (in the loop: the step before the first one does this, with values and weights of 0)
+      int x = x0 + 32;
+      bool next = sees.some(x);
+      for (int i = -1; i < steps; ++i, x -= 32) {
+        const int stage = i >> kStepsLog2, j = i & (kSteps - 1);
+        const bool work = next && i >= 0;
+        next = i + 1 < steps && sees.some(x - 32);
+        const bool run = work || next;                     // (rows that see nothing of this step may need the products of the next one)
+        u32x4 vf[F::DT], p[RT];
+        if (work) {
+          const u32x4* const from = slot_of(i) + kValues;
+#pragma unroll
+          for (int d = 0; d < kEarly; ++d) vf[d] = from[d * 64];
+          weigh_step(i, x, p);
+        } else {
+#pragma unroll
+          for (int d = 0; d < F::DT; ++d) vf[d] = u32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int r = 0; r < RT; ++r) p[r] = u32x4{0, 0, 0, 0};
         }
-        products_of(0);
-        products_of(1);
-        __builtin_amdgcn_s_setprio(0);
+        if ((i < 0 || j == (late ? kSteps / 2 : 0)) && stage + 1 < stages) {
+          convert(stage + 1);
+          if (stage + 2 < stages) fetch(stage + 2);
+        }
+        const auto read_values = [&](int from_d) {
+          const u32x4* const from = slot_of(i) + kValues;
+#pragma unroll
+          for (int d = 0; d < F::DT / 2; ++d) vf[from_d + d] = from[(from_d + d) * 64];
+        };
+        if constexpr (kLean) {
+          if (work) {
+            add_values<F, RT, 0, F::DT / 2>(vf, p, st);
+            read_values(F::DT / 2);
+            add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
+          }
+          if (j == kSteps - 1) __syncthreads();
+          if (run) {
+            read_keys(i + 1, 0);
+            read_keys(i + 1, 1);
+          }
+        } else {
+          if (kEarly < F::DT && work) read_values(F::DT / 2);                // (before the barrier: the stage's place is written behind it)
+          if (j == kSteps - 1) __syncthreads();
+          if (run) {
+            __builtin_amdgcn_s_setprio(1);
+            if (kEarly == F::DT) read_keys(i + 1, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            add_values<F, RT, 0, F::DT / 2>(vf, p, st);
+            __builtin_amdgcn_sched_barrier(0);
+            read_keys(i + 1, kEarly == F::DT ? 1 : 0);
+            __builtin_amdgcn_sched_barrier(0);
+            add_values<F, RT, F::DT / 2, F::DT>(vf, p, st);
+            __builtin_amdgcn_sched_barrier(0);
+            if (kEarly < F::DT) read_keys(i + 1, 1);
+          }
+        }
+        if (run) {
+          products_of(0);
+          products_of(1);
+          __builtin_amdgcn_s_setprio(0);
+        }
       }
     }
     const Args& a = arguments();

@@ -113,6 +113,8 @@ struct Steps {
   // some row might see one of the keys; every row sees all of them
   FCR_HOST_DEVICE bool some(int x) const { return x < prefix || (x < high && x > low); }
   FCR_HOST_DEVICE bool whole(int x) const { return (uint32_t)(x - fast) < (uint32_t)fasts || x <= prefix - 32; }
+  // of all steps from `first` down to `last`
+  FCR_HOST_DEVICE bool whole(int first, int last) const { return (last >= fast && first - fast < fasts) || first <= prefix - 32; }
 };
 
 }  // namespace fcr_tree
