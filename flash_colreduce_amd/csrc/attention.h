@@ -39,6 +39,8 @@ struct Args {
   const float* slopes;         // [H G] or null
   const int32_t* prefix;       // [B] or null
   int window;                  // INT32_MAX: none
+  int whole;                   // 1: items may be taken whole, a workgroup for each (see items_are_whole), 2: they are, 0: they are not
+  Div all_heads;               // by B H
 };
 }  // namespace fcr_tree
 

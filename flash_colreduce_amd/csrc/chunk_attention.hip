@@ -24,7 +24,29 @@ template <int THREADS, int ROWS>
 struct ChunkDeal {
   int at, end, b, h, tile, blk, nb;
   Sight seen;
-  __device__ __forceinline__ bool start(const Args& a, int wg, int* scan) {   // scan: THREADS / 64 + 4 words of LDS
+  // What is found goes through locals to one place: stores on several ways would be joined into one to an address that is chosen, and the deal would stay in
+  // memory, where nothing is known to be uniform.
+  struct Found {
+    int at, end, b, h, tile, blk;     // end below 0: the item is taken whole
+    bool any;
+  };
+  // An item for this workgroup of a launch of one for each: the last tiles, which see the most keys, first, and tiles of one head on one die (workgroups are
+  // dealt to 8 dies in turn) where the number of heads is a multiple of 8.
+  static __device__ __forceinline__ Found one(const Args& a) {
+    const int rank = (int)a.all_heads.of(blockIdx.x), bh = blockIdx.x - rank * a.all_heads.d, b = (int)a.heads.of((uint32_t)bh);
+    return Found{0, -1, b, bh - b * a.H, a.row_tiles - 1 - rank, 0, rank < a.row_tiles};
+  }
+  __device__ __forceinline__ bool start(const Args& a, int wg, int* scan) {   // scan: THREADS / 64 + 4 words of LDS (twice the first where a.whole is 1)
+    const Found f = a.whole == 2 ? one(a) : dealt(a, wg, scan);
+    if (!f.any) return false;
+    b = __builtin_amdgcn_readfirstlane(f.b), h = __builtin_amdgcn_readfirstlane(f.h), tile = __builtin_amdgcn_readfirstlane(f.tile);
+    blk = __builtin_amdgcn_readfirstlane(f.blk), at = __builtin_amdgcn_readfirstlane(f.at);
+    look(a);
+    const int last = __builtin_amdgcn_readfirstlane(f.end);
+    end = last < 0 ? nb : last;
+    return true;
+  }
+  static __device__ __forceinline__ Found dealt(const Args& a, int wg, int* scan) {
     constexpr int waves = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const bool by_head = a.context.sh != 0;
@@ -36,10 +58,17 @@ struct ChunkDeal {
       if (by_head) eb = (int)a.heads.of((uint32_t)e), eh = e - eb * a.H;
       return view_of(a, eb, eh, t * ROWS, t * ROWS + ROWS).blocks();
     };
-    int mine = 0;
-    for (int p = p0; p < p1; ++p) mine += blocks_of_pair(p);
+    int mine = 0, most = 0;
+    for (int p = p0; p < p1; ++p) {
+      const int blocks = blocks_of_pair(p);
+      mine += blocks, most = max(most, blocks);
+    }
     const int upto = sum_up_to(mine);
     if (lane == 63) scan[wave] = upto;
+    if (a.whole) {
+      for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o));
+      if (lane == 63) scan[waves + 4 + wave] = most;
+    }
     __syncthreads();
     int sum = 0, before = upto - mine;
 #pragma unroll
@@ -49,9 +78,14 @@ struct ChunkDeal {
     }
     const int total = __builtin_amdgcn_readfirstlane(sum) * times, per = (int)a.all.of((uint32_t)(total + a.wgs - 1));
     if (wg == 0 && tid == 0) a.first[0] = per;
-    at = wg * per;                                      // (wgs * per is total + wgs at most: checked by the host to fit)
-    end = min(at + per, total);
-    if (at >= end) return false;
+    if (a.whole) {
+#pragma unroll
+      for (int i = 0; i < waves; ++i) most = max(most, scan[waves + 4 + i]);
+      if (items_are_whole(__builtin_amdgcn_readfirstlane(most), per, pairs * times, a.wgs)) return one(a);
+      if (blockIdx.x >= (unsigned)a.wgs) return Found{0, 0, 0, 0, 0, 0, false};
+    }
+    const int at = wg * per, end = min(at + per, total);   // (wgs * per is total + wgs at most: checked by the host to fit)
+    if (at >= end) return Found{0, 0, 0, 0, 0, 0, false};
     // the pair that has block x of its entries, and the blocks in front of it
     int* const found = scan + waves;
     const auto find = [&](int x) {
@@ -63,8 +97,6 @@ struct ChunkDeal {
       __syncthreads();
     };
     find(by_head ? at : (int)a.heads.of((uint32_t)at));
-    // (everything found goes through locals to one place: stores on several ways would be joined into one to an address that is chosen, and the deal
-    // would stay in memory, where nothing is known to be uniform)
     int pair = __builtin_amdgcn_readfirstlane(found[0]), in_front = __builtin_amdgcn_readfirstlane(found[1]);
     const int entry = (int)a.per_head.of((uint32_t)pair), q0 = entry * a.row_tiles;
     int place = at - times * in_front, head = 0;
@@ -93,12 +125,8 @@ struct ChunkDeal {
       pair = __builtin_amdgcn_readfirstlane(found[0]), in_front = __builtin_amdgcn_readfirstlane(found[1]);
       place = from + place - in_front;
     }
-    b = by_head ? (int)a.heads.of((uint32_t)entry) : entry;
-    h = __builtin_amdgcn_readfirstlane(by_head ? entry - b * a.H : head);
-    tile = pair - q0;
-    blk = __builtin_amdgcn_readfirstlane(place);
-    look(a);
-    return true;
+    const int b = by_head ? (int)a.heads.of((uint32_t)entry) : entry;
+    return Found{at, end, b, by_head ? entry - b * a.H : head, pair - q0, place, true};
   }
   __device__ __forceinline__ void look(const Args& a) {
     seen = view_of(a, b, h, tile * ROWS, tile * ROWS + ROWS);
@@ -164,7 +192,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
   // registers: 128 rows over 4 x 8 heads of 8192 bf16 keys of 128 elements 57 -> 54 us, 1024 rows of 256 elements 451 -> 413, int8 393 -> 383.
   // (fp16 and bf16 rows of 256 elements still spill 15, bf16 of 128 and e4m3 of 256 two.)
   // With 64 elements, where nothing spills, 1 to 10 % are lost.
-  constexpr bool kPiped = W <= 2;
+  constexpr bool kPiped = W == 1 || (W == 2 && !F::codes);
   constexpr int kEarly = W == 1 || (W == 2 && F::codes) ? F::DT : F::DT / 2;                     // value operands that fit next to the weights
   static_assert(kTiles * (kApart ? 2 : 1) == WAVES * kMine, "every wave has its share of a stage");
   __shared__ u32x4 operands[kRing * kStep];
@@ -172,7 +200,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
   __shared__ float most[kRing][2];                                       // the largest scale of a tile's values
   __shared__ int2 flags[kRing];                                          // a tile's page is there, and (bit 1) one of its values was not finite
   __shared__ float rest[WAVES][RT][16];                                  // powers of two that rows' scores are still to be multiplied by
-  __shared__ int scan[WAVES + 4];
+  __shared__ int scan[2 * WAVES + 4];
   const int wg = range_of(args, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const Lane<F> at(threadIdx.x & 63);
@@ -579,7 +607,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
 // form: see form_of.  false: there is no such kernel
 template <bool BENT, int CD, int W>
 bool launch_chunk(const Args& a, int form, hipStream_t s) {
-  const dim3 grid((unsigned)a.wgs);
+  const dim3 grid((unsigned)(a.whole ? std::max(a.wgs, a.B * a.H * a.row_tiles) : a.wgs));
   if (form == 1) {
     hipLaunchKernelGGL((few_attention_kernel<Chunk<BENT>, CD, W>), grid, dim3(256), 0, s, a);
   } else if (form == 8) {
@@ -651,6 +679,8 @@ int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* ta
   a.cap2 = cap * log2e;
   a.scale2 = cap != 0.0f ? scale * (2.0f * log2e) / cap : scale * log2e;
   if (!isfinite(a.scale2) || !isfinite(a.cap2)) return fail(FCR_E_SCALE, "scale over cap must be finite");
+  a.whole = plan.form == 1 ? 0 : whole_items_of(plan.items, plan.wgs);
+  a.all_heads.set((uint32_t)(B * cache->H));
   const int w = (cache->D + 63) / 64;
   hipStream_t s = static_cast<hipStream_t>(stream);
   bool there;
@@ -661,7 +691,7 @@ int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* ta
     default: there = fcr_tree::chunk_e4m3(a, w, plan.form, s); break;
   }
   if (!there) return fail(FCR_E_SHAPE, "no kernel for these sizes");
-  if ((rc = launched("chunk attention"))) return rc;
+  if ((rc = launched("chunk attention")) || a.whole == 2) return rc;
   return join(a, plan, s);
 }
 

@@ -117,4 +117,15 @@ struct Steps {
   FCR_HOST_DEVICE bool whole(int first, int last) const { return (last >= fast && first - fast < fasts) || first <= prefix - 32; }
 };
 
+// Items of many rows may be taken whole, a workgroup for each, by a launch of as many (0: no, too few; 1: if items_are_whole says so; 2: yes, there are so many that
+// none is large): nothing is cut and joined, but the last workgroups may leave others idle.
+FCR_HOST_DEVICE inline int whole_items_of(int64_t items, int wgs) { return 4 * items < wgs ? 0 : items < 8ll * wgs ? 1 : 2; }
+// The time of either distribution in blocks: what runs once per piece costs about three, the join of what was cut five.  Whole items take as long as the longest of them or, where
+// there is more than one for a workgroup, an eighth longer than their mean.
+FCR_HOST_DEVICE inline bool items_are_whole(int longest, int per, int items, int wgs) {
+  const int rounds = quotient_up(items, wgs);
+  const int whole = items <= wgs ? longest : most_of_two(longest, per + per / 8);
+  return whole + 3 * rounds <= per + 3 * (rounds + 1) + 5;
+}
+
 }  // namespace fcr_tree
