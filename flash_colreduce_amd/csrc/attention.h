@@ -1339,10 +1339,11 @@ using fcr_detail::launched;
 struct Plan {
   int form;                  // see form_of
   int tile_rows, row_tiles, wgs;
+  int held;                  // workgroups that the chip holds at once: wgs where there is work for them
   int64_t items, first_bytes, bytes;
 };
 // What depends on sizes alone.  false: too large.
-bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Plan& p) {
+bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Plan& p, int per_cu = 0) {
   const int64_t rows = (int64_t)T * G;
   const int w = (D + 63) / 64;
   p.form = form_of(rows, w, codes);
@@ -1354,8 +1355,9 @@ bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Pl
   p.row_tiles = (int)tiles;
   // As many as the CUs hold at once: one of eight waves, or of four that take more than 256 registers (8 x 8 heads of 1000 bf16 keys of 256
   // elements 21 us, 28 with twice as many, one behind the other); two of the others.
-  int64_t wgs = (p.form == 8 || (!codes && w > 2) ? 1 : 2) * (int64_t)fcr_detail::chip_cus_of_current_device();
-  if (blocks < wgs) wgs = blocks;
+  if (!per_cu || p.form != 1) per_cu = p.form == 8 || (!codes && w > 2) ? 1 : 2;
+  p.held = per_cu * fcr_detail::chip_cus_of_current_device();
+  const int64_t wgs = std::min(blocks, (int64_t)p.held);
   p.wgs = (int)((wgs + 7) / 8 * 8);
   p.first_bytes = (kFirst * 4 + p.items * 8 + 15) / 16 * 16;
   p.bytes = p.first_bytes + 2ll * p.wgs * p.tile_rows * (D + 4) * 4;
@@ -1365,7 +1367,7 @@ bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Pl
 // What both entry points are given, but for the cache itself: checked, and put into `a`.
 int check_queries(Args& a, Plan& plan, const void* q, const fcr_cache& cache, const int32_t* table, int64_t table_stride, int table_pages, const int32_t* context,
                   const int64_t* context_strides, void* out, float* lse, void* ws, size_t ws_bytes, int dtype, int B, int G, int T, const int64_t* q_strides,
-                  float scale) {
+                  float scale, int per_cu = 0) {
   const int rc = check_table(table, table_stride, table_pages, cache.page_size, B);
   if (rc) return rc;
   if (!q || !q_strides || !context || !context_strides || !out || !ws) return fail(FCR_E_NULL, "null pointer argument");
@@ -1374,7 +1376,7 @@ int check_queries(Args& a, Plan& plan, const void* q, const fcr_cache& cache, co
   const int H = cache.H, D = cache.D;
   const int64_t capacity = (int64_t)table_pages * cache.page_size;
   if (G < 1 || T < 1 || T > (1 << 24) || G > (1 << 24) || (int64_t)B * H > (1 << 24) || (int64_t)H * G > (1 << 24) ||
-      !plan_of(has_codes(cache.dtype), B, H, G, T, D, capacity, plan))
+      !plan_of(has_codes(cache.dtype), B, H, G, T, D, capacity, plan, per_cu))
     return fail(FCR_E_SHAPE, "G and T must be >= 1; B, H, G, T and the table are too large for one call otherwise");
   if (!isfinite(scale)) return fail(FCR_E_SCALE, "scale must be finite");
   bool ok = q_strides[3] == 1 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;

@@ -17,34 +17,39 @@ __device__ __forceinline__ Sight view_of(const Args& a, int b, int h, int r0, in
   return Sight(a.context.of(b, h), a.tree_lengths ? constant_at(a.tree_lengths + b) : a.T, a.prefix ? constant_at(a.prefix + b) : 0, a.window, a.T, a.positions,
                (int)a.G.of((uint32_t)r0), (int)a.G.of((uint32_t)(min(r1, a.rows) - 1)));
 }
-// Blocks of all items laid end to end, `per` of them for every workgroup, found from the lengths on the device.  A thread adds up the blocks of some consecutive
-// (entry, tile) pairs, an entry being a sequence, or one of its heads where these differ in length; all heads of a sequence have the same number S of blocks.  A place
-// among the blocks is then found in two steps: its entry, by the place over the number of heads, and the tile, by what is left of the place over S.
+// Blocks of all items laid end to end, each item behind some places for what runs once (once_of), `per` places for every workgroup, found from the lengths on the device; or
+// items taken whole.  A thread adds up the blocks of some consecutive
+// (entry, tile) pairs, an entry being a sequence, or one of its heads where these differ in length; all heads of a sequence have the same number S of places.  A place
+// is then found in two steps: its entry, by the place over the number of heads, and the tile, by what is left of the place over S.
 template <int THREADS, int ROWS>
 struct ChunkDeal {
-  int at, end, b, h, tile, blk, nb;
+  int at, end, b, h, tile, blk, nb, once;
   Sight seen;
+  // `at` and `end` are places; the piece is of blocks [blk, stop()) of the item's nb.
   // What is found goes through locals to one place: stores on several ways would be joined into one to an address that is chosen, and the deal would stay in
   // memory, where nothing is known to be uniform.
   struct Found {
-    int at, end, b, h, tile, blk;     // end below 0: the item is taken whole
+    int at, end, b, h, tile, blk;     // blk: the place in the item; end below 0: it is taken whole
+    int once;
     bool any;
   };
   // An item for this workgroup of a launch of one for each: the last tiles, which see the most keys, first, and tiles of one head on one die (workgroups are
   // dealt to 8 dies in turn) where the number of heads is a multiple of 8.
   static __device__ __forceinline__ Found one(const Args& a) {
     const int rank = (int)a.all_heads.of(blockIdx.x), bh = blockIdx.x - rank * a.all_heads.d, b = (int)a.heads.of((uint32_t)bh);
-    return Found{0, -1, b, bh - b * a.H, a.row_tiles - 1 - rank, 0, rank < a.row_tiles};
+    return Found{0, -1, b, bh - b * a.H, a.row_tiles - 1 - rank, 0, 0, rank < a.row_tiles};
   }
-  __device__ __forceinline__ bool start(const Args& a, int wg, int* scan) {   // scan: THREADS / 64 + 4 words of LDS (twice the first where a.whole is 1)
+  __device__ __forceinline__ bool start(const Args& a, int wg, int* scan) {   // scan: THREADS / 64 + 4 words of LDS and, where a.whole is 1, THREADS / 64 more
     const Found f = a.whole == 2 ? one(a) : dealt(a, wg, scan);
     if (!f.any) return false;
     b = __builtin_amdgcn_readfirstlane(f.b), h = __builtin_amdgcn_readfirstlane(f.h), tile = __builtin_amdgcn_readfirstlane(f.tile);
-    blk = __builtin_amdgcn_readfirstlane(f.blk), at = __builtin_amdgcn_readfirstlane(f.at);
+    blk = __builtin_amdgcn_readfirstlane(f.blk), at = __builtin_amdgcn_readfirstlane(f.at), once = __builtin_amdgcn_readfirstlane(f.once);
     look(a);
     const int last = __builtin_amdgcn_readfirstlane(f.end);
     end = last < 0 ? nb : last;
-    return true;
+    const int skipped = max(once - blk, 0);
+    at += skipped, blk += skipped - once;
+    return at < end;                                    // (else the next workgroup has the first part of this item)
   }
   static __device__ __forceinline__ Found dealt(const Args& a, int wg, int* scan) {
     constexpr int waves = THREADS / 64;
@@ -52,46 +57,80 @@ struct ChunkDeal {
     const bool by_head = a.context.sh != 0;
     const int entries = by_head ? a.B * a.H : a.B, times = by_head ? 1 : a.H, pairs = entries * a.row_tiles;
     const int each = (pairs + THREADS - 1) / THREADS, p0 = min(tid * each, pairs), p1 = min(p0 + each, pairs);
-    const auto blocks_of_pair = [&](int p) {
+    int once = 0;
+    const auto weight_of_pair = [&](int p) {
       const int e = (int)a.per_head.of((uint32_t)p), t = p - e * a.row_tiles;
       int eb = e, eh = 0;
       if (by_head) eb = (int)a.heads.of((uint32_t)e), eh = e - eb * a.H;
-      return view_of(a, eb, eh, t * ROWS, t * ROWS + ROWS).blocks();
+      return view_of(a, eb, eh, t * ROWS, t * ROWS + ROWS).blocks() + once;
     };
     int mine = 0, most = 0;
     for (int p = p0; p < p1; ++p) {
-      const int blocks = blocks_of_pair(p);
+      const int blocks = weight_of_pair(p);
       mine += blocks, most = max(most, blocks);
     }
-    const int upto = sum_up_to(mine);
-    if (lane == 63) scan[wave] = upto;
+    int before, sum;                                    // in front of this thread's, and all
+    const auto add_up = [&](int x) {
+      const int upto = sum_up_to(x);
+      if (lane == 63) scan[wave] = upto;
+      __syncthreads();
+      sum = 0, before = upto - x;
+#pragma unroll
+      for (int i = 0; i < waves; ++i) {
+        before += i < wave ? scan[i] : 0;
+        sum += scan[i];
+      }
+    };
     if (a.whole) {
       for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o));
       if (lane == 63) scan[waves + 4 + wave] = most;
     }
-    __syncthreads();
-    int sum = 0, before = upto - mine;
-#pragma unroll
-    for (int i = 0; i < waves; ++i) {
-      before += i < wave ? scan[i] : 0;
-      sum += scan[i];
-    }
-    const int total = __builtin_amdgcn_readfirstlane(sum) * times, per = (int)a.all.of((uint32_t)(total + a.wgs - 1));
-    if (wg == 0 && tid == 0) a.first[0] = per;
+    add_up(mine);
+    int total = __builtin_amdgcn_readfirstlane(sum) * times, per = (int)a.all.of((uint32_t)(total + a.wgs - 1));
+    const int more = once_of(per, ROWS != 16), weights = total + more * pairs * times, each_weight = (int)a.all.of((uint32_t)(weights + a.wgs - 1));
+    if (wg == 0 && tid == 0) a.first[0] = each_weight;
     if (a.whole) {
 #pragma unroll
       for (int i = 0; i < waves; ++i) most = max(most, scan[waves + 4 + i]);
-      if (items_are_whole(__builtin_amdgcn_readfirstlane(most), per, pairs * times, a.wgs)) return one(a);
-      if (blockIdx.x >= (unsigned)a.wgs) return Found{0, 0, 0, 0, 0, 0, false};
+      if (items_are_whole(__builtin_amdgcn_readfirstlane(most) + more, each_weight, pairs * times, a.wgs, ROWS != 16)) return one(a);
+      if (blockIdx.x >= (unsigned)a.wgs) return Found{0, 0, 0, 0, 0, 0, 0, false};
     }
+    if (ROWS == 16 && a.row_tiles == 1 && pieces_are_tried(entries, THREADS, per, 1, false)) {
+      // Pieces of one item each, as in tree_attention.
+      const int blocks = mine;
+      const int longest = most_of(per, most_allowed(per, 1, false), [&](int p) {
+        mine = tid < entries ? pieces_of(blocks, p) : 0;
+        __syncthreads();
+        add_up(mine);
+        return __builtin_amdgcn_readfirstlane(sum) * times <= a.wgs;
+      });
+      if (longest) {
+        if (wg == 0 && tid == 0) a.first[0] = longest;
+        if (wg >= __builtin_amdgcn_readfirstlane(sum) * times) return Found{0, 0, 0, 0, 0, 0, 0, false};
+        int* const found = scan + waves;
+        const int x = by_head ? wg : (int)a.heads.of((uint32_t)wg);
+        if (x >= before && x < before + mine) found[0] = tid, found[1] = before, found[2] = blocks;
+        __syncthreads();
+        const int entry = __builtin_amdgcn_readfirstlane(found[0]), nb = __builtin_amdgcn_readfirstlane(found[2]), pieces = pieces_of(nb, longest);
+        int piece = wg - times * __builtin_amdgcn_readfirstlane(found[1]), head = 0;
+        if (!by_head) head = (int)((uint32_t)piece / (uint32_t)pieces), piece -= head * pieces;
+        const int length = piece_length(nb, pieces), b = by_head ? (int)a.heads.of((uint32_t)entry) : entry;
+        return Found{0, least_of(length, nb - piece * length), b, by_head ? entry - b * a.H : head, 0, piece * length, 0, true};
+      }
+      mine = blocks;
+      __syncthreads();
+      add_up(mine);
+    }
+    once = more, per = each_weight, total = weights;
+    before += once * p0, mine += once * (p1 - p0), sum += once * pairs;
     const int at = wg * per, end = min(at + per, total);   // (wgs * per is total + wgs at most: checked by the host to fit)
-    if (at >= end) return Found{0, 0, 0, 0, 0, 0, false};
-    // the pair that has block x of its entries, and the blocks in front of it
+    if (at >= end) return Found{0, 0, 0, 0, 0, 0, 0, false};
+    // the pair that has place x of its entries, and the places in front of it
     int* const found = scan + waves;
     const auto find = [&](int x) {
       if (x >= before && x < before + mine) {
         int p = p0, s = before;
-        for (int blocks = blocks_of_pair(p); x >= s + blocks; blocks = blocks_of_pair(p)) s += blocks, ++p;
+        for (int weight = weight_of_pair(p); x >= s + weight; weight = weight_of_pair(p)) s += weight, ++p;
         found[0] = p, found[1] = s;
       }
       __syncthreads();
@@ -101,15 +140,15 @@ struct ChunkDeal {
     const int entry = (int)a.per_head.of((uint32_t)pair), q0 = entry * a.row_tiles;
     int place = at - times * in_front, head = 0;
     if (a.row_tiles == 1) {
-      const int blocks = __builtin_amdgcn_readfirstlane(blocks_of_pair(pair));
-      if (!by_head) head = (int)((uint32_t)place / (uint32_t)blocks), place -= head * blocks;
+      const int weight = __builtin_amdgcn_readfirstlane(weight_of_pair(pair));
+      if (!by_head) head = (int)((uint32_t)place / (uint32_t)weight), place -= head * weight;
     } else {
-      // blocks in front of the entry's pairs and behind them
+      // places in front of the entry's pairs and behind them
       const int q1 = q0 + a.row_tiles;
       const auto mark = [&](int q, int to) {
         if (p0 <= q && q < p1) {
           int s = before;
-          for (int p = p0; p < q; ++p) s += blocks_of_pair(p);
+          for (int p = p0; p < q; ++p) s += weight_of_pair(p);
           found[to] = s;
         } else if (q == pairs && tid == 0) {
           found[to] = sum;
@@ -118,15 +157,15 @@ struct ChunkDeal {
       mark(q0, 2);
       mark(q1, 3);
       __syncthreads();
-      const int from = __builtin_amdgcn_readfirstlane(found[2]), blocks = __builtin_amdgcn_readfirstlane(found[3]) - from;
+      const int from = __builtin_amdgcn_readfirstlane(found[2]), weight = __builtin_amdgcn_readfirstlane(found[3]) - from;
       place = at - times * from;
-      if (!by_head) head = (int)((uint32_t)place / (uint32_t)blocks), place -= head * blocks;
+      if (!by_head) head = (int)((uint32_t)place / (uint32_t)weight), place -= head * weight;
       find(from + place);
       pair = __builtin_amdgcn_readfirstlane(found[0]), in_front = __builtin_amdgcn_readfirstlane(found[1]);
       place = from + place - in_front;
     }
     const int b = by_head ? (int)a.heads.of((uint32_t)entry) : entry;
-    return Found{at, end, b, by_head ? entry - b * a.H : head, pair - q0, place, true};
+    return Found{at, end, b, by_head ? entry - b * a.H : head, pair - q0, place, once, true};
   }
   __device__ __forceinline__ void look(const Args& a) {
     seen = view_of(a, b, h, tile * ROWS, tile * ROWS + ROWS);
@@ -143,7 +182,7 @@ struct ChunkDeal {
   }
   // To the next piece; false: there is none.
   __device__ __forceinline__ bool next(const Args& a) {
-    at += stop() - blk;
+    at += stop() - blk + once;
     if (at >= end) return false;
     blk = 0;
     if (++tile == a.row_tiles) {
@@ -158,7 +197,7 @@ struct ChunkDeal {
 template <bool BENT>
 struct Chunk {
   static constexpr bool bent = BENT, rising = false;
-  static constexpr int kScan = 4;
+  static constexpr int kScan = 8;
   template <int THREADS>
   using Deal = ChunkDeal<THREADS, 16>;
   static __device__ __forceinline__ uint32_t seen_by(const Args& a, const Sight& v, int, int row, int pos, uint32_t there, int g) {
@@ -651,12 +690,19 @@ bool fcr_tree::chunk_e4m3(const Args& a, int w, int form, hipStream_t s) { retur
 #endif
 
 #if FCR_HAS(0)
+namespace {
+// Workgroups of few_attention_kernel in a launch for each CU, where not as many as tree_attention takes: rows of 64 elements leave registers for three and more.  One token
+// of 16 sequences over 8 heads of 8192 e4m3 keys of 64 elements, 4 queries each: 39 us with two, 37 with three, 41 with four; of 128 elements 8 x 8 heads of 16384 keys 55 and
+// 57 with three.
+int few_per_cu(int D) { return D <= 64 ? 3 : 0; }
+}  // namespace
+
 extern "C" {
 
 size_t fcr_chunk_attention_bytes(int B, int H, int G, int T, int D, int64_t positions) {
   Plan p[2];             // for either kind of cache
   if (B < 1 || H < 1 || G < 1 || T < 1 || D < 16 || D > 256 || positions < 1 || positions > (1 << 30) || (int64_t)B * H > (1 << 24)) return 0;
-  return plan_of(true, B, H, G, T, D, positions, p[0]) && plan_of(false, B, H, G, T, D, positions, p[1]) ? (size_t)std::max(p[0].bytes, p[1].bytes) : 0;
+  return plan_of(true, B, H, G, T, D, positions, p[0], few_per_cu(D)) && plan_of(false, B, H, G, T, D, positions, p[1], few_per_cu(D)) ? (size_t)std::max(p[0].bytes, p[1].bytes) : 0;
 }
 
 int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages,
@@ -668,7 +714,8 @@ int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* ta
   Plan plan;
   Args a = {};
   if (window < 0) return fail(FCR_E_SHAPE, "window must be >= 0");
-  if ((rc = check_queries(a, plan, q, *cache, table, table_stride, table_pages, context, context_strides, out, lse, ws, ws_bytes, dtype, B, G, T, q_strides, scale)))
+  if ((rc = check_queries(a, plan, q, *cache, table, table_stride, table_pages, context, context_strides, out, lse, ws, ws_bytes, dtype, B, G, T, q_strides, scale,
+                          few_per_cu(cache->D))))
     return rc;
   if (!isfinite(cap) || cap < 0.0f) return fail(FCR_E_SCALE, "cap must be finite and >= 0");
   a.tree_lengths = counts;
@@ -679,7 +726,8 @@ int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* ta
   a.cap2 = cap * log2e;
   a.scale2 = cap != 0.0f ? scale * (2.0f * log2e) / cap : scale * log2e;
   if (!isfinite(a.scale2) || !isfinite(a.cap2)) return fail(FCR_E_SCALE, "scale over cap must be finite");
-  a.whole = plan.form == 1 ? 0 : whole_items_of(plan.items, plan.wgs);
+  const int64_t positions = (int64_t)table_pages * cache->page_size, near = (int64_t)window + plan.tile_rows / G + 2 * 128;
+  a.whole = whole_items_of(plan.items, plan.held, ((window && !prefix ? std::min(positions, near) : positions) + 127) / 128, plan.form != 1);
   a.all_heads.set((uint32_t)(B * cache->H));
   const int w = (cache->D + 63) / 64;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -67,7 +67,7 @@ FCR_HOST_DEVICE inline int most_of_two(int a, int b) { return a > b ? a : b; }
 // What tokens first .. last of a sequence (those that it has) see in chunk_attention: keys of [lo, n) and [0, prefix), and no others; keys of [all_lo, all_hi) and
 // [0, prefix), every token.  Blocks that begin at gap_at or behind it (a number of keys) lie `gap` keys further back than their number says: between the
 // prefix and lo no key is seen.  They are taken from the last one to the first: where scores lose a slope times the distance the largest weights come first, and
-// the reference of a row rises once, not with every step towards the token (two prompts of up to 4096 biased tokens, 16 heads: PROMPT us).  (context
+// the reference of a row rises once, not with every step towards the token (two prompts of up to 4096 biased tokens, 16 heads: 306 -> 240 us).  (context
 // up to 2^30, T up to 2^24.)
 constexpr int kNoKey = 0x7fff0000;           // above every n
 struct Sight {
@@ -117,15 +117,25 @@ struct Steps {
   FCR_HOST_DEVICE bool whole(int first, int last) const { return (last >= fast && first - fast < fasts) || first <= prefix - 32; }
 };
 
-// Items of many rows may be taken whole, a workgroup for each, by a launch of as many (0: no, too few; 1: if items_are_whole says so; 2: yes, there are so many that
-// none is large): nothing is cut and joined, but the last workgroups may leave others idle.
-FCR_HOST_DEVICE inline int whole_items_of(int64_t items, int wgs) { return 4 * items < wgs ? 0 : items < 8ll * wgs ? 1 : 2; }
-// The time of either distribution in blocks: what runs once per piece costs about three, the join of what was cut five.  Whole items take as long as the longest of them or, where
-// there is more than one for a workgroup, an eighth longer than their mean.
-FCR_HOST_DEVICE inline bool items_are_whole(int longest, int per, int items, int wgs) {
-  const int rounds = quotient_up(items, wgs);
-  const int whole = items <= wgs ? longest : most_of_two(longest, per + per / 8);
-  return whole + 3 * rounds <= per + 3 * (rounds + 1) + 5;
+// Items of chunk_attention may be taken whole, a workgroup for each, by a launch of as many: nothing is cut and joined, tiles of one head run together on one die, but the last
+// workgroups may leave others idle.  2: they are, without a look at the lengths or the launch that joins, where the longest that there can be (blocks of it) is no more
+// than some for each that a workgroup gets: keys of tall tiles (many rows) are bound by the matrix instructions wherever they are, few rows by memory, of which
+// the last workgroups have the more.  1: if items_are_whole says so.  0: no.
+//   One token of 8 heads of fp16 keys of 128 elements, us, cut and whole: 450 keys 10.9, 9.2; 900 11.3, 13.5; of 16 sequences 18.9, 16.3; 2000 of 64, of drawn lengths 64, 55.
+//   Many rows: 4 chunks of 512 tokens, 8 heads of 4 queries, behind 1000 keys 104, 73; 16 of 300 tokens of 256 elements 247, 215.
+FCR_HOST_DEVICE inline int whole_items_of(int64_t items, int held, int64_t longest, bool tall) {
+  if (longest * held <= (tall ? 2 * held + 12 * items : 4 * held + 16 * items)) return 2;
+  return (tall ? 4 * items : items) >= held ? 1 : 0;
+}
+// Blocks that what runs once for an item counts as where items are laid end to end: workgroups that have many short ones would take longer than the others.  No more
+// than half of a workgroup's blocks, or where there are few a part of them would get nothing else.  16 chunks of 128 tokens behind up to 2000 keys of 128 elements, 8 heads of 4
+// queries: 121 us without, 85 with them (five: 91); 64 heads of 8192 tokens 1520 and 1200; one token of 64 sequences of up to 2000 e4m3 keys 52 and 38.
+FCR_HOST_DEVICE inline int once_of(int per, bool tall) { return least_of(tall ? 3 : 1, per / 2); }
+// Whether items of these weights (blocks and what runs once) are better taken whole.  They take as long as the longest of them or, where there is more than one for
+// a workgroup, as their mean and a part of the longest; cut ones as their mean, what runs once for a second piece, and the join.  8 heads of 4096 fp16 tokens, two prompts:
+// 131 us cut and 154 whole; 4 chunks of 512 tokens, one behind 8192 keys, the others behind 512: 122 and 277, all behind 8192 370 and 340.
+FCR_HOST_DEVICE inline bool items_are_whole(int longest, int per, int items, int held, bool tall) {
+  return (items <= held ? longest : most_of_two(longest, per + longest / 8)) <= per + (tall ? 6 : 5);
 }
 
 }  // namespace fcr_tree

@@ -248,6 +248,21 @@ def test_many_blocks_per_workgroup(shape, kind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [(F16, F16), (E4M3, BF16)])
+@pytest.mark.parametrize("b,h,g,t,n,d", [(70, 8, 2, 1, 2500, 16), (9, 4, 1, 300, 1500, 32), (9, 4, 1, 300, 200, 32), (130, 8, 1, 1, 300, 64), (24, 4, 2, 20, 900, 64)])
+def test_items_whole_and_cut(kind, dtype, b, h, g, t, n, d):
+    """Many items, of one length, of drawn lengths, one long among short ones, of nothing but for one, of own lengths for each head."""
+    query, cache, table, _ = problem(b, h, g, t, n, d, 16, kind, dtype)
+    draw = torch.Generator().manual_seed(n)
+    full = torch.full((b,), n, dtype=torch.int32)
+    drawn, tokens = torch.randint(0, n + 1, (b,), generator=draw).int(), torch.randint(0, t + 1, (b,), generator=draw).int()
+    one, last = torch.full((b,), 3, dtype=torch.int32), torch.zeros(b, dtype=torch.int32)
+    one[b // 2], last[-1] = n, t
+    for context, counts in ((full, None), (drawn, tokens), (one, None), (full, last), (torch.randint(0, n + 1, (b, h), generator=draw).int(), tokens)):
+        check(query, cache, table, context, counts=counts)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind,dtype", KINDS)
 @pytest.mark.parametrize("t,d", [(6, 64), (130, 128), (3, 256)])
 def test_what_hidden_rows_hold_has_no_influence(kind, dtype, t, d):
