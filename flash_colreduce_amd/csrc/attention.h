@@ -1342,11 +1342,11 @@ struct Plan {
   int held;                  // workgroups that the chip holds at once: wgs where there is work for them
   int64_t items, first_bytes, bytes;
 };
-// What depends on sizes alone.  false: too large.
-bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Plan& p, int per_cu = 0) {
+// What depends on sizes alone.  per_cu: workgroups of few_attention_kernel for each CU; form: not form_of's.  false: too large.
+bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Plan& p, int per_cu = 0, int form = 0) {
   const int64_t rows = (int64_t)T * G;
   const int w = (D + 63) / 64;
-  p.form = form_of(rows, w, codes);
+  p.form = form ? form : form_of(rows, w, codes);
   p.tile_rows = rows_of_tile(p.form, w);
   const int64_t tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.items = (int64_t)B * H * tiles;
@@ -1364,10 +1364,11 @@ bool plan_of(bool codes, int B, int H, int G, int T, int D, int64_t capacity, Pl
   return true;
 }
 
-// What both entry points are given, but for the cache itself: checked, and put into `a`.
+// What both entry points are given, but for the cache itself: checked, and put into `a`; plan_for(plan) as plan_of.
+template <class PlanFor>
 int check_queries(Args& a, Plan& plan, const void* q, const fcr_cache& cache, const int32_t* table, int64_t table_stride, int table_pages, const int32_t* context,
                   const int64_t* context_strides, void* out, float* lse, void* ws, size_t ws_bytes, int dtype, int B, int G, int T, const int64_t* q_strides,
-                  float scale, int per_cu = 0) {
+                  float scale, PlanFor plan_for) {
   const int rc = check_table(table, table_stride, table_pages, cache.page_size, B);
   if (rc) return rc;
   if (!q || !q_strides || !context || !context_strides || !out || !ws) return fail(FCR_E_NULL, "null pointer argument");
@@ -1376,7 +1377,7 @@ int check_queries(Args& a, Plan& plan, const void* q, const fcr_cache& cache, co
   const int H = cache.H, D = cache.D;
   const int64_t capacity = (int64_t)table_pages * cache.page_size;
   if (G < 1 || T < 1 || T > (1 << 24) || G > (1 << 24) || (int64_t)B * H > (1 << 24) || (int64_t)H * G > (1 << 24) ||
-      !plan_of(has_codes(cache.dtype), B, H, G, T, D, capacity, plan, per_cu))
+      !plan_for(plan))
     return fail(FCR_E_SHAPE, "G and T must be >= 1; B, H, G, T and the table are too large for one call otherwise");
   if (!isfinite(scale)) return fail(FCR_E_SCALE, "scale must be finite");
   bool ok = q_strides[3] == 1 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;

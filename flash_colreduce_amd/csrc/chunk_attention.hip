@@ -695,14 +695,31 @@ namespace {
 // of 16 sequences over 8 heads of 8192 e4m3 keys of 64 elements, 4 queries each: 39 us with two, 37 with three, 41 with four; of 128 elements 8 x 8 heads of 16384 keys 55 and
 // 57 with three.
 int few_per_cu(int D) { return D <= 64 ? 3 : 0; }
+// Blocks that an item of a plan has at most; window: 0 where there is none, or a prefix, whose length only the device knows.
+int64_t most_blocks(const Plan& p, int64_t positions, int window, int G) {
+  return ((window ? std::min(positions, (int64_t)window + p.tile_rows / G + 2 * kBlock) : positions) + kBlock - 1) / kBlock;
+}
+// few_attention_kernel takes more rows than form_of gives it, in tiles of 16, where the chip has few of them: it starts faster and its items are many, so that they run at once and
+// need not be cut.  us, by it and by the kernel for many rows, at the largest size on its side and the next one: 8 x 8 fp16 heads of 128 rows of 128 elements, 1564 keys 36.0, 41.6,
+// 256 rows, 464 keys 26.5, 31.9, 1564 keys 63.4, 49.4; of 64 elements 256 rows, 464 keys 16.7, 22.0, 1564 keys 39.2, 35.4; of 256 elements 128 rows, 464 keys 32.5, 39.9, 1564 keys
+// 72.0, 57.7; e4m3 keys of 128 elements, 512 rows, 178 keys 24.9, 25.7, 528 keys 40.7, 38.4.  One item of 64 rows of 128 elements and 114 keys: 7.5, 16.0.
+bool chunk_plan(bool codes, int B, int H, int G, int T, int D, int64_t positions, int window, Plan& p) {
+  if (plan_of(codes, B, H, G, T, D, positions, p, few_per_cu(D), 1) && p.items * (most_blocks(p, positions, window, G) + 2) <= 15ll * p.held) return true;
+  return plan_of(codes, B, H, G, T, D, positions, p, few_per_cu(D));
+}
 }  // namespace
 
 extern "C" {
 
 size_t fcr_chunk_attention_bytes(int B, int H, int G, int T, int D, int64_t positions) {
-  Plan p[2];             // for either kind of cache
   if (B < 1 || H < 1 || G < 1 || T < 1 || D < 16 || D > 256 || positions < 1 || positions > (1 << 30) || (int64_t)B * H > (1 << 24)) return 0;
-  return plan_of(true, B, H, G, T, D, positions, p[0], few_per_cu(D)) && plan_of(false, B, H, G, T, D, positions, p[1], few_per_cu(D)) ? (size_t)std::max(p[0].bytes, p[1].bytes) : 0;
+  size_t bytes = 0;
+  for (int i = 0; i < 4; ++i) {                         // for either kind of cache, whatever the window is
+    Plan p;
+    if (!chunk_plan(i & 1, B, H, G, T, D, positions, i >> 1, p)) return 0;
+    bytes = std::max(bytes, (size_t)p.bytes);
+  }
+  return bytes;
 }
 
 int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages,
@@ -714,8 +731,9 @@ int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* ta
   Plan plan;
   Args a = {};
   if (window < 0) return fail(FCR_E_SHAPE, "window must be >= 0");
+  const int64_t positions = (int64_t)table_pages * cache->page_size;
   if ((rc = check_queries(a, plan, q, *cache, table, table_stride, table_pages, context, context_strides, out, lse, ws, ws_bytes, dtype, B, G, T, q_strides, scale,
-                          few_per_cu(cache->D))))
+                          [&](Plan& p) { return chunk_plan(has_codes(cache->dtype), B, cache->H, G, T, cache->D, positions, prefix ? 0 : window, p); })))
     return rc;
   if (!isfinite(cap) || cap < 0.0f) return fail(FCR_E_SCALE, "cap must be finite and >= 0");
   a.tree_lengths = counts;
@@ -726,8 +744,7 @@ int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* ta
   a.cap2 = cap * log2e;
   a.scale2 = cap != 0.0f ? scale * (2.0f * log2e) / cap : scale * log2e;
   if (!isfinite(a.scale2) || !isfinite(a.cap2)) return fail(FCR_E_SCALE, "scale over cap must be finite");
-  const int64_t positions = (int64_t)table_pages * cache->page_size, near = (int64_t)window + plan.tile_rows / G + 2 * 128;
-  a.whole = whole_items_of(plan.items, plan.held, ((window && !prefix ? std::min(positions, near) : positions) + 127) / 128, plan.form != 1);
+  a.whole = whole_items_of(plan.items, plan.held, most_blocks(plan, positions, prefix ? 0 : window, G), plan.form != 1);
   a.all_heads.set((uint32_t)(B * cache->H));
   const int w = (cache->D + 63) / 64;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -98,7 +98,8 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
   Plan plan;
   Args a = {};
   if (mask && T > 46340) return fail(FCR_E_SHAPE, "a mask of more than 2^31 bytes");
-  if ((rc = check_queries(a, plan, q, *cache, table, table_stride, table_pages, context, context_strides, out, lse, ws, ws_bytes, dtype, B, G, T, q_strides, scale)))
+  if ((rc = check_queries(a, plan, q, *cache, table, table_stride, table_pages, context, context_strides, out, lse, ws, ws_bytes, dtype, B, G, T, q_strides, scale,
+                          [&](Plan& p) { return plan_of(has_codes(cache->dtype), B, cache->H, G, T, cache->D, (int64_t)table_pages * cache->page_size, p); })))
     return rc;
   if (mask_stride < 0) return fail(FCR_E_STRIDE, "strides must be >= 0");
   a.tree_lengths = tree_lengths;
