@@ -336,8 +336,8 @@ def chunk_attention(query: torch.Tensor, cache: KVCache, table: torch.Tensor, co
             raise ValueError(f"{name} must be int32 ({b},) on the cache's device. Got {tuple(x.shape)} {x.dtype}.")
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (hq,) or slopes.device != dev):
         raise ValueError(f"slopes must be float32 ({hq},) on the cache's device. Got {tuple(slopes.shape)} {slopes.dtype}.")
-    if cap is not None and not 0 < cap < math.inf:
-        raise ValueError(f"cap must be positive and finite. Got {cap}.")
+    if cap is not None and not 2.0**-149 <= cap < math.inf:
+        raise ValueError(f"cap must be positive and finite, and not below fp32's least number. Got {cap}.")
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1. Got {window}.")
     if scale is None:

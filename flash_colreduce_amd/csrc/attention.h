@@ -449,7 +449,8 @@ __device__ __forceinline__ void weigh(const f32x4 (&k_scale)[2], const f32x4 (&v
 }
 
 // Scores that are capped, c tanh(s / c) = c - 2 c / (1 + 2^x) with x = s 2 log2(e) / c, which the products' scale gives; or that lose a slope times the distance
-// between a token and a key.  In base 2, and in 32 bits: next to 0 the difference is off by 2^-24 c.  Costs a score an fma, two transcendental
+// between a token and a key.  In base 2, and in 32 bits: next to 0 the difference is off by 2^-22 c, for caps of 128 a sixteenth of what the rounding of weights to 11 bits
+// costs; with larger ones it is formed next to 0 as a quotient (Lambert's continued fraction of tanh, six terms, off by 2^-31).  Costs a score an fma, two transcendental
 // instructions and an addition; or a conversion's share, an addition and an fma.
 template <int RT>
 struct Bend {
@@ -466,6 +467,12 @@ struct Bend {
       slope2[r] = sloped ? a.slopes[h * (int)a.G.d + (int)(row - t * a.G.d)] * 1.44269504088896340736f : 0.0f;
     }
   }
+  __device__ __forceinline__ float wide(float x) const {
+    const float y = x * 0.34657359027997265471f, z = y * y;              // ln(2) / 2
+    const float quotient = y * __builtin_fmaf(__builtin_fmaf(21.0f, z, 1260.0f), z, 10395.0f) *
+                           __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fmaf(z + 210.0f, z, 4725.0f), z, 10395.0f));
+    return cap2 * (fabsf(y) < 1.0f ? quotient : __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), 1.0f));
+  }
   // The products s of 32 keys from pos on become scores; nothing is left to multiply them by.
   __device__ __forceinline__ void of(f32x4 (&k_scale)[2], int pos, int g, f32x4 (&s)[RT][2]) const {
 #pragma unroll
@@ -474,7 +481,14 @@ struct Bend {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[r][t][i] *= k_scale[t][i];
-    if (cap2 != 0.0f) {
+    if (__builtin_expect(cap2 > 128.0f * 1.44269504088896340736f, 0)) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[r][t][i] = wide(s[r][t][i]);
+    } else if (cap2 != 0.0f) {
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll

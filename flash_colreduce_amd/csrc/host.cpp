@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <limits>
 
 #include "fcr.h"
 
@@ -480,7 +481,7 @@ PyObject* chunk_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (args[6] != Py_None) {
     if (!PyFloat_CheckExact(args[6])) Py_RETURN_NONE;
     cap = PyFloat_AS_DOUBLE(args[6]);
-    if (!(cap > 0.0) || !std::isfinite(cap)) Py_RETURN_NONE;
+    if (!(cap >= std::numeric_limits<float>::denorm_min()) || !std::isfinite(cap)) Py_RETURN_NONE;
   }
   long long window = 0;
   if (args[8] != Py_None) {

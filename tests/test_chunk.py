@@ -56,12 +56,13 @@ def ref_chunk(query, cache, table, context, scale=None, counts=None, cap=None, s
         out[bi, hi, sees] = out[bi, hi, sees] + p[bi, hi, sees, at][:, None] * bad
     # As for tree_attention: weights rounded to fp16 (bf16 against a bf16 cache), those under 2^-14 of the largest to half of fp16's smallest step; scores are
     # sums of D products, each off by 2^-24 of the sum of magnitudes, and exp2's 2^-21.  A cap adds, in steps of 2^-24 of it: 1 for its own rounding, 2 for the
-    # reciprocal's last bit, 1 for the exponential's and 2 for what is fed to it, twice for safety 12: under 2^-20; it makes no error before it larger.  A slope times a
+    # reciprocal's last bit, 1 for the exponential's and 2 for what is fed to it, twice for safety 12: under 2^-20; it makes no error before it larger.  Above 128 it
+    # is formed so that these are steps of the score instead.  A slope times a
     # distance is rounded three times (slope in base 2, product, sum): 2^-22 of it.
     rounding = HALF_STEP[BF16 if cache.k.dtype == BF16 else F16]
     v1 = torch.where(v0.isfinite(), v0, 0.0).abs()
     magnitude = torch.where(any_seen.transpose(2, 3) & seen, q.abs() @ torch.where(k0.isfinite(), k0, 0.0).abs().transpose(-1, -2) * abs(scale), 0.0).amax(-1)
-    ds = (d + 8) * 2.0 ** -24 * magnitude + 2.0 ** -21 + (0 if cap is None else cap * 2.0 ** -20)
+    ds = (d + 8) * 2.0 ** -24 * magnitude + 2.0 ** -21 + (0 if cap is None else cap * 2.0 ** -20 if cap <= 128 else magnitude * 2.0 ** -20)
     if slopes is not None:
         ds = ds + 2.0 ** -22 * (slopes.double()[None, :, None, None] * distance * seen).abs().amax(-1)
     weighted = p @ v1
@@ -315,7 +316,7 @@ def test_what_hidden_rows_hold_has_no_influence(kind, dtype, t, d, places):
 def test_scores_at_the_ends(kind, dtype):
     """Scores far above a cap, slopes that leave one key, negative ones, scales of 0 and below, caps next to 0 and above all scores."""
     query, cache, table, context = problem(2, 2, 2, 20, 200, 64, 16, kind, dtype, spread=2.0)
-    for how in (dict(scale=50.0, cap=1.0), dict(scale=0.0, cap=3.0), dict(scale=-0.3, cap=20.0), dict(cap=1e-3), dict(cap=1e6), dict(slopes=torch.full((4,), 100.0)),
+    for how in (dict(scale=50.0, cap=1.0), dict(scale=0.0, cap=3.0), dict(scale=-0.3, cap=20.0), dict(cap=1e-3), dict(cap=128.0), dict(cap=130.0), dict(cap=1e6), dict(scale=30.0, cap=200.0), dict(cap=1e30), dict(slopes=torch.full((4,), 100.0)),
                 dict(slopes=torch.full((4,), -0.3)), dict(slopes=torch.zeros(4), window=7), dict(scale=3.0, slopes=torch.tensor([0.0, 1e-4, 2.0, -1.0]), cap=30.0)):
         check(query, cache, table, context, **how)
         check(query[:, :, :3], cache, table, context, **how)
@@ -483,7 +484,7 @@ def test_refusals_on_the_device():
     bad = [dict(query=query.float()), dict(query=query.bfloat16()), dict(query=query[:, :3]), dict(query=query[..., :32]), dict(query=query[0]), dict(query=query.cpu()),
            dict(table=table.long()), dict(table=table[:1]), dict(context=context.long()), dict(context=context[:1]), dict(counts=ints.long()), dict(counts=ints[:1]),
            dict(prefix=ints.float()), dict(prefix=ints[:, None]), dict(slopes=torch.ones(3, device="cuda")), dict(slopes=torch.ones(4, device="cuda").half()),
-           dict(slopes=torch.ones(4)), dict(cap=0.0), dict(cap=-1.0), dict(cap=math.inf), dict(cap=math.nan), dict(window=0), dict(window=-5)]
+           dict(slopes=torch.ones(4)), dict(cap=0.0), dict(cap=-1.0), dict(cap=1e-46), dict(cap=math.inf), dict(cap=math.nan), dict(window=0), dict(window=-5)]
     for over in bad:
         a = {**dict(query=query, table=table, context=context), **over}
         with pytest.raises(ValueError):
