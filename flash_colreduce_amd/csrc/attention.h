@@ -452,19 +452,24 @@ __device__ __forceinline__ void weigh(const f32x4 (&k_scale)[2], const f32x4 (&v
 // between a token and a key.  In base 2, and in 32 bits: next to 0 the difference is off by 2^-22 c, for caps of 128 a sixteenth of what the rounding of weights to 11 bits
 // costs; with larger ones it is formed next to 0 as a quotient (Lambert's continued fraction of tanh, six terms, off by 2^-31).  Costs a score an fma, two transcendental
 // instructions and an addition; or a conversion's share, an addition and an fma.
-template <int RT>
+// BENT: 1, capped; 2, with slopes, and a cap perhaps; 0, neither.  (One kernel for caps and slopes spilled up to 126 registers: 4 chunks of 512 tokens behind 8192 fp16 keys of
+// 128 elements, 8 heads of 4 queries, capped, 430 us by it and 413 by its own, two biased prompts of 4096 tokens, 16 heads, 215 and 203; both at once 446 and 467.)  Keys behind
+// every token of the rows take their distance as it is, an fma with what is common to a row; others its magnitude, an instruction more.
+template <int RT, int BENT>
 struct Bend {
   float cap2, slope2[RT];
   int place[RT];           // of a row's token
-  bool sloped;
+  int first;               // of the rows' first one
   __device__ __forceinline__ void load(const Args& a, int h, int row0, int context, int col) {
     cap2 = a.cap2;
-    sloped = a.slopes != nullptr;
+    if constexpr (BENT == 2) {
+      first = __builtin_amdgcn_readfirstlane(context + (int)a.G.of((uint32_t)min(row0, a.rows - 1)));
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const uint32_t row = (uint32_t)min(row0 + 16 * r + col, a.rows - 1), t = a.G.of(row);
-      place[r] = context + (int)t;
-      slope2[r] = sloped ? a.slopes[h * (int)a.G.d + (int)(row - t * a.G.d)] * 1.44269504088896340736f : 0.0f;
+      for (int r = 0; r < RT; ++r) {
+        const uint32_t row = (uint32_t)min(row0 + 16 * r + col, a.rows - 1), t = a.G.of(row);
+        place[r] = context + (int)t;
+        slope2[r] = a.slopes[h * (int)a.G.d + (int)(row - t * a.G.d)] * 1.44269504088896340736f;
+      }
     }
   }
   __device__ __forceinline__ float wide(float x) const {
@@ -473,14 +478,7 @@ struct Bend {
                            __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fmaf(z + 210.0f, z, 4725.0f), z, 10395.0f));
     return cap2 * (fabsf(y) < 1.0f ? quotient : __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), 1.0f));
   }
-  // The products s of 32 keys from pos on become scores; nothing is left to multiply them by.
-  __device__ __forceinline__ void of(f32x4 (&k_scale)[2], int pos, int g, f32x4 (&s)[RT][2]) const {
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[r][t][i] *= k_scale[t][i];
+  __device__ __forceinline__ void capped(f32x4 (&s)[RT][2]) const {
     if (__builtin_expect(cap2 > 128.0f * 1.44269504088896340736f, 0)) {
 #pragma unroll
       for (int r = 0; r < RT; ++r)
@@ -488,7 +486,7 @@ struct Bend {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[r][t][i] = wide(s[r][t][i]);
-    } else if (cap2 != 0.0f) {
+    } else {
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -497,14 +495,36 @@ struct Bend {
           for (int i = 0; i < 4; ++i)
             s[r][t][i] = __builtin_fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[r][t][i])), cap2);
     }
-    if (sloped) {
+  }
+  // The products s of 32 keys from pos on become scores; nothing is left to multiply them by.
+  __device__ __forceinline__ void of(f32x4 (&k_scale)[2], int pos, int g, f32x4 (&s)[RT][2]) const {
+    const bool behind = BENT == 2 && pos + 31 <= first, late = BENT == 1 || cap2 != 0.0f;
+    if (BENT == 1 || !behind || __builtin_expect(late, 0)) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const float first = (float)(place[r] - pos - 4 * g);
+      for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[r][t][i] = __builtin_fmaf(-slope2[r], fabsf(first - (float)(16 * t + i)), s[r][t][i]);
+          for (int i = 0; i < 4; ++i) s[r][t][i] *= k_scale[t][i];
+      if (BENT == 1 || __builtin_expect(late, 0)) capped(s);
+      if constexpr (BENT == 2) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float away = (float)(place[r] - pos - 4 * g);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[r][t][i] = __builtin_fmaf(-slope2[r], fabsf(away - (float)(16 * t + i)), s[r][t][i]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float off = -slope2[r] * (float)(place[r] - pos - 4 * g);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[r][t][i] = __builtin_fmaf(s[r][t][i], k_scale[t][i], __builtin_fmaf(slope2[r], (float)(16 * t + i), off));
       }
     }
 #pragma unroll
@@ -814,7 +834,7 @@ __device__ __forceinline__ int range_of(const Args& a, int block) { return (bloc
 
 // How tree_attention cuts its work, and what its rows see.
 struct Tree {
-  static constexpr bool bent = false;              // scores are products times a scale
+  static constexpr int bent = 0;                   // scores are products times a scale
   static constexpr bool rising = true;             // the last keys come last
   static constexpr int kScan = 2;                  // words of LDS behind those of the waves
   template <int THREADS>
@@ -865,7 +885,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) f
       by = __builtin_amdgcn_ldexpf(by, -up);            // (of the lane's row)
     }
     q.arrive();
-    Bend<1> bend;
+    Bend<1, P::bent> bend;
     if constexpr (P::bent) bend.load(a, h, deal.tile * 16, view.context, at.col);
     State<F, 1> st;
     st.clear();

@@ -200,9 +200,10 @@ struct ChunkDeal {
   }
 };
 
-template <bool BENT>
+template <int BENT>
 struct Chunk {
-  static constexpr bool bent = BENT, rising = false;
+  static constexpr int bent = BENT;
+  static constexpr bool rising = false;
   static constexpr int kScan = 8;
   template <int THREADS>
   using Deal = ChunkDeal<THREADS, 16>;
@@ -223,7 +224,7 @@ struct Chunk {
 // steps that none sees.  What a step costs beside its products and weights is kept small, since it is the vector and scalar instructions of two waves that a SIMD
 // spends its time on: a step is a slot of a ring in LDS at one address, what the wave sees of it follows from one number that falls by 32 (Steps), and what is used once per
 // stage is formed there from the arguments.
-template <bool BENT, int CD, int W, int WAVES>
+template <int BENT, int CD, int W, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args args) {
   using F = Form<CD, W>;
   constexpr int RT = tall_tiles(W), kKeys = tall_keys(W, WAVES), kSteps = kKeys / 32, kTiles = kKeys / 16, kStepsLog2 = kSteps == 4 ? 2 : 1;
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
       by = __builtin_amdgcn_ldexpf(by, -least);
     }
     q.arrive();
-    Bend<RT> bend;
+    Bend<RT, BENT> bend;
     if constexpr (BENT) bend.load(arguments(), h, row0, view.context, at.col);
     State<F, RT> st;
     st.clear();
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
 }
 
 // form: see form_of.  false: there is no such kernel
-template <bool BENT, int CD, int W>
+template <int BENT, int CD, int W>
 bool launch_chunk(const Args& a, int form, hipStream_t s) {
   const dim3 grid((unsigned)(a.whole ? std::max(a.wgs, a.B * a.H * a.row_tiles) : a.wgs));
   if (form == 1) {
@@ -662,15 +663,18 @@ bool launch_chunk(const Args& a, int form, hipStream_t s) {
   }
   return true;
 }
+template <int BENT, int CD>
+bool launch_chunk(const Args& a, int w, int form, hipStream_t s) {
+  switch (w) {
+    case 1: return launch_chunk<BENT, CD, 1>(a, form, s);
+    case 2: return launch_chunk<BENT, CD, 2>(a, form, s);
+    case 3: return launch_chunk<BENT, CD, 3>(a, form, s);
+    default: return launch_chunk<BENT, CD, 4>(a, form, s);
+  }
+}
 template <int CD>
 bool launch_chunk(const Args& a, int w, int form, hipStream_t s) {
-  const bool bent = a.cap2 != 0.0f || a.slopes;
-  switch (w) {
-    case 1: return bent ? launch_chunk<true, CD, 1>(a, form, s) : launch_chunk<false, CD, 1>(a, form, s);
-    case 2: return bent ? launch_chunk<true, CD, 2>(a, form, s) : launch_chunk<false, CD, 2>(a, form, s);
-    case 3: return bent ? launch_chunk<true, CD, 3>(a, form, s) : launch_chunk<false, CD, 3>(a, form, s);
-    default: return bent ? launch_chunk<true, CD, 4>(a, form, s) : launch_chunk<false, CD, 4>(a, form, s);
-  }
+  return a.slopes ? launch_chunk<2, CD>(a, w, form, s) : a.cap2 != 0.0f ? launch_chunk<1, CD>(a, w, form, s) : launch_chunk<0, CD>(a, w, form, s);
 }
 }  // namespace
 
