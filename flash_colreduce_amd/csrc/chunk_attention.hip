@@ -284,11 +284,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
       }
       look(src, stage + 1);
     };
-    look(source(), 0);
-    fetch(0);
     Queries<F, RT> q;
     float by = arguments().scale2;
     q.load(arguments(), b, h, row0, at);
+    look(source(), 0);
+    fetch(0);
     __syncthreads();                                                     // (the piece before has been used)
     bool apart = false;
     if (F::codes && arguments().bf16) {
