@@ -10,7 +10,7 @@
 // often end up on the other side of one).  First kernel: sums of pieces of the row, many workgroups, each of which finds the row by itself (a few
 // gathers); second one: the piece, then the element.
 // One sequence, 4 tokens of 32000 fp32 probabilities with what they were drawn from: 10 us, two launches and a chain of loads (tokens, their probabilities, sums, the piece); 64 of 7
-// tokens of 131072: 23 us, 67 MB, 2.9 TB/s of them; 16 trees of 63 of 100003 bf16 ones: 17 us, of which 6 find the path, a thread for each token.
+// tokens of 131072: 23 us, 67 MB, 2.9 TB/s of them; 16 trees of 63 of 100003 bf16 ones: 15 us, of which 4 find the path, a thread for each token.
 // cache_accept and cache_reserve are bound by one launch and a chain of loads: 16 rows of 8 heads of 128 bf16 elements 5.3 us, 63 int8 rows of 32 heads and 64 sequences
 // 7.0; a page here and there for 48 sequences, and back, 9.6 us together (two launches); pages for 256 prompts and back 40 us, 33000 entries of a table each way through
 // one workgroup, 0.45 us for 1024, so that their order on the stack is that of the sequences without a second launch.
@@ -150,8 +150,9 @@ __device__ __forceinline__ int count_of(const VerifyArgs& a, int b) { return a.c
 
 template <int DT>
 __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
-  __shared__ double p_of[kMostDrafted];
-  __shared__ int token_of[kMostDrafted], parent_of[kMostDrafted];     // -1: none of V; kMostDrafted: not there
+  __shared__ __attribute__((aligned(16))) double p_of[kMostDrafted];
+  __shared__ float uniform_of[kMostDrafted], q_of[kMostDrafted];
+  __shared__ __attribute__((aligned(16))) int token_of[kMostDrafted], parent_of[kMostDrafted];     // -1: none of V; kMostDrafted: not there
   __shared__ int up[2][kMostDrafted];                                 // bit 31: not taken; else the predecessor + 1
   __shared__ uint64_t path[kMostDrafted / 64];
   __shared__ int hidden;
@@ -167,6 +168,8 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
     parent_of[i] = there ? parent : kMostDrafted;
     token_of[i] = known ? (int)x : -1;
     p_of[i] = there && known ? weight(number<DT>(target + (parent + 1) * a.target_r, x)) : 0.0;
+    uniform_of[i] = a.uniform[(int64_t)b * a.T + i];
+    q_of[i] = a.draft && known ? number<DT>(a.draft + b * a.draft_b + i * a.draft_r, x) : 0.0f;
   }
   __syncthreads();
   if (a.parents && !a.draft) {
@@ -176,8 +179,12 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
     for (int i = tid, k = 0; i < count; i += kThreads, ++k) {
       const int parent = parent_of[i], token = token_of[i];
       bool found = false;
-#pragma unroll 4
-      for (int j = 0; j < i; ++j) found |= (parent_of[j] == parent) & (token_of[j] == token);
+#pragma unroll 2
+      for (int j = 0; j < i; j += 4) {
+        const int4 p = *reinterpret_cast<const int4*>(parent_of + j), x = *reinterpret_cast<const int4*>(token_of + j);
+        found |= ((p.x == parent) & (x.x == token)) | ((p.y == parent) & (x.y == token) & (j + 1 < i)) | ((p.z == parent) & (x.z == token) & (j + 2 < i)) |
+                 ((p.w == parent) & (x.w == token) & (j + 3 < i));
+      }
       again |= (found ? 1u : 0u) << k;
     }
     __syncthreads();
@@ -189,14 +196,21 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
     const int parent = parent_of[i];
     bool taken = parent != kMostDrafted && token_of[i] >= 0;
     if (taken) {
-      const double u = a.uniform[(int64_t)b * a.T + parent + 1];
+      const double u = uniform_of[parent + 1];
       if (a.draft) {
-        taken = u * weight(number<DT>(a.draft + b * a.draft_b + i * a.draft_r, token_of[i])) < p_of[i];
+        taken = u * weight(q_of[i]) < p_of[i];
       } else {
         double low = 0.0;
         if (a.parents) {
-#pragma unroll 4
-          for (int j = 0; j < i; ++j) low += parent_of[j] == parent ? p_of[j] : 0.0;
+#pragma unroll 2
+          for (int j = 0; j < i; j += 4) {
+            const int4 p = *reinterpret_cast<const int4*>(parent_of + j);
+            const double2 w0 = *reinterpret_cast<const double2*>(p_of + j), w1 = *reinterpret_cast<const double2*>(p_of + j + 2);
+            low += p.x == parent ? w0.x : 0.0;
+            low += (p.y == parent) & (j + 1 < i) ? w0.y : 0.0;
+            low += (p.z == parent) & (j + 2 < i) ? w1.x : 0.0;
+            low += (p.w == parent) & (j + 3 < i) ? w1.y : 0.0;
+          }
         }
         taken = low <= u && u < low + p_of[i];
       }
