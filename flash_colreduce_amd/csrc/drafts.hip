@@ -12,7 +12,7 @@
 // One sequence, 4 tokens of 32000 fp32 probabilities with what they were drawn from: 10 us, two launches and a chain of loads (tokens, their probabilities, sums, the piece); 64 of 7
 // tokens of 131072: 23 us, 67 MB, 2.9 TB/s of them; 16 trees of 63 of 100003 bf16 ones: 15 us, of which 4 find the path, a thread for each token.
 // cache_accept and cache_reserve are bound by one launch and a chain of loads: 16 rows of 8 heads of 128 bf16 elements 5.3 us, 63 int8 rows of 32 heads and 64 sequences
-// 7.0; a page here and there for 48 sequences, and back, 9.6 us together (two launches); pages for 256 prompts and back 40 us, 33000 entries of a table each way through
+// 5.4; a page here and there for 48 sequences, and back, 9.6 us together (two launches); pages for 256 prompts and back 40 us, 33000 entries of a table each way through
 // one workgroup, 0.45 us for 1024, so that their order on the stack is that of the sequences without a second launch.
 
 #include "paged.h"
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kThreads) cache_accept_kernel(AcceptArgs a) {
   const int b = (int)a.H.of(blockIdx.x), h = (int)(blockIdx.x - b * a.H.d), tid = threadIdx.x;
   const int context = max(a.context.of(b, h), 0), n = min(max(a.accepted[b], 0), a.T);
   if (which == 0 && tid == 0 && (h == 0 || a.by_head)) a.out[a.by_head ? blockIdx.x : b] = context + n;
-  const int each = kThreads / (int)a.pieces.d, mine = (int)a.pieces.of(tid), piece = tid - mine * (int)a.pieces.d;
+  const int each = (int)blockDim.x / (int)a.pieces.d, mine = (int)a.pieces.of(tid), piece = tid - mine * (int)a.pieces.d;
   for (int i0 = 0; i0 < n; i0 += each) {
     const int i = i0 + mine;
     bool move = mine < each && i < n;
@@ -617,7 +617,10 @@ int fcr_cache_accept(const fcr_cache* cache, const int32_t* table, int64_t table
   a.path = path, a.accepted = accepted, a.out = out, a.T = T, a.by_head = context_strides[1] != 0;
   a.H.set((uint32_t)cache->H);
   a.pieces.set((uint32_t)(cache->D * element_bytes(cache->dtype) / 16));
-  hipLaunchKernelGGL(cache_accept_kernel, dim3((unsigned)(B * cache->H), 2), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+  // Half the threads where there are more workgroups than the CUs hold at once: most of a tree's tokens do not stand, and so most threads have nothing to move.  8 of 63 rows of 32
+  // int8 heads and 64 sequences 6.7 -> 5.1 us, 50 of them 11.6 -> 11.2; for 8 heads of one sequence all 63 bf16 rows of 256 elements 3.5 with 256 threads, 4.4 with 128.
+  const int threads = 2ll * B * cache->H >= 8ll * fcr_detail::chip_cus_of_current_device() ? kThreads / 2 : kThreads;
+  hipLaunchKernelGGL(cache_accept_kernel, dim3((unsigned)(B * cache->H), 2), dim3(threads), 0, static_cast<hipStream_t>(stream), a);
   return launched("cache_accept_kernel");
 }
 

@@ -410,7 +410,7 @@ def paths(B, T, accepted, seed):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16, I8, E4M3])
-@pytest.mark.parametrize("B, H, T, D, ps", [(1, 1, 1, 16, 16), (2, 3, 7, 64, 16), (3, 2, 63, 80, 32), (2, 2, 300, 256, 16), (1, 5, 100, 176, 48), (5, 8, 16, 128, 128)])
+@pytest.mark.parametrize("B, H, T, D, ps", [(1, 1, 1, 16, 16), (2, 3, 7, 64, 16), (3, 2, 63, 80, 32), (2, 2, 300, 256, 16), (1, 5, 100, 176, 48), (5, 8, 16, 128, 128), (130, 8, 40, 96, 16)])
 def test_accept(dtype, B, H, T, D, ps):
     rng = random.Random(T)
     for turn in range(2):
