@@ -448,6 +448,10 @@ __device__ __forceinline__ void weigh(const f32x4 (&k_scale)[2], const f32x4 (&v
   for (int r = 0; r < RT; ++r) st.l[r] = sum[r];
 }
 
+constexpr float kWideCap = 128.0f * 1.44269504088896340736f;
+// What scores under a cap are formed less: a softmax does not see it, and the log-sum-exp takes it back (below caps where it would cost them bits).
+__device__ __forceinline__ float left_off(const Args& a) { return a.cap2 <= kWideCap ? a.cap2 : 0.0f; }
+
 // Scores that are capped, c tanh(s / c) = c - 2 c / (1 + 2^x) with x = s 2 log2(e) / c, which the products' scale gives; or that lose a slope times the distance
 // between a token and a key.  In base 2, and in 32 bits: next to 0 the difference is off by 2^-22 c, for caps of 128 a sixteenth of what the rounding of weights to 11 bits
 // costs; with larger ones it is formed next to 0 as a quotient (Lambert's continued fraction of tanh, six terms, off by 2^-31).  Costs a score an fma, two transcendental
@@ -479,7 +483,7 @@ struct Bend {
     return cap2 * (fabsf(y) < 1.0f ? quotient : __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), 1.0f));
   }
   __device__ __forceinline__ void capped(f32x4 (&s)[RT][2]) const {
-    if (__builtin_expect(cap2 > 128.0f * 1.44269504088896340736f, 0)) {
+    if (__builtin_expect(cap2 > kWideCap, 0)) {
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -492,11 +496,13 @@ struct Bend {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s[r][t][i] = __builtin_fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[r][t][i])), cap2);
+          for (int i = 0; i < 4; ++i) {
+            s[r][t][i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[r][t][i]));
+            if constexpr (BENT == 2) s[r][t][i] *= -2.0f * cap2;
+          }
     }
   }
-  // The products s of 32 keys from pos on become scores; nothing is left to multiply them by.
+  // The products s of 32 keys from pos on become scores, to be multiplied by k_scale (and less left_off).
   __device__ __forceinline__ void of(f32x4 (&k_scale)[2], int pos, int g, f32x4 (&s)[RT][2]) const {
     const bool behind = BENT == 2 && pos + 31 <= first, late = BENT == 1 || cap2 != 0.0f;
     if (BENT == 1 || !behind || __builtin_expect(late, 0)) {
@@ -527,8 +533,9 @@ struct Bend {
           for (int i = 0; i < 4; ++i) s[r][t][i] = __builtin_fmaf(s[r][t][i], k_scale[t][i], __builtin_fmaf(slope2[r], (float)(16 * t + i), off));
       }
     }
+    const float by = BENT == 1 && !(cap2 > kWideCap) ? -2.0f * cap2 : 1.0f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) k_scale[t] = f32x4{1, 1, 1, 1};
+    for (int t = 0; t < 2; ++t) k_scale[t] = f32x4{by, by, by, by};
   }
 };
 
@@ -978,7 +985,7 @@ __global__ void __launch_bounds__(256, (W <= 2 || Form<CD, W>::codes) ? 2 : 1) f
       if (final) {
         const Output out(a_end, b, h, row, l);
         emit<F>(a_end, out, d0, x, 1.0f / l);
-        if (a_end.lse && first) a_end.lse[out.row] = out.none ? -INFINITY : m + __builtin_amdgcn_logf(l);
+        if (a_end.lse && first) a_end.lse[out.row] = out.none ? -INFINITY : m + __builtin_amdgcn_logf(l) + (P::bent ? left_off(a_end) : 0.0f);
       } else {
         float* const to = slot + (int64_t)at.col * (a_end.D + 4);
         emit_part<F>(to, d0, x);
@@ -1361,7 +1368,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Args a, int tile_ro
     for (int j = 0; j < 4; ++j) x[j] = out.none ? 0.0f : x[j] * inverse;
     *reinterpret_cast<u32x2*>(a.out + (out.row * a.D + d) * 2) = a.bf16 ? u32x2{pack2<FCR_DTYPE_BF16>(x[0], x[1]), pack2<FCR_DTYPE_BF16>(x[2], x[3])}
                                                                        : u32x2{pack2<FCR_DTYPE_F16>(x[0], x[1]), pack2<FCR_DTYPE_F16>(x[2], x[3])};
-    if (a.lse && d == 0) a.lse[out.row] = out.none ? -INFINITY : m + __builtin_amdgcn_logf(l);
+    if (a.lse && d == 0) a.lse[out.row] = out.none ? -INFINITY : m + __builtin_amdgcn_logf(l) + left_off(a);
   }
 }
 #endif

@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
           for (int d = 0; d < F::DT; ++d) x[d] = st.o[r][d][i];
           emit<F>(a, out, Lane<F>::elements_of(a.D, 4 * at.g + i), x, inverse);
         }
-        if (a.lse && at.g == 0) a.lse[out.row] = out.none ? -INFINITY : st.m[r] + __builtin_amdgcn_logf(l);
+        if (a.lse && at.g == 0) a.lse[out.row] = out.none ? -INFINITY : st.m[r] + __builtin_amdgcn_logf(l) + (BENT ? left_off(a) : 0.0f);
       } else {
         float* const to = slot + (int64_t)((wave * RT + r) * 16 + at.col) * (a.D + 4);
 #pragma unroll
