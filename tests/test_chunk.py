@@ -496,3 +496,33 @@ def test_refusals_on_the_device():
     assert out.shape == (2, 4, 0, 64) and lse.shape == (2, 4, 0)
     out, lse = fca.chunk_attention(query, cache, table[:, :0], context, return_lse2=True)
     assert not out.any() and lse.isneginf().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(12))
+def test_random_calls(seed):
+    """Calls of any kind, five for each seed."""
+    rng = random.Random(seed)
+    for _ in range(5):
+        kind, dtype = rng.choice(KINDS)
+        h, g, t = rng.choice([1, 2, 3, 8]), rng.choice([1, 2, 4, 7]), rng.choice([1, 1, 2, 5, rng.randint(1, 40), rng.randint(1, 400)])
+        n, d, page = rng.choice([0, 3, rng.randint(0, 300), rng.randint(0, 3000)]), 16 * rng.randint(1, 16), rng.choice([16, 32, 48, 128])
+        b = rng.randint(1, max(1, min(200, 40000000 // (h * g * t * (n + t) * d))))
+        query, cache, table, context = problem(b, h, g, t, n, d, page, kind, dtype)
+        draw = torch.Generator().manual_seed(seed)
+        how = {}
+        if rng.random() < 0.5:
+            how["counts"] = torch.randint(0, t + 1, (b,), generator=draw).int()
+        if rng.random() < 0.4:
+            how["cap"] = rng.choice([0.5, 5.0, 30.0, 300.0])
+        if rng.random() < 0.3:
+            how["slopes"] = slopes_of(h * g) * rng.choice([1.0, 0.01, -0.001])
+        if rng.random() < 0.4:
+            how["window"] = rng.randint(1, n + t + 5)
+        if rng.random() < 0.4:
+            how["prefix"] = torch.randint(0, n + t + 2, (b,), generator=draw).int()
+        if rng.random() < 0.6:
+            context = torch.randint(0, n + 1, (b, h) if rng.random() < 0.3 else (b,), generator=draw).int()
+        if rng.random() < 0.2:
+            table[rng.randrange(b), rng.randrange(table.shape[1])] = -1
+        check(query, cache, table, context, **how)
