@@ -266,7 +266,8 @@ def test_many_blocks_per_workgroup(shape, kind, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,dtype", [(F16, F16), (E4M3, BF16)])
-@pytest.mark.parametrize("b,h,g,t,n,d", [(70, 8, 2, 1, 2500, 16), (9, 4, 1, 300, 1500, 32), (9, 4, 1, 300, 200, 32), (130, 8, 1, 1, 300, 64), (24, 4, 2, 20, 900, 64)])
+@pytest.mark.parametrize("b,h,g,t,n,d", [(70, 8, 2, 1, 2500, 16), (9, 4, 1, 300, 1500, 32), (9, 4, 1, 300, 200, 32), (130, 8, 1, 1, 300, 64), (24, 4, 2, 20, 900, 64),
+                                         (45, 4, 1, 400, 100, 64), (40, 2, 4, 200, 60, 128)])
 def test_items_whole_and_cut(kind, dtype, b, h, g, t, n, d):
     """Many items, of one length, of drawn lengths, one long among short ones, of nothing but for one, of own lengths for each head."""
     query, cache, table, _ = problem(b, h, g, t, n, d, 16, kind, dtype)
