@@ -318,7 +318,7 @@ def chunk_attention(query: torch.Tensor, cache: KVCache, table: torch.Tensor, co
     Returns (B, Hq, T, D) of query's type, and with return_lse2 the base-2 log-sum-exp of every row's scores, fp32 (B, Hq, T).  A row that sees nothing (or that the
     sequence does not have, or whose every score is -inf) is zeros, its log-sum-exp -inf.  What hidden rows of the cache hold, NaNs included, has no
     influence.  Probabilities are rounded to fp16 (bf16 against a bf16 cache) as they multiply the values, sums are fp32.  The last bits of a
-    sequence's result depend on how the work was cut, and so on the lengths of the others in the batch."""
+    sequence's result depend on how the work was cut, and so on the lengths of the others in the batch and on the table's width."""
     out = _host().chunk_attention(query, cache, table, context, scale, counts, cap, slopes, window, prefix, return_lse2)
     if out is not None:
         return out
