@@ -312,7 +312,7 @@ def chunk_attention(query: torch.Tensor, cache: KVCache, table: torch.Tensor, co
     prefix, int32 (B,), besides those every j < prefix[b], also behind it (tokens of an image, or the first ones that a window is to keep).  counts,
     int32 (B,): sequences that have fewer than T new tokens.
 
-    A score is scale * q.k, scale 1/sqrt(D) by default; with cap it becomes cap * tanh(score / cap), and with slopes, fp32 (Hq,), slopes[head] * |i - j| is
+    A score is scale * q.k, scale 1/sqrt(D) by default; with cap (at most 2.35e38) it becomes cap * tanh(score / cap), and with slopes, fp32 (Hq,), slopes[head] * |i - j| is
     taken off it.  Positions are those in the cache: after cache_keep they are not those in the text, and distances and windows go by what is left.
 
     Returns (B, Hq, T, D) of query's type, and with return_lse2 the base-2 log-sum-exp of every row's scores, fp32 (B, Hq, T).  A row that sees nothing (or that the

@@ -35,7 +35,7 @@ struct Args {
   int wgs;                     // workgroups of the launch
   int positions;               // that a row of the table names
   // of chunk_attention
-  float cap2;                  // scores in base 2 are capped at this (scale2 then is what the cap's exponential takes); 0: as they are
+  float cap2;                  // scores in base 2 are capped at this (scale2 then is what the cap's exponential takes, up to kWideCap); 0: as they are
   const float* slopes;         // [H G] or null
   const int32_t* prefix;       // [B] or null
   int window;                  // INT32_MAX: none
@@ -452,7 +452,8 @@ constexpr float kWideCap = 128.0f * 1.44269504088896340736f;
 // What scores under a cap are formed less: a softmax does not see it, and the log-sum-exp takes it back (below caps where it would cost them bits).  An fma of each score: 409 -> 397 us.
 __device__ __forceinline__ float left_off(const Args& a) { return a.cap2 <= kWideCap ? a.cap2 : 0.0f; }
 
-// Scores that are capped, c tanh(s / c) = c - 2 c / (1 + 2^x) with x = s 2 log2(e) / c, which the products' scale gives; or that lose a slope times the distance
+// Scores that are capped, c tanh(s / c) = c - 2 c / (1 + 2^x) with x = s 2 log2(e) / c, which the products' scale gives (caps above 128: it gives s log2(e), since x of
+// the largest caps has no bits left in 32); or that lose a slope times the distance
 // between a token and a key.  In base 2, and in 32 bits: next to 0 the difference is off by 2^-22 c, for caps of 128 a sixteenth of what the rounding of weights to 11 bits
 // costs; with larger ones it is formed next to 0 as a quotient (Lambert's continued fraction of tanh, six terms, off by 2^-31).  A cap costs a score two transcendental
 // instructions, a multiplication and an addition, a slope an fma, 397 and 346 us for 4 chunks of 512 tokens behind 8192 fp16 keys of 128 elements, 8 heads of 4 queries, that take 300 without.
@@ -476,20 +477,25 @@ struct Bend {
       }
     }
   }
-  __device__ __forceinline__ float wide(float x) const {
-    const float y = x * 0.34657359027997265471f, z = y * y;              // ln(2) / 2
-    const float quotient = y * __builtin_fmaf(__builtin_fmaf(21.0f, z, 1260.0f), z, 10395.0f) *
-                           __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fmaf(z + 210.0f, z, 4725.0f), z, 10395.0f));
-    return cap2 * (fabsf(y) < 1.0f ? quotient : __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), 1.0f));
+  // x: a score in base 2.  Next to 0 it is multiplied by tanh(y) / y, y = x / cap2; by16 = 16 / cap2, which no cap leaves subnormal.
+  __device__ __forceinline__ float wide(float x, float by16) const {
+    const float y = x * 0.0625f * by16, z = y * y;
+    const float ratio = __builtin_fmaf(__builtin_fmaf(21.0f, z, 1260.0f), z, 10395.0f) *
+                        __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fmaf(z + 210.0f, z, 4725.0f), z, 10395.0f));
+    const float e = __builtin_amdgcn_exp2f(y * 2.88539008177792681472f);      // e^(2 y)
+    return fabsf(y) < 1.0f ? x * ratio : cap2 * __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
   }
   __device__ __forceinline__ void capped(f32x4 (&s)[RT][2]) const {
     if (__builtin_expect(cap2 > kWideCap, 0)) {
+      float sixteenth = cap2 * 0.0625f;
+      asm volatile("" : "+v"(sixteenth));                                  // (formed here, not kept)
+      const float by16 = __builtin_amdgcn_rcpf(sixteenth);
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[r][t][i] = wide(s[r][t][i]);
+          for (int i = 0; i < 4; ++i) s[r][t][i] = wide(s[r][t][i], by16);
     } else {
 #pragma unroll
       for (int r = 0; r < RT; ++r)

@@ -764,8 +764,9 @@ int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* ta
   a.window = window ? window : INT32_MAX;
   constexpr float log2e = 1.44269504088896340736f;
   a.cap2 = cap * log2e;
-  a.scale2 = cap != 0.0f ? scale * (2.0f * log2e) / cap : scale * log2e;
-  if (!isfinite(a.scale2) || !isfinite(a.cap2)) return fail(FCR_E_SCALE, "scale over cap must be finite");
+  a.scale2 = cap != 0.0f && a.cap2 <= kWideCap ? scale * (2.0f * log2e) / cap : scale * log2e;
+  if (!isfinite(a.cap2)) return fail(FCR_E_SCALE, "cap in base 2 (1.4427 cap) must be finite");
+  if (!isfinite(a.scale2)) return fail(FCR_E_SCALE, "scale over cap must be finite");
   a.whole = whole_items_of(plan.items, plan.held, most_blocks(plan, positions, prefix ? 0 : window, G), plan.form != 1);
   a.all_heads.set((uint32_t)(B * cache->H));
   const int w = (cache->D + 63) / 64;

@@ -324,6 +324,23 @@ def test_scores_at_the_ends(kind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("cap", [1e36, 1e37, 1e38, 2.35e38])
+def test_the_largest_caps(kind, dtype, cap):
+    """Caps next to which every score is small leave them as they are, whatever powers of two codes and bf16 queries bring with them; scores as large as the caps."""
+    query, cache, table, context = problem(2, 2, 2, 20, 200, 64, 16, kind, dtype, spread=2.0)
+    for how in (dict(), dict(slopes=slopes_of(4), counts=torch.tensor([20, 7]).int()), dict(scale=3e-4), dict(scale=1e34)):
+        check(query, cache, table, context, cap=cap, **how)
+        check(query[:, :, :3], cache, table, context, cap=cap, **how)
+
+
+def test_caps_past_32_bits_are_refused():
+    """What a cap is in base 2 has to be a number, too; the text says which of the two it was."""
+    assert _chunk_c(cap=2.4e38) == -6 and b"cap in base 2" in _lib.load().fcr_last_error()
+    assert _chunk_c(cap=1e-38, scale=1e3) == -6 and b"scale over cap" in _lib.load().fcr_last_error()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [F16, BF16])
 @pytest.mark.parametrize("t,places", [(3, same), (100, same), (100, wide)])
 def test_scores_that_are_not_finite(kind, t, places):
