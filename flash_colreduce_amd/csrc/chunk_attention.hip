@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_attention_kernel(Args arg
   __shared__ u32x4 operands[kRing * kStep];
   __shared__ __attribute__((aligned(16))) float scales[kRing][2][32];    // of keys, of values
   __shared__ float most[kRing][2];                                       // the largest scale of a tile's values
-  __shared__ int2 flags[kRing];                                          // a tile's page is there, and (bit 1) one of its values was not finite
+  __shared__ __attribute__((aligned(16))) int2 flags[kRing];             // a tile's page is there, and (bit 1) one of its values was not finite
   __shared__ float rest[WAVES][RT][16];                                  // powers of two that rows' scores are still to be multiplied by
   __shared__ int scan[2 * WAVES + 4];
   const int wg = range_of(args, blockIdx.x);

@@ -3,6 +3,7 @@ import ctypes
 import math
 import os
 import random
+import re
 import subprocess
 
 import pytest
@@ -165,6 +166,23 @@ def test_blocks_of_a_tile_hold_every_key_that_it_sees(sight):
             assert wave_some or not any(step & s for s in rows)
         # and no block without a reason
         assert out[0] <= max(1, len({j // 128 for j in seen_by_any}) + 1)
+
+
+def test_shared_arrays_that_are_read_16_bytes_at_a_time_are_aligned_for_it():
+    """By their elements' type or by their declaration: where the compiler happens to put them is no promise."""
+    csrc, wide_reads = os.path.join(ROOT, "flash_colreduce_amd", "csrc"), 0
+    for name in sorted(os.listdir(csrc)):
+        text = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
+        for kernel in re.split(r"__global__", text)[1:]:
+            arrays = {}
+            for aligned, kind, names in re.findall(r"__shared__\s+(?:__attribute__\(\(aligned\((\d+)\)\)\)\s+)?(\w+)\s+([^;]+);", kernel):
+                for array in re.findall(r"(\w+)(?:\[[^\]]*\])+", names):
+                    arrays[array] = int(aligned or 0) >= 16 or kind in ("u32x4", "f32x4", "int4")
+            for array in re.findall(r"reinterpret_cast<\s*(?:const\s+)?(?:u32x4|f32x4|int4|double2)\s*\*>\(\s*(\w+)", kernel):
+                if array in arrays:
+                    wide_reads += 1
+                    assert arrays[array], (name, array)
+    assert wide_reads >= 4
 
 
 def _chunk_c(**over):
