@@ -704,22 +704,9 @@ namespace {
 // of 16 sequences over 8 heads of 8192 e4m3 keys of 64 elements, 4 queries each: 39 us with two, 37 with three, 41 with four; of 128 elements 8 x 8 heads of 16384 keys 55 and
 // 57 with three.
 int few_per_cu(int D) { return D <= 64 ? 3 : 0; }
-// Blocks that an item of a plan has at most; window: 0 where there is none, or a prefix, whose length only the device knows.
-int64_t most_blocks(const Plan& p, int64_t positions, int window, int G) {
-  return ((window ? std::min(positions, (int64_t)window + p.tile_rows / G + 2 * kBlock) : positions) + kBlock - 1) / kBlock;
-}
-// few_attention_kernel takes more rows than form_of gives it, in tiles of 16, where the chip has few of them: it starts faster and its items are many, so that they run at once and
-// need not be cut.  us, by it and by the kernel for many rows, at the largest size on its side and the next one: 8 x 8 fp16 heads of 128 rows of 128 elements, 1564 keys 36.0, 41.6,
-// 256 rows, 464 keys 26.5, 31.9, 1564 keys 63.4, 49.4; of 64 elements 256 rows, 464 keys 16.7, 22.0, 1564 keys 39.2, 35.4; of 256 elements 128 rows, 464 keys 32.5, 39.9, 1564 keys
-// 72.0, 57.7; e4m3 keys of 128 elements, 512 rows, 178 keys 24.9, 25.7, 528 keys 40.7, 38.4.  One item of 64 rows of 128 elements and 114 keys: 7.5, 16.0.
-bool few_rows(const Plan& p, int64_t longest) { return p.items * (longest + 2) <= 15ll * p.held; }
-// Tiles of 128 rows, two workgroups to a CU, instead of 256, where there are more than the chip holds and they are short or mostly of keys that only some of the rows see: less is
-// multiplied that is hidden, and what runs once for one tile runs beside the other one's products.  fp16, us, 128 rows and 256: 64 elements, 128 prompts of 384 tokens, 16 heads, 159, 230;
-// 8 of 2048 of 8 heads of 4 queries 261, 272, 2 of 4096 of 16 heads 148, 141; 64 chunks of 64 behind 300 keys 42, 44, 16 of 512 behind 2000 265, 267; 128 elements: 16 of 768
-// 196, 206, 8 of 1024 152, 145, 32 of 256 behind 500 keys 184, 181.
-bool half_tiles(const Plan& p, int64_t longest, int D, int64_t positions, int T) {
-  return p.items > p.held && (positions <= 2ll * T ? longest <= (D <= 64 ? 16 : 6) : D <= 64 && longest <= 6);
-}
+int64_t most_blocks(const Plan& p, int64_t positions, int window, int G) { return most_blocks_of(positions, window, p.tile_rows, G); }
+bool few_rows(const Plan& p, int64_t longest) { return takes_few_rows(p.items, p.held, longest); }
+bool half_tiles(const Plan& p, int64_t longest, int D, int64_t positions, int T) { return takes_half_tiles(p.items, p.held, longest, D, positions, T); }
 bool chunk_plan(bool codes, int B, int H, int G, int T, int D, int64_t positions, int window, Plan& p) {
   if (plan_of(codes, B, H, G, T, D, positions, p, few_per_cu(D), 1) && few_rows(p, most_blocks(p, positions, window, G))) return true;
   if (D <= 128 && (int64_t)T * G > 128 && plan_of(codes, B, H, G, T, D, positions, p, 0, 4) && half_tiles(p, most_blocks(p, positions, window, G), D, positions, T)) return true;

@@ -6,6 +6,8 @@
 // tells the join how many blocks others have; from that the join knows how many workgroups these are (followers), one behind the other.
 #pragma once
 
+#include <stdint.h>
+
 #include "div.h"
 
 namespace fcr_tree {
@@ -116,6 +118,24 @@ struct Steps {
   // of all steps from `first` down to `last`
   FCR_HOST_DEVICE bool whole(int first, int last) const { return (last >= fast && first - fast < fasts) || first <= prefix - 32; }
 };
+
+// Blocks that an item of chunk_attention has at most; window: 0 where there is none, or a prefix, whose length only the device knows.
+FCR_HOST_DEVICE inline int64_t most_blocks_of(int64_t positions, int window, int tile_rows, int G) {
+  const int64_t near = (int64_t)window + tile_rows / G + 2 * kBlock;
+  return ((window && near < positions ? near : positions) + kBlock - 1) / kBlock;
+}
+// few_attention_kernel takes more rows than form_of gives it, in tiles of 16, where the chip has few of them: it starts faster and its items are many, so that they run at once and
+// need not be cut.  us, by it and by the kernel for many rows, at the largest size on its side and the next one: 8 x 8 fp16 heads of 128 rows of 128 elements, 1564 keys 36.0, 41.6,
+// 256 rows, 464 keys 26.5, 31.9, 1564 keys 63.4, 49.4; of 64 elements 256 rows, 464 keys 16.7, 22.0, 1564 keys 39.2, 35.4; of 256 elements 128 rows, 464 keys 32.5, 39.9, 1564 keys
+// 72.0, 57.7; e4m3 keys of 128 elements, 512 rows, 178 keys 24.9, 25.7, 528 keys 40.7, 38.4.  One item of 64 rows of 128 elements and 114 keys: 7.5, 16.0.
+FCR_HOST_DEVICE inline bool takes_few_rows(int64_t items, int held, int64_t longest) { return items * (longest + 2) <= 15ll * held; }
+// Tiles of 128 rows, two workgroups to a CU, instead of 256, where there are more than the chip holds and they are short or mostly of keys that only some of the rows see: less is
+// multiplied that is hidden, and what runs once for one tile runs beside the other one's products.  fp16, us, 128 rows and 256: 64 elements, 128 prompts of 384 tokens, 16 heads, 159, 230;
+// 8 of 2048 of 8 heads of 4 queries 261, 272, 2 of 4096 of 16 heads 148, 141; 64 chunks of 64 behind 300 keys 42, 44, 16 of 512 behind 2000 265, 267; 128 elements: 16 of 768
+// 196, 206, 8 of 1024 152, 145, 32 of 256 behind 500 keys 184, 181.
+FCR_HOST_DEVICE inline bool takes_half_tiles(int64_t items, int held, int64_t longest, int D, int64_t positions, int T) {
+  return items > held && (positions <= 2ll * T ? longest <= (D <= 64 ? 16 : 6) : D <= 64 && longest <= 6);
+}
 
 // Items of chunk_attention may be taken whole, a workgroup for each, by a launch of as many: nothing is cut and joined, tiles of one head run together on one die, but the last
 // workgroups may leave others idle.  2: they are, without a look at the lengths or the launch that joins, where the longest that there can be (blocks of it) is no more

@@ -168,6 +168,52 @@ def test_blocks_of_a_tile_hold_every_key_that_it_sees(sight):
         assert out[0] <= max(1, len({j // 128 for j in seen_by_any}) + 1)
 
 
+@pytest.fixture(scope="module")
+def tile_rule(tmp_path_factory):
+    """The kernel that csrc/deal.h gives a call of more than 128 rows of at most 128 elements, on 256 compute units: 1, 4 or 8."""
+    tmp = tmp_path_factory.mktemp("tiles")
+    (tmp / "t.cpp").write_text(
+        '#include "deal.h"\nusing namespace fcr_tree;\n'
+        'extern "C" int form(int codes, int B, int H, int G, int T, int D, int positions, int window) {\n'
+        '  const int w = (D + 63) / 64, rows = T * G, small = rows_of_tile(1, w), half = rows_of_tile(4, w);\n'
+        '  const int64_t heads = (int64_t)B * H;\n'
+        '  if (takes_few_rows(heads * quotient_up(rows, small), 256 * (w == 1 ? 3 : 2), most_blocks_of(positions, window, small, G))) return 1;\n'
+        '  if (takes_half_tiles(heads * quotient_up(rows, half), 512, most_blocks_of(positions, window, half, G), D, positions, T)) return 4;\n'
+        '  return form_of(rows, w, codes); }\n')
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "flash_colreduce_amd", "csrc"), str(tmp / "t.cpp"), "-o",
+                    str(tmp / "t.so")], check=True)
+    return ctypes.CDLL(str(tmp / "t.so")).form
+
+
+# (B, H, G, T, context, D, page), window: several tiles of 128 rows to a head, more of them than the chip holds; prompts, and a window far behind the first key
+HALVES = [((33, 8, 1, 150, 350, 64, 16), 300), ((34, 8, 2, 75, 400, 48, 16), 130), ((33, 8, 1, 300, 20, 64, 16), None), ((33, 8, 1, 270, 0, 128, 16), None),
+          ((45, 4, 3, 130, 100, 112, 16), None)]
+
+
+@pytest.mark.parametrize("shape,window", HALVES)
+def test_many_short_tiles_are_of_128_rows(shape, window, tile_rule):
+    b, h, g, t, n, d, page = shape
+    positions = -(-(n + t) // page) * page
+    assert all(tile_rule(codes, b, h, g, t, d, positions, window or 0) == 4 for codes in (0, 1))
+    assert tile_rule(0, 1, h, g, 4000, d, 1 << 20, 0) == 8 and tile_rule(0, 1, 1, g, t, d, positions, window or 0) == 1
+    assert (positions > 2 * t) == (window is not None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [(F16, F16), (BF16, BF16), (I8, BF16), (E4M3, F16)])
+@pytest.mark.parametrize("shape,window", HALVES)
+def test_tiles_of_128_rows(shape, window, kind, dtype):
+    """Behind a window, and with everything that becomes of scores; ragged counts, contexts of own length for each head."""
+    b, h, g, t, n, d, page = shape
+    query, cache, table, context = problem(*shape, kind, dtype)
+    draw = torch.Generator().manual_seed(t)
+    counts, context = torch.randint(0, t + 1, (b,), generator=draw).int(), torch.randint(0, n + 1, (b, h), generator=draw).int()
+    counts[0], context[0] = t, n
+    for how in (dict(), dict(cap=3.0), dict(slopes=slopes_of(h * g), counts=counts), dict(cap=200.0, slopes=slopes_of(h * g) * 0.1)):
+        got = call(query, cache, table, context, window=window, **how)
+        compare_attention(*got, ref_chunk(query, cache, table, context, window=window, **how))
+
+
 def test_shared_arrays_that_are_read_16_bytes_at_a_time_are_aligned_for_it():
     """By their elements' type or by their declaration: where the compiler happens to put them is no promise."""
     csrc, wide_reads = os.path.join(ROOT, "flash_colreduce_amd", "csrc"), 0
