@@ -1,5 +1,5 @@
-// How the work of tree_attention is cut, in whole numbers: the kernels', the join's and the host's side of it.  Plain C++, so that it can be
-// tested without a device.
+// How the work of tree_attention and chunk_attention is cut, in whole numbers: the kernels', the join's and the host's side of it.  Plain C++, so that it can be
+// tested without a device.  Sight, Steps and what stands behind them are chunk_attention's alone.
 //
 // An item is 16 rows and more of a (sequence, head) and all of its keys, in blocks of kBlock.  Blocks of all items are laid end to end and every workgroup
 // takes `per` of them, or (most_of) items are cut into pieces of one item each, a workgroup for each.  Of an item that was cut the workgroup with its first part
@@ -50,8 +50,8 @@ FCR_HOST_DEVICE inline int piece_length(int blocks, int pieces) { return quotien
 // Workgroups behind the one with an item's first part that have parts of it: `others` blocks are theirs.  unit: `per`, or the pieces' `most`.
 FCR_HOST_DEVICE inline int followers(int others, int unit) { return others <= 0 ? 0 : quotient_up(others, unit); }
 
-// Which kernel takes `rows` rows of a (sequence, head) of at most 64 w elements: 1, few_attention_kernel; 4 and 8, tall_attention_kernel of as many
-// waves (4: of at most 128 elements, see tall_tiles).
+// Which kernel takes `rows` rows of a (sequence, head) of at most 64 w elements: 1, few_attention_kernel; 4 and 8, tall_attention_kernel (chunk_attention:
+// chunk_attention_kernel) of as many waves (4: of at most 128 elements, see tall_tiles).
 // Both sides, us, at 4 sequences x 8 heads x 8192 keys, int8 (bf16): 48 rows of 64 elements 33 (31) by form 1, 37 (33) by form 4, 64 rows 38
 // (35) and 38 (34); of 128 elements 42 (45) and 47 (46), 48 (52) and 49 (47); 48 rows of 256 elements 59 (89) by form 1, 62 (61) by form 8, 64
 // rows 69 (108) and 65 (67); 128 rows of 128 elements 58 (57) by form 4, 60 (64) by form 8, 192 rows 77 (79) and 72 (74).

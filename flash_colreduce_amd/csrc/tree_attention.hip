@@ -30,7 +30,7 @@
 //
 // Distribution: the (batch, head, row tile) items are cut into blocks of 128 keys, laid end to end, and every workgroup takes the same
 // number of blocks, found from the lengths on the device; or, where that takes little longer, one piece of one item.  Parts of an item that
-// was cut are joined by tree_join_kernel, in the order of the keys.
+// was cut are joined by attention_join_kernel, in the order of the keys.
 
 #include "attention.h"
 
