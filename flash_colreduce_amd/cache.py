@@ -309,8 +309,8 @@ def chunk_attention(query: torch.Tensor, cache: KVCache, table: torch.Tensor, co
 
     query is (B, Hq, T, D), fp16 or bf16 (the cache's type if that is one of them), Hq a multiple of the cache's heads: heads h*G .. h*G+G-1 attend to
     head h.  Token t has position i = context[b] + t (or context[b, h] + t) and sees positions j <= i, with window (at least 1) only those above i - window; with
-    prefix, int32 (B,), besides those every j < prefix[b], also behind it (tokens of an image, or the first ones that a window is to keep).  counts,
-    int32 (B,): sequences that have fewer than T new tokens.
+    prefix, int32 (B,), besides those every j < prefix[b], also behind it, up to the sequence's last new token (tokens of an image, or the first ones that a window is
+    to keep: the two are one number, so a prefix whose tokens see each other never leaves a window).  counts, int32 (B,): sequences that have fewer than T new tokens.
 
     A score is scale * q.k, scale 1/sqrt(D) by default; with cap (at most 2.35e38) it becomes cap * tanh(score / cap), and with slopes, fp32 (Hq,), slopes[head] * |i - j| is
     taken off it.  Positions are those in the cache: after cache_keep they are not those in the text, and distances and windows go by what is left.
@@ -318,7 +318,12 @@ def chunk_attention(query: torch.Tensor, cache: KVCache, table: torch.Tensor, co
     Returns (B, Hq, T, D) of query's type, and with return_lse2 the base-2 log-sum-exp of every row's scores, fp32 (B, Hq, T).  A row that sees nothing (or that the
     sequence does not have, or whose every score is -inf) is zeros, its log-sum-exp -inf.  What hidden rows of the cache hold, NaNs included, has no
     influence.  Probabilities are rounded to fp16 (bf16 against a bf16 cache) as they multiply the values, sums are fp32.  The last bits of a
-    sequence's result depend on how the work was cut, and so on the lengths of the others in the batch and on the table's width."""
+    sequence's result depend on how the work was cut, and so on the lengths of the others in the batch and on the table's width.
+
+    Lengths are known on the device only: how many rows a workgroup takes, and whether parts are joined, goes by the positions that the table names, and with a window and no
+    prefix by the window.  Short sequences behind a table that has room for long ones run faster with a view of the columns that are in use, table[:, :n]: one that
+    is 65536 positions wide takes 128 prompts of 384 tokens, 16 heads of 64 elements, from 159 to 261 us, 512 tokens of 16 heads behind 16 from 14 to 34, 17 tokens of two
+    sequences behind 300 from 7 to 12.5, and two prompts of 4096 nowhere."""
     out = _host().chunk_attention(query, cache, table, context, scale, counts, cap, slopes, window, prefix, return_lse2)
     if out is not None:
         return out

@@ -376,7 +376,8 @@ int fcr_tree_attention(const void* q, const fcr_cache* cache, const int32_t* tab
  * are scale q k, with cap > 0 then cap tanh(. / cap), with slopes ([H*G], fp32, may be NULL) then less slopes[head] |i - j|; lse is that of the scores so
  * formed.  Tokens from counts on get zeros and -inf.  With a cap a score of +-infinity is +-cap.  Positions that no token of a tile sees are not read.
  * ws: fcr_chunk_attention_bytes(B, H, G, T, D, table_pages * page_size) bytes, as above; the same limits.  cap must be >= 0,
- * cap log2(e) and scale / cap finite in fp32.
+ * cap log2(e) and scale / cap finite in fp32.  How the work is cut goes by table_pages, as lengths are known on the device only: with short sequences, say no more
+ * pages than the longest of them needs (the stride stays).
  */
 size_t fcr_chunk_attention_bytes(int B, int H, int G, int T, int D, int64_t positions);
 int fcr_chunk_attention(const void* q, const fcr_cache* cache, const int32_t* table, int64_t table_stride, int table_pages,
