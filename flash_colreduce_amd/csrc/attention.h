@@ -456,9 +456,11 @@ __device__ __forceinline__ float left_off(const Args& a) { return a.cap2 <= kWid
 // the largest caps has no bits left in 32); or that lose a slope times the distance
 // between a token and a key.  In base 2, and in 32 bits: next to 0 the difference is off by 2^-22 c, for caps of 128 a sixteenth of what the rounding of weights to 11 bits
 // costs; with larger ones it is formed next to 0 as a quotient (Lambert's continued fraction of tanh, six terms, off by 2^-31).  A cap costs a score two transcendental
-// instructions, a multiplication and an addition, a slope an fma, 397 and 346 us for 4 chunks of 512 tokens behind 8192 fp16 keys of 128 elements, 8 heads of 4 queries, that take 300 without.
+// instructions, a multiplication and an addition, a slope an fma, 387 and 342 us for 4 chunks of 512 tokens behind 8192 fp16 keys of 128 elements, 8 heads of 4 queries, that take 295 without.
 // BENT: 1, capped; 2, with slopes, and a cap perhaps; 0, neither.  (One kernel for caps and slopes spilled up to 126 registers: 4 chunks of 512 tokens behind 8192 fp16 keys of
-// 128 elements, 8 heads of 4 queries, capped, 430 us by it and 413 by its own, two biased prompts of 4096 tokens, 16 heads, 215 and 203; both at once 446 and 467.)  Keys behind
+// 128 elements, 8 heads of 4 queries, capped, 430 us by it and 413 by its own, two biased prompts of 4096 tokens, 16 heads, 215 and 203; both at once 446 and 467.
+// Of the three the one with neither spills where rows have 128 elements of 16 bits, 33 registers (fp16) and 44 (bf16) with eight waves, 42 and 72 with four, in the steps on the borders of what rows see; the
+// straight-line code has none of it.  All three spill 18 to 20 where they have 256.)  Keys behind
 // every token of the rows take their distance as it is, an fma with what is common to a row; others its magnitude, an instruction more.
 template <int RT, int BENT>
 struct Bend {

@@ -9,10 +9,10 @@
 // are dealt, since tiles of one sequence have different numbers of them (ChunkDeal); and Bend, behind the products.
 //
 // few_attention_kernel: one token of 48 sequences over 8 heads of up to 4096 e4m3 keys of 128 elements, 4 queries each, capped: 70 us, 4.4 TB/s; two chunks of 17 tokens,
-// 4 heads of 2 queries, behind up to 300 fp16 keys of 64 elements with slopes: 7.3 us, one launch and a chain of loads: lengths, table, keys.
+// 4 heads of 2 queries, behind up to 300 fp16 keys of 64 elements with slopes: 7.6 us, one launch and a chain of loads: lengths, table, keys.
 // chunk_attention_kernel, bound by vector and matrix instructions of two waves to a SIMD that run next to each other for a fifth of the time: a prompt of 8192 tokens, 8 heads of
-// 8 queries, fp16, 128 elements: 1180 us, 930 TFLOP/s; 4 chunks of 512 behind 8192 keys, 8 heads of 4: 300 to 340 us by the card, 830 to 945 TFLOP/s; two biased bf16 prompts of up to 4096 tokens,
-// 16 heads: 180 us; two of 2048 behind up to 16384 keys of 96 fp16 elements that see 1024 and a prefix of 64: 75 us.
+// 8 queries, fp16, 128 elements: 1163 us, 946 TFLOP/s; 4 chunks of 512 behind 8192 keys, 8 heads of 4: 295 us, 955 TFLOP/s; two biased bf16 prompts of up to 4096 tokens,
+// 16 heads: 132 to 204 us by the drawn lengths; two of 2048 behind up to 16384 keys of 96 fp16 elements that see 1024 and a prefix of 64: 77 us.
 
 #include "attention.h"
 

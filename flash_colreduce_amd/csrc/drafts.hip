@@ -10,9 +10,9 @@
 // often end up on the other side of one).  First kernel: sums of pieces of the row, many workgroups, each of which finds the row by itself (a few
 // gathers); second one: the piece, then the element.
 // One sequence, 4 tokens of 32000 fp32 probabilities with what they were drawn from: 10 us, two launches and a chain of loads (tokens, their probabilities, sums, the piece); 64 of 7
-// tokens of 131072: 23 us, 67 MB, 2.9 TB/s of them; 16 trees of 63 of 100003 bf16 ones: 15 us, of which 4 find the path, a thread for each token.
-// cache_accept and cache_reserve are bound by one launch and a chain of loads: 16 rows of 8 heads of 128 bf16 elements 5.3 us, 63 int8 rows of 32 heads and 64 sequences
-// 6.1; a page here and there for 48 sequences, and back, 9.6 us together (two launches); pages for 256 prompts and back 40 us, 33000 entries of a table each way through
+// tokens of 131072: 24 us, 67 MB, 2.8 TB/s of them; 16 trees of 63 of 100003 bf16 ones: 14.5 us, 10 of them the first launch: tokens, their probabilities, siblings and the path, one behind the other.
+// cache_accept and cache_reserve are bound by one launch and a chain of loads: 16 rows of 8 heads of 128 bf16 elements 5.2 us, 63 int8 rows of 32 heads and 64 sequences
+// 5.8; a page here and there for 48 sequences, and back, 9.5 us together (two launches); pages for 256 prompts and back 40 us, 33000 entries of a table each way through
 // one workgroup, 0.45 us for 1024, so that their order on the stack is that of the sequences without a second launch.
 
 #include "paged.h"
