@@ -8,6 +8,9 @@ to where they belong (cache_accept), and room for the next ones (cache_reserve).
     context = cache_accept(cache, table, context, path, accepted)             # each layer's cache
     cache_reserve(pool, table, context, page_size)                            # pages of what was rejected go back
 
+Models that cap their scores, bias them by distance or limit them to a window attend to a drafted chain by chunk_attention; tree_attention, which trees need, has plain
+scores only.
+
 The reference has none of this.  The kernels are csrc/drafts.hip behind the C ABI (include/fcr.h); nothing here has a gradient.  Every call is
 asynchronous on the current stream of its operands' device and allocates with torch only; all of them can be captured into a graph.
 """
